@@ -85,6 +85,33 @@ int pgd_matrix_upload_q6k(pgd_dev* dev, const void* blocks, int n_out, int n_in,
  * 283-289 like the k-quants. Format ids 3 and 4 in pgd_matrix_info. */
 int pgd_matrix_upload_q8_0(pgd_dev* dev, const void* blocks, int n_out, int n_in, pgd_matrix** out);
 int pgd_matrix_upload_q5_0(pgd_dev* dev, const void* blocks, int n_out, int n_in, pgd_matrix** out);
+/* ---- MXFP4 (OCP microscaling formats v1.0; no reference counterpart) --------
+ * Blocks of 32 consecutive elements of a row: 4-bit codes (bit 3 the sign, then
+ * 0 .5 1 1.5 2 3 4 6) and one scale byte s that stands for 2^(s - 127); s = 255
+ * makes the block NaN. Row-major planes: codes, element 2 i of a row in the low
+ * nibble of byte i, and one scale byte per block. Format id 5 in
+ * pgd_matrix_info; pgd_matrix_dequant and the pgd_matrix_gemv* entry points that
+ * take f32 / f16 rows take these matrices too. n_in is a multiple of 32.
+ *
+ * upload: host planes, codes [n_out][n_in / 2], scales [n_out][n_in / 32]. */
+int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* scales, int n_out, int n_in,
+                            pgd_matrix** out);
+/* The same from device planes, code rows ldc bytes apart (a multiple of 16, the
+ * plane 16-byte aligned), scale rows lds bytes (a multiple of 4, 4-byte
+ * aligned). Queued on the handle's stream: the planes may go once it has run. */
+int pgd_matrix_from_mxfp4_dev(pgd_dev* dev, const uint8_t* codes, int ldc, const uint8_t* scales, int lds, int n_out,
+                              int n_in, pgd_matrix** out);
+/* Rows x [nrows, k] of f32 (x_type 0), f16 (1) or bf16 (2), row stride ldx
+ * elements (a multiple of 8; x 16-byte aligned), to MXFP4 planes with strides as
+ * above. A block's scale is the power of two of its largest magnitude over 4
+ * (s at most 252, at least 0); codes are x / scale rounded to nearest, ties to
+ * the even code, magnitudes above 6 to 6. A block with an infinity or NaN gets
+ * s = 255 and codes 0. values (nullable; row stride ldv, a multiple of 4,
+ * 16-byte aligned) receives the f32 values that codes and scales stand for.
+ * Bytes of a plane's row past its codes or scales are left as they were. */
+int pgd_mxfp4_quantize_dev(pgd_dev* dev, const void* x, int x_type, int ldx, int nrows, int k, uint8_t* codes, int ldc,
+                           uint8_t* scales, int lds, float* values, int ldv);
+
 /* Seeded synthetic matrix: N(0, std) weights quantized on the device (no
  * reference counterpart: the reference only loads checkpoints). */
 int pgd_matrix_synth(pgd_dev* dev, int fmt, int n_out, int n_in, uint64_t seed, uint64_t key, float std,
@@ -102,13 +129,23 @@ int pgd_matrix_dequant(const pgd_matrix* m, int row0, int rows, float* out);
 int pgd_matrix_gemv(const pgd_matrix* m, const float* x, int nrows, float* y);
 /* Device form. x f32 (x_f16 = 0) or IEEE f16 (x_f16 = 1), row stride ldx
  * elements (multiple of 8); y row stride ldy; res (nullable) adds a residual
- * y = res + W.x (replaces affine_gemv_res, qwen3_gemv.rs:289-306). */
+ * y = res + W.x (replaces affine_gemv_res, qwen3_gemv.rs:289-306).
+ * MXFP4 matrices also take bf16 rows (x_f16 = 2), and x must be 16-byte
+ * aligned; every x enters the products exactly, sums are f32. */
 int pgd_matrix_gemv_dev(const pgd_matrix* m, const void* x, int x_f16, int ldx, int nrows, float* y,
                         int ldy, const float* res, int ldres);
 /* mid = silu(gate . x) * (up . x); replaces affine_gemv2_silu
  * (qwen3_gemv.rs:256-286). */
 int pgd_matrix_gemv_swiglu_dev(const pgd_matrix* gate, const pgd_matrix* up, const float* x, int ldx,
                                int nrows, float* mid, int ldm);
+/* Products of MXFP4 rows (planes as pgd_mxfp4_quantize_dev writes them, strides
+ * as there; each plane nrows rows) with MXFP4 matrices, on the scaled 4-bit
+ * matrix instructions with f32 sums: y = W.x, plus res (nullable) as in
+ * pgd_matrix_gemv_dev, and mid = silu(gate.x) * (up.x). Any nrows >= 0. */
+int pgd_matrix_gemv_mx_dev(const pgd_matrix* m, const uint8_t* codes, int ldc, const uint8_t* scales, int lds, int nrows,
+                           float* y, int ldy, const float* res, int ldres);
+int pgd_matrix_gemv_swiglu_mx_dev(const pgd_matrix* gate, const pgd_matrix* up, const uint8_t* codes, int ldc,
+                                  const uint8_t* scales, int lds, int nrows, float* mid, int ldm);
 /* A8 activations converted once into matrix-core operands, shared by every
  * A8 matrix of width k (the reference shares one x across several matrices
  * the same way: gemv_shared / affine_gemv_n, qwen3_gemv.rs:149-253).

@@ -11,6 +11,7 @@
 #include "../../include/pagoda_hip.h"
 #include "common.h"
 #include "device.h"
+#include "mxfp4.h"
 #include "ops.h"
 #include "quant.h"
 
@@ -214,6 +215,68 @@ int pgd_matrix_upload_q5_0(pgd_dev* dev, const void* blocks, int n_out, int n_in
   return upload_kq(dev, FMT_Q5_0, blocks, n_out, n_in, out);
 }
 
+int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* scales, int n_out, int n_in,
+                            pgd_matrix** out) {
+  pgd_matrix* held = nullptr;
+  int rc = guard([&] {
+    PGD_CHECK(codes && scales, kErrArg, "null argument");
+    DeviceScope scope(dev);
+    new_matrix(dev, FMT_MXFP4, n_out, n_in, out, &held);
+    const size_t nc = (size_t)n_out * (n_in / 2), ns = (size_t)n_out * (n_in / kMxBlock);
+    DevBuf c(nc), sc(ns);
+    hipStream_t s = dev->stream;
+    PGD_HIP(hipMemcpyAsync(c.p, codes, nc, hipMemcpyHostToDevice, s));
+    PGD_HIP(hipMemcpyAsync(sc.p, scales, ns, hipMemcpyHostToDevice, s));
+    mx_tile(held->m, MxPlanes{c.as<uint8_t>(), n_in / 2, sc.as<uint8_t>(), n_in / kMxBlock}, s);
+    PGD_HIP(hipStreamSynchronize(s));
+    *out = held;
+  });
+  if (rc && held) pgd_matrix_free(held);
+  return rc;
+}
+
+// Row-major planes of rows of n_in columns, as every entry point takes them.
+static MxPlanes planes(const uint8_t* codes, int ldc, const uint8_t* scales, int lds, int n_in) {
+  PGD_CHECK(codes && scales, kErrArg, "null argument");
+  PGD_CHECK(reinterpret_cast<uintptr_t>(codes) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0, kErrArg,
+            "MXFP4 codes must be 16-byte and scales 4-byte aligned");
+  PGD_CHECK(ldc >= n_in / 2 && ldc % 16 == 0, kErrShape, "MXFP4 code stride must be >= n_in / 2 and a multiple of 16");
+  PGD_CHECK(lds >= n_in / kMxBlock && lds % 4 == 0, kErrShape,
+            "MXFP4 scale stride must be >= n_in / 32 and a multiple of 4");
+  return MxPlanes{codes, ldc, scales, lds};
+}
+
+int pgd_matrix_from_mxfp4_dev(pgd_dev* dev, const uint8_t* codes, int ldc, const uint8_t* scales, int lds, int n_out,
+                              int n_in, pgd_matrix** out) {
+  pgd_matrix* held = nullptr;
+  int rc = guard([&] {
+    PGD_CHECK(n_out > 0 && n_in > 0, kErrShape, "matrix dims must be positive");
+    const MxPlanes p = planes(codes, ldc, scales, lds, n_in);
+    DeviceScope scope(dev);
+    new_matrix(dev, FMT_MXFP4, n_out, n_in, out, &held);
+    mx_tile(held->m, p, dev->stream);
+    *out = held;
+  });
+  if (rc && held) pgd_matrix_free(held);
+  return rc;
+}
+
+int pgd_mxfp4_quantize_dev(pgd_dev* dev, const void* x, int x_type, int ldx, int nrows, int k, uint8_t* codes, int ldc,
+                           uint8_t* scales, int lds, float* values, int ldv) {
+  return guard([&] {
+    PGD_CHECK(dev && x, kErrArg, "null argument");
+    PGD_CHECK(x_type >= X_F32 && x_type <= X_BF16, kErrArg, "rows are f32 (0), f16 (1) or bf16 (2)");
+    PGD_CHECK(nrows >= 0 && k > 0 && k % kMxBlock == 0, kErrShape, "MXFP4 rows: width must be a multiple of 32");
+    PGD_CHECK(ldx >= k && ldx % 8 == 0, kErrShape, "ldx must be >= k and a multiple of 8");
+    PGD_CHECK(reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(values) % 16 == 0, kErrArg,
+              "rows and values must be 16-byte aligned");
+    PGD_CHECK(!values || (ldv >= k && ldv % 4 == 0), kErrShape, "ldv must be >= k and a multiple of 4");
+    planes(codes, ldc, scales, lds, k);
+    DeviceScope scope(dev);
+    mx_quantize(x, x_type, ldx, nrows, k, codes, ldc, scales, lds, values, ldv, dev->stream);
+  });
+}
+
 int pgd_matrix_synth(pgd_dev* dev, int fmt, int n_out, int n_in, uint64_t seed, uint64_t key, float std,
                      pgd_matrix** out) {
   pgd_matrix* held = nullptr;
@@ -297,6 +360,31 @@ int pgd_matrix_gemv_swiglu_dev(const pgd_matrix* gate, const pgd_matrix* up, con
     PGD_CHECK(ldm >= gate->m.n_out, kErrShape, "swiglu output stride");
     DeviceScope scope(gate->dev);
     qmat_gemv_swiglu(gate->m, up->m, x, ldx, nrows, mid, ldm, gate->dev->stream);
+  });
+}
+
+int pgd_matrix_gemv_mx_dev(const pgd_matrix* m, const uint8_t* codes, int ldc, const uint8_t* scales, int lds, int nrows,
+                           float* y, int ldy, const float* res, int ldres) {
+  return guard([&] {
+    PGD_CHECK(m && y, kErrArg, "null argument");
+    PGD_CHECK(m->m.fmt == FMT_MXFP4, kErrFormat, "MXFP4 rows feed MXFP4 matrices");
+    const MxPlanes p = planes(codes, ldc, scales, lds, m->m.n_in);
+    PGD_CHECK(ldy >= m->m.n_out && (!res || ldres >= m->m.n_out), kErrShape, "gemv output stride");
+    DeviceScope scope(m->dev);
+    mx_gemv_planes(m->m, nullptr, p, nrows, MxOut{y, ldy, res, ldres}, m->dev->stream);
+  });
+}
+
+int pgd_matrix_gemv_swiglu_mx_dev(const pgd_matrix* gate, const pgd_matrix* up, const uint8_t* codes, int ldc,
+                                  const uint8_t* scales, int lds, int nrows, float* mid, int ldm) {
+  return guard([&] {
+    PGD_CHECK(gate && up && mid, kErrArg, "null argument");
+    PGD_CHECK(gate->dev == up->dev, kErrArg, "gate and up live on different devices");
+    PGD_CHECK(gate->m.fmt == FMT_MXFP4 && up->m.fmt == FMT_MXFP4, kErrFormat, "MXFP4 rows feed MXFP4 matrices");
+    const MxPlanes p = planes(codes, ldc, scales, lds, gate->m.n_in);
+    PGD_CHECK(ldm >= gate->m.n_out, kErrShape, "swiglu output stride");
+    DeviceScope scope(gate->dev);
+    mx_gemv_planes(gate->m, &up->m, p, nrows, MxOut{mid, ldm, nullptr, 0}, gate->dev->stream);
   });
 }
 

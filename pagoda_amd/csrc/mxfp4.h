@@ -1,0 +1,82 @@
+// mxfp4.h — MXFP4 (OCP microscaled 4-bit floating point) operands: the public
+// row-major planes, the device layout of matrices, and the launchers.
+//
+// A block is 32 consecutive elements of a row: 4-bit codes (sign, 2 exponent
+// and 1 mantissa bits: 0 .5 1 1.5 2 3 4 6) and one scale byte s that stands for
+// 2^(s - 127); s = 255 makes the block NaN.
+//
+// Planes (activations, and what a matrix is made of): codes [rows][ldc bytes],
+// element 2 i of a row in the low nibble of byte i, and scales [rows][lds bytes].
+//
+// Matrices: tiles of 16 rows by 128 columns, [row tile][k tile]. Lane l of a
+// wave owns row l % 16 and block l / 16 of a tile, which is what one lane feeds
+// the 16x16x128 scaled matrix instruction: codes [64 lanes][16 B], scales
+// [64 lanes][1 B]. Rows and columns of the last tiles past the matrix are zeros.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "quant.h"
+
+namespace pgd {
+
+enum XType : int { X_F32 = 0, X_F16 = 1, X_BF16 = 2 };
+inline int xtype_bytes(int t) { return t == X_F32 ? 4 : 2; }
+
+constexpr int kMxBlock = 32, kMxTileN = 16, kMxTileK = 128;
+
+inline int mx_row_tiles(int n) { return (n + kMxTileN - 1) / kMxTileN; }
+inline int mx_k_tiles(int k) { return (k + kMxTileK - 1) / kMxTileK; }
+inline size_t mx_code_bytes(int n, int k) { return (size_t)mx_row_tiles(n) * mx_k_tiles(k) * 1024; }
+inline size_t mx_scale_bytes(int n, int k) { return (size_t)mx_row_tiles(n) * mx_k_tiles(k) * 64; }
+
+// Row-major planes on the device.
+struct MxPlanes {
+  const uint8_t* codes;
+  int ldc;  // bytes, a multiple of 16
+  const uint8_t* scales;
+  int lds;  // bytes, a multiple of 4
+};
+
+// Rows of x (XType, stride ldx elements) to planes; values (nullable, row
+// stride ldv) receives what the codes stand for.
+void mx_quantize(const void* x, int type, int ldx, int rows, int k, uint8_t* codes, int ldc, uint8_t* scales, int lds,
+                 float* values, int ldv, hipStream_t s);
+// planes of n_out rows into the planes of an allocated FMT_MXFP4 matrix
+void mx_tile(QMat& m, const MxPlanes& p, hipStream_t s);
+void mx_dequant(const QMat& m, int row0, int rows, float* out, hipStream_t s);
+
+// What a product's epilogue does.
+struct MxOut {
+  float* y;
+  int ldy;
+  const float* res;  // nullable; may be y
+  int ldres;
+};
+// y = W x (+ res), or with up: y = silu(W x) * (up x). x is rows of XType in
+// device memory, or planes.
+void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, int rows, const MxOut& o, hipStream_t s);
+void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, const MxOut& o, hipStream_t s);
+
+namespace mx {
+
+// One product launch. Activation rows are planes (codes set), or bf16 terms:
+// row r is the sum over t < terms of the bf16 rows x[t * term_stride + r * ldx].
+struct Args {
+  const uint8_t *wc, *ws;  // matrix codes, scales
+  const uint8_t *uc, *us;  // the up matrix's (SwiGLU), or null
+  int n_out, nt, kt, nblk;  // outputs; row tiles, k tiles, 32-element blocks of a row
+  int rows;
+  MxPlanes p;
+  const uint16_t* x;
+  size_t ldx, term_stride;
+  int terms;
+  MxOut o;
+};
+
+// A few rows: see gemv_mx.hip.
+void run_few(const Args& a, hipStream_t s);
+
+}  // namespace mx
+}  // namespace pgd

@@ -1,0 +1,249 @@
+// mxfp4.hip — MXFP4 operands: quantization, matrix tiling, dequantization, the
+// exact split of activation rows into bf16 terms, and the product front end.
+#include <algorithm>
+#include <mutex>
+
+#include "common.h"
+#include "gemv_impl.h"
+#include "mxfp4.h"
+#include "mxfp4_dev.h"
+
+namespace pgd {
+
+using namespace mx;
+
+namespace {
+
+// Eight consecutive elements of a row as f32.
+template <int TYPE>
+__device__ inline void load8(const void* x, size_t at, float (&v)[8]) {
+  if constexpr (TYPE == X_F32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
+    const float4 a = p[0], b = p[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (TYPE == X_BF16) {
+        v[2 * i] = __builtin_bit_cast(float, w[i] << 16);
+        v[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xffff0000u);
+      } else {
+        v[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
+        v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
+      }
+    }
+  }
+}
+
+// Units (8 elements) of a row go to a power of two of threads, at most 256; the
+// rest of a 256-thread workgroup takes further rows.
+struct RowGrid {
+  dim3 grid, block;
+  RowGrid(int units, int rows) {
+    int bx = 1;
+    while (bx < units && bx < 256) bx *= 2;
+    block = dim3(bx, 256 / bx);
+    grid = dim3((units + bx - 1) / bx, std::min((rows + (int)block.y - 1) / (int)block.y, 65535));
+  }
+};
+
+// A block's scale byte is the exponent of its largest magnitude less 2 (6 = 1.5
+// 2^2 is the largest code), codes are rounded to nearest, ties to the even code,
+// and saturate at 6: the conversion instruction's own rounding. Four threads
+// share a block. Bound by HBM: each element is read once and written once.
+template <int TYPE>
+__global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ x, int ldx, int rows, int units,
+                                                       uint8_t* __restrict__ codes, int ldc,
+                                                       uint8_t* __restrict__ scales, int lds,
+                                                       float* __restrict__ values, int ldv) {
+  const int u = blockIdx.x * blockDim.x + threadIdx.x;
+  if (u >= units) return;  // (units is a multiple of 4: a block's threads stay together)
+  const int step = gridDim.y * blockDim.y;
+  for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += step) {
+    float v[8];
+    load8<TYPE>(x, (size_t)r * ldx + (size_t)u * 8, v);
+    // magnitudes as bits: a NaN's exceed an infinity's, so nothing is lost to a maximum
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    const int e = (int)(top >> 23);
+    const int sc = e == 255 ? 255 : max(e - 2, 0);
+    const float scale = __builtin_bit_cast(float, (uint32_t)sc << 23);
+    uint32_t c = 0;
+    if (sc != 255) c = fp4_pack8(v, scale);
+    *reinterpret_cast<uint32_t*>(codes + (size_t)r * ldc + (size_t)u * 4) = c;
+    if ((u & 3) == 0) scales[(size_t)r * lds + (u >> 2)] = (uint8_t)sc;
+    if (values) {
+      float o[8];
+      fp4_unpack8(c, scale, o);
+      float* d = values + (size_t)r * ldv + (size_t)u * 8;
+      reinterpret_cast<float4*>(d)[0] = make_float4(o[0], o[1], o[2], o[3]);
+      reinterpret_cast<float4*>(d)[1] = make_float4(o[4], o[5], o[6], o[7]);
+    }
+  }
+}
+
+// One block (16 code bytes and its scale) per thread into its place in the tiles.
+__global__ __launch_bounds__(256) void tile_kernel(MxPlanes p, int n_out, int nblk, int kt, uint8_t* __restrict__ codes,
+                                                   uint8_t* __restrict__ scales) {
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b >= nblk) return;
+  const int step = gridDim.y * blockDim.y;
+  for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < n_out; r += step) {
+    const size_t tile = (size_t)(r >> 4) * kt + (b >> 2);
+    const int lane = (r & 15) + 16 * (b & 3);
+    const uint4 c = *reinterpret_cast<const uint4*>(p.codes + (size_t)r * p.ldc + (size_t)b * 16);
+    *reinterpret_cast<uint4*>(codes + tile * 1024 + lane * 16) = c;
+    scales[tile * 64 + lane] = p.scales[(size_t)r * p.lds + b];
+  }
+}
+
+__global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict__ codes,
+                                                      const uint8_t* __restrict__ scales, int row0, int rows, int units,
+                                                      int kt, float* __restrict__ out) {
+  const int u = blockIdx.x * blockDim.x + threadIdx.x;
+  if (u >= units) return;
+  const int step = gridDim.y * blockDim.y;
+  for (int i = blockIdx.y * blockDim.y + threadIdx.y; i < rows; i += step) {
+    const int r = row0 + i, b = u >> 2;
+    const size_t tile = (size_t)(r >> 4) * kt + (b >> 2);
+    const int lane = (r & 15) + 16 * (b & 3);
+    const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + tile * 1024 + lane * 16 + (u & 3) * 4);
+    float o[8];
+    fp4_unpack8(c, e8m0_f32(scales[tile * 64 + lane]), o);
+    float* d = out + (size_t)i * units * 8 + (size_t)u * 8;
+    reinterpret_cast<float4*>(d)[0] = make_float4(o[0], o[1], o[2], o[3]);
+    reinterpret_cast<float4*>(d)[1] = make_float4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+// x = t0 + t1 + t2 exactly: each term is the truncation to bf16 (8 significant
+// bits) of what is left, so 3 terms hold the 24 bits of an f32, 2 the 11 of an
+// f16. An infinity or NaN is its first term alone (a NaN stays one: its bits
+// below bf16 are or-ed in). Columns [k, ldt) are zeros, which the last k tile reads.
+template <int TYPE, int TERMS>
+__global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, int ldx, int rows, int units,
+                                                    uint16_t* __restrict__ out, int ldt, size_t term_stride) {
+  const int u = blockIdx.x * blockDim.x + threadIdx.x;
+  if (u * 8 >= ldt) return;
+  const int step = gridDim.y * blockDim.y;
+  for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += step) {
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (u < units) load8<TYPE>(x, (size_t)r * ldx + (size_t)u * 8, v);
+    uint32_t t[TERMS][4];
+    split_terms8<TERMS>(v, t);
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i)
+      *reinterpret_cast<uint4*>(out + i * term_stride + (size_t)r * ldt + (size_t)u * 8) =
+          make_uint4(t[i][0], t[i][1], t[i][2], t[i][3]);
+  }
+}
+
+Args make_args(const QMat& w, const QMat* up, int rows, const MxOut& o) {
+  Args a{};
+  a.wc = w.p0;
+  a.ws = w.p1;
+  if (up) {
+    a.uc = up->p0;
+    a.us = up->p1;
+  }
+  a.n_out = w.n_out;
+  a.nt = mx_row_tiles(w.n_out);
+  a.kt = mx_k_tiles(w.n_in);
+  a.nblk = w.n_in / kMxBlock;
+  a.rows = rows;
+  a.o = o;
+  return a;
+}
+
+void check(const QMat& w, const QMat* up, int rows) {
+  PGD_CHECK(w.fmt == FMT_MXFP4 && (!up || up->fmt == FMT_MXFP4), kErrFormat, "not an MXFP4 matrix");
+  PGD_CHECK(!up || (up->n_out == w.n_out && up->n_in == w.n_in), kErrShape, "swiglu gate/up shapes differ");
+  PGD_CHECK(rows >= 0, kErrShape, "gemv rows");
+}
+
+// The terms lie in the stream's scratch between the two launches. Held over
+// both, so that no other host thread's call on the stream is queued between
+// them or replaces the buffer.
+std::mutex g_terms;
+
+}  // namespace
+
+void mx_quantize(const void* x, int type, int ldx, int rows, int k, uint8_t* codes, int ldc, uint8_t* scales, int lds,
+                 float* values, int ldv, hipStream_t s) {
+  if (rows == 0) return;
+  const int units = k / 8;
+  const RowGrid g(units, rows);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, g.grid, g.block, 0, s, x, ldx, rows, units, codes, ldc, scales, lds, values, ldv);
+  };
+  if (type == X_F32) go(quantize_kernel<X_F32>);
+  else if (type == X_F16) go(quantize_kernel<X_F16>);
+  else go(quantize_kernel<X_BF16>);
+  PGD_HIP(hipGetLastError());
+}
+
+void mx_tile(QMat& m, const MxPlanes& p, hipStream_t s) {
+  const int nblk = m.n_in / kMxBlock;
+  const RowGrid g(nblk, m.n_out);
+  hipLaunchKernelGGL(tile_kernel, g.grid, g.block, 0, s, p, m.n_out, nblk, mx_k_tiles(m.n_in), m.p0, m.p1);
+  PGD_HIP(hipGetLastError());
+}
+
+void mx_dequant(const QMat& m, int row0, int rows, float* out, hipStream_t s) {
+  if (rows == 0) return;
+  const int units = m.n_in / 8;
+  const RowGrid g(units, rows);
+  hipLaunchKernelGGL(dequant_kernel, g.grid, g.block, 0, s, m.p0, m.p1, row0, rows, units, mx_k_tiles(m.n_in), out);
+  PGD_HIP(hipGetLastError());
+}
+
+void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, int rows, const MxOut& o, hipStream_t s) {
+  check(w, up, rows);
+  PGD_CHECK(type >= X_F32 && type <= X_BF16, kErrArg, "activations are f32 (0), f16 (1) or bf16 (2)");
+  PGD_CHECK(ldx >= w.n_in && ldx % 8 == 0, kErrShape, "gemv ldx must be >= n_in and a multiple of 8");
+  PGD_CHECK(reinterpret_cast<uintptr_t>(x) % 16 == 0, kErrArg, "MXFP4 activations must be 16-byte aligned");
+  if (rows == 0) return;
+  Args a = make_args(w, up, rows, o);
+  a.terms = type == X_F32 ? 3 : type == X_F16 ? 2 : 1;
+  if (type == X_BF16 && w.n_in % kMxTileK == 0) {  // the rows are their own term
+    a.x = static_cast<const uint16_t*>(x);
+    a.ldx = ldx;
+    run_few(a, s);
+    return;
+  }
+  // a captured graph would keep the scratch's address, which a later call may replace
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  PGD_HIP(hipStreamIsCapturing(s, &cap));
+  PGD_CHECK(cap == hipStreamCaptureStatusNone, kErrState,
+            "these MXFP4 activation rows need scratch memory: capture bf16 rows of whole 128-column tiles, or MXFP4 rows");
+  const int ldt = a.kt * kMxTileK;
+  std::lock_guard<std::mutex> lock(g_terms);
+  a.term_stride = (size_t)rows * ldt;
+  auto* t = static_cast<uint16_t*>(gemv::gemv_scratch(s, a.terms * a.term_stride * sizeof(uint16_t), 8));
+  a.x = t;
+  a.ldx = ldt;
+  const RowGrid g(ldt / 8, rows);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, g.grid, g.block, 0, s, x, ldx, rows, w.n_in / 8, t, ldt, a.term_stride);
+  };
+  if (type == X_F32) go(terms_kernel<X_F32, 3>);
+  else if (type == X_F16) go(terms_kernel<X_F16, 2>);
+  else go(terms_kernel<X_BF16, 1>);
+  PGD_HIP(hipGetLastError());
+  run_few(a, s);
+}
+
+void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, const MxOut& o, hipStream_t s) {
+  check(w, up, rows);
+  if (rows == 0) return;
+  Args a = make_args(w, up, rows, o);
+  a.p = x;
+  run_few(a, s);
+}
+
+}  // namespace pgd

@@ -8,6 +8,7 @@
 
 #include "common.h"
 #include "gemv_impl.h"
+#include "mxfp4.h"
 #include "ops.h"
 #include "quant.h"
 
@@ -498,6 +499,7 @@ double qmat_algo_bytes(const QMat& m) {
     case FMT_Q6K: return n * 6.5625 / 8.0;
     case FMT_Q8_0: return n * 8.5 / 8.0;
     case FMT_Q5_0: return n * 5.5 / 8.0;
+    case FMT_MXFP4: return n * 4.25 / 8.0;
   }
   return 0.0;
 }
@@ -542,6 +544,10 @@ void qmat_alloc(QMat& m, int fmt, int n_out, int n_in, hipStream_t s) {
     place(0, rows * n_in / 2);
     place(1, rows * m.nsb * 4);
     place(2, rows * m.nsb * 2);
+  } else if (fmt == FMT_MXFP4) {
+    PGD_CHECK(n_in % kMxBlock == 0, kErrShape, "MXFP4 n_in must be a multiple of 32");
+    place(0, mx_code_bytes(n_out, n_in));
+    place(1, mx_scale_bytes(n_out, n_in));
   } else {
     throw Error{kErrFormat, "unknown matrix format"};
   }
@@ -650,6 +656,7 @@ void qmat_upload_kq(QMat& m, const uint8_t* blocks, hipStream_t s) {
 
 void qmat_dequant(const QMat& m, int row0, int rows, float* out, hipStream_t s) {
   PGD_CHECK(row0 >= 0 && rows >= 0 && row0 + rows <= m.n_out, kErrShape, "dequant row range");
+  if (m.fmt == FMT_MXFP4) return mx_dequant(m, row0, rows, out, s);
   launch_dequant(m, row0, rows, nullptr, out, m.n_in, s);
 }
 
@@ -661,6 +668,7 @@ void qmat_gemv(const QMat& m, const void* x, int x_f16, int ldx, int nrows, floa
                int ldres, hipStream_t s) {
   PGD_CHECK(nrows >= 0, kErrShape, "gemv rows");
   PGD_CHECK(ldx >= m.n_in && ldx % 8 == 0, kErrShape, "gemv ldx must be >= n_in and a multiple of 8");
+  if (m.fmt == FMT_MXFP4) return mx_gemv(m, nullptr, x, x_f16, ldx, nrows, MxOut{y, ldy, res, ldres}, s);
   if (nrows == 0) return;
   GemvArgs a = make_args(m);
   a.x = x;
@@ -677,6 +685,7 @@ void qmat_gemv_swiglu(const QMat& gate, const QMat& up, const float* x, int ldx,
   PGD_CHECK(gate.fmt == up.fmt && gate.n_out == up.n_out && gate.n_in == up.n_in, kErrShape,
             "swiglu gate/up shapes differ");
   PGD_CHECK(ldx >= gate.n_in && ldx % 8 == 0, kErrShape, "gemv ldx must be >= n_in and a multiple of 8");
+  if (gate.fmt == FMT_MXFP4) return mx_gemv(gate, &up, x, X_F32, ldx, nrows, MxOut{mid, ldm, nullptr, 0}, s);
   if (nrows == 0) return;
   GemvArgs a = make_args(gate);
   a.u0 = up.p0;

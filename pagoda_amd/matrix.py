@@ -8,8 +8,10 @@ import numpy as np
 from ._lib import call
 from .device import Device
 
-FMT_A8, FMT_Q4K, FMT_Q6K, FMT_Q8_0, FMT_Q5_0 = 0, 1, 2, 3, 4
-FMT_NAMES = {FMT_A8: "a8", FMT_Q4K: "q4k", FMT_Q6K: "q6k", FMT_Q8_0: "q8_0", FMT_Q5_0: "q5_0"}
+FMT_A8, FMT_Q4K, FMT_Q6K, FMT_Q8_0, FMT_Q5_0, FMT_MXFP4 = 0, 1, 2, 3, 4, 5
+FMT_NAMES = {FMT_A8: "a8", FMT_Q4K: "q4k", FMT_Q6K: "q6k", FMT_Q8_0: "q8_0", FMT_Q5_0: "q5_0", FMT_MXFP4: "mxfp4"}
+# activation rows of MXFP4 products and of mxfp4_quantize_dev
+X_F32, X_F16, X_BF16 = 0, 1, 2
 
 
 def _ptr(a: np.ndarray) -> C.c_void_p:
@@ -24,6 +26,13 @@ def act_bytes(nrows: int, k: int) -> int:
 
 def act_prep_dev(dev: Device, x_ptr: int, ldx: int, nrows: int, k: int, act_ptr: int) -> None:
     call("pgd_act_prep_dev", dev.handle, C.c_void_p(x_ptr), ldx, nrows, k, C.c_void_p(act_ptr))
+
+
+def mxfp4_quantize_dev(dev: Device, x_ptr: int, x_type: int, ldx: int, nrows: int, k: int, codes_ptr: int, ldc: int,
+                       scales_ptr: int, lds: int, values_ptr: int = 0, ldv: int = 0) -> None:
+    """Rows of f32 / f16 / bf16 (x_type) to MXFP4 planes; values_ptr also receives the values they stand for."""
+    call("pgd_mxfp4_quantize_dev", dev.handle, C.c_void_p(x_ptr), x_type, ldx, nrows, k, C.c_void_p(codes_ptr), ldc,
+         C.c_void_p(scales_ptr), lds, C.c_void_p(values_ptr or None), ldv)
 
 
 class Matrix:
@@ -62,6 +71,24 @@ class Matrix:
         return cls(dev, h)
 
     @classmethod
+    def upload_mxfp4(cls, dev: Device, codes: np.ndarray, scales: np.ndarray, n_out: int, n_in: int):
+        """MXFP4 planes, row-major: codes [n_out, n_in / 2], scales [n_out, n_in / 32]."""
+        codes = np.ascontiguousarray(codes, np.uint8)
+        scales = np.ascontiguousarray(scales, np.uint8)
+        assert codes.size == n_out * (n_in // 2) and scales.size == n_out * (n_in // 32)
+        h = C.c_void_p()
+        call("pgd_matrix_upload_mxfp4", dev.handle, _ptr(codes), _ptr(scales), n_out, n_in, C.byref(h))
+        return cls(dev, h)
+
+    @classmethod
+    def from_mxfp4_dev(cls, dev: Device, codes_ptr: int, ldc: int, scales_ptr: int, lds: int, n_out: int, n_in: int):
+        """MXFP4 planes in device memory (queued: they may go once the handle's stream has passed)."""
+        h = C.c_void_p()
+        call("pgd_matrix_from_mxfp4_dev", dev.handle, C.c_void_p(codes_ptr), ldc, C.c_void_p(scales_ptr), lds, n_out,
+             n_in, C.byref(h))
+        return cls(dev, h)
+
+    @classmethod
     def synth(cls, dev: Device, fmt: int, n_out: int, n_in: int, seed: int, key: int, std: float = 0.02):
         h = C.c_void_p()
         call("pgd_matrix_synth", dev.handle, fmt, n_out, n_in, C.c_uint64(seed), C.c_uint64(key), C.c_float(std), C.byref(h))
@@ -93,8 +120,9 @@ class Matrix:
         call("pgd_matrix_gemv", self.handle, _ptr(x2), x2.shape[0], _ptr(y))
         return y[0] if squeeze else y
 
-    def gemv_dev(self, x_ptr: int, ldx: int, nrows: int, y_ptr: int, ldy: int, x_f16: bool = False,
+    def gemv_dev(self, x_ptr: int, ldx: int, nrows: int, y_ptr: int, ldy: int, x_f16: int = False,
                  res_ptr: int = 0, ldres: int = 0) -> None:
+        """x_f16: f32 rows (False), f16 (True), or for MXFP4 matrices X_F32 / X_F16 / X_BF16."""
         call("pgd_matrix_gemv_dev", self.handle, C.c_void_p(x_ptr), int(x_f16), ldx, nrows, C.c_void_p(y_ptr), ldy,
              C.c_void_p(res_ptr or None), ldres)
 
@@ -121,3 +149,15 @@ class Matrix:
     @staticmethod
     def gemv_swiglu_dev(gate: "Matrix", up: "Matrix", x_ptr: int, ldx: int, nrows: int, mid_ptr: int, ldm: int):
         call("pgd_matrix_gemv_swiglu_dev", gate.handle, up.handle, C.c_void_p(x_ptr), ldx, nrows, C.c_void_p(mid_ptr), ldm)
+
+    def gemv_mx_dev(self, codes_ptr: int, ldc: int, scales_ptr: int, lds: int, nrows: int, y_ptr: int, ldy: int,
+                    res_ptr: int = 0, ldres: int = 0) -> None:
+        """MXFP4 rows (planes) times this MXFP4 matrix."""
+        call("pgd_matrix_gemv_mx_dev", self.handle, C.c_void_p(codes_ptr), ldc, C.c_void_p(scales_ptr), lds, nrows,
+             C.c_void_p(y_ptr), ldy, C.c_void_p(res_ptr or None), ldres)
+
+    @staticmethod
+    def gemv_swiglu_mx_dev(gate: "Matrix", up: "Matrix", codes_ptr: int, ldc: int, scales_ptr: int, lds: int,
+                           nrows: int, mid_ptr: int, ldm: int):
+        call("pgd_matrix_gemv_swiglu_mx_dev", gate.handle, up.handle, C.c_void_p(codes_ptr), ldc,
+             C.c_void_p(scales_ptr), lds, nrows, C.c_void_p(mid_ptr), ldm)
