@@ -75,8 +75,9 @@ struct Args {
   MxOut o;
 };
 
-// A few rows: see gemv_mx.hip.
+// A few rows (gemv_mx.hip), many (gemm_mx.hip), and whichever suits.
 void run_few(const Args& a, hipStream_t s);
+void run_many(const Args& a, hipStream_t s);
 
 }  // namespace mx
 }  // namespace pgd

@@ -160,6 +160,11 @@ Args make_args(const QMat& w, const QMat* up, int rows, const MxOut& o) {
   return a;
 }
 
+void run(const Args& a, hipStream_t s) {
+  if (a.rows <= 64) run_few(a, s);
+  else run_many(a, s);
+}
+
 void check(const QMat& w, const QMat* up, int rows) {
   PGD_CHECK(w.fmt == FMT_MXFP4 && (!up || up->fmt == FMT_MXFP4), kErrFormat, "not an MXFP4 matrix");
   PGD_CHECK(!up || (up->n_out == w.n_out && up->n_in == w.n_in), kErrShape, "swiglu gate/up shapes differ");
@@ -213,7 +218,7 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   if (type == X_BF16 && w.n_in % kMxTileK == 0) {  // the rows are their own term
     a.x = static_cast<const uint16_t*>(x);
     a.ldx = ldx;
-    run_few(a, s);
+    run(a, s);
     return;
   }
   // a captured graph would keep the scratch's address, which a later call may replace
@@ -235,7 +240,7 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   else if (type == X_F16) go(terms_kernel<X_F16, 2>);
   else go(terms_kernel<X_BF16, 1>);
   PGD_HIP(hipGetLastError());
-  run_few(a, s);
+  run(a, s);
 }
 
 void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, const MxOut& o, hipStream_t s) {
@@ -243,7 +248,7 @@ void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, 
   if (rows == 0) return;
   Args a = make_args(w, up, rows, o);
   a.p = x;
-  run_few(a, s);
+  run(a, s);
 }
 
 }  // namespace pgd
