@@ -62,6 +62,12 @@ __global__ __launch_bounds__(64 * T::W, T::W / 4) void gemm_kernel(Args a, int n
   const int i16 = lane & 15, q = lane >> 4;
   const int wm = wave / T::WN, wn = wave % T::WN;
 
+  // An activation load takes 64 B (a k tile's codes, or a block's terms) of each
+  // of 16 rows, four neighbouring lanes a row, so that they leave as one request.
+  // The four 16 B parts of row i lie in LDS in the order 0..3 ^ i / 4: then the
+  // 16 lanes that read one part of 16 rows at once meet no bank twice.
+  const int lr = lane >> 2, lp = (lane & 3) ^ (lane >> 4);
+  const int swz = i16 >> 2;
   // this wave's loads: sources without the k tile's offset
   const uint8_t* src[T::NL];
 #pragma unroll
@@ -69,10 +75,10 @@ __global__ __launch_bounds__(64 * T::W, T::W / 4) void gemm_kernel(Args a, int n
     const int j = wave * T::NL + k;
     if (j < T::XI) {
       if constexpr (T::FP4) {
-        src[k] = a.p.codes + (size_t)min(m0 + j * 16 + i16, a.rows - 1) * a.p.ldc;
-      } else {  // block j % 4 of 16 rows, 16 B (8 columns) per lane
-        src[k] = reinterpret_cast<const uint8_t*>(a.x + (size_t)min(m0 + (j >> 2) * 16 + i16, a.rows - 1) * a.ldx) +
-                 (j & 3) * 64 + q * 16;
+        src[k] = a.p.codes + (size_t)min(m0 + j * 16 + lr, a.rows - 1) * a.p.ldc;
+      } else {  // block j % 4 of 16 rows
+        src[k] = reinterpret_cast<const uint8_t*>(a.x + (size_t)min(m0 + (j >> 2) * 16 + lr, a.rows - 1) * a.ldx) +
+                 (j & 3) * 64 + lp * 16;
       }
     } else {  // row tile f of the stage: a wave's NF tiles, gate before up
       const int f = j - T::XI, w = f / NF, t = f % NF;
@@ -102,7 +108,7 @@ __global__ __launch_bounds__(64 * T::W, T::W / 4) void gemm_kernel(Args a, int n
       const uint8_t* p;
       if (j < T::XI) {
         // (past a row's last block: that block again, its weights are zero)
-        if constexpr (T::FP4) p = src[k] + (size_t)min(lk * 4 + q, a.nblk - 1) * 16;
+        if constexpr (T::FP4) p = src[k] + (size_t)min(lk * 4 + lp, a.nblk - 1) * 16;
         else p = src[k] + (size_t)lk * (kMxTileK * 2) + lterm * a.term_stride * 2;
       } else {
         p = src[k] + (size_t)lk * 1024;
@@ -129,7 +135,7 @@ __global__ __launch_bounds__(64 * T::W, T::W / 4) void gemm_kernel(Args a, int n
       sw[n] = ws[n * 64];
     }
     if constexpr (T::FP4) {
-      const uint8_t* xp = st + wm * MF * 1024 + lane * 16;
+      const uint8_t* xp = st + wm * MF * 1024 + i16 * 64 + (q ^ swz) * 16;
       const uint8_t* xs = st + T::X + T::WI * 1024 + (wm * MF * 16 + i16) * 4 + q;
       const bool in_row = ck * 4 + q < a.nblk;  // (scale bytes past the row may be anything)
 #pragma unroll
@@ -140,7 +146,7 @@ __global__ __launch_bounds__(64 * T::W, T::W / 4) void gemm_kernel(Args a, int n
         for (int n = 0; n < NF; ++n) acc[n][m] = mfma_fp4(w[n], sw[n], x, sx, acc[n][m]);
       }
     } else {
-      const uint8_t* xp = st + wm * MF * 4096 + q * 1024 + i16 * 16;
+      const uint8_t* xp = st + wm * MF * 4096 + q * 1024 + i16 * 64;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         bf8 wf[NF];
@@ -148,7 +154,7 @@ __global__ __launch_bounds__(64 * T::W, T::W / 4) void gemm_kernel(Args a, int n
         for (int n = 0; n < NF; ++n) wf[n] = fp4_bf16x8(reinterpret_cast<const uint32_t*>(&w[n])[j], e8m0_f32(sw[n]));
 #pragma unroll
         for (int m = 0; m < MF; ++m) {
-          const bf8 x = *reinterpret_cast<const bf8*>(xp + m * 4096 + j * 256);
+          const bf8 x = *reinterpret_cast<const bf8*>(xp + m * 4096 + (j ^ swz) * 16);
 #pragma unroll
           for (int n = 0; n < NF; ++n) acc[n][m] = mfma_bf16(wf[n], x, acc[n][m]);
         }
