@@ -96,9 +96,9 @@ int pgd_matrix_upload_q5_0(pgd_dev* dev, const void* blocks, int n_out, int n_in
  * upload: host planes, codes [n_out][n_in / 2], scales [n_out][n_in / 32]. */
 int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* scales, int n_out, int n_in,
                             pgd_matrix** out);
-/* The same from device planes, code rows ldc bytes apart (a multiple of 16, the
- * plane 16-byte aligned), scale rows lds bytes (a multiple of 4, 4-byte
- * aligned). Queued on the handle's stream: the planes may go once it has run. */
+/* The same from device planes, code rows ldc and scale rows lds bytes apart
+ * (multiples of 16, the planes 16-byte aligned). Queued on the handle's stream:
+ * the planes may go once it has run. */
 int pgd_matrix_from_mxfp4_dev(pgd_dev* dev, const uint8_t* codes, int ldc, const uint8_t* scales, int lds, int n_out,
                               int n_in, pgd_matrix** out);
 /* Rows x [nrows, k] of f32 (x_type 0), f16 (1) or bf16 (2), row stride ldx

@@ -238,11 +238,11 @@ int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* s
 // Row-major planes of rows of n_in columns, as every entry point takes them.
 static MxPlanes planes(const uint8_t* codes, int ldc, const uint8_t* scales, int lds, int n_in) {
   PGD_CHECK(codes && scales, kErrArg, "null argument");
-  PGD_CHECK(reinterpret_cast<uintptr_t>(codes) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0, kErrArg,
-            "MXFP4 codes must be 16-byte and scales 4-byte aligned");
+  PGD_CHECK(reinterpret_cast<uintptr_t>(codes) % 16 == 0 && reinterpret_cast<uintptr_t>(scales) % 16 == 0, kErrArg,
+            "MXFP4 planes must be 16-byte aligned");
   PGD_CHECK(ldc >= n_in / 2 && ldc % 16 == 0, kErrShape, "MXFP4 code stride must be >= n_in / 2 and a multiple of 16");
-  PGD_CHECK(lds >= n_in / kMxBlock && lds % 4 == 0, kErrShape,
-            "MXFP4 scale stride must be >= n_in / 32 and a multiple of 4");
+  PGD_CHECK(lds >= n_in / kMxBlock && lds % 16 == 0, kErrShape,
+            "MXFP4 scale stride must be >= n_in / 32 and a multiple of 16");
   return MxPlanes{codes, ldc, scales, lds};
 }
 

@@ -36,7 +36,7 @@ struct MxPlanes {
   const uint8_t* codes;
   int ldc;  // bytes, a multiple of 16
   const uint8_t* scales;
-  int lds;  // bytes, a multiple of 4
+  int lds;  // bytes, a multiple of 16 (upload: any)
 };
 
 // Rows of x (XType, stride ldx elements) to planes; values (nullable, row

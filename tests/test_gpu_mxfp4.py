@@ -85,7 +85,7 @@ def test_quantize_bit_for_bit(dev, buf, t, rows, k):
     top = {F32: np.finfo(np.float32).max, F16: 60000, BF16: mx.bf16_f32(np.uint16([0x7F7F]))[0]}[t]
     raw, x = mx.rows_of(np.clip(x, -np.float32(top), np.float32(top)), t)
     assert np.isfinite(x).all()
-    ldx, ldc, lds, ldv = k + 8, pad16(k // 2) + 16, pad16(k // 32) + 4, k + 4
+    ldx, ldc, lds, ldv = k + 8, pad16(k // 2) + 16, pad16(k // 32) + 16, k + 4
     dx = buf.up(mx.padded(raw, ldx, raw.dtype.type(77)))
     shape = (max(rows, 1),)
     codes, scales = np.full(shape + (ldc,), 0xA5, np.uint8), np.full(shape + (lds,), 0x5A, np.uint8)
@@ -114,11 +114,12 @@ def test_quantize_nonfinite_blocks(dev, buf, t):
     raw[0, 5], raw[2, 127] = bad
     raw[3, 64] = {F32: -np.inf, F16: -np.inf, BF16: 0xFF80}[t]
     hit = [(0, 0), (2, 3), (3, 2)]
-    codes, scales = np.zeros((4, 64), np.uint8), np.zeros((4, 4), np.uint8)
+    codes, scales = np.zeros((4, 64), np.uint8), np.zeros((4, 16), np.uint8)
     dx, dc, ds, dv = buf.up(raw), buf.up(codes), buf.up(scales), buf.up(x)
-    mxfp4_quantize_dev(dev, dx, t, 128, 4, 128, dc, 64, ds, 4, dv, 128)
+    mxfp4_quantize_dev(dev, dx, t, 128, 4, 128, dc, 64, ds, 16, dv, 128)
     gc, gs, gv = buf.down(dc, codes), buf.down(ds, scales), buf.down(dv, x)
-    want_c, want_s = mx.quantize(v)
+    want_c, s = mx.quantize(v)
+    want_s = mx.padded(s, 16, np.uint8(0))
     for r, b in hit:
         want_s[r, b] = 255
         want_c[r, 16 * b:16 * b + 16] = 0
@@ -141,7 +142,7 @@ def test_matrix_holds_its_planes(dev, buf, n, k):
         want = mx.values(codes, scales).astype(np.float32)
     m = Matrix.upload_mxfp4(dev, codes, scales, n, k)
     assert (m.fmt, m.n_out, m.n_in) == (5, n, k) and m.algo_bytes == n * k * 4.25 / 8
-    ldc, lds = pad16(k // 2) + 32, pad16(k // 32) + 4
+    ldc, lds = pad16(k // 2) + 32, pad16(k // 32) + 16
     d = Matrix.from_mxfp4_dev(dev, buf.up(mx.padded(codes, ldc, np.uint8(0xFF))), ldc,
                               buf.up(mx.padded(scales, lds, np.uint8(0xFF))), lds, n, k)
     for w in (m, d):
@@ -177,7 +178,7 @@ def run_planes(dev, buf, m, planes, res=None, up=None, ldc_more=0, ldy_more=0, y
 
     codes, scales = planes
     rows, n, k = codes.shape[0], m.n_out, m.n_in
-    ldc, lds, ldy = k // 2 + ldc_more, (k // 32 + 3) // 4 * 4, n + ldy_more
+    ldc, lds, ldy = k // 2 + ldc_more, pad16(k // 32), n + ldy_more
     y = np.full((rows + 1, ldy), 55.0, np.float32)
     py = buf.up(np.concatenate([np.zeros(y_off, np.float32), y.ravel()])) + 4 * y_off
     pc, ps = buf.up(mx.padded(codes, ldc, np.uint8(0x77))), buf.up(mx.padded(scales, lds, np.uint8(0xFF)))
@@ -323,8 +324,8 @@ def test_feed_forward_in_mxfp4(dev, buf):
         gv, uv, dv = (mx.values(*p) for p in planes)
         px, pmid, py = buf.up(x), buf.up(np.zeros((rows, i), np.float32)), buf.up(x)
         pc, ps = buf.up(np.zeros((rows, i), np.uint8)), buf.up(np.zeros((rows, 16), np.uint8))
-        mxfp4_quantize_dev(dev, px, F32, h, rows, h, pc, h // 2, ps, 8)
-        Matrix.gemv_swiglu_mx_dev(gate, up, pc, h // 2, ps, 8, rows, pmid, i)
+        mxfp4_quantize_dev(dev, px, F32, h, rows, h, pc, h // 2, ps, 16)
+        Matrix.gemv_swiglu_mx_dev(gate, up, pc, h // 2, ps, 16, rows, pmid, i)
         mxfp4_quantize_dev(dev, pmid, F32, i, rows, i, pc, i // 2, ps, 16)
         down.gemv_mx_dev(pc, i // 2, ps, 16, rows, py, h, py, h)
         mid, y = buf.down(pmid, np.zeros((rows, i), np.float32)), buf.down(py, x)

@@ -34,16 +34,16 @@ def code(name, *args):
 A = 0x10000
 
 
-QUANT = dict(dev=A, x=A, t=0, ldx=64, rows=2, k=64, codes=A, ldc=32, scales=A, lds=4, values=None, ldv=0)
+QUANT = dict(dev=A, x=A, t=0, ldx=64, rows=2, k=64, codes=A, ldc=32, scales=A, lds=16, values=None, ldv=0)
 
 
 @pytest.mark.parametrize("change,want", [
     (dict(dev=None), ARG), (dict(x=None), ARG), (dict(codes=None), ARG), (dict(scales=None), ARG),
-    (dict(t=3), ARG), (dict(t=-1), ARG), (dict(x=A + 4), ARG), (dict(codes=A + 8), ARG), (dict(scales=A + 2), ARG),
+    (dict(t=3), ARG), (dict(t=-1), ARG), (dict(x=A + 4), ARG), (dict(codes=A + 8), ARG), (dict(scales=A + 8), ARG),
     (dict(values=A + 4, ldv=64), ARG), (dict(values=A, ldv=60), SHAPE), (dict(values=A, ldv=66), SHAPE),
     (dict(rows=-1), SHAPE), (dict(k=0), SHAPE), (dict(k=-32), SHAPE), (dict(k=48), SHAPE),
     (dict(ldx=56), SHAPE), (dict(ldx=68), SHAPE), (dict(ldc=16), SHAPE), (dict(ldc=40), SHAPE),
-    (dict(lds=0), SHAPE), (dict(lds=6), SHAPE),
+    (dict(lds=0), SHAPE), (dict(lds=4), SHAPE), (dict(lds=24), SHAPE),
 ])
 def test_quantize_refuses(change, want):
     a = dict(QUANT, **change)
@@ -51,14 +51,14 @@ def test_quantize_refuses(change, want):
                 a["scales"], a["lds"], a["values"], a["ldv"]) == want
 
 
-PROD = dict(m={}, codes=A, ldc=32, scales=A, lds=4, rows=2, y=A, ldy=48, res=None, ldres=0)
+PROD = dict(m={}, codes=A, ldc=32, scales=A, lds=16, rows=2, y=A, ldy=48, res=None, ldres=0)
 
 
 @pytest.mark.parametrize("change,want", [
     (dict(m=None), ARG), (dict(y=None), ARG), (dict(codes=None), ARG), (dict(scales=None), ARG),
     (dict(m=dict(fmt=0)), FORMAT), (dict(m=dict(fmt=1)), FORMAT),
-    (dict(codes=A + 4), ARG), (dict(scales=A + 1), ARG), (dict(ldc=24), SHAPE), (dict(ldc=16), SHAPE),
-    (dict(lds=3), SHAPE), (dict(ldy=47), SHAPE), (dict(res=A, ldres=47), SHAPE),
+    (dict(codes=A + 4), ARG), (dict(scales=A + 4), ARG), (dict(ldc=24), SHAPE), (dict(ldc=16), SHAPE),
+    (dict(lds=8), SHAPE), (dict(ldy=47), SHAPE), (dict(res=A, ldres=47), SHAPE),
 ])
 def test_product_of_planes_refuses(change, want):
     a = dict(PROD, **change)
@@ -73,21 +73,21 @@ def test_product_of_planes_refuses(change, want):
 ])
 def test_pair_of_planes_refuses(gate, up, want):
     g, u = handle(**gate), handle(**up) if up is not None else None
-    assert code("pgd_matrix_gemv_swiglu_mx_dev", C.byref(g), C.byref(u) if u is not None else None, A, 32, A, 4, 2, A,
+    assert code("pgd_matrix_gemv_swiglu_mx_dev", C.byref(g), C.byref(u) if u is not None else None, A, 32, A, 16, 2, A,
                 48) == want
 
 
 @pytest.mark.parametrize("name,args,want", [
     ("pgd_matrix_upload_mxfp4", (A, None, A, 16, 32), ARG),
     ("pgd_matrix_upload_mxfp4", (None, A, A, 16, 32), ARG),
-    ("pgd_matrix_from_mxfp4_dev", (A, None, 16, A, 4, 16, 32), ARG),
-    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, None, 4, 16, 32), ARG),
-    ("pgd_matrix_from_mxfp4_dev", (A, A, 8, A, 4, 16, 32), SHAPE),
-    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 2, 16, 32), SHAPE),
-    ("pgd_matrix_from_mxfp4_dev", (A, A + 8, 16, A, 4, 16, 32), ARG),
-    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 4, 0, 32), SHAPE),
-    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 4, 16, 0), SHAPE),
-    ("pgd_matrix_from_mxfp4_dev", (None, A, 16, A, 4, 16, 32), ARG),
+    ("pgd_matrix_from_mxfp4_dev", (A, None, 16, A, 16, 16, 32), ARG),
+    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, None, 16, 16, 32), ARG),
+    ("pgd_matrix_from_mxfp4_dev", (A, A, 8, A, 16, 16, 32), SHAPE),
+    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 4, 16, 32), SHAPE),
+    ("pgd_matrix_from_mxfp4_dev", (A, A + 8, 16, A, 16, 16, 32), ARG),
+    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 16, 0, 32), SHAPE),
+    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 16, 16, 0), SHAPE),
+    ("pgd_matrix_from_mxfp4_dev", (None, A, 16, A, 16, 16, 32), ARG),
 ])
 def test_matrix_from_planes_refuses(name, args, want):
     out = C.c_void_p()
