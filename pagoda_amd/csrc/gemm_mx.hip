@@ -10,9 +10,11 @@
 // Rows of several bf16 terms take one stage per term and k tile: all terms of a
 // row add to the same f32 sums.
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 #include "common.h"
+#include "gemv_impl.h"
 #include "mxfp4.h"
 #include "mxfp4_dev.h"
 
@@ -20,148 +22,181 @@ namespace pgd {
 namespace mx {
 namespace {
 
-// 64 lanes' 16 (4) bytes from global memory to consecutive places from the LDS
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ const void* uniform(const void* p) {
+  const uint64_t b = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const void*>((uint64_t)uniform((uint32_t)(b >> 32)) << 32 | uniform((uint32_t)b));
+}
+// 64 lanes' 16 (4) bytes from base + off to consecutive places from the LDS
 // address `to` on. Written in assembly (no output registers) because the
 // compiler would otherwise let later LDS reads wait for these loads to land;
 // the waits are the kernel's own.
-__device__ __forceinline__ void dma16(const void* g, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(g) : "memory");
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(to)), "v"(off), "s"(uniform(base)) : "memory");
 }
-__device__ __forceinline__ void dma4(const void* g, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(g) : "memory");
+__device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(uniform(to)), "v"(off), "s"(uniform(base)) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(uniform(to)), "v"(from) : "memory");
 }
 
 template <bool FP4_, int BM_, int BN_, int WM_, int WN_, int S_, int OCC_ = 1>
 struct Shape {
-  static constexpr int OCC = OCC_;
   static constexpr bool FP4 = FP4_;
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_, OCC = OCC_;
   static constexpr int W = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
-  // a stage's loads: 1 KiB of codes or terms each, and 256 B of weight scales
-  // (the last may reach past the tile), NL and NS of them to a wave
-  static constexpr int XI = BM / 16 * (FP4 ? 1 : 4), WI = BN / 16, WS = (BN + 63) / 64;
-  static constexpr int NL = (XI + WI + W - 1) / W, NS = (WS + W - 1) / W, LOADS = NL + NS;
-  static constexpr int X = XI * 1024, SC = X + WI * 1024, BYTES = SC + WS * 256;
+  // A wave's loads of a stage: NX of activations (XB bytes each, 4 or 16 a lane),
+  // NL KiB of weight codes, NS times 256 B of weight scales (where there are
+  // fewer than waves, several waves load the same bytes to the same place)
+  static constexpr int X = BM * (FP4 ? 64 : 256), XB = X / 1024 % W == 0 ? 1024 : 256, NX = X / XB / W;
+  static constexpr int NL = BN / 16 / W, WS = BN / 64, NS = WS > W ? WS / W : 1, LOADS = NX + NL + NS;
+  static constexpr int SC = X + BN * 64, BYTES = SC + BN * 4;
   // activation scales: every fourth stage brings those of 4 k tiles, 16 B of a
   // row, into the other of two slots behind the ring
-  static constexpr int XS = FP4 ? (BM + 63) / 64 : 0, NX = (XS + W - 1) / W;
+  static constexpr int XS = FP4 ? (BM + 63) / 64 : 0, NXS = XS > W ? XS / W : 1;
   static constexpr int RING = S * BYTES, LDS = RING + 2 * XS * 1024;
+  static_assert((!FP4 || MF == 1 || MF % 2 == 0) && X / XB % W == 0 && BN / 16 % W == 0 && (WS <= W || WS % W == 0) && (XS <= W || XS % W == 0));
   static_assert(S >= 2 && S <= (FP4 ? 5 : 8) && LDS * OCC <= 160 * 1024);
 };
 
 template <class T, int EPI>
 __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args a, int nmb, int nnb, int per_xcd, bool vec) {
-  constexpr bool DUAL = EPI == MX_SWIGLU;
+  constexpr bool DUAL = EPI == MX_SWIGLU || EPI == MX_PART2;
   constexpr int MF = T::MF, NF = T::NF, S = T::S;
   constexpr int NW = DUAL ? NF / 2 : NF;      // a wave's row tiles of outputs
   constexpr int NB = DUAL ? T::BN / 32 : T::BN / 16;  // the workgroup's
+  static_assert(!DUAL || (NF % 2 == 0 && (T::NL == NF || NW % T::NL == 0)));
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  const uint32_t lds0 = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem);
   // XCD x takes the contiguous range [x per_xcd, (x + 1) per_xcd) of blocks
-  // (workgroups are dealt to the 8 XCDs in turn), ordered in groups of 8 row
-  // blocks, in a group output block by output block
-  const int gi = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if (gi >= nmb * nnb) return;
+  // (workgroups are dealt to the 8 XCDs in turn): range of k tiles by range, in
+  // a range in groups of 8 row blocks, in a group output block by output block
+  int gi = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (gi >= nmb * nnb * a.splits) return;
+  const int split = uniform((uint32_t)(gi / (nmb * nnb)));  // (divisions leave the scalar unit)
+  gi -= split * nmb * nnb;
+  const int k0 = uniform((uint32_t)((long long)split * a.kt / a.splits)), k1 = uniform((uint32_t)((long long)(split + 1) * a.kt / a.splits));
   const int g0 = gi / (8 * nnb) * 8, gw = min(8, nmb - g0), in = gi - g0 * nnb;
-  const int m0 = (g0 + in % gw) * T::BM, nt0 = in / gw * NB;
+  const int m0 = uniform((uint32_t)((g0 + in % gw) * T::BM)), nt0 = uniform((uint32_t)(in / gw * NB));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i16 = lane & 15, q = lane >> 4;
+  const int i16 = lane & 15, q = lane >> 4, swz = i16 >> 2;
   const int wm = wave / T::WN, wn = wave % T::WN;
 
-  // An activation load takes 64 B (a k tile's codes, or a block's terms) of each
-  // of 16 rows, four neighbouring lanes a row, so that they leave as one request.
-  // The four 16 B parts of row i lie in LDS in the order 0..3 ^ i / 4: then the
-  // 16 lanes that read one part of 16 rows at once meet no bank twice.
-  const int lr = lane >> 2, lp = (lane & 3) ^ (lane >> 4);
-  const int swz = i16 >> 2;
-  // this wave's loads: sources without the k tile's offset (a wave with fewer
-  // repeats the last: the same bytes to the same place)
-  const uint8_t* src[T::NL];
+  // Where the bytes at LDS offset p of a stage come from, relative to the block's
+  // first row and the k tile. A 16-row tile (a block of it, for bf16 terms) is 16
+  // rows of 64 B, so that neighbouring lanes of a load leave as one request; the
+  // four 16 B parts of row i lie in the order 0..3 ^ i / 4: then the 16 lanes that
+  // read one part of 16 rows at once meet no bank twice. Rows past the last are
+  // that row again, and are not stored.
+  const int last = a.rows - 1 - m0;
+  uint32_t xo[T::NX], cut[T::NX];
+#pragma unroll
+  for (int k = 0; k < T::NX; ++k) {
+    const int p = (wave * T::NX + k) * T::XB + lane * (T::XB / 64);
+    const int i = (p >> 6) & 15, part = ((p >> 4) & 3) ^ (i >> 2);
+    if constexpr (T::FP4) {
+      xo[k] = (uint32_t)min((p >> 10) * 16 + i, last) * (uint32_t)a.p.ldc + part * 16 + (p & 15);
+      // in the last k tile, blocks past the row's last are that one again (their weights are zero)
+      cut[k] = max(part - ((a.nblk - 1) & 3), 0) * 16;
+    } else {
+      xo[k] = (uint32_t)min((p >> 12) * 16 + i, last) * (uint32_t)(a.ldx * 2) + ((p >> 10) & 3) * 64 + part * 16 + (p & 15);
+    }
+  }
+  const uint8_t* xb = T::FP4 ? a.p.codes + (size_t)m0 * a.p.ldc : reinterpret_cast<const uint8_t*>(a.x + (size_t)m0 * a.ldx);
+  // row tile f of the stage: a wave's NF tiles, gate before up
+  auto tile_of = [&](int f, bool& up) {
+    const int w = f / NF, t = f % NF;
+    up = DUAL && t >= NW;
+    return (size_t)min(nt0 + w * NW + (up ? t - NW : t), a.nt - 1);
+  };
+  const uint8_t *wb[T::NL], *sb[T::NS];
+  const uint32_t wo = lane * 16;
 #pragma unroll
   for (int k = 0; k < T::NL; ++k) {
-    const int j = min(wave * T::NL + k, T::XI + T::WI - 1);
-    if (j < T::XI) {
-      if constexpr (T::FP4) {
-        src[k] = a.p.codes + (size_t)min(m0 + j * 16 + lr, a.rows - 1) * a.p.ldc;
-      } else {  // block j % 4 of 16 rows
-        src[k] = reinterpret_cast<const uint8_t*>(a.x + (size_t)min(m0 + (j >> 2) * 16 + lr, a.rows - 1) * a.ldx) +
-                 (j & 3) * 64 + lp * 16;
-      }
-    } else {  // row tile f of the stage: a wave's NF tiles, gate before up
-      const int f = j - T::XI, w = f / NF, t = f % NF;
-      const bool up = DUAL && t >= NW;
-      const size_t nt = min(nt0 + w * NW + (up ? t - NW : t), a.nt - 1);
-      src[k] = (up ? a.uc : a.wc) + nt * a.kt * 1024 + lane * 16;
-    }
+    bool up;
+    const size_t nt = tile_of(wave * T::NL + k, up);
+    wb[k] = (up ? a.uc : a.wc) + (nt * a.kt + k0) * 1024;
   }
-  const uint8_t* ssrc[T::NS];
 #pragma unroll
-  for (int k = 0; k < T::NS; ++k) {
-    const int f = min(wave * T::NS + k, T::WS - 1) * 4 + q, w = f / NF, t = f % NF;
-    const bool up = DUAL && t >= NW;
-    const size_t nt = min(nt0 + w * NW + (up ? t - NW : t), a.nt - 1);
-    ssrc[k] = (up ? a.us : a.ws) + nt * a.kt * 64 + i16 * 4;
+  for (int k = 0; k < T::NS; ++k) {  // 4 row tiles a load, 16 lanes each
+    bool up;
+    const size_t nt = tile_of((wave * T::NS + k) % T::WS * 4 + q, up);
+    sb[k] = (up ? a.us : a.ws) + (nt * a.kt + k0) * 64 + i16 * 4;
   }
-  const uint8_t* xsrc[T::FP4 ? T::NX : 1];
-  if constexpr (T::FP4) {
+  const uint8_t* xsb = a.p.scales + (T::FP4 ? (size_t)m0 * a.p.lds : 0);
+  uint32_t xso[T::NXS];
 #pragma unroll
-    for (int k = 0; k < T::NX; ++k)
-      xsrc[k] = a.p.scales + (size_t)min(m0 + min(wave * T::NX + k, T::XS - 1) * 64 + lane, a.rows - 1) * a.p.lds;
-  }
-  // stage t: k tile t / terms, term t % terms; kt and term follow the loads
-  const int terms = T::FP4 ? 1 : a.terms, steps = a.kt * terms;
-  int lk = 0, lterm = 0;
-  auto issue = [&](uint32_t st) {
+  for (int k = 0; k < T::NXS; ++k)
+    xso[k] = T::FP4 ? (uint32_t)min((wave * T::NXS + k) % max(T::XS, 1) * 64 + lane, last) * (uint32_t)a.p.lds : 0;
+
+  // The loads' k tile and term. Past the last stage they repeat its k tile into
+  // slots that nothing reads: every wave has the same number in flight.
+  const int terms = T::FP4 ? 1 : a.terms, steps = (k1 - k0) * terms;
+  int lk = k0, lterm = 0;
+  const size_t term_bytes = a.term_stride * 2;
+  const uint8_t* xk = xb + (size_t)k0 * (T::FP4 ? 64 : 256);  // of k tile lk, term lterm
+  bool first = true;
+  auto issue = [&](uint32_t slot) {
+    const uint32_t st = lds0 + slot;
     if constexpr (T::FP4) {  // (first: sync() may wait for these loads of a stage that it lets fly)
-      if ((lk & 3) == 0) {
+      if ((lk & 3) == 0 || first) {
+        first = false;
 #pragma unroll
-        for (int k = 0; k < T::NX; ++k)
-          dma16(xsrc[k] + (size_t)lk * 4, lds0 + T::RING + (((lk >> 2) & 1) * T::XS + min(wave * T::NX + k, T::XS - 1)) * 1024);
+        for (int k = 0; k < T::NXS; ++k)
+          dma16(xsb + (size_t)(lk & ~3) * 4, xso[k],
+                lds0 + T::RING + (((lk >> 2) & 1) * T::XS + (wave * T::NXS + k) % T::XS) * 1024);
       }
     }
+    const bool end = lk == a.kt - 1;
 #pragma unroll
-    for (int k = 0; k < T::NL; ++k) {
-      const int j = min(wave * T::NL + k, T::XI + T::WI - 1);
-      const uint8_t* p;
-      if (j < T::XI) {
-        // (past a row's last block: that block again, its weights are zero)
-        if constexpr (T::FP4) p = src[k] + (size_t)min(lk * 4 + lp, a.nblk - 1) * 16;
-        else p = src[k] + (size_t)lk * (kMxTileK * 2) + lterm * a.term_stride * 2;
-      } else {
-        p = src[k] + (size_t)lk * 1024;
-      }
-      dma16(p, st + j * 1024);
+    for (int k = 0; k < T::NX; ++k) {
+      const uint32_t to = st + (wave * T::NX + k) * T::XB;
+      uint32_t off = xo[k];
+      if constexpr (T::FP4) off -= end ? cut[k] : 0;
+      if constexpr (T::XB == 1024) dma16(xk, off, to);
+      else dma4(xk, off, to);
     }
 #pragma unroll
-    for (int k = 0; k < T::NS; ++k)
-      dma4(ssrc[k] + (size_t)lk * 64, st + T::SC + min(wave * T::NS + k, T::WS - 1) * 256);
-    if (++lterm == terms) {
-      lterm = 0;
-      lk = min(lk + 1, a.kt - 1);  // (the loads past the last stage fill slots that nothing reads)
+    for (int k = 0; k < T::NL; ++k) dma16(wb[k], wo, st + T::X + (wave * T::NL + k) * 1024);
+#pragma unroll
+    for (int k = 0; k < T::NS; ++k) dma4(sb[k], st + T::SC + (wave * T::NS + k) % T::WS * 256);
+    // (no branches: the pointers stay in registers)
+    const int more = T::FP4 ? lk + 1 < k1 : (lterm == terms - 1 && lk + 1 < k1);
+    if constexpr (T::FP4) {
+      xk += more * 64;
+    } else {
+      const int wrap = lterm == terms - 1;
+      xk += wrap ? more * 256 - (ptrdiff_t)term_bytes * (terms - 1) : (ptrdiff_t)term_bytes;
+      lterm = wrap ? 0 : lterm + 1;
     }
+    lk += more;
+#pragma unroll
+    for (int k = 0; k < T::NL; ++k) wb[k] += more * 1024;
+#pragma unroll
+    for (int k = 0; k < T::NS; ++k) sb[k] += more * 64;
   };
 
   f4 acc[NF][MF] = {};
-  // LDS operands of a stage: its weights' codes and scales, and activations (FP4:
-  // the whole k tile and its scales, else the quarter that matrix instruction j takes)
+  // LDS operands of a stage: its weights' codes and scales, and of bf16 terms the
+  // quarter that matrix instruction j takes
   struct WFrag {
     uint4 c[NF];
     uint32_t s[NF];
   };
-  auto read_w = [&](WFrag& f, const uint8_t* st) {
-    const uint8_t* ws = st + T::SC + wn * NF * 64 + lane;
-    const uint8_t* wp = st + T::X + wn * NF * 1024 + lane * 16;
+  auto read_w = [&](WFrag& f, uint32_t slot) {
+    const uint8_t* ws = smem + slot + T::SC + wn * NF * 64 + lane;
+    const uint8_t* wp = smem + slot + T::X + wn * NF * 1024 + lane * 16;
 #pragma unroll
     for (int n = 0; n < NF; ++n) {
       f.c[n] = *reinterpret_cast<const uint4*>(wp + n * 1024);
       f.s[n] = ws[n * 64];
     }
   };
-  auto read_x = [&](uint4 (&x)[MF], const uint8_t* st, int j) {
-    const uint8_t* xp = T::FP4 ? st + wm * MF * 1024 + i16 * 64 + (q ^ swz) * 16
-                               : st + wm * MF * 4096 + q * 1024 + i16 * 64 + (j ^ swz) * 16;
+  auto read_x = [&](uint4 (&x)[MF], uint32_t slot, int j) {
+    const uint8_t* xp = smem + slot + wm * MF * 4096 + q * 1024 + i16 * 64 + (j ^ swz) * 16;
 #pragma unroll
-    for (int m = 0; m < MF; ++m) x[m] = *reinterpret_cast<const uint4*>(xp + m * (T::FP4 ? 1024 : 4096));
+    for (int m = 0; m < MF; ++m) x[m] = *reinterpret_cast<const uint4*>(xp + m * 4096);
   };
   // A stage has landed for every wave, and every wave has read the slot that the
   // next loads fill. `fly` stages stay in flight.
@@ -174,81 +209,112 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
     asm volatile("" ::: "memory");
   };
   uint32_t here = 0;  // the slot of the stage in use
-  auto after = [&](uint32_t slot) { return slot + T::BYTES == S * T::BYTES ? 0 : slot + T::BYTES; };
-  // All of the next stage's first operands are read under this stage's last
-  // matrix instructions: the reads' latency and the barrier are hidden.
+  auto advance = [&] { here = here + T::BYTES == S * T::BYTES ? 0 : here + T::BYTES; };
+  // Reads go out before the matrix instructions of what was read before: their
+  // latency and the barrier's are hidden (the scheduler would put each next to its use).
+  auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
 #pragma unroll
-  for (int i = 0; i < S; ++i) issue(lds0 + i * T::BYTES);
+  for (int i = 0; i < S; ++i) issue(i * T::BYTES);
   sync(std::integral_constant<int, S - 1>{});
   if constexpr (T::FP4) {
-    struct Frag {
-      WFrag w;
-      uint4 x[MF];
-      uint32_t s[MF];
+    // a stage in two halves of its row tiles
+    constexpr int H = MF > 1 ? MF / 2 : 1;
+    struct Half {
+      uint4 x[H];
+      uint32_t s[H];
     };
-    auto read = [&](Frag& f, const uint8_t* st, int kt) {
-      read_w(f.w, st);
-      read_x(f.x, st, 0);
-      const uint8_t* xs = smem + T::RING + ((kt >> 2) & 1) * (T::XS * 1024) + (wm * MF * 16 + i16) * 16 + (kt & 3) * 4 + q;
-      const bool in_row = kt * 4 + q < a.nblk;  // (scale bytes past the row may be anything)
+    auto read_half = [&](Half& f, int half, int kt) {
+      const uint8_t* xp = smem + here + (wm * MF + half * H) * 1024 + i16 * 64 + (q ^ swz) * 16;
+      const uint8_t* xs = smem + T::RING + ((kt >> 2) & 1) * (T::XS * 1024) + ((wm * MF + half * H) * 16 + i16) * 16 + (kt & 3) * 4 + q;
 #pragma unroll
-      for (int m = 0; m < MF; ++m) {
-        const uint32_t b = xs[m * 256];
-        f.s[m] = in_row ? b : 127;
+      for (int m = 0; m < H; ++m) {
+        f.x[m] = *reinterpret_cast<const uint4*>(xp + m * 1024);
+        f.s[m] = xs[m * 256];
       }
     };
-    auto step = [&](int t, const Frag& f, Frag& next) {
-      sync(std::integral_constant<int, S - 2>{});
-      issue(lds0 + here);
-      here = after(here);
-      read(next, smem + here, t + 1);
+    auto mma = [&](const WFrag& w, Half& f, int half, int kt) {
+      if (kt == a.kt - 1 && kt * 4 + q >= a.nblk) {  // (scale bytes past the row may be anything)
 #pragma unroll
-      for (int m = 0; m < MF; ++m)
+        for (int m = 0; m < H; ++m) f.s[m] = 127;
+      }
 #pragma unroll
-        for (int n = 0; n < NF; ++n) acc[n][m] = mfma_fp4(f.w.c[n], f.w.s[n], f.x[m], f.s[m], acc[n][m]);
+      for (int m = 0; m < H; ++m)
+#pragma unroll
+        for (int n = 0; n < NF; ++n)
+          acc[n][half * H + m] = mfma_fp4(w.c[n], w.s[n], f.x[m], f.s[m], acc[n][half * H + m]);
+      fence();
     };
-    Frag f0, f1;
-    read(f0, smem, 0);
+    WFrag w0, w1;
+    Half lo, hi;
+    auto step = [&](int kt, const WFrag& w, WFrag& next) {
+      if constexpr (MF > 1) {
+        read_half(hi, 1, kt);
+        fence();
+        mma(w, lo, 0, kt);
+      } else {
+        hi = lo;
+      }
+      sync(std::integral_constant<int, S - 2>{});
+      issue(here);
+      advance();
+      read_w(next, here);
+      read_half(lo, 0, kt + 1);
+      fence();
+      mma(w, hi, MF > 1, kt);
+    };
+    read_w(w0, 0);
+    read_half(lo, 0, k0);
     for (int t = 0;;) {
-      step(t, f0, f1);
+      step(k0 + t, w0, w1);
       if (++t == steps) break;
-      step(t, f1, f0);
+      step(k0 + t, w1, w0);
       if (++t == steps) break;
     }
   } else {
-    auto mma = [&](const WFrag& w, const uint4 (&x)[MF], int j) {
-      bf8 wf[NF];
+    auto decode = [&](bf8 (&wf)[NF], const WFrag& w, int j) {
 #pragma unroll
       for (int n = 0; n < NF; ++n) wf[n] = fp4_bf16x8(reinterpret_cast<const uint32_t*>(&w.c[n])[j], e8m0_f32(w.s[n]));
+    };
+    auto mma = [&](const bf8 (&wf)[NF], const uint4 (&x)[MF]) {
 #pragma unroll
       for (int m = 0; m < MF; ++m)
 #pragma unroll
         for (int n = 0; n < NF; ++n) acc[n][m] = mfma_bf16(wf[n], __builtin_bit_cast(bf8, x[m]), acc[n][m]);
+      // the next quarter's conversions in the shadows of these
+#pragma unroll
+      for (int i = 0; i < MF * NF; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (4 * NF + MF * NF - 1) / (MF * NF), 0);
+      }
+      fence();
     };
-    auto step = [&](const WFrag& w, WFrag& next, uint4 (&x0)[MF], uint4 (&x1)[MF]) {
-      const uint8_t* st = smem + here;
-      read_x(x1, st, 1);
-      mma(w, x0, 0);
-      read_x(x0, st, 2);
-      mma(w, x1, 1);
-      read_x(x1, st, 3);
-      mma(w, x0, 2);
-      sync(std::integral_constant<int, S - 2>{});
-      issue(lds0 + here);
-      here = after(here);
-      read_w(next, smem + here);
-      read_x(x0, smem + here, 0);
-      mma(w, x1, 3);
-    };
-    WFrag w0, w1;
+    WFrag w;
     uint4 x0[MF], x1[MF];
-    read_w(w0, smem);
-    read_x(x0, smem, 0);
-    for (int t = 0;;) {
-      step(w0, w1, x0, x1);
-      if (++t == steps) break;
-      step(w1, w0, x0, x1);
-      if (++t == steps) break;
+    bf8 f0[NF], f1[NF];
+    read_w(w, 0);
+    read_x(x0, 0, 0);
+    decode(f0, w, 0);
+    for (int t = 0; t < steps; ++t) {
+      read_x(x1, here, 1);
+      fence();
+      decode(f1, w, 1);
+      mma(f0, x0);
+      read_x(x0, here, 2);
+      fence();
+      decode(f0, w, 2);
+      mma(f1, x1);
+      read_x(x1, here, 3);
+      fence();
+      decode(f1, w, 3);
+      mma(f0, x0);
+      sync(std::integral_constant<int, S - 2>{});
+      issue(here);
+      advance();
+      read_w(w, here);
+      read_x(x0, here, 0);
+      fence();
+      mma(f1, x1);
+      decode(f0, w, 0);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS outlives the workgroup
@@ -260,8 +326,14 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
     for (int n = 0; n < NW; ++n) {
       const int o = (nt0 + wn * NW + n) * 16 + q * 4;
       if (o >= a.n_out) continue;
+      if constexpr (EPI == MX_PART || EPI == MX_PART2) {
+        float* p = a.part + (size_t)split * a.part_stride + (size_t)r * (a.nt * 16) + o;
+        *reinterpret_cast<f4*>(p) = acc[n][m];
+        if constexpr (DUAL) *reinterpret_cast<f4*>(p + a.part_stride / 2) = acc[n + NW][m];
+        continue;
+      }
       f4 v = acc[n][m];
-      if constexpr (DUAL) {
+      if constexpr (EPI == MX_SWIGLU) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = swiglu(v[e], acc[n + NW][m][e]);
       }
@@ -270,31 +342,78 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
   }
 }
 
+// Sums of the ranges in range order, then the epilogue: four outputs of a row per thread.
+template <int EPI>
+__global__ __launch_bounds__(256) void join_kernel(Args a, bool vec) {
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (n >= a.n_out) return;
+  for (int r = blockIdx.y; r < a.rows; r += gridDim.y) {
+    const float* p = a.part + (size_t)r * (a.nt * 16) + n;
+    f4 v = {}, u = {};
+#pragma unroll 4
+    for (int i = 0; i < a.splits; ++i) {
+      v += *reinterpret_cast<const f4*>(p + (size_t)i * a.part_stride);
+      if constexpr (EPI == MX_SWIGLU) u += *reinterpret_cast<const f4*>(p + (size_t)i * a.part_stride + a.part_stride / 2);
+    }
+    if constexpr (EPI == MX_SWIGLU) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = swiglu(v[e], u[e]);
+    }
+    store4<EPI>(a, vec, r, n, v);
+  }
+}
+
 template <class T, int EPI>
-void launch(const Args& a, hipStream_t s) {
-  const int nb = EPI == MX_SWIGLU ? T::BN / 32 : T::BN / 16;
+void launch_blocks(const Args& a, hipStream_t s) {
+  const int nb = EPI == MX_SWIGLU || EPI == MX_PART2 ? T::BN / 32 : T::BN / 16;
   const long long nmb = (a.rows + (long long)T::BM - 1) / T::BM, nnb = (a.nt + nb - 1) / nb;
-  PGD_CHECK(nmb * nnb < (1ll << 30), kErrShape, "too many outputs for one MXFP4 product");
-  const int per_xcd = (int)((nmb * nnb + 7) / 8);
+  PGD_CHECK(nmb * nnb * a.splits < (1ll << 30), kErrShape, "too many outputs for one MXFP4 product");
+  // (the lanes' offsets in a block's rows are 32 bits)
+  PGD_CHECK((T::FP4 ? (size_t)std::max(a.p.ldc, a.p.lds) : a.ldx * 2) * T::BM < (1ull << 32), kErrShape,
+            "activation row stride");
+  const int per_xcd = (int)((nmb * nnb * a.splits + 7) / 8);
   PGD_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, EPI>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS));
-  hipLaunchKernelGGL((gemm_kernel<T, EPI>), dim3(per_xcd * 8), dim3(64 * T::W), T::LDS, s, a, (int)nmb, (int)nnb, per_xcd,
-                     rows_vec(a.o));
+  hipLaunchKernelGGL((gemm_kernel<T, EPI>), dim3(per_xcd * 8), dim3(64 * T::W), T::LDS, s, a, (int)nmb, (int)nnb,
+                     per_xcd, rows_vec(a.o));
   PGD_HIP(hipGetLastError());
 }
 
+// The ranges' sums lie in the stream's scratch between the two launches. Held
+// over both, so that no other host thread's call on the stream is queued
+// between them or replaces the buffer.
+std::mutex g_part;
+
 template <class T>
-void launch_epi(const Args& a, hipStream_t s) {
-  if (a.uc) launch<T, MX_SWIGLU>(a, s);
-  else if (a.o.res) launch<T, MX_RES>(a, s);
-  else launch<T, MX_STORE>(a, s);
+void launch(Args a, int splits, hipStream_t s) {
+  a.splits = splits;
+  if (splits == 1) {
+    if (a.uc) launch_blocks<T, MX_SWIGLU>(a, s);
+    else if (a.o.res) launch_blocks<T, MX_RES>(a, s);
+    else launch_blocks<T, MX_STORE>(a, s);
+    return;
+  }
+  std::lock_guard<std::mutex> lock(g_part);
+  a.part_stride = (size_t)(a.uc ? 2 : 1) * a.rows * a.nt * 16;
+  a.part = static_cast<float*>(gemv::gemv_scratch(s, splits * a.part_stride * sizeof(float), 9));
+  const dim3 grid((a.nt * 4 + 255) / 256, std::min(a.rows, 65535));
+  auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, rows_vec(a.o)); };
+  if (a.uc) {
+    launch_blocks<T, MX_PART2>(a, s);
+    join(join_kernel<MX_SWIGLU>);
+  } else {
+    launch_blocks<T, MX_PART>(a, s);
+    if (a.o.res) join(join_kernel<MX_RES>);
+    else join(join_kernel<MX_STORE>);
+  }
+  PGD_HIP(hipGetLastError());
 }
 
 }  // namespace
 
 void run_many(const Args& a, hipStream_t s) {
-  if (a.p.codes) launch_epi<Shape<true, 256, 256, 2, 4, 3>>(a, s);
-  else launch_epi<Shape<false, 128, 256, 2, 4, 3>>(a, s);
+  if (a.p.codes) launch<Shape<true, 256, 256, 2, 4, 3>>(a, 1, s);
+  else launch<Shape<false, 128, 256, 2, 4, 3>>(a, 1, s);
 }
 
 }  // namespace mx

@@ -73,6 +73,10 @@ struct Args {
   size_t ldx, term_stride;
   int terms;
   MxOut o;
+  // set by run_many: ranges of k tiles, and where their sums go
+  int splits;
+  float* part;
+  size_t part_stride;
 };
 
 // A few rows (gemv_mx.hip), many (gemm_mx.hip), and whichever suits.

@@ -80,7 +80,8 @@ __device__ inline f4 mfma_fp4(uint4 w, uint32_t ws, uint4 x, uint32_t xs, f4 c) 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, (int)ws, 0, (int)xs);
 }
 
-enum { MX_STORE = 0, MX_RES = 1, MX_SWIGLU = 2 };
+// (PART, PART2: sums of a range of k tiles, of one matrix or of the pair)
+enum { MX_STORE = 0, MX_RES = 1, MX_SWIGLU = 2, MX_PART = 3, MX_PART2 = 4 };
 
 // silu(g) * u in f32: expf's error (an ulp or so) is that of the f32 products' sums
 __device__ inline float swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
