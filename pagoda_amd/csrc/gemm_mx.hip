@@ -368,9 +368,6 @@ void launch_blocks(const Args& a, hipStream_t s) {
   const int nb = EPI == MX_SWIGLU || EPI == MX_PART2 ? T::BN / 32 : T::BN / 16;
   const long long nmb = (a.rows + (long long)T::BM - 1) / T::BM, nnb = (a.nt + nb - 1) / nb;
   PGD_CHECK(nmb * nnb * a.splits < (1ll << 30), kErrShape, "too many outputs for one MXFP4 product");
-  // (the lanes' offsets in a block's rows are 32 bits)
-  PGD_CHECK((T::FP4 ? (size_t)std::max(a.p.ldc, a.p.lds) : a.ldx * 2) * T::BM < (1ull << 32), kErrShape,
-            "activation row stride");
   const int per_xcd = (int)((nmb * nnb * a.splits + 7) / 8);
   PGD_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, EPI>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS));
@@ -409,11 +406,72 @@ void launch(Args a, int splits, hipStream_t s) {
   PGD_HIP(hipGetLastError());
 }
 
+// The shapes, largest first.
+using P0 = Shape<true, 128, 256, 1, 4, 3, 2>;
+using P1 = Shape<true, 128, 128, 2, 2, 4, 2>;
+using P2 = Shape<true, 64, 128, 1, 4, 4, 2>;
+using P3 = Shape<true, 32, 128, 1, 4, 5, 2>;
+using T0 = Shape<false, 64, 256, 1, 4, 2, 2>;
+using T1 = Shape<false, 64, 128, 1, 4, 3, 2>;
+using T2 = Shape<false, 32, 128, 1, 4, 4, 2>;
+
+// Microseconds of a launch, of a stage and of the rest of a block where a CU runs
+// two blocks and where it runs one, and of joining ranges (a launch, and each MB of
+// their sums). Least squares over 12 matrices from 300 x 8192 to 151936 x 896 with
+// 2..4000 rows, 1..24 ranges: 5% (bf16 terms) to 10% (planes) rms off.
+struct Cost {
+  int bm, bn;
+  float launch, stage2, block2, stage1, block1, join, mb;
+};
+constexpr Cost kPlanes[4] = {{128, 256, 5.46f, 0.987f, 3.91f, 0.628f, 2.24f, 2.35f, 0.265f},
+                             {128, 128, 4.89f, 0.593f, 3.38f, 0.410f, 0.83f, 2.73f, 0.274f},
+                             {64, 128, 4.18f, 0.403f, 1.76f, 0.298f, 0.22f, 2.95f, 0.314f},
+                             {32, 128, 2.36f, 0.401f, 1.86f, 0.243f, 1.61f, 3.25f, 0.279f}};
+constexpr Cost kTerms[3] = {{64, 256, 5.92f, 1.303f, 1.53f, 0.805f, 0.00f, 2.13f, 0.295f},
+                            {64, 128, 4.43f, 0.792f, 2.24f, 0.495f, 0.15f, 2.45f, 0.267f},
+                            {32, 128, 3.14f, 0.496f, 2.13f, 0.342f, 0.80f, 2.64f, 0.296f}};
+
+double cost_us(const Cost& c, const Args& a, int splits) {
+  const int pair = a.uc ? 2 : 1;
+  const long long blocks = (long long)((a.rows + c.bm - 1) / c.bm) * ((a.nt * 16ll * pair + c.bn - 1) / c.bn) * splits;
+  const long long per_cu = (blocks + 255) / 256;
+  const double stages = (a.kt + splits - 1) / splits * (a.p.codes ? 1 : a.terms);
+  double us = c.launch + (double)(per_cu / 2) * (stages * c.stage2 + c.block2);
+  if (per_cu % 2) us += stages * c.stage1 + c.block1;
+  if (splits > 1) us += c.join + c.mb * 4e-6 * splits * a.rows * a.nt * 16.0 * pair;
+  return us;
+}
+
 }  // namespace
 
-void run_many(const Args& a, hipStream_t s) {
-  if (a.p.codes) launch<Shape<true, 256, 256, 2, 4, 3>>(a, 1, s);
-  else launch<Shape<false, 128, 256, 2, 4, 3>>(a, 1, s);
+Many plan_many(const Args& a, bool scratch) {
+  Many best{0, 1, 1e30};
+  const int shapes = a.p.codes ? 4 : 3;
+  for (int i = 0; i < shapes; ++i) {
+    const Cost& c = a.p.codes ? kPlanes[i] : kTerms[i];
+    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24}) {
+      if (splits > 1 && (!scratch || splits * 2 > a.kt)) break;
+      const double us = cost_us(c, a, splits);
+      if (us < best.us) best = Many{i, splits, us};
+    }
+  }
+  return best;
+}
+
+void run_many(const Args& a, const Many& m, hipStream_t s) {
+  if (a.p.codes) {
+    switch (m.shape) {
+      case 0: return launch<P0>(a, m.splits, s);
+      case 1: return launch<P1>(a, m.splits, s);
+      case 2: return launch<P2>(a, m.splits, s);
+      default: return launch<P3>(a, m.splits, s);
+    }
+  }
+  switch (m.shape) {
+    case 0: return launch<T0>(a, m.splits, s);
+    case 1: return launch<T1>(a, m.splits, s);
+    default: return launch<T2>(a, m.splits, s);
+  }
 }
 
 }  // namespace mx

@@ -22,7 +22,11 @@ namespace {
 
 constexpr int kWaves = 8;
 
-// One k tile of a batch row tile.
+// How a launch holds its activations: planes, bf16 terms, or (at most 16 terms of
+// rows, k of any multiple of 32) rows of an XType, which the kernel splits itself.
+enum { PLANES = 0, TERMS = 1, ROWS = 2 };  // ROWS + XType
+
+// One k tile of a batch row tile, as the matrix instructions take it.
 template <bool FP4>
 struct XFrag;
 template <>
@@ -35,46 +39,117 @@ struct XFrag<false> {
   uint4 c[4];
 };
 
-// A lane's batch row of each row tile. Lanes past the last row read that one
-// again: column m of a product depends on row m alone, and theirs are dropped.
-template <bool FP4>
-struct XRow;
-template <>
-struct XRow<true> {
-  const uint8_t *codes, *scales;
-  XRow() = default;
-  __device__ XRow(const Args& a, int m, int q) {
-    m = min(m, a.rows - 1);
-    codes = a.p.codes + (size_t)m * a.p.ldc;
-    scales = a.p.scales + (size_t)m * a.p.lds;
+// The activations of MT row tiles: load() asks for a k tile, frags() turns what
+// came into operands. Lanes past the last row read that one again: column m of a
+// product depends on row m alone, and theirs are dropped.
+//
+// Two neighbouring values of a row per lane, split into terms and put into the
+// wave's own LDS as 16 rows of 256 B, the 16 B parts of row m in the order
+// 0..15 ^ m: a lane's operand is one part of row lane % 16.
+template <int KIND, int MT>
+struct X {
+  static_assert(KIND >= ROWS && MT == 1);
+  static constexpr int TYPE = KIND - ROWS, T = TYPE == X_F32 ? 3 : TYPE == X_F16 ? 2 : 1, R = 16 / T;
+  using Raw = uint32_t[R][TYPE == X_F32 ? 2 : 1];
+  uint8_t* lds;
+  __device__ X(const Args&, int, uint8_t* l) : lds(l) {}
+  __device__ void load(const Args& a, int kt, int lane, Raw& f) const {
+    const int k = kt * kMxTileK + lane * 2;
+    const bool in = k < a.nblk * kMxBlock;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r >= a.rows) break;
+      const size_t at = (size_t)r * a.ldx + k;
+      if constexpr (TYPE == X_F32) {
+        const uint2 v = in ? *reinterpret_cast<const uint2*>(static_cast<const float*>(a.raw) + at) : make_uint2(0, 0);
+        f[r][0] = v.x;
+        f[r][1] = v.y;
+      } else {
+        f[r][0] = in ? *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.raw) + at) : 0;
+      }
+    }
+  }
+  __device__ void frags(const Args& a, int, int lane, const Raw& f, XFrag<false> (&x)[1]) const {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r >= a.rows) break;
+      float v[2];
+      if constexpr (TYPE == X_F32) {
+        v[0] = __builtin_bit_cast(float, f[r][0]);
+        v[1] = __builtin_bit_cast(float, f[r][1]);
+      } else if constexpr (TYPE == X_F16) {
+        v[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)f[r][0]);
+        v[1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(f[r][0] >> 16));
+      } else {
+        v[0] = __builtin_bit_cast(float, f[r][0] << 16);
+        v[1] = __builtin_bit_cast(float, f[r][0] & 0xffff0000u);
+      }
+      uint32_t t[T];
+      split_terms2<T>(v, t);
+#pragma unroll
+      for (int i = 0; i < T; ++i) {
+        const int m = i * a.rows + r;
+        *reinterpret_cast<uint32_t*>(lds + m * 256 + (((lane >> 2) ^ m) & 15) * 16 + (lane & 3) * 4) = t[i];
+      }
+    }
+    asm volatile("" ::: "memory");  // (one wave's LDS accesses run in order)
+    const int m = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[0].c[j] = *reinterpret_cast<const uint4*>(lds + m * 256 + ((q * 4 + j) ^ m) * 16);
+    asm volatile("" ::: "memory");
+  }
+};
+template <int MT>
+struct X<PLANES, MT> {
+  using Raw = XFrag<true>[MT];
+  const uint8_t *codes[MT], *scales[MT];
+  __device__ X(const Args& a, int lane, uint8_t*) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = min(m * 16 + (lane & 15), a.rows - 1);
+      codes[m] = a.p.codes + (size_t)r * a.p.ldc;
+      scales[m] = a.p.scales + (size_t)r * a.p.lds;
+    }
   }
   // Blocks past the row's last: any codes (the weights are zero there), a scale of 1.
-  __device__ XFrag<true> load(const Args& a, int kt, int q) const {
-    const int b = kt * 4 + q, bc = min(b, a.nblk - 1);
-    XFrag<true> f;
-    f.c = *reinterpret_cast<const uint4*>(codes + (size_t)bc * 16);
-    f.s = b < a.nblk ? scales[bc] : 127;
-    return f;
-  }
-};
-template <>
-struct XRow<false> {
-  const uint16_t* x;
-  XRow() = default;
-  __device__ XRow(const Args& a, int m, int q) {
-    m = min(m, a.rows * a.terms - 1);
-    const int t = m / a.rows;
-    x = a.x + t * a.term_stride + (size_t)(m - t * a.rows) * a.ldx + q * 32;
-  }
-  __device__ XFrag<false> load(const Args& a, int kt, int q) const {
-    XFrag<false> f;
-    const uint4* p = reinterpret_cast<const uint4*>(x + (size_t)kt * kMxTileK);
+  __device__ void load(const Args& a, int kt, int lane, Raw& f) const {
+    const int b = kt * 4 + (lane >> 4), bc = min(b, a.nblk - 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f.c[j] = p[j];
-    return f;
+    for (int m = 0; m < MT; ++m) {
+      f[m].c = *reinterpret_cast<const uint4*>(codes[m] + (size_t)bc * 16);
+      const uint32_t s = scales[m][bc];
+      f[m].s = b < a.nblk ? s : 127;
+    }
+  }
+  __device__ void frags(const Args&, int, int, const Raw& f, XFrag<true> (&x)[MT]) const {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) x[m] = f[m];
   }
 };
-
+template <int MT>
+struct X<TERMS, MT> {
+  using Raw = XFrag<false>[MT];
+  const uint16_t* x[MT];
+  __device__ X(const Args& a, int lane, uint8_t*) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = min(m * 16 + (lane & 15), a.rows * a.terms - 1), t = r / a.rows;
+      x[m] = a.x + t * a.term_stride + (size_t)(r - t * a.rows) * a.ldx + (lane >> 4) * 32;
+    }
+  }
+  __device__ void load(const Args&, int kt, int, Raw& f) const {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const uint4* p = reinterpret_cast<const uint4*>(x[m] + (size_t)kt * kMxTileK);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[m].c[j] = p[j];
+    }
+  }
+  __device__ void frags(const Args&, int, int, const Raw& f, XFrag<false> (&x)[MT]) const {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) x[m] = f[m];
+  }
+};
 template <int MT>
 __device__ inline void mma(uint4 w, uint32_t ws, const XFrag<true> (&x)[MT], f4 (&acc)[MT]) {
 #pragma unroll
@@ -93,25 +168,27 @@ __device__ inline void mma(uint4 w, uint32_t ws, const XFrag<false> (&x)[MT], f4
   }
 }
 
-template <bool FP4, int MT, int NT, int EPI>
+template <int KIND, int MT, int NT, int EPI>
 __global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, bool vec) {
   constexpr int NM = EPI == MX_SWIGLU ? 2 : 1;  // matrices
-  __shared__ f4 part[kWaves][NM][NT][MT][64];
+  constexpr bool FP4 = KIND == PLANES;
+  __shared__ union {
+    f4 part[kWaves][NM][NT][MT][64];
+    uint8_t x[kWaves][KIND >= ROWS ? 4096 : 16];
+  } lds;
+  auto& part = lds.part;
   // this workgroup's batch rows
   const int r0 = blockIdx.y * chunk;
   a.rows = min(chunk, a.rows - r0);
   if constexpr (FP4) {
     a.p.codes += (size_t)r0 * a.p.ldc;
     a.p.scales += (size_t)r0 * a.p.lds;
-  } else {
+  } else if constexpr (KIND == TERMS) {
     a.x += (size_t)r0 * a.ldx;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int q = lane >> 4;
   const int nt0 = blockIdx.x * NT;
-  XRow<FP4> xr[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) xr[m] = XRow<FP4>(a, m * 16 + (lane & 15), q);
+  const X<KIND, MT> xs(a, lane, lds.x[wave]);
   const uint8_t *wc[NM][NT], *ws[NM][NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -124,19 +201,37 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, boo
     }
   }
   f4 acc[NM][NT][MT] = {};
-  const int k1 = (int)((long long)(wave + 1) * a.kt / kWaves);
-  for (int kt = (int)((long long)wave * a.kt / kWaves); kt < k1; ++kt) {
-    XFrag<FP4> x[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) x[m] = xr[m].load(a, kt, q);
+  // this wave's k tiles
+  struct Tile {
+    uint4 w[NM][NT];
+    uint32_t s[NM][NT];
+    typename X<KIND, MT>::Raw x;
+  };
+  auto load = [&](Tile& t, int kt) {
 #pragma unroll
     for (int i = 0; i < NM; ++i)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const uint4 w = *reinterpret_cast<const uint4*>(wc[i][t] + (size_t)kt * 1024);
-        mma<MT>(w, ws[i][t][(size_t)kt * 64], x, acc[i][t]);
+      for (int n = 0; n < NT; ++n) {
+        t.w[i][n] = *reinterpret_cast<const uint4*>(wc[i][n] + (size_t)kt * 1024);
+        t.s[i][n] = ws[i][n][(size_t)kt * 64];
       }
+    xs.load(a, kt, lane, t.x);
+  };
+  auto products = [&](const Tile& t, int kt) {
+    XFrag<FP4> x[MT];
+    xs.frags(a, kt, lane, t.x, x);
+#pragma unroll
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma<MT>(t.w[i][n], t.s[i][n], x, acc[i][n]);
+  };
+  const int k1 = (int)((long long)(wave + 1) * a.kt / kWaves);
+  for (int kt = (int)((long long)wave * a.kt / kWaves); kt < k1; ++kt) {
+    Tile t;
+    load(t, kt);
+    products(t, kt);
   }
+  if constexpr (KIND >= ROWS) __syncthreads();  // (the sums take the place of the activations)
 #pragma unroll
   for (int i = 0; i < NM; ++i)
 #pragma unroll
@@ -164,21 +259,20 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, boo
   }
 }
 
-template <bool FP4, int MT, int EPI>
+template <int KIND, int MT, int EPI>
 void launch(const Args& a, int chunk, hipStream_t s) {
   constexpr int NT = EPI == MX_SWIGLU || MT > 2 ? 1 : 2;
   // (grid y is at most 65535: the rest goes to further launches)
   Args b = a;
-  for (int r0 = 0; r0 < a.rows; r0 += chunk * 65535) {
+  for (long long r0 = 0; r0 < a.rows; r0 += b.rows) {
     b.rows = (int)std::min<long long>(a.rows - r0, (long long)chunk * 65535);
-    hipLaunchKernelGGL((few_kernel<FP4, MT, NT, EPI>), dim3((a.nt + NT - 1) / NT, (b.rows + chunk - 1) / chunk),
+    hipLaunchKernelGGL((few_kernel<KIND, MT, NT, EPI>), dim3((a.nt + NT - 1) / NT, (b.rows + chunk - 1) / chunk),
                        dim3(64 * kWaves), 0, s, b, chunk, rows_vec(a.o));
     PGD_HIP(hipGetLastError());
-    if (b.rows == a.rows - r0) break;
-    if constexpr (FP4) {
+    if constexpr (KIND == PLANES) {
       b.p.codes += (size_t)b.rows * b.p.ldc;
       b.p.scales += (size_t)b.rows * b.p.lds;
-    } else {
+    } else if constexpr (KIND == TERMS) {
       b.x += (size_t)b.rows * b.ldx;
     }
     b.o.y += (size_t)b.rows * b.o.ldy;
@@ -186,30 +280,65 @@ void launch(const Args& a, int chunk, hipStream_t s) {
   }
 }
 
-template <bool FP4, int MT>
+template <int KIND, int MT>
 void launch_epi(const Args& a, int chunk, hipStream_t s) {
-  if (a.uc) launch<FP4, MT, MX_SWIGLU>(a, chunk, s);
-  else if (a.o.res) launch<FP4, MT, MX_RES>(a, chunk, s);
-  else launch<FP4, MT, MX_STORE>(a, chunk, s);
+  if (a.uc) launch<KIND, MT, MX_SWIGLU>(a, chunk, s);
+  else if (a.o.res) launch<KIND, MT, MX_RES>(a, chunk, s);
+  else launch<KIND, MT, MX_STORE>(a, chunk, s);
 }
 
-template <bool FP4>
+template <int KIND>
 void launch_rows(const Args& a, hipStream_t s) {
-  const int terms = FP4 ? 1 : a.terms;
+  const int terms = KIND == PLANES ? 1 : a.terms;
   const int chunk = std::min(a.rows, 64 / terms);
   switch ((chunk * terms + 15) / 16) {
-    case 1: return launch_epi<FP4, 1>(a, chunk, s);
-    case 2: return launch_epi<FP4, 2>(a, chunk, s);
-    case 3: return launch_epi<FP4, 3>(a, chunk, s);
-    default: return launch_epi<FP4, 4>(a, chunk, s);
+    case 1: return launch_epi<KIND, 1>(a, chunk, s);
+    case 2: return launch_epi<KIND, 2>(a, chunk, s);
+    case 3: return launch_epi<KIND, 3>(a, chunk, s);
+    default: return launch_epi<KIND, 4>(a, chunk, s);
   }
 }
 
 }  // namespace
 
+// Splitting rows inside the launch saves another one and the scratch between them
+// (2.6 us), and costs each workgroup about 0.05 + 0.03 (rows * terms) us per k tile
+// of a wave: measured for 1, 2, 4, 5 and 8 rows over 12 matrices from 300 x 17408
+// to 151936 x 896, where more than 5 workgroups per CU always lose.
+bool few_split_ok(int rows, int type) { return rows <= (type == X_F32 ? 5 : type == X_F16 ? 8 : 4); }
+bool few_split_pays(const Args& a, int type) {
+  const int terms = type == X_F32 ? 3 : type == X_F16 ? 2 : 1;
+  return few_split_ok(a.rows, type) && (a.uc ? a.nt : (a.nt + 1) / 2) <= 1280 &&
+         (a.kt + kWaves - 1) / kWaves * (0.05 + 0.03 * a.rows * terms) <= 2.2;
+}
+
+// Microseconds of a launch; per 256 workgroups, their weight tiles and their
+// activation tiles; per k tile, and row of terms of it (1..4 row tiles of rows).
+// Fitted with the costs in gemm_mx.hip: 10 to 15% rms off.
+double few_us(const Args& a) {
+  static constexpr float kPlanes[4][6] = {{5.17f, 0.088f, 0.0239f, 0.00015f, 0.0f, 0.0016f},
+                                          {4.41f, 0.333f, 0.0107f, 0.0015f, 0.023f, 0.0019f},
+                                          {3.87f, 0.392f, 0.0134f, 0.0018f, 0.0f, 0.0030f},
+                                          {3.45f, 0.511f, 0.0312f, 0.0015f, 0.0f, 0.0029f}};
+  static constexpr float kTerms[4][6] = {{4.42f, 0.214f, 0.0176f, 0.0037f, 0.012f, 0.0033f},
+                                         {3.70f, 0.478f, 0.0087f, 0.0060f, 0.029f, 0.0041f},
+                                         {3.06f, 0.180f, 0.0f, 0.0071f, 0.0f, 0.0052f},
+                                         {2.84f, 0.516f, 0.0f, 0.0053f, 0.0f, 0.0051f}};
+  const int terms = a.p.codes ? 1 : a.terms, chunk = std::min(a.rows, 64 / terms), x = chunk * terms, mt = (x + 15) / 16;
+  const int tiles = a.uc ? 1 : mt > 2 ? 1 : 2;
+  const double wg = (double)((a.nt + tiles - 1) / tiles) * ((a.rows + chunk - 1) / chunk) / 256.0;
+  const float* c = a.p.codes ? kPlanes[mt - 1] : kTerms[mt - 1];
+  return c[0] + wg * (c[1] + a.kt * (c[2] * tiles * (a.uc ? 2 : 1) + c[3] * x)) + a.kt * (c[4] + c[5] * x);
+}
+
 void run_few(const Args& a, hipStream_t s) {
-  if (a.p.codes) launch_rows<true>(a, s);
-  else launch_rows<false>(a, s);
+  if (a.p.codes) return launch_rows<PLANES>(a, s);
+  if (a.x) return launch_rows<TERMS>(a, s);
+  switch (a.raw_type) {
+    case X_F32: return launch_epi<ROWS + X_F32, 1>(a, a.rows, s);
+    case X_F16: return launch_epi<ROWS + X_F16, 1>(a, a.rows, s);
+    default: return launch_epi<ROWS + X_BF16, 1>(a, a.rows, s);
+  }
 }
 
 }  // namespace mx

@@ -61,8 +61,9 @@ void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, 
 
 namespace mx {
 
-// One product launch. Activation rows are planes (codes set), or bf16 terms:
-// row r is the sum over t < terms of the bf16 rows x[t * term_stride + r * ldx].
+// One product launch. Activation rows are planes (codes set), bf16 terms (x set:
+// row r is the sum over t < terms of the bf16 rows x[t * term_stride + r * ldx]),
+// or raw, rows of an XType with stride ldx (few_split_ok of them).
 struct Args {
   const uint8_t *wc, *ws;  // matrix codes, scales
   const uint8_t *uc, *us;  // the up matrix's (SwiGLU), or null
@@ -72,6 +73,8 @@ struct Args {
   const uint16_t* x;
   size_t ldx, term_stride;
   int terms;
+  const void* raw;
+  int raw_type;
   MxOut o;
   // set by run_many: ranges of k tiles, and where their sums go
   int splits;
@@ -79,9 +82,21 @@ struct Args {
   size_t part_stride;
 };
 
-// A few rows (gemv_mx.hip), many (gemm_mx.hip), and whichever suits.
+// A few rows (gemv_mx.hip): in 64-row (of terms) chunks, its estimated
+// microseconds; whether it can split a.rows rows of a type itself, and whether
+// that beats splitting them first.
 void run_few(const Args& a, hipStream_t s);
-void run_many(const Args& a, hipStream_t s);
+double few_us(const Args& a);
+bool few_split_ok(int rows, int type);
+bool few_split_pays(const Args& a, int type);
+// Many rows (gemm_mx.hip): the block shape and ranges of k tiles estimated
+// fastest (more than one range only if scratch memory may be used).
+struct Many {
+  int shape, splits;
+  double us;
+};
+Many plan_many(const Args& a, bool scratch);
+void run_many(const Args& a, const Many& m, hipStream_t s);
 
 }  // namespace mx
 }  // namespace pgd

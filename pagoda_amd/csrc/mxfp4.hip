@@ -121,10 +121,8 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict_
   }
 }
 
-// x = t0 + t1 + t2 exactly: each term is the truncation to bf16 (8 significant
-// bits) of what is left, so 3 terms hold the 24 bits of an f32, 2 the 11 of an
-// f16. An infinity or NaN is its first term alone (a NaN stays one: its bits
-// below bf16 are or-ed in). Columns [k, ldt) are zeros, which the last k tile reads.
+// Rows as TERMS planes of bf16 terms (split_terms2). Columns [k, ldt) are zeros,
+// which the last k tile reads.
 template <int TYPE, int TERMS>
 __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, int ldx, int rows, int units,
                                                     uint16_t* __restrict__ out, int ldt, size_t term_stride) {
@@ -134,12 +132,16 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
   for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += step) {
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (u < units) load8<TYPE>(x, (size_t)r * ldx + (size_t)u * 8, v);
-    uint32_t t[TERMS][4];
-    split_terms8<TERMS>(v, t);
+    uint32_t t[4][TERMS];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float pair[2] = {v[2 * j], v[2 * j + 1]};
+      split_terms2<TERMS>(pair, t[j]);
+    }
 #pragma unroll
     for (int i = 0; i < TERMS; ++i)
       *reinterpret_cast<uint4*>(out + i * term_stride + (size_t)r * ldt + (size_t)u * 8) =
-          make_uint4(t[i][0], t[i][1], t[i][2], t[i][3]);
+          make_uint4(t[0][i], t[1][i], t[2][i], t[3][i]);
   }
 }
 
@@ -160,9 +162,23 @@ Args make_args(const QMat& w, const QMat* up, int rows, const MxOut& o) {
   return a;
 }
 
-void run(const Args& a, hipStream_t s) {
-  if (a.rows <= 64) run_few(a, s);
-  else run_many(a, s);
+// A captured graph would keep the address of scratch memory, which a later call
+// may replace: captured launches use none.
+bool scratch_allowed(hipStream_t s) {
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  PGD_HIP(hipStreamIsCapturing(s, &cap));
+  return cap == hipStreamCaptureStatusNone;
+}
+
+void run(const Args& a, bool scratch, hipStream_t s) {
+  // (the many-row kernel's lanes hold offsets in 128 rows, and 16 row tiles of the matrix, in 32 bits)
+  const size_t stride = a.p.codes ? std::max(a.p.ldc, a.p.lds) : a.ldx * 2;
+  const bool near = stride < ((size_t)1 << 24);
+  if (near) {
+    const Many m = plan_many(a, scratch);
+    if (m.us < few_us(a)) return run_many(a, m, s);
+  }
+  run_few(a, s);
 }
 
 void check(const QMat& w, const QMat* up, int rows) {
@@ -215,17 +231,23 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   if (rows == 0) return;
   Args a = make_args(w, up, rows, o);
   a.terms = type == X_F32 ? 3 : type == X_F16 ? 2 : 1;
+  const bool scratch = scratch_allowed(s);
   if (type == X_BF16 && w.n_in % kMxTileK == 0) {  // the rows are their own term
     a.x = static_cast<const uint16_t*>(x);
     a.ldx = ldx;
-    run(a, s);
+    run(a, scratch, s);
     return;
   }
-  // a captured graph would keep the scratch's address, which a later call may replace
-  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-  PGD_HIP(hipStreamIsCapturing(s, &cap));
-  PGD_CHECK(cap == hipStreamCaptureStatusNone, kErrState,
-            "these MXFP4 activation rows need scratch memory: capture bf16 rows of whole 128-column tiles, or MXFP4 rows");
+  if (few_split_pays(a, type) || (!scratch && few_split_ok(rows, type))) {
+    a.raw = x;
+    a.raw_type = type;
+    a.ldx = ldx;
+    run_few(a, s);
+    return;
+  }
+  PGD_CHECK(scratch, kErrState,
+            "splitting these MXFP4 activation rows needs scratch memory: under capture, at most 5 f32, 8 f16 or 4 bf16 "
+            "rows, any bf16 rows of whole 128-column tiles, or MXFP4 rows");
   const int ldt = a.kt * kMxTileK;
   std::lock_guard<std::mutex> lock(g_terms);
   a.term_stride = (size_t)rows * ldt;
@@ -240,7 +262,7 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   else if (type == X_F16) go(terms_kernel<X_F16, 2>);
   else go(terms_kernel<X_BF16, 1>);
   PGD_HIP(hipGetLastError());
-  run(a, s);
+  run(a, true, s);
 }
 
 void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, const MxOut& o, hipStream_t s) {
@@ -248,7 +270,7 @@ void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, 
   if (rows == 0) return;
   Args a = make_args(w, up, rows, o);
   a.p = x;
-  run(a, s);
+  run(a, scratch_allowed(s), s);
 }
 
 }  // namespace pgd

@@ -47,26 +47,26 @@ __device__ inline bf8 fp4_bf16x8(uint32_t c, float scale) {
   return (bf8){a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
 }
 
-// Eight values as TERMS bf16 terms, pairs packed low first (see terms_kernel).
+// x = t0 + t1 + t2 exactly: each term is the truncation to bf16 (8 significant
+// bits) of what is left, so 3 terms hold the 24 bits of an f32, 2 the 11 of an
+// f16. An infinity or NaN is its first term alone (a NaN stays one: its bits
+// below bf16 are or-ed in). Two values, the terms packed low first.
 template <int TERMS>
-__device__ inline void split_terms8(float (&v)[8], uint32_t (&t)[TERMS][4]) {
+__device__ inline void split_terms2(float (&v)[2], uint32_t (&t)[TERMS]) {
 #pragma unroll
   for (int i = 0; i < TERMS; ++i) {
+    uint32_t h[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t h[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float& x = v[2 * j + e];
-        const uint32_t b = __builtin_bit_cast(uint32_t, x);
-        uint32_t hi = b & 0xffff0000u;
-        const bool fin = (b & 0x7f800000u) != 0x7f800000u;
-        if (!fin && (b & 0x007fffffu)) hi |= 0x00400000u;  // a NaN
-        if (i + 1 < TERMS) x = fin ? x - __builtin_bit_cast(float, hi) : 0.0f;
-        h[e] = hi;
-      }
-      t[i][j] = (h[0] >> 16) | h[1];
+    for (int e = 0; e < 2; ++e) {
+      float& x = v[e];
+      const uint32_t b = __builtin_bit_cast(uint32_t, x);
+      uint32_t hi = b & 0xffff0000u;
+      const bool fin = (b & 0x7f800000u) != 0x7f800000u;
+      if (!fin && (b & 0x007fffffu)) hi |= 0x00400000u;  // a NaN
+      if (i + 1 < TERMS) x = fin ? x - __builtin_bit_cast(float, hi) : 0.0f;
+      h[e] = hi;
     }
+    t[i] = (h[0] >> 16) | h[1];
   }
 }
 
