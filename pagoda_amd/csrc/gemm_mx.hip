@@ -8,7 +8,8 @@
 // the barrier retires is filled with the stage S - 1 ahead.
 //
 // Rows of several bf16 terms take one stage per term and k tile: all terms of a
-// row add to the same f32 sums.
+// row add to the same f32 sums. Rows in digits (mxfp4.hip) take six matrix
+// instructions of the 4-bit rate instead of three terms' twelve of the bf16 rate.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -41,23 +42,26 @@ __device__ __forceinline__ void dma4(const void* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(uniform(to)), "v"(from) : "memory");
 }
 
-template <bool FP4_, int BM_, int BN_, int WM_, int WN_, int S_, int OCC_ = 1>
+enum { PLANES = 0, TERMS = 1, DIGITS = 2 };  // how the activations come (Args)
+
+template <int KIND_, int BM_, int BN_, int WM_, int WN_, int S_, int OCC_ = 1>
 struct Shape {
-  static constexpr bool FP4 = FP4_;
+  static constexpr int KIND = KIND_;
+  static constexpr bool FP4 = KIND == PLANES, DIG = KIND == DIGITS;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_, OCC = OCC_;
   static constexpr int W = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16;
   // A wave's loads of a stage: NX of activations (XB bytes each, 4 or 16 a lane),
   // NL KiB of weight codes, NS times 256 B of weight scales (where there are
   // fewer than waves, several waves load the same bytes to the same place)
-  static constexpr int X = BM * (FP4 ? 64 : 256), XB = X / 1024 % W == 0 ? 1024 : 256, NX = X / XB / W;
-  static constexpr int NL = BN / 16 / W, WS = BN / 64, NS = WS > W ? WS / W : 1, LOADS = NX + NL + NS;
-  static constexpr int SC = X + BN * 64, BYTES = SC + BN * 4;
+  static constexpr int X = BM / 16 * (FP4 ? 1024 : DIG ? kMxDigitTile : 4096), XB = X / 1024 % W == 0 ? 1024 : 256, NX = X / XB / W;
+  static constexpr int NL = BN / 16 / W, WS = BN / 64, NS = WS > W ? WS / W : 1, LOADS = NX + NL + NS + DIG;
+  static constexpr int SC = X + BN * 64, DS = SC + BN * 4, BYTES = DS + (DIG ? BM * 4 : 0);
   // activation scales: every fourth stage brings those of 4 k tiles, 16 B of a
   // row, into the other of two slots behind the ring
   static constexpr int XS = FP4 ? (BM + 63) / 64 : 0, NXS = XS > W ? XS / W : 1;
   static constexpr int RING = S * BYTES, LDS = RING + 2 * XS * 1024;
   static_assert((!FP4 || MF == 1 || MF % 2 == 0) && X / XB % W == 0 && BN / 16 % W == 0 && (WS <= W || WS % W == 0) && (XS <= W || XS % W == 0));
-  static_assert(S >= 2 && S <= (FP4 ? 5 : 8) && LDS * OCC <= 160 * 1024);
+  static_assert(S >= 2 && S <= (FP4 ? 5 : 8) && LDS * OCC <= 160 * 1024 && (!DIG || (BM <= 64 && XB == 1024)));
 };
 
 template <class T, int EPI>
@@ -95,7 +99,10 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
   for (int k = 0; k < T::NX; ++k) {
     const int p = (wave * T::NX + k) * T::XB + lane * (T::XB / 64);
     const int i = (p >> 6) & 15, part = ((p >> 4) & 3) ^ (i >> 2);
-    if constexpr (T::FP4) {
+    if constexpr (T::DIG) {  // whole tiles, as they lie
+      const int f = p / kMxDigitTile;
+      xo[k] = (uint32_t)min(f, last >> 4) * (uint32_t)(a.kt * kMxDigitTile) + (p - f * kMxDigitTile);
+    } else if constexpr (T::FP4) {
       xo[k] = (uint32_t)min((p >> 10) * 16 + i, last) * (uint32_t)a.p.ldc + part * 16 + (p & 15);
       // in the last k tile, blocks past the row's last are that one again (their weights are zero)
       cut[k] = max(part - ((a.nblk - 1) & 3), 0) * 16;
@@ -103,7 +110,12 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
       xo[k] = (uint32_t)min((p >> 12) * 16 + i, last) * (uint32_t)(a.ldx * 2) + ((p >> 10) & 3) * 64 + part * 16 + (p & 15);
     }
   }
-  const uint8_t* xb = T::FP4 ? a.p.codes + (size_t)m0 * a.p.ldc : reinterpret_cast<const uint8_t*>(a.x + (size_t)m0 * a.ldx);
+  const uint8_t* xb = T::FP4   ? a.p.codes + (size_t)m0 * a.p.ldc
+                      : T::DIG ? a.d + (size_t)(m0 >> 4) * a.kt * kMxDigitTile
+                               : reinterpret_cast<const uint8_t*>(a.x + (size_t)m0 * a.ldx);
+  // digits' scales: 64 B of each row tile
+  const uint32_t dso = (uint32_t)min(q, last >> 4) * (uint32_t)(a.kt * 64) + i16 * 4;
+  const uint8_t* dsb = T::DIG ? a.ds + ((size_t)(m0 >> 4) * a.kt + k0) * 64 : nullptr;
   // row tile f of the stage: a wave's NF tiles, gate before up
   auto tile_of = [&](int f, bool& up) {
     const int w = f / NF, t = f % NF;
@@ -132,10 +144,10 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
 
   // The loads' k tile and term. Past the last stage they repeat its k tile into
   // slots that nothing reads: every wave has the same number in flight.
-  const int terms = T::FP4 ? 1 : a.terms, steps = (k1 - k0) * terms;
+  const int terms = T::KIND == TERMS ? a.terms : 1, steps = (k1 - k0) * terms;
   int lk = k0, lterm = 0;
   const size_t term_bytes = a.term_stride * 2;
-  const uint8_t* xk = xb + (size_t)k0 * (T::FP4 ? 64 : 256);  // of k tile lk, term lterm
+  const uint8_t* xk = xb + (size_t)k0 * (T::FP4 ? 64 : T::DIG ? kMxDigitTile : 256);  // of k tile lk, term lterm
   bool first = true;
   auto issue = [&](uint32_t slot) {
     const uint32_t st = lds0 + slot;
@@ -161,10 +173,14 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
     for (int k = 0; k < T::NL; ++k) dma16(wb[k], wo, st + T::X + (wave * T::NL + k) * 1024);
 #pragma unroll
     for (int k = 0; k < T::NS; ++k) dma4(sb[k], st + T::SC + (wave * T::NS + k) % T::WS * 256);
+    if constexpr (T::DIG) {
+      if (q < T::BM / 16) dma4(dsb, dso, st + T::DS);
+    }
     // (no branches: the pointers stay in registers)
-    const int more = T::FP4 ? lk + 1 < k1 : (lterm == terms - 1 && lk + 1 < k1);
-    if constexpr (T::FP4) {
-      xk += more * 64;
+    const int more = T::KIND != TERMS ? lk + 1 < k1 : (lterm == terms - 1 && lk + 1 < k1);
+    if constexpr (T::KIND != TERMS) {
+      xk += more * (T::FP4 ? 64 : kMxDigitTile);
+      if constexpr (T::DIG) dsb += more * 64;
     } else {
       const int wrap = lterm == terms - 1;
       xk += wrap ? more * 256 - (ptrdiff_t)term_bytes * (terms - 1) : (ptrdiff_t)term_bytes;
@@ -268,6 +284,64 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
       step(k0 + t, w0, w1);
       if (++t == steps) break;
       step(k0 + t, w1, w0);
+      if (++t == steps) break;
+    }
+  } else if constexpr (T::DIG) {
+    // Three digits of a row tile at a time, the next three read under their products.
+    struct Digits {
+      uint4 lo[3];
+      uint2 hi[3];
+    };
+    auto read_digits = [&](Digits& f, int g) {
+      const uint8_t* xp = smem + here + (wm * MF + (g >> 1)) * kMxDigitTile + lane * 16;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int d = (g & 1) * 3 + i;
+        f.lo[i] = *reinterpret_cast<const uint4*>(xp + d * 1024);
+        f.hi[i] = *reinterpret_cast<const uint2*>(xp + 6144 + (d >> 1) * 1024 + (d & 1) * 8);
+      }
+    };
+    struct Stage {
+      WFrag w;
+      uint32_t s[MF];
+    };
+    auto read_stage = [&](Stage& f) {
+      read_w(f.w, here);
+#pragma unroll
+      for (int m = 0; m < MF; ++m) f.s[m] = smem[here + T::DS + (wm * MF + m) * 64 + lane];
+    };
+    Digits even, odd;
+    auto step = [&](const Stage& f, Stage& next) {
+#pragma unroll
+      for (int g = 0; g < 2 * MF; ++g) {
+        Digits &now = g & 1 ? odd : even, &then = g & 1 ? even : odd;
+        if (g + 1 < 2 * MF) {
+          read_digits(then, g + 1);
+        } else {
+          sync(std::integral_constant<int, S - 2>{});
+          issue(here);
+          advance();
+          read_stage(next);
+          read_digits(then, 0);
+        }
+        fence();
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint32_t s = f.s[g >> 1] - 5 * ((g & 1) * 3 + i);
+#pragma unroll
+          for (int n = 0; n < NF; ++n)
+            acc[n][g >> 1] = mfma_fp4_fp6(f.w.c[n], f.w.s[n], now.lo[i], now.hi[i], s, acc[n][g >> 1]);
+        }
+        fence();
+      }
+    };
+    Stage f0, f1;
+    read_stage(f0);
+    read_digits(even, 0);
+    for (int t = 0;;) {
+      step(f0, f1);
+      if (++t == steps) break;
+      step(f1, f0);
       if (++t == steps) break;
     }
   } else {
@@ -407,13 +481,15 @@ void launch(Args a, int splits, hipStream_t s) {
 }
 
 // The shapes, largest first.
-using P0 = Shape<true, 128, 256, 1, 4, 3, 2>;
-using P1 = Shape<true, 128, 128, 2, 2, 4, 2>;
-using P2 = Shape<true, 64, 128, 1, 4, 4, 2>;
-using P3 = Shape<true, 32, 128, 1, 4, 5, 2>;
-using T0 = Shape<false, 64, 256, 1, 4, 2, 2>;
-using T1 = Shape<false, 64, 128, 1, 4, 3, 2>;
-using T2 = Shape<false, 32, 128, 1, 4, 4, 2>;
+using P0 = Shape<PLANES, 128, 256, 1, 4, 3, 2>;
+using P1 = Shape<PLANES, 128, 128, 2, 2, 4, 2>;
+using P2 = Shape<PLANES, 64, 128, 1, 4, 4, 2>;
+using P3 = Shape<PLANES, 32, 128, 1, 4, 5, 2>;
+using D0 = Shape<DIGITS, 64, 256, 2, 2, 3>;
+using D1 = Shape<DIGITS, 32, 128, 1, 2, 3, 2>;
+using T0 = Shape<TERMS, 64, 256, 1, 4, 2, 2>;
+using T1 = Shape<TERMS, 64, 128, 1, 4, 3, 2>;
+using T2 = Shape<TERMS, 32, 128, 1, 4, 4, 2>;
 
 // Microseconds of a launch, of a stage and of the rest of a block where a CU runs
 // two blocks and where it runs one, and of joining ranges (a launch, and each MB of
@@ -467,6 +543,7 @@ void run_many(const Args& a, const Many& m, hipStream_t s) {
       default: return launch<P3>(a, m.splits, s);
     }
   }
+  if (a.d) return launch<D0>(a, m.splits, s);
   switch (m.shape) {
     case 0: return launch<T0>(a, m.splits, s);
     case 1: return launch<T1>(a, m.splits, s);

@@ -61,9 +61,13 @@ void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, 
 
 namespace mx {
 
+constexpr int kMxDigitTile = 9216;  // 6 digits of 24 B a lane
+
 // One product launch. Activation rows are planes (codes set), bf16 terms (x set:
 // row r is the sum over t < terms of the bf16 rows x[t * term_stride + r * ldx]),
-// or raw, rows of an XType with stride ldx (few_split_ok of them).
+// raw, rows of an XType with stride ldx (few_split_ok of them), or digits (d, ds
+// set): tiles of 16 rows by 128 columns, kMxDigitTile bytes of e2m3 codes and 64
+// block exponents each, [row tile][k tile].
 struct Args {
   const uint8_t *wc, *ws;  // matrix codes, scales
   const uint8_t *uc, *us;  // the up matrix's (SwiGLU), or null
@@ -75,6 +79,7 @@ struct Args {
   int terms;
   const void* raw;
   int raw_type;
+  const uint8_t *d, *ds;
   MxOut o;
   // set by run_many: ranges of k tiles, and where their sums go
   int splits;

@@ -145,6 +145,59 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
   }
 }
 
+// Rows in six base-32 digits. A block with largest magnitude below 2^(e - 126) (e
+// the biased exponent, 25 at least) is held in steps of 2^(e - 155): 30 bits, so
+// its values are exact to the last of their 24 where they are above 1/64 of the
+// largest, and within 2^-30 of it elsewhere (f32 sums of its products keep 24).
+// Digits -16..15 of that whole number, the top one to 16, are e2m3 codes (u / 8 is
+// code u up to 16), digit i scaled by 2^(e - 127 - 5 i). A wave takes one tile of 16
+// rows by 128 columns, lane l block l / 16 of row l % 16. A block with an infinity
+// or NaN is NaN. Rows and columns past the matrix are zeros.
+template <int TYPE>
+__global__ __launch_bounds__(256) void digits_kernel(const void* __restrict__ x, int ldx, int rows, int nblk, int kt,
+                                                     long long tiles, uint8_t* __restrict__ d,
+                                                     uint8_t* __restrict__ ds) {
+  const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tile >= tiles) return;
+  const int lane = threadIdx.x & 63;
+  const int row = (int)(tile / kt) * 16 + (lane & 15), b = (int)(tile % kt) * 4 + (lane >> 4);
+  float v[4][8] = {};
+  if (row < rows && b < nblk) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load8<TYPE>(x, (size_t)row * ldx + (size_t)b * kMxBlock + j * 8, v[j]);
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i >> 3][i & 7]) & 0x7fffffffu);
+  const int e = max((int)(top >> 23), 25);
+  uint32_t q[6][6] = {};  // [digit][dword]
+  if (e != 255) {
+    // (2^(155 - e) in two factors: it may pass the largest f32)
+    const float up = __builtin_bit_cast(float, (uint32_t)(127 + (155 - e) / 2) << 23);
+    const float up2 = __builtin_bit_cast(float, (uint32_t)(127 + (155 - e) - (155 - e) / 2) << 23);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      int n = __float2int_rn(v[i >> 3][i & 7] * up * up2);
+#pragma unroll
+      for (int k = 5; k >= 0; --k) {
+        const int u = k ? ((n + 16) & 31) - 16 : n;
+        n = (n - u) >> 5;
+        const uint32_t code = (uint32_t)abs(u) | (u < 0 ? 32u : 0u);
+        const int bit = 6 * i, w = bit >> 5, o = bit & 31;
+        q[k][w] |= code << o;
+        if (o > 26) q[k][w + 1] |= code >> (32 - o);
+      }
+    }
+  }
+  uint8_t* out = d + (size_t)tile * kMxDigitTile + lane * 16;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    *reinterpret_cast<uint4*>(out + k * 1024) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
+    *reinterpret_cast<uint2*>(out + 6144 + (k >> 1) * 1024 + (k & 1) * 8) = make_uint2(q[k][4], q[k][5]);
+  }
+  ds[(size_t)tile * 64 + lane] = (uint8_t)e;
+}
+
 Args make_args(const QMat& w, const QMat* up, int rows, const MxOut& o) {
   Args a{};
   a.wc = w.p0;
@@ -248,8 +301,23 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   PGD_CHECK(scratch, kErrState,
             "splitting these MXFP4 activation rows needs scratch memory: under capture, at most 5 f32, 8 f16 or 4 bf16 "
             "rows, any bf16 rows of whole 128-column tiles, or MXFP4 rows");
-  const int ldt = a.kt * kMxTileK;
   std::lock_guard<std::mutex> lock(g_terms);
+  if (type != X_BF16 && rows > 64) {
+    const long long tiles = (long long)((rows + 15) / 16) * a.kt;
+    auto* d = static_cast<uint8_t*>(gemv::gemv_scratch(s, (size_t)tiles * (kMxDigitTile + 64), 8));
+    a.d = d;
+    a.ds = d + (size_t)tiles * kMxDigitTile;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, s, x, ldx, rows, a.nblk, a.kt, tiles, d,
+                         d + (size_t)tiles * kMxDigitTile);
+    };
+    if (type == X_F32) go(digits_kernel<X_F32>);
+    else go(digits_kernel<X_F16>);
+    PGD_HIP(hipGetLastError());
+    run_many(a, plan_many(a, true), s);
+    return;
+  }
+  const int ldt = a.kt * kMxTileK;
   a.term_stride = (size_t)rows * ldt;
   auto* t = static_cast<uint16_t*>(gemv::gemv_scratch(s, a.terms * a.term_stride * sizeof(uint16_t), 8));
   a.x = t;

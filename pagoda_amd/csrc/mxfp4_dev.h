@@ -80,6 +80,13 @@ __device__ inline f4 mfma_fp4(uint4 w, uint32_t ws, uint4 x, uint32_t xs, f4 c) 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, (int)ws, 0, (int)xs);
 }
 
+// The same with the 32 e2m3 codes (24 bytes) of the lane's activation block.
+__device__ inline f4 mfma_fp4_fp6(uint4 w, uint32_t ws, uint4 lo, uint2 hi, uint32_t xs, f4 c) {
+  const i8v a = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
+  const i8v b = {(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 2, 0, (int)ws, 0, (int)xs);
+}
+
 // (PART, PART2: sums of a range of k tiles, of one matrix or of the pair)
 enum { MX_STORE = 0, MX_RES = 1, MX_SWIGLU = 2, MX_PART = 3, MX_PART2 = 4 };
 
