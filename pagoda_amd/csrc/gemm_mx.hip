@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 #include "gemv_impl.h"
@@ -38,9 +39,6 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t t
 __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(uniform(to)), "v"(off), "s"(uniform(base)) : "memory");
 }
-__device__ __forceinline__ void dma4(const void* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(uniform(to)), "v"(from) : "memory");
-}
 
 enum { PLANES = 0, TERMS = 1, DIGITS = 2 };  // how the activations come (Args)
 
@@ -64,6 +62,16 @@ struct Shape {
   static_assert(S >= 2 && S <= (FP4 ? 5 : 8) && LDS * OCC <= 160 * 1024 && (!DIG || (BM <= 64 && XB == 1024)));
 };
 
+// f(0), .., f(N - 1) with constant arguments
+template <class F, int... I>
+__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  each(f, std::make_integer_sequence<int, N>{});
+}
+
 template <class T, int EPI>
 __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args a, int nmb, int nnb, int per_xcd, bool vec) {
   constexpr bool DUAL = EPI == MX_SWIGLU || EPI == MX_PART2;
@@ -84,21 +92,24 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
   const int g0 = gi / (8 * nnb) * 8, gw = min(8, nmb - g0), in = gi - g0 * nnb;
   const int m0 = uniform((uint32_t)((g0 + in % gw) * T::BM)), nt0 = uniform((uint32_t)(in / gw * NB));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i16 = lane & 15, q = lane >> 4, swz = i16 >> 2;
+  const int i16 = lane & 15, q = lane >> 4;
+  auto h = [](int g) { return (0x78 >> (2 * g)) & 3; };
+  const int swz = h(i16 >> 2);
   const int wm = wave / T::WN, wn = wave % T::WN;
 
   // Where the bytes at LDS offset p of a stage come from, relative to the block's
   // first row and the k tile. A 16-row tile (a block of it, for bf16 terms) is 16
   // rows of 64 B, so that neighbouring lanes of a load leave as one request; the
-  // four 16 B parts of row i lie in the order 0..3 ^ i / 4: then the 16 lanes that
-  // read one part of 16 rows at once meet no bank twice. Rows past the last are
-  // that row again, and are not stored.
+  // four 16 B parts of row i lie in the order 0..3 ^ h(i / 4). An LDS read of 16 B a
+  // lane takes lanes 0-3, 12-15, 20-27 at once (then the others of 32): with h = 0 2
+  // 3 1 these meet no bank twice, whether the lanes' parts differ (codes: part l /
+  // 16) or not (terms). Rows past the last are that row again, and are not stored.
   const int last = a.rows - 1 - m0;
   uint32_t xo[T::NX], cut[T::NX];
 #pragma unroll
   for (int k = 0; k < T::NX; ++k) {
     const int p = (wave * T::NX + k) * T::XB + lane * (T::XB / 64);
-    const int i = (p >> 6) & 15, part = ((p >> 4) & 3) ^ (i >> 2);
+    const int i = (p >> 6) & 15, part = ((p >> 4) & 3) ^ h(i >> 2);
     if constexpr (T::DIG) {  // whole tiles, as they lie
       const int f = p / kMxDigitTile;
       xo[k] = (uint32_t)min(f, last >> 4) * (uint32_t)(a.kt * kMxDigitTile) + (p - f * kMxDigitTile);
@@ -130,12 +141,15 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
     const size_t nt = tile_of(wave * T::NL + k, up);
     wb[k] = (up ? a.uc : a.wc) + (nt * a.kt + k0) * 1024;
   }
+  // weight scales, 4 row tiles a load: the gate's of the workgroup, then the up matrix's
 #pragma unroll
-  for (int k = 0; k < T::NS; ++k) {  // 4 row tiles a load, 16 lanes each
-    bool up;
-    const size_t nt = tile_of((wave * T::NS + k) % T::WS * 4 + q, up);
-    sb[k] = (up ? a.us : a.ws) + (nt * a.kt + k0) * 64 + i16 * 4;
+  for (int k = 0; k < T::NS; ++k) {
+    const int u = (wave * T::NS + k) % T::WS;
+    const bool up = DUAL && u >= NB / 4;
+    const size_t g = min(nt0 / 4 + (up ? u - NB / 4 : u), (a.nt - 1) / 4);
+    sb[k] = (up ? a.us : a.ws) + (g * a.kt + k0) * 256;
   }
+  const uint32_t wso = lane * 4;
   const uint8_t* xsb = a.p.scales + (T::FP4 ? (size_t)m0 * a.p.lds : 0);
   uint32_t xso[T::NXS];
 #pragma unroll
@@ -172,7 +186,7 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
 #pragma unroll
     for (int k = 0; k < T::NL; ++k) dma16(wb[k], wo, st + T::X + (wave * T::NL + k) * 1024);
 #pragma unroll
-    for (int k = 0; k < T::NS; ++k) dma4(sb[k], st + T::SC + (wave * T::NS + k) % T::WS * 256);
+    for (int k = 0; k < T::NS; ++k) dma4(sb[k], wso, st + T::SC + (wave * T::NS + k) % T::WS * 256);
     if constexpr (T::DIG) {
       if (q < T::BM / 16) dma4(dsb, dso, st + T::DS);
     }
@@ -190,25 +204,34 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
 #pragma unroll
     for (int k = 0; k < T::NL; ++k) wb[k] += more * 1024;
 #pragma unroll
-    for (int k = 0; k < T::NS; ++k) sb[k] += more * 64;
+    for (int k = 0; k < T::NS; ++k) sb[k] += more * 256;
   };
 
   f4 acc[NF][MF] = {};
   // LDS operands of a stage: its weights' codes and scales, and of bf16 terms the
   // quarter that matrix instruction j takes
+  // (scales: byte n % 4 of register n / 4 of a matrix's NW tiles; a wave with fewer
+  // than 4 tiles shifts its own down)
+  constexpr int NM = DUAL ? 2 : 1, SG = (NW + 3) / 4;
+  static_assert(NB % 4 == 0 && (NW % 4 == 0 || 4 % NW == 0));
   struct WFrag {
     uint4 c[NF];
-    uint32_t s[NF];
+    uint32_t s[NM][SG];
   };
   auto read_w = [&](WFrag& f, uint32_t slot) {
-    const uint8_t* ws = smem + slot + T::SC + wn * NF * 64 + lane;
+    const uint8_t* ws = smem + slot + T::SC + (wn * NW >> 2) * 256 + lane * 4;
     const uint8_t* wp = smem + slot + T::X + wn * NF * 1024 + lane * 16;
 #pragma unroll
-    for (int n = 0; n < NF; ++n) {
-      f.c[n] = *reinterpret_cast<const uint4*>(wp + n * 1024);
-      f.s[n] = ws[n * 64];
-    }
+    for (int n = 0; n < NF; ++n) f.c[n] = *reinterpret_cast<const uint4*>(wp + n * 1024);
+#pragma unroll
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+      for (int g = 0; g < SG; ++g) {
+        f.s[i][g] = *reinterpret_cast<const uint32_t*>(ws + (i * (NB / 4) + g) * 256);
+        if constexpr (NW < 4) f.s[i][g] >>= 8 * (wn * NW & 3);
+      }
   };
+  auto ws_of = [](const WFrag& f, int n) { return f.s[n / NW][n % NW / 4]; };
   auto read_x = [&](uint4 (&x)[MF], uint32_t slot, int j) {
     const uint8_t* xp = smem + slot + wm * MF * 4096 + q * 1024 + i16 * 64 + (j ^ swz) * 16;
 #pragma unroll
@@ -255,9 +278,10 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
       }
 #pragma unroll
       for (int m = 0; m < H; ++m)
-#pragma unroll
-        for (int n = 0; n < NF; ++n)
-          acc[n][half * H + m] = mfma_fp4(w.c[n], w.s[n], f.x[m], f.s[m], acc[n][half * H + m]);
+        each<NF>([&](auto n) {
+          f4& c = acc[n][half * H + m];
+          c = mfma_fp4<n % NW % 4, 0>(w.c[n], ws_of(w, n), fp4_operand(f.x[m]), f.s[m], c);
+        });
       fence();
     };
     WFrag w0, w1;
@@ -289,16 +313,18 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
   } else if constexpr (T::DIG) {
     // Three digits of a row tile at a time, the next three read under their products.
     struct Digits {
-      uint4 lo[3];
-      uint2 hi[3];
+      i8v x[3];
     };
     auto read_digits = [&](Digits& f, int g) {
-      const uint8_t* xp = smem + here + (wm * MF + (g >> 1)) * kMxDigitTile + lane * 16;
+      const uint8_t* xp = smem + here + (wm * MF + (g >> 1)) * kMxDigitTile;
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
         const int d = (g & 1) * 3 + i;
-        f.lo[i] = *reinterpret_cast<const uint4*>(xp + d * 1024);
-        f.hi[i] = *reinterpret_cast<const uint2*>(xp + 6144 + (d >> 1) * 1024 + (d & 1) * 8);
+        const uint4 lo = *reinterpret_cast<const uint4*>(xp + lane * 16 + d * 1024);
+        const uint2 hi = *reinterpret_cast<const uint2*>(xp + lane * 8 + 6144 + d * 512);
+        f.x[i] = (i8v){(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, 0, 0};
+        // (joined into one read with the next digit's, hi would land outside its operand's registers)
+        asm volatile("" ::: "memory");
       }
     };
     struct Stage {
@@ -328,9 +354,9 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
           const uint32_t s = f.s[g >> 1] - 5 * ((g & 1) * 3 + i);
-#pragma unroll
-          for (int n = 0; n < NF; ++n)
-            acc[n][g >> 1] = mfma_fp4_fp6(f.w.c[n], f.w.s[n], now.lo[i], now.hi[i], s, acc[n][g >> 1]);
+          each<NF>([&](auto n) {
+            acc[n][g >> 1] = mfma_fp4<n % NW % 4, 0, true>(f.w.c[n], ws_of(f.w, n), now.x[i], s, acc[n][g >> 1]);
+          });
         }
         fence();
       }
@@ -347,7 +373,7 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
   } else {
     auto decode = [&](bf8 (&wf)[NF], const WFrag& w, int j) {
 #pragma unroll
-      for (int n = 0; n < NF; ++n) wf[n] = fp4_bf16x8(reinterpret_cast<const uint32_t*>(&w.c[n])[j], e8m0_f32(w.s[n]));
+      for (int n = 0; n < NF; ++n) wf[n] = fp4_bf16x8(reinterpret_cast<const uint32_t*>(&w.c[n])[j], e8m0_f32(ws_of(w, n) >> (8 * (n % NW % 4)) & 255));
     };
     auto mma = [&](const bf8 (&wf)[NF], const uint4 (&x)[MF]) {
 #pragma unroll

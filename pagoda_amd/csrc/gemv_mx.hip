@@ -150,15 +150,16 @@ struct X<TERMS, MT> {
     for (int m = 0; m < MT; ++m) x[m] = f[m];
   }
 };
-template <int MT>
+// (the weights' scale is byte B of ws)
+template <int B, int MT>
 __device__ inline void mma(uint4 w, uint32_t ws, const XFrag<true> (&x)[MT], f4 (&acc)[MT]) {
 #pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = mfma_fp4(w, ws, x[m].c, x[m].s, acc[m]);
+  for (int m = 0; m < MT; ++m) acc[m] = mfma_fp4<B, 0>(w, ws, fp4_operand(x[m].c), x[m].s, acc[m]);
 }
 // Matrix instruction j takes elements 8 j .. 8 j + 7 of each lane's block.
-template <int MT>
+template <int B, int MT>
 __device__ inline void mma(uint4 w, uint32_t ws, const XFrag<false> (&x)[MT], f4 (&acc)[MT]) {
-  const float s = e8m0_f32(ws);
+  const float s = e8m0_f32(ws >> (8 * B) & 255);
   const uint32_t c[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -187,43 +188,49 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, boo
     a.x += (size_t)r0 * a.ldx;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nt0 = blockIdx.x * NT;
+  // Workgroups are dealt to the 8 XCDs in turn: those whose row tiles' scales lie
+  // together (four tiles) follow each other on one XCD, and find them in its L2.
+  constexpr int NG = 4 / NT;
+  const int id = blockIdx.x >> 3;
+  const int nt0 = (((id / NG) * 8 + (blockIdx.x & 7)) * NG + id % NG) * NT;
+  if (nt0 >= a.nt) return;
   const X<KIND, MT> xs(a, lane, lds.x[wave]);
-  const uint8_t *wc[NM][NT], *ws[NM][NT];
+  // (the scales of NT row tiles are neighbouring bytes)
+  const uint8_t *wc[NM][NT], *ws[NM];
+  const size_t sat = mx_scale_off(nt0, 0, a.kt, lane);
+  ws[0] = a.ws + sat;
+  if constexpr (NM == 2) ws[1] = a.us + sat;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const size_t tile = (size_t)min(nt0 + t, a.nt - 1) * a.kt;
-    wc[0][t] = a.wc + tile * 1024 + lane * 16;
-    ws[0][t] = a.ws + tile * 64 + lane;
-    if constexpr (NM == 2) {
-      wc[1][t] = a.uc + tile * 1024 + lane * 16;
-      ws[1][t] = a.us + tile * 64 + lane;
-    }
+    const size_t at = (size_t)min(nt0 + t, a.nt - 1) * a.kt * 1024 + lane * 16;
+    wc[0][t] = a.wc + at;
+    if constexpr (NM == 2) wc[1][t] = a.uc + at;
   }
   f4 acc[NM][NT][MT] = {};
   // this wave's k tiles
   struct Tile {
     uint4 w[NM][NT];
-    uint32_t s[NM][NT];
+    uint32_t s[NM];
     typename X<KIND, MT>::Raw x;
   };
   auto load = [&](Tile& t, int kt) {
 #pragma unroll
-    for (int i = 0; i < NM; ++i)
+    for (int i = 0; i < NM; ++i) {
+      const uint8_t* s = ws[i] + (size_t)kt * 256;
+      t.s[i] = NT == 2 ? *reinterpret_cast<const uint16_t*>(s) : *s;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        t.w[i][n] = *reinterpret_cast<const uint4*>(wc[i][n] + (size_t)kt * 1024);
-        t.s[i][n] = ws[i][n][(size_t)kt * 64];
-      }
+      for (int n = 0; n < NT; ++n) t.w[i][n] = *reinterpret_cast<const uint4*>(wc[i][n] + (size_t)kt * 1024);
+    }
     xs.load(a, kt, lane, t.x);
   };
   auto products = [&](const Tile& t, int kt) {
     XFrag<FP4> x[MT];
     xs.frags(a, kt, lane, t.x, x);
 #pragma unroll
-    for (int i = 0; i < NM; ++i)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mma<MT>(t.w[i][n], t.s[i][n], x, acc[i][n]);
+    for (int i = 0; i < NM; ++i) {
+      mma<0, MT>(t.w[i][0], t.s[i], x, acc[i][0]);
+      if constexpr (NT == 2) mma<1, MT>(t.w[i][1], t.s[i], x, acc[i][1]);
+    }
   };
   const int k1 = (int)((long long)(wave + 1) * a.kt / kWaves);
   for (int kt = (int)((long long)wave * a.kt / kWaves); kt < k1; ++kt) {
@@ -266,7 +273,7 @@ void launch(const Args& a, int chunk, hipStream_t s) {
   Args b = a;
   for (long long r0 = 0; r0 < a.rows; r0 += b.rows) {
     b.rows = (int)std::min<long long>(a.rows - r0, (long long)chunk * 65535);
-    hipLaunchKernelGGL((few_kernel<KIND, MT, NT, EPI>), dim3((a.nt + NT - 1) / NT, (b.rows + chunk - 1) / chunk),
+    hipLaunchKernelGGL((few_kernel<KIND, MT, NT, EPI>), dim3((a.nt + 31) / 32 * (32 / NT), (b.rows + chunk - 1) / chunk),
                        dim3(64 * kWaves), 0, s, b, chunk, rows_vec(a.o));
     PGD_HIP(hipGetLastError());
     if constexpr (KIND == PLANES) {

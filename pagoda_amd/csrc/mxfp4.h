@@ -10,8 +10,10 @@
 //
 // Matrices: tiles of 16 rows by 128 columns, [row tile][k tile]. Lane l of a
 // wave owns row l % 16 and block l / 16 of a tile, which is what one lane feeds
-// the 16x16x128 scaled matrix instruction: codes [64 lanes][16 B], scales
-// [64 lanes][1 B]. Rows and columns of the last tiles past the matrix are zeros.
+// the 16x16x128 scaled matrix instruction: codes [64 lanes][16 B]. The scales of
+// four row tiles lie together, [row tile / 4][k tile][64 lanes][4 B]: a lane's four
+// bytes are one register, of which the instruction picks one. Rows and columns of
+// the last tiles past the matrix are zeros.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -29,7 +31,11 @@ constexpr int kMxBlock = 32, kMxTileN = 16, kMxTileK = 128;
 inline int mx_row_tiles(int n) { return (n + kMxTileN - 1) / kMxTileN; }
 inline int mx_k_tiles(int k) { return (k + kMxTileK - 1) / kMxTileK; }
 inline size_t mx_code_bytes(int n, int k) { return (size_t)mx_row_tiles(n) * mx_k_tiles(k) * 1024; }
-inline size_t mx_scale_bytes(int n, int k) { return (size_t)mx_row_tiles(n) * mx_k_tiles(k) * 64; }
+inline size_t mx_scale_bytes(int n, int k) { return (size_t)((mx_row_tiles(n) + 3) / 4) * mx_k_tiles(k) * 256; }
+// scale byte of lane `lane` of a tile
+__host__ __device__ inline size_t mx_scale_off(int row_tile, int k_tile, int kt, int lane) {
+  return (((size_t)(row_tile >> 2) * kt + k_tile) * 64 + lane) * 4 + (row_tile & 3);
+}
 
 // Row-major planes on the device.
 struct MxPlanes {

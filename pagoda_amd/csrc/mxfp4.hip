@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void tile_kernel(MxPlanes p, int n_out, int nb
     const int lane = (r & 15) + 16 * (b & 3);
     const uint4 c = *reinterpret_cast<const uint4*>(p.codes + (size_t)r * p.ldc + (size_t)b * 16);
     *reinterpret_cast<uint4*>(codes + tile * 1024 + lane * 16) = c;
-    scales[tile * 64 + lane] = p.scales[(size_t)r * p.lds + b];
+    scales[mx_scale_off(r >> 4, b >> 2, kt, lane)] = p.scales[(size_t)r * p.lds + b];
   }
 }
 
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict_
     const int lane = (r & 15) + 16 * (b & 3);
     const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + tile * 1024 + lane * 16 + (u & 3) * 4);
     float o[8];
-    fp4_unpack8(c, e8m0_f32(scales[tile * 64 + lane]), o);
+    fp4_unpack8(c, e8m0_f32(scales[mx_scale_off(r >> 4, b >> 2, kt, lane)]), o);
     float* d = out + (size_t)i * units * 8 + (size_t)u * 8;
     reinterpret_cast<float4*>(d)[0] = make_float4(o[0], o[1], o[2], o[3]);
     reinterpret_cast<float4*>(d)[1] = make_float4(o[4], o[5], o[6], o[7]);
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256) void digits_kernel(const void* __restrict__ x,
 #pragma unroll
   for (int k = 0; k < 6; ++k) {
     *reinterpret_cast<uint4*>(out + k * 1024) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
-    *reinterpret_cast<uint2*>(out + 6144 + (k >> 1) * 1024 + (k & 1) * 8) = make_uint2(q[k][4], q[k][5]);
+    *reinterpret_cast<uint2*>(out + 6144 + k * 512 - lane * 8) = make_uint2(q[k][4], q[k][5]);
   }
   ds[(size_t)tile * 64 + lane] = (uint8_t)e;
 }

@@ -73,19 +73,14 @@ __device__ inline void split_terms2(float (&v)[2], uint32_t (&t)[TERMS]) {
 // D[16 weight rows n][16 batch rows m]: lane l holds n = 4 (l / 16) + 0..3 of
 // m = l % 16. Lane l feeds row l % 16 of either side.
 __device__ inline f4 mfma_bf16(bf8 w, bf8 x, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0); }
-// 128 columns of fp4 codes, lane l block l / 16, with that block's scale bytes
-__device__ inline f4 mfma_fp4(uint4 w, uint32_t ws, uint4 x, uint32_t xs, f4 c) {
+// 128 columns of fp4 codes, lane l block l / 16, with those blocks' scales in byte
+// WB (XB) of ws (xs); the activations' codes fp4, or e2m3 in 24 bytes (X6).
+template <int WB, int XB, bool X6 = false>
+__device__ inline f4 mfma_fp4(uint4 w, uint32_t ws, i8v x, uint32_t xs, f4 c) {
   const i8v a = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
-  const i8v b = {(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, (int)ws, 0, (int)xs);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, c, 4, X6 ? 2 : 4, WB, (int)ws, XB, (int)xs);
 }
-
-// The same with the 32 e2m3 codes (24 bytes) of the lane's activation block.
-__device__ inline f4 mfma_fp4_fp6(uint4 w, uint32_t ws, uint4 lo, uint2 hi, uint32_t xs, f4 c) {
-  const i8v a = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
-  const i8v b = {(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 2, 0, (int)ws, 0, (int)xs);
-}
+__device__ inline i8v fp4_operand(uint4 x) { return (i8v){(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0}; }
 
 // (PART, PART2: sums of a range of k tiles, of one matrix or of the pair)
 enum { MX_STORE = 0, MX_RES = 1, MX_SWIGLU = 2, MX_PART = 3, MX_PART2 = 4 };
