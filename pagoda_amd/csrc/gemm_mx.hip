@@ -40,8 +40,6 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t to
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(uniform(to)), "v"(off), "s"(uniform(base)) : "memory");
 }
 
-enum { PLANES = 0, TERMS = 1, DIGITS = 2 };  // how the activations come (Args)
-
 template <int KIND_, int BM_, int BN_, int WM_, int WN_, int S_, int OCC_ = 1>
 struct Shape {
   static constexpr int KIND = KIND_;
@@ -51,15 +49,15 @@ struct Shape {
   // A wave's loads of a stage: NX of activations (XB bytes each, 4 or 16 a lane),
   // NL KiB of weight codes, NS times 256 B of weight scales (where there are
   // fewer than waves, several waves load the same bytes to the same place)
-  static constexpr int X = BM / 16 * (FP4 ? 1024 : DIG ? kMxDigitTile : 4096), XB = X / 1024 % W == 0 ? 1024 : 256, NX = X / XB / W;
+  static constexpr int X = BM / 16 * (FP4 ? 1024 : DIG ? kMxDigitTile : 4096), XB = DIG || X / 1024 % W == 0 ? 1024 : 256, XU = X / XB, NX = (XU + W - 1) / W;
   static constexpr int NL = BN / 16 / W, WS = BN / 64, NS = WS > W ? WS / W : 1, LOADS = NX + NL + NS + DIG;
   static constexpr int SC = X + BN * 64, DS = SC + BN * 4, BYTES = DS + (DIG ? BM * 4 : 0);
   // activation scales: every fourth stage brings those of 4 k tiles, 16 B of a
   // row, into the other of two slots behind the ring
   static constexpr int XS = FP4 ? (BM + 63) / 64 : 0, NXS = XS > W ? XS / W : 1;
   static constexpr int RING = S * BYTES, LDS = RING + 2 * XS * 1024;
-  static_assert((!FP4 || MF == 1 || MF % 2 == 0) && X / XB % W == 0 && BN / 16 % W == 0 && (WS <= W || WS % W == 0) && (XS <= W || XS % W == 0));
-  static_assert(S >= 2 && S <= (FP4 ? 5 : 8) && LDS * OCC <= 160 * 1024 && (!DIG || (BM <= 64 && XB == 1024)));
+  static_assert((!FP4 || MF == 1 || MF % 2 == 0) && (DIG || XU % W == 0) && BN / 16 % W == 0 && (WS <= W || WS % W == 0) && (XS <= W || XS % W == 0));
+  static_assert(S >= 2 && S <= (FP4 ? 5 : 8) && LDS * OCC <= 160 * 1024 && (!DIG || BM <= 64));
 };
 
 // f(0), .., f(N - 1) with constant arguments
@@ -108,7 +106,7 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
   uint32_t xo[T::NX], cut[T::NX];
 #pragma unroll
   for (int k = 0; k < T::NX; ++k) {
-    const int p = (wave * T::NX + k) * T::XB + lane * (T::XB / 64);
+    const int p = min(wave * T::NX + k, T::XU - 1) * T::XB + lane * (T::XB / 64);
     const int i = (p >> 6) & 15, part = ((p >> 4) & 3) ^ h(i >> 2);
     if constexpr (T::DIG) {  // whole tiles, as they lie
       const int f = p / kMxDigitTile;
@@ -177,7 +175,7 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
     const bool end = lk == a.kt - 1;
 #pragma unroll
     for (int k = 0; k < T::NX; ++k) {
-      const uint32_t to = st + (wave * T::NX + k) * T::XB;
+      const uint32_t to = st + min(wave * T::NX + k, T::XU - 1) * T::XB;
       uint32_t off = xo[k];
       if constexpr (T::FP4) off -= end ? cut[k] : 0;
       if constexpr (T::XB == 1024) dma16(xk, off, to);
@@ -511,33 +509,36 @@ using P0 = Shape<PLANES, 128, 256, 1, 4, 3, 2>;
 using P1 = Shape<PLANES, 128, 128, 2, 2, 4, 2>;
 using P2 = Shape<PLANES, 64, 128, 1, 4, 4, 2>;
 using P3 = Shape<PLANES, 32, 128, 1, 4, 5, 2>;
-using D0 = Shape<DIGITS, 64, 256, 2, 2, 3>;
-using D1 = Shape<DIGITS, 32, 128, 1, 2, 3, 2>;
 using T0 = Shape<TERMS, 64, 256, 1, 4, 2, 2>;
 using T1 = Shape<TERMS, 64, 128, 1, 4, 3, 2>;
 using T2 = Shape<TERMS, 32, 128, 1, 4, 4, 2>;
+using D0 = Shape<DIGITS, 32, 256, 1, 4, 2, 2>;
+using D1 = Shape<DIGITS, 32, 128, 2, 2, 3, 2>;
 
 // Microseconds of a launch, of a stage and of the rest of a block where a CU runs
 // two blocks and where it runs one, and of joining ranges (a launch, and each MB of
-// their sums). Least squares over 12 matrices from 300 x 8192 to 151936 x 896 with
-// 2..4000 rows, 1..24 ranges: 5% (bf16 terms) to 10% (planes) rms off.
+// their sums). Least squares over 11 matrices from 300 x 8192 to 151936 x 896 with
+// 2..4000 rows, 1..24 ranges: 4 to 8% rms off. What they choose takes 1.008 times the
+// fastest choice on the average of those, 1.19 at most.
 struct Cost {
   int bm, bn;
   float launch, stage2, block2, stage1, block1, join, mb;
 };
-constexpr Cost kPlanes[4] = {{128, 256, 5.46f, 0.987f, 3.91f, 0.628f, 2.24f, 2.35f, 0.265f},
-                             {128, 128, 4.89f, 0.593f, 3.38f, 0.410f, 0.83f, 2.73f, 0.274f},
-                             {64, 128, 4.18f, 0.403f, 1.76f, 0.298f, 0.22f, 2.95f, 0.314f},
-                             {32, 128, 2.36f, 0.401f, 1.86f, 0.243f, 1.61f, 3.25f, 0.279f}};
-constexpr Cost kTerms[3] = {{64, 256, 5.92f, 1.303f, 1.53f, 0.805f, 0.00f, 2.13f, 0.295f},
-                            {64, 128, 4.43f, 0.792f, 2.24f, 0.495f, 0.15f, 2.45f, 0.267f},
-                            {32, 128, 3.14f, 0.496f, 2.13f, 0.342f, 0.80f, 2.64f, 0.296f}};
+constexpr Cost kPlanes[] = {{128, 256, 6.45f, 0.995f, 3.90f, 0.630f, 2.13f, 1.66f, 0.269f},
+                            {128, 128, 5.46f, 0.595f, 3.80f, 0.403f, 0.88f, 2.15f, 0.272f},
+                            {64, 128, 4.93f, 0.396f, 2.17f, 0.293f, 0.07f, 2.52f, 0.299f},
+                            {32, 128, 3.60f, 0.360f, 2.47f, 0.256f, 1.24f, 2.56f, 0.310f}};
+constexpr Cost kTerms[] = {{64, 256, 6.22f, 1.311f, 1.13f, 0.813f, 0.00f, 1.85f, 0.282f},
+                           {64, 128, 5.00f, 0.809f, 2.22f, 0.518f, 0.11f, 2.08f, 0.249f},
+                           {32, 128, 3.63f, 0.512f, 2.19f, 0.382f, 0.61f, 2.38f, 0.281f}};
+constexpr Cost kDigits[] = {{32, 256, 6.56f, 1.218f, 2.22f, 0.796f, 0.78f, 2.19f, 0.293f},
+                            {32, 128, 5.73f, 0.757f, 2.58f, 0.526f, 1.24f, 2.14f, 0.278f}};
 
 double cost_us(const Cost& c, const Args& a, int splits) {
   const int pair = a.uc ? 2 : 1;
   const long long blocks = (long long)((a.rows + c.bm - 1) / c.bm) * ((a.nt * 16ll * pair + c.bn - 1) / c.bn) * splits;
   const long long per_cu = (blocks + 255) / 256;
-  const double stages = (a.kt + splits - 1) / splits * (a.p.codes ? 1 : a.terms);
+  const double stages = (a.kt + splits - 1) / splits * (a.kind == TERMS ? a.terms : 1);
   double us = c.launch + (double)(per_cu / 2) * (stages * c.stage2 + c.block2);
   if (per_cu % 2) us += stages * c.stage1 + c.block1;
   if (splits > 1) us += c.join + c.mb * 4e-6 * splits * a.rows * a.nt * 16.0 * pair;
@@ -548,20 +549,19 @@ double cost_us(const Cost& c, const Args& a, int splits) {
 
 Many plan_many(const Args& a, bool scratch) {
   Many best{0, 1, 1e30};
-  const int shapes = a.p.codes ? 4 : 3;
-  for (int i = 0; i < shapes; ++i) {
-    const Cost& c = a.p.codes ? kPlanes[i] : kTerms[i];
-    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24}) {
+  const Cost* costs = a.kind == PLANES ? kPlanes : a.kind == TERMS ? kTerms : kDigits;
+  const int shapes = a.kind == PLANES ? 4 : a.kind == TERMS ? 3 : 2;
+  for (int i = 0; i < shapes; ++i)
+    for (int splits : {1, 2, 3, 4, 6, 8, 10, 12, 16, 24}) {
       if (splits > 1 && (!scratch || splits * 2 > a.kt)) break;
-      const double us = cost_us(c, a, splits);
+      const double us = cost_us(costs[i], a, splits);
       if (us < best.us) best = Many{i, splits, us};
     }
-  }
   return best;
 }
 
 void run_many(const Args& a, const Many& m, hipStream_t s) {
-  if (a.p.codes) {
+  if (a.kind == PLANES) {
     switch (m.shape) {
       case 0: return launch<P0>(a, m.splits, s);
       case 1: return launch<P1>(a, m.splits, s);
@@ -569,7 +569,7 @@ void run_many(const Args& a, const Many& m, hipStream_t s) {
       default: return launch<P3>(a, m.splits, s);
     }
   }
-  if (a.d) return launch<D0>(a, m.splits, s);
+  if (a.kind == DIGITS) return m.shape == 0 ? launch<D0>(a, m.splits, s) : launch<D1>(a, m.splits, s);
   switch (m.shape) {
     case 0: return launch<T0>(a, m.splits, s);
     case 1: return launch<T1>(a, m.splits, s);

@@ -22,9 +22,8 @@ namespace {
 
 constexpr int kWaves = 8;
 
-// How a launch holds its activations: planes, bf16 terms, or (at most 16 terms of
-// rows, k of any multiple of 32) rows of an XType, which the kernel splits itself.
-enum { PLANES = 0, TERMS = 1, ROWS = 2 };  // ROWS + XType
+// (KIND: PLANES, TERMS, or ROWS + XType for rows the launch splits itself: at most 16
+// terms of rows, k any multiple of 32)
 
 // One k tile of a batch row tile, as the matrix instructions take it.
 template <bool FP4>
@@ -323,24 +322,24 @@ bool few_split_pays(const Args& a, int type) {
 // activation tiles; per k tile, and row of terms of it (1..4 row tiles of rows).
 // Fitted with the costs in gemm_mx.hip: 10 to 15% rms off.
 double few_us(const Args& a) {
-  static constexpr float kPlanes[4][6] = {{5.17f, 0.088f, 0.0239f, 0.00015f, 0.0f, 0.0016f},
-                                          {4.41f, 0.333f, 0.0107f, 0.0015f, 0.023f, 0.0019f},
-                                          {3.87f, 0.392f, 0.0134f, 0.0018f, 0.0f, 0.0030f},
-                                          {3.45f, 0.511f, 0.0312f, 0.0015f, 0.0f, 0.0029f}};
-  static constexpr float kTerms[4][6] = {{4.42f, 0.214f, 0.0176f, 0.0037f, 0.012f, 0.0033f},
-                                         {3.70f, 0.478f, 0.0087f, 0.0060f, 0.029f, 0.0041f},
-                                         {3.06f, 0.180f, 0.0f, 0.0071f, 0.0f, 0.0052f},
-                                         {2.84f, 0.516f, 0.0f, 0.0053f, 0.0f, 0.0051f}};
-  const int terms = a.p.codes ? 1 : a.terms, chunk = std::min(a.rows, 64 / terms), x = chunk * terms, mt = (x + 15) / 16;
+  static constexpr float kPlanes[4][6] = {{5.16f, 0.066f, 0.0257f, 0.00017f, 0.0005f, 0.0020f},
+                                          {4.54f, 0.296f, 0.0188f, 0.0013f, 0.020f, 0.0024f},
+                                          {4.04f, 0.384f, 0.0173f, 0.0018f, 0.0f, 0.0032f},
+                                          {3.75f, 0.425f, 0.0333f, 0.0016f, 0.0f, 0.0029f}};
+  static constexpr float kTerms[4][6] = {{4.28f, 0.223f, 0.0171f, 0.0039f, 0.019f, 0.0033f},
+                                         {3.64f, 0.497f, 0.0179f, 0.0047f, 0.047f, 0.0038f},
+                                         {3.15f, 0.142f, 0.0f, 0.0072f, 0.0f, 0.0053f},
+                                         {3.45f, 0.400f, 0.0f, 0.0060f, 0.0f, 0.0050f}};
+  const int terms = a.kind == PLANES ? 1 : a.terms, chunk = std::min(a.rows, 64 / terms), x = chunk * terms, mt = (x + 15) / 16;
   const int tiles = a.uc ? 1 : mt > 2 ? 1 : 2;
   const double wg = (double)((a.nt + tiles - 1) / tiles) * ((a.rows + chunk - 1) / chunk) / 256.0;
-  const float* c = a.p.codes ? kPlanes[mt - 1] : kTerms[mt - 1];
+  const float* c = a.kind == PLANES ? kPlanes[mt - 1] : kTerms[mt - 1];
   return c[0] + wg * (c[1] + a.kt * (c[2] * tiles * (a.uc ? 2 : 1) + c[3] * x)) + a.kt * (c[4] + c[5] * x);
 }
 
 void run_few(const Args& a, hipStream_t s) {
-  if (a.p.codes) return launch_rows<PLANES>(a, s);
-  if (a.x) return launch_rows<TERMS>(a, s);
+  if (a.kind == PLANES) return launch_rows<PLANES>(a, s);
+  if (a.kind == TERMS) return launch_rows<TERMS>(a, s);
   switch (a.raw_type) {
     case X_F32: return launch_epi<ROWS + X_F32, 1>(a, a.rows, s);
     case X_F16: return launch_epi<ROWS + X_F16, 1>(a, a.rows, s);

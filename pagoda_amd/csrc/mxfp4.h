@@ -69,16 +69,22 @@ namespace mx {
 
 constexpr int kMxDigitTile = 9216;  // 6 digits of 24 B a lane
 
-// One product launch. Activation rows are planes (codes set), bf16 terms (x set:
-// row r is the sum over t < terms of the bf16 rows x[t * term_stride + r * ldx]),
-// raw, rows of an XType with stride ldx (few_split_ok of them), or digits (d, ds
-// set): tiles of 16 rows by 128 columns, kMxDigitTile bytes of e2m3 codes and 64
-// block exponents each, [row tile][k tile].
+// How a launch holds its activation rows:
+//   PLANES  p: the MXFP4 planes
+//   TERMS   x: row r is the sum over t < terms of the bf16 rows
+//           x[t * term_stride + r * ldx], of whole 128-column tiles
+//   DIGITS  d, ds: six base-32 digits (mxfp4.hip), in tiles of 16 rows by 128
+//           columns, [row tile][k tile]: kMxDigitTile bytes of e2m3 codes, 64 scales
+//   ROWS    raw: rows of an XType with stride ldx, split by the launch itself
+enum Kind : int { PLANES = 0, TERMS = 1, DIGITS = 2, ROWS = 3 };
+
+// One product launch.
 struct Args {
   const uint8_t *wc, *ws;  // matrix codes, scales
   const uint8_t *uc, *us;  // the up matrix's (SwiGLU), or null
   int n_out, nt, kt, nblk;  // outputs; row tiles, k tiles, 32-element blocks of a row
   int rows;
+  Kind kind;
   MxPlanes p;
   const uint16_t* x;
   size_t ldx, term_stride;
@@ -93,14 +99,14 @@ struct Args {
   size_t part_stride;
 };
 
-// A few rows (gemv_mx.hip): in 64-row (of terms) chunks, its estimated
-// microseconds; whether it can split a.rows rows of a type itself, and whether
-// that beats splitting them first.
+// A few rows (gemv_mx.hip; planes, terms or rows): in 64-row (of terms) chunks, its
+// estimated microseconds; whether it can split that many rows of a type itself, and
+// whether that beats splitting them first.
 void run_few(const Args& a, hipStream_t s);
 double few_us(const Args& a);
 bool few_split_ok(int rows, int type);
 bool few_split_pays(const Args& a, int type);
-// Many rows (gemm_mx.hip): the block shape and ranges of k tiles estimated
+// Many rows (gemm_mx.hip; planes, terms or digits): the block shape and ranges of k tiles estimated
 // fastest (more than one range only if scratch memory may be used).
 struct Many {
   int shape, splits;

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
   }
 }
 
-// Rows in six base-32 digits. A block with largest magnitude below 2^(e - 126) (e
+// f32 rows in six base-32 digits. A block with largest magnitude below 2^(e - 126) (e
 // the biased exponent, 25 at least) is held in steps of 2^(e - 155): 30 bits, so
 // its values are exact to the last of their 24 where they are above 1/64 of the
 // largest, and within 2^-30 of it elsewhere (f32 sums of its products keep 24).
@@ -153,8 +153,7 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
 // code u up to 16), digit i scaled by 2^(e - 127 - 5 i). A wave takes one tile of 16
 // rows by 128 columns, lane l block l / 16 of row l % 16. A block with an infinity
 // or NaN is NaN. Rows and columns past the matrix are zeros.
-template <int TYPE>
-__global__ __launch_bounds__(256) void digits_kernel(const void* __restrict__ x, int ldx, int rows, int nblk, int kt,
+__global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x, int ldx, int rows, int nblk, int kt,
                                                      long long tiles, uint8_t* __restrict__ d,
                                                      uint8_t* __restrict__ ds) {
   const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -164,7 +163,7 @@ __global__ __launch_bounds__(256) void digits_kernel(const void* __restrict__ x,
   float v[4][8] = {};
   if (row < rows && b < nblk) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load8<TYPE>(x, (size_t)row * ldx + (size_t)b * kMxBlock + j * 8, v[j]);
+    for (int j = 0; j < 4; ++j) load8<X_F32>(x, (size_t)row * ldx + (size_t)b * kMxBlock + j * 8, v[j]);
   }
   uint32_t top = 0;
 #pragma unroll
@@ -223,15 +222,26 @@ bool scratch_allowed(hipStream_t s) {
   return cap == hipStreamCaptureStatusNone;
 }
 
-void run(const Args& a, bool scratch, hipStream_t s) {
+// The plan of a launch: few, or many with their plan.
+struct Plan {
+  bool few;
+  Many many;
+  double us() const { return many.us; }
+};
+Plan plan(const Args& a, bool scratch) {
   // (the many-row kernel's lanes hold offsets in 128 rows, and 16 row tiles of the matrix, in 32 bits)
-  const size_t stride = a.p.codes ? std::max(a.p.ldc, a.p.lds) : a.ldx * 2;
-  const bool near = stride < ((size_t)1 << 24);
-  if (near) {
-    const Many m = plan_many(a, scratch);
-    if (m.us < few_us(a)) return run_many(a, m, s);
-  }
-  run_few(a, s);
+  const size_t stride = a.kind == PLANES ? std::max(a.p.ldc, a.p.lds) : a.ldx * 2;
+  Plan p{true, Many{0, 1, 1e30}};
+  if (a.kind == DIGITS || stride < ((size_t)1 << 24)) p = Plan{false, plan_many(a, scratch)};
+  if (a.kind == DIGITS) return p;
+  const double few = few_us(a);
+  if (few <= p.many.us) p = Plan{true, Many{0, 1, few}};
+  return p;
+}
+
+void run(const Args& a, const Plan& p, hipStream_t s) {
+  if (p.few) run_few(a, s);
+  else run_many(a, p.many, s);
 }
 
 void check(const QMat& w, const QMat* up, int rows) {
@@ -284,14 +294,16 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   if (rows == 0) return;
   Args a = make_args(w, up, rows, o);
   a.terms = type == X_F32 ? 3 : type == X_F16 ? 2 : 1;
+  a.kind = TERMS;
   const bool scratch = scratch_allowed(s);
   if (type == X_BF16 && w.n_in % kMxTileK == 0) {  // the rows are their own term
     a.x = static_cast<const uint16_t*>(x);
     a.ldx = ldx;
-    run(a, scratch, s);
+    run(a, plan(a, scratch), s);
     return;
   }
   if (few_split_pays(a, type) || (!scratch && few_split_ok(rows, type))) {
+    a.kind = ROWS;
     a.raw = x;
     a.raw_type = type;
     a.ldx = ldx;
@@ -301,36 +313,39 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   PGD_CHECK(scratch, kErrState,
             "splitting these MXFP4 activation rows needs scratch memory: under capture, at most 5 f32, 8 f16 or 4 bf16 "
             "rows, any bf16 rows of whole 128-column tiles, or MXFP4 rows");
+  const int ldt = a.kt * kMxTileK;
+  a.ldx = ldt;
+  Plan p = plan(a, true);
+  if (type == X_F32 && rows > 16) {
+    // digits: 8.5 bytes of each value read and written instead of 10, and half the matrix instructions' time
+    Args d = a;
+    d.kind = DIGITS;
+    const Plan pd = plan(d, true);
+    if (pd.us() + 8.5 / 4.5e6 * rows * ldt < p.us() + 10 / 4.5e6 * rows * ldt) a = d, p = pd;
+  }
   std::lock_guard<std::mutex> lock(g_terms);
-  if (type != X_BF16 && rows > 64) {
+  if (a.kind == DIGITS) {
     const long long tiles = (long long)((rows + 15) / 16) * a.kt;
     auto* d = static_cast<uint8_t*>(gemv::gemv_scratch(s, (size_t)tiles * (kMxDigitTile + 64), 8));
+    auto* ds = d + (size_t)tiles * kMxDigitTile;
     a.d = d;
-    a.ds = d + (size_t)tiles * kMxDigitTile;
+    a.ds = ds;
+    hipLaunchKernelGGL(digits_kernel, dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, s, static_cast<const float*>(x), ldx,
+                       rows, a.nblk, a.kt, tiles, d, ds);
+  } else {
+    a.term_stride = (size_t)rows * ldt;
+    auto* t = static_cast<uint16_t*>(gemv::gemv_scratch(s, a.terms * a.term_stride * sizeof(uint16_t), 8));
+    a.x = t;
+    const RowGrid g(ldt / 8, rows);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, s, x, ldx, rows, a.nblk, a.kt, tiles, d,
-                         d + (size_t)tiles * kMxDigitTile);
+      hipLaunchKernelGGL(kernel, g.grid, g.block, 0, s, x, ldx, rows, w.n_in / 8, t, ldt, a.term_stride);
     };
-    if (type == X_F32) go(digits_kernel<X_F32>);
-    else go(digits_kernel<X_F16>);
-    PGD_HIP(hipGetLastError());
-    run_many(a, plan_many(a, true), s);
-    return;
+    if (type == X_F32) go(terms_kernel<X_F32, 3>);
+    else if (type == X_F16) go(terms_kernel<X_F16, 2>);
+    else go(terms_kernel<X_BF16, 1>);
   }
-  const int ldt = a.kt * kMxTileK;
-  a.term_stride = (size_t)rows * ldt;
-  auto* t = static_cast<uint16_t*>(gemv::gemv_scratch(s, a.terms * a.term_stride * sizeof(uint16_t), 8));
-  a.x = t;
-  a.ldx = ldt;
-  const RowGrid g(ldt / 8, rows);
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, g.grid, g.block, 0, s, x, ldx, rows, w.n_in / 8, t, ldt, a.term_stride);
-  };
-  if (type == X_F32) go(terms_kernel<X_F32, 3>);
-  else if (type == X_F16) go(terms_kernel<X_F16, 2>);
-  else go(terms_kernel<X_BF16, 1>);
   PGD_HIP(hipGetLastError());
-  run(a, true, s);
+  run(a, p, s);
 }
 
 void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, const MxOut& o, hipStream_t s) {
@@ -338,7 +353,8 @@ void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, 
   if (rows == 0) return;
   Args a = make_args(w, up, rows, o);
   a.p = x;
-  run(a, scratch_allowed(s), s);
+  a.kind = PLANES;
+  run(a, plan(a, scratch_allowed(s)), s);
 }
 
 }  // namespace pgd

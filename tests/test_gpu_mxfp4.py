@@ -267,8 +267,8 @@ def test_rows_enter_exactly(dev, buf, t, rows):
 @pytest.mark.parametrize("rows", [1, 30, 200])
 def test_nonfinite_stays_in_its_row_and_column(dev, buf, rows):
     """A NaN or infinity among a row's values makes that row's outputs non-finite (NaN for a
-    NaN; an infinity keeps its sign in few rows and in bf16, and is a NaN in many rows of f32
-    or f16), a NaN block of weights its output's; no other row or output."""
+    NaN; an infinity keeps its sign in f16, bf16 and few f32 rows, and may be a NaN in many f32
+    rows), a NaN block of weights its output's; no other row or output."""
     rng = np.random.default_rng(rows)
     n, k = 100, 160
     codes, scales = weights(rng, n, k)
@@ -288,7 +288,7 @@ def test_nonfinite_stays_in_its_row_and_column(dev, buf, rows):
         got = run_rows(dev, buf, m, raw, t)
         live = [c for c in range(n) if c != 17]
         assert np.isnan(got[:, 17]).all()
-        assert (got[0, live] == np.inf).all() if rows <= 64 or t == BF16 else np.isnan(got[0, live]).all()
+        assert (got[0, live] == np.inf).all() or (t == F32 and rows > 16 and np.isnan(got[0, live]).all())
         if rows > 1:
             assert np.isnan(got[rows - 1]).all()
         mid = slice(1, rows - 1)
