@@ -137,7 +137,7 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
   for (int k = 0; k < T::NL; ++k) {
     bool up;
     const size_t nt = tile_of(wave * T::NL + k, up);
-    wb[k] = (up ? a.uc : a.wc) + (nt * a.kt + k0) * 1024;
+    wb[k] = (up ? a.up : a.w) + mx_code_off((int)nt, k0, a.kt);
   }
   // weight scales, 4 row tiles a load: the gate's of the workgroup, then the up matrix's
 #pragma unroll
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
     const int u = (wave * T::NS + k) % T::WS;
     const bool up = DUAL && u >= NB / 4;
     const size_t g = min(nt0 / 4 + (up ? u - NB / 4 : u), (a.nt - 1) / 4);
-    sb[k] = (up ? a.us : a.ws) + (g * a.kt + k0) * 256;
+    sb[k] = (up ? a.up : a.w) + mx_scale_off((int)g * 4, k0, a.kt, 0);
   }
   const uint32_t wso = lane * 4;
   const uint8_t* xsb = a.p.scales + (T::FP4 ? (size_t)m0 * a.p.lds : 0);
@@ -200,9 +200,9 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
     }
     lk += more;
 #pragma unroll
-    for (int k = 0; k < T::NL; ++k) wb[k] += more * 1024;
+    for (int k = 0; k < T::NL; ++k) wb[k] += more * kMxStep;
 #pragma unroll
-    for (int k = 0; k < T::NS; ++k) sb[k] += more * 256;
+    for (int k = 0; k < T::NS; ++k) sb[k] += more * kMxStep;
   };
 
   f4 acc[NF][MF] = {};
@@ -483,17 +483,17 @@ template <class T>
 void launch(Args a, int splits, hipStream_t s) {
   a.splits = splits;
   if (splits == 1) {
-    if (a.uc) launch_blocks<T, MX_SWIGLU>(a, s);
+    if (a.up) launch_blocks<T, MX_SWIGLU>(a, s);
     else if (a.o.res) launch_blocks<T, MX_RES>(a, s);
     else launch_blocks<T, MX_STORE>(a, s);
     return;
   }
   std::lock_guard<std::mutex> lock(g_part);
-  a.part_stride = (size_t)(a.uc ? 2 : 1) * a.rows * a.nt * 16;
+  a.part_stride = (size_t)(a.up ? 2 : 1) * a.rows * a.nt * 16;
   a.part = static_cast<float*>(gemv::gemv_scratch(s, splits * a.part_stride * sizeof(float), 9));
   const dim3 grid((a.nt * 4 + 255) / 256, std::min(a.rows, 65535));
   auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, rows_vec(a.o)); };
-  if (a.uc) {
+  if (a.up) {
     launch_blocks<T, MX_PART2>(a, s);
     join(join_kernel<MX_SWIGLU>);
   } else {
@@ -535,7 +535,7 @@ constexpr Cost kDigits[] = {{32, 256, 6.56f, 1.218f, 2.22f, 0.796f, 0.78f, 2.19f
                             {32, 128, 5.73f, 0.757f, 2.58f, 0.526f, 1.24f, 2.14f, 0.278f}};
 
 double cost_us(const Cost& c, const Args& a, int splits) {
-  const int pair = a.uc ? 2 : 1;
+  const int pair = a.up ? 2 : 1;
   const long long blocks = (long long)((a.rows + c.bm - 1) / c.bm) * ((a.nt * 16ll * pair + c.bn - 1) / c.bn) * splits;
   const long long per_cu = (blocks + 255) / 256;
   const double stages = (a.kt + splits - 1) / splits * (a.kind == TERMS ? a.terms : 1);

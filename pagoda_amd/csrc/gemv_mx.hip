@@ -1,11 +1,11 @@
 // gemv_mx.hip — MXFP4 products of a few rows.
 //
-// A workgroup of 8 waves owns NT row tiles of the matrix (of both matrices for
-// the gate/up pair) and up to MT 16-row tiles of batch rows; its waves split
-// the k tiles into 8 contiguous ranges, so a tile's weights (1 KiB of codes and
-// 64 B of scales per k tile) are read once, in lane order, straight into the
-// registers that feed the matrix instructions. The ranges' sums meet in LDS and
-// are added in range order, so results do not depend on timing.
+// A workgroup owns NT row tiles of the matrix (of both matrices for the gate/up
+// pair) and up to MT 16-row tiles of batch rows; its KW waves take the k tiles in
+// turn, so a tile's weights (1 KiB of codes and 64 B of scales per k tile) are read
+// once, in lane order, straight into the registers that feed the matrix
+// instructions. The waves' sums meet in LDS and are added in wave order, so results
+// do not depend on timing.
 //
 // Activation rows held as several bf16 terms take one matrix row per term and
 // batch row (term t of row r is row t * rows + r), and the terms' sums are added
@@ -19,8 +19,6 @@
 namespace pgd {
 namespace mx {
 namespace {
-
-constexpr int kWaves = 8;
 
 // (KIND: PLANES, TERMS, or ROWS + XType for rows the launch splits itself: at most 16
 // terms of rows, k any multiple of 32)
@@ -168,13 +166,13 @@ __device__ inline void mma(uint4 w, uint32_t ws, const XFrag<false> (&x)[MT], f4
   }
 }
 
-template <int KIND, int MT, int NT, int EPI>
-__global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, bool vec) {
+template <int KIND, int MT, int NT, int EPI, int KW>
+__global__ __launch_bounds__(64 * KW) void few_kernel(Args a, int chunk, bool vec) {
   constexpr int NM = EPI == MX_SWIGLU ? 2 : 1;  // matrices
   constexpr bool FP4 = KIND == PLANES;
   __shared__ union {
-    f4 part[kWaves][NM][NT][MT][64];
-    uint8_t x[kWaves][KIND >= ROWS ? 4096 : 16];
+    f4 part[KW][NM][NT][MT][64];
+    uint8_t x[KW][KIND >= ROWS ? 4096 : 16];
   } lds;
   auto& part = lds.part;
   // this workgroup's batch rows
@@ -197,13 +195,13 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, boo
   // (the scales of NT row tiles are neighbouring bytes)
   const uint8_t *wc[NM][NT], *ws[NM];
   const size_t sat = mx_scale_off(nt0, 0, a.kt, lane);
-  ws[0] = a.ws + sat;
-  if constexpr (NM == 2) ws[1] = a.us + sat;
+  ws[0] = a.w + sat;
+  if constexpr (NM == 2) ws[1] = a.up + sat;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const size_t at = (size_t)min(nt0 + t, a.nt - 1) * a.kt * 1024 + lane * 16;
-    wc[0][t] = a.wc + at;
-    if constexpr (NM == 2) wc[1][t] = a.uc + at;
+    const size_t at = mx_code_off(min(nt0 + t, a.nt - 1), 0, a.kt) + lane * 16;
+    wc[0][t] = a.w + at;
+    if constexpr (NM == 2) wc[1][t] = a.up + at;
   }
   f4 acc[NM][NT][MT] = {};
   // this wave's k tiles
@@ -215,10 +213,10 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, boo
   auto load = [&](Tile& t, int kt) {
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
-      const uint8_t* s = ws[i] + (size_t)kt * 256;
+      const uint8_t* s = ws[i] + (size_t)kt * kMxStep;
       t.s[i] = NT == 2 ? *reinterpret_cast<const uint16_t*>(s) : *s;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) t.w[i][n] = *reinterpret_cast<const uint4*>(wc[i][n] + (size_t)kt * 1024);
+      for (int n = 0; n < NT; ++n) t.w[i][n] = *reinterpret_cast<const uint4*>(wc[i][n] + (size_t)kt * kMxStep);
     }
     xs.load(a, kt, lane, t.x);
   };
@@ -231,11 +229,15 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, boo
       if constexpr (NT == 2) mma<1, MT>(t.w[i][1], t.s[i], x, acc[i][1]);
     }
   };
-  const int k1 = (int)((long long)(wave + 1) * a.kt / kWaves);
-  for (int kt = (int)((long long)wave * a.kt / kWaves); kt < k1; ++kt) {
-    Tile t;
-    load(t, kt);
-    products(t, kt);
+  // (two k tiles' loads together measured 8% faster for one row of f32, 3% slower for planes)
+  constexpr int U = MT == 1 && !FP4 ? 2 : 1;
+  for (int kt = wave; kt < a.kt; kt += U * KW) {
+    Tile t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(t[u], min(kt + u * KW, a.kt - 1));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u == 0 || kt + u * KW < a.kt) products(t[u], kt + u * KW);
   }
   if constexpr (KIND >= ROWS) __syncthreads();  // (the sums take the place of the activations)
 #pragma unroll
@@ -245,15 +247,15 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(Args a, int chunk, boo
 #pragma unroll
       for (int m = 0; m < MT; ++m) part[wave][i][t][m][lane] = acc[i][t][m];
   __syncthreads();
-  // four outputs of one row per thread: ranges in order, terms in order
+  // four outputs of one row per thread: waves in order, terms in order
   const int terms = FP4 ? 1 : a.terms;
-  for (int o = threadIdx.x; o < NT * 4 * a.rows; o += 64 * kWaves) {
+  for (int o = threadIdx.x; o < NT * 4 * a.rows; o += 64 * KW) {
     const int t = o / (4 * a.rows), rem = o - t * 4 * a.rows, nq = rem / a.rows, r = rem - nq * a.rows;
     f4 v[NM] = {};
     for (int term = 0; term < terms; ++term) {
       const int m = term * a.rows + r;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w)
+      for (int w = 0; w < KW; ++w)
 #pragma unroll
         for (int i = 0; i < NM; ++i) v[i] += part[w][i][t][m >> 4][nq * 16 + (m & 15)];
     }
@@ -272,8 +274,13 @@ void launch(const Args& a, int chunk, hipStream_t s) {
   Args b = a;
   for (long long r0 = 0; r0 < a.rows; r0 += b.rows) {
     b.rows = (int)std::min<long long>(a.rows - r0, (long long)chunk * 65535);
-    hipLaunchKernelGGL((few_kernel<KIND, MT, NT, EPI>), dim3((a.nt + 31) / 32 * (32 / NT), (b.rows + chunk - 1) / chunk),
-                       dim3(64 * kWaves), 0, s, b, chunk, rows_vec(a.o));
+    const dim3 grid((a.nt + 31) / 32 * (32 / NT), (b.rows + chunk - 1) / chunk);
+    auto go = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, b, chunk, rows_vec(a.o)); };
+    // (one f32 row, 1088 pairs of row tiles: 20.4 us with 4 waves, 22.2 with 8; 8 MXFP4
+    // rows, 160 workgroups: 16.2 with 4, 11.1 with 8)
+    const bool wide = (long long)(a.nt + NT - 1) / NT * grid.y >= 512;
+    if (wide) go(few_kernel<KIND, MT, NT, EPI, 4>, 4);
+    else go(few_kernel<KIND, MT, NT, EPI, 8>, 8);
     PGD_HIP(hipGetLastError());
     if constexpr (KIND == PLANES) {
       b.p.codes += (size_t)b.rows * b.p.ldc;
@@ -288,7 +295,7 @@ void launch(const Args& a, int chunk, hipStream_t s) {
 
 template <int KIND, int MT>
 void launch_epi(const Args& a, int chunk, hipStream_t s) {
-  if (a.uc) launch<KIND, MT, MX_SWIGLU>(a, chunk, s);
+  if (a.up) launch<KIND, MT, MX_SWIGLU>(a, chunk, s);
   else if (a.o.res) launch<KIND, MT, MX_RES>(a, chunk, s);
   else launch<KIND, MT, MX_STORE>(a, chunk, s);
 }
@@ -314,8 +321,8 @@ void launch_rows(const Args& a, hipStream_t s) {
 bool few_split_ok(int rows, int type) { return rows <= (type == X_F32 ? 5 : type == X_F16 ? 8 : 4); }
 bool few_split_pays(const Args& a, int type) {
   const int terms = type == X_F32 ? 3 : type == X_F16 ? 2 : 1;
-  return few_split_ok(a.rows, type) && (a.uc ? a.nt : (a.nt + 1) / 2) <= 1280 &&
-         (a.kt + kWaves - 1) / kWaves * (0.05 + 0.03 * a.rows * terms) <= 2.2;
+  return few_split_ok(a.rows, type) && (a.up ? a.nt : (a.nt + 1) / 2) <= 1280 &&
+         (a.kt + 7) / 8 * (0.05 + 0.03 * a.rows * terms) <= 2.2;
 }
 
 // Microseconds of a launch; per 256 workgroups, their weight tiles and their
@@ -331,10 +338,10 @@ double few_us(const Args& a) {
                                          {3.15f, 0.142f, 0.0f, 0.0072f, 0.0f, 0.0053f},
                                          {3.45f, 0.400f, 0.0f, 0.0060f, 0.0f, 0.0050f}};
   const int terms = a.kind == PLANES ? 1 : a.terms, chunk = std::min(a.rows, 64 / terms), x = chunk * terms, mt = (x + 15) / 16;
-  const int tiles = a.uc ? 1 : mt > 2 ? 1 : 2;
+  const int tiles = a.up ? 1 : mt > 2 ? 1 : 2;
   const double wg = (double)((a.nt + tiles - 1) / tiles) * ((a.rows + chunk - 1) / chunk) / 256.0;
   const float* c = a.kind == PLANES ? kPlanes[mt - 1] : kTerms[mt - 1];
-  return c[0] + wg * (c[1] + a.kt * (c[2] * tiles * (a.uc ? 2 : 1) + c[3] * x)) + a.kt * (c[4] + c[5] * x);
+  return c[0] + wg * (c[1] + a.kt * (c[2] * tiles * (a.up ? 2 : 1) + c[3] * x)) + a.kt * (c[4] + c[5] * x);
 }
 
 void run_few(const Args& a, hipStream_t s) {

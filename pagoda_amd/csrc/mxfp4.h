@@ -8,12 +8,13 @@
 // Planes (activations, and what a matrix is made of): codes [rows][ldc bytes],
 // element 2 i of a row in the low nibble of byte i, and scales [rows][lds bytes].
 //
-// Matrices: tiles of 16 rows by 128 columns, [row tile][k tile]. Lane l of a
-// wave owns row l % 16 and block l / 16 of a tile, which is what one lane feeds
-// the 16x16x128 scaled matrix instruction: codes [64 lanes][16 B]. The scales of
-// four row tiles lie together, [row tile / 4][k tile][64 lanes][4 B]: a lane's four
-// bytes are one register, of which the instruction picks one. Rows and columns of
-// the last tiles past the matrix are zeros.
+// Matrices: tiles of 16 rows by 128 columns. Lane l of a wave owns row l % 16 and
+// block l / 16 of a tile, which is what one lane feeds the 16x16x128 scaled matrix
+// instruction: 16 B of codes. Four row tiles and their scales lie together as one
+// step of [row tile / 4][k tile]: codes [4][64 lanes][16 B], then scales [64 lanes]
+// [4 B], a lane's four bytes one register of which the instruction picks one. So
+// 64 rows stream through memory as one run of 4352 B steps. Rows and columns of the
+// last tiles past the matrix are zeros.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -30,11 +31,14 @@ constexpr int kMxBlock = 32, kMxTileN = 16, kMxTileK = 128;
 
 inline int mx_row_tiles(int n) { return (n + kMxTileN - 1) / kMxTileN; }
 inline int mx_k_tiles(int k) { return (k + kMxTileK - 1) / kMxTileK; }
-inline size_t mx_code_bytes(int n, int k) { return (size_t)mx_row_tiles(n) * mx_k_tiles(k) * 1024; }
-inline size_t mx_scale_bytes(int n, int k) { return (size_t)((mx_row_tiles(n) + 3) / 4) * mx_k_tiles(k) * 256; }
-// scale byte of lane `lane` of a tile
+constexpr int kMxStep = 4352, kMxStepScales = 4096;
+inline size_t mx_bytes(int n, int k) { return (size_t)((mx_row_tiles(n) + 3) / 4) * mx_k_tiles(k) * kMxStep; }
+// codes of lane 0 of a tile, and the scale byte of lane `lane` of it
+__host__ __device__ inline size_t mx_code_off(int row_tile, int k_tile, int kt) {
+  return ((size_t)(row_tile >> 2) * kt + k_tile) * kMxStep + (row_tile & 3) * 1024;
+}
 __host__ __device__ inline size_t mx_scale_off(int row_tile, int k_tile, int kt, int lane) {
-  return (((size_t)(row_tile >> 2) * kt + k_tile) * 64 + lane) * 4 + (row_tile & 3);
+  return ((size_t)(row_tile >> 2) * kt + k_tile) * kMxStep + kMxStepScales + lane * 4 + (row_tile & 3);
 }
 
 // Row-major planes on the device.
@@ -80,8 +84,7 @@ enum Kind : int { PLANES = 0, TERMS = 1, DIGITS = 2, ROWS = 3 };
 
 // One product launch.
 struct Args {
-  const uint8_t *wc, *ws;  // matrix codes, scales
-  const uint8_t *uc, *us;  // the up matrix's (SwiGLU), or null
+  const uint8_t *w, *up;  // the matrix, and the up matrix (SwiGLU) or null
   int n_out, nt, kt, nblk;  // outputs; row tiles, k tiles, 32-element blocks of a row
   int rows;
   Kind kind;

@@ -88,33 +88,29 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ 
 }
 
 // One block (16 code bytes and its scale) per thread into its place in the tiles.
-__global__ __launch_bounds__(256) void tile_kernel(MxPlanes p, int n_out, int nblk, int kt, uint8_t* __restrict__ codes,
-                                                   uint8_t* __restrict__ scales) {
+__global__ __launch_bounds__(256) void tile_kernel(MxPlanes p, int n_out, int nblk, int kt, uint8_t* __restrict__ w) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= nblk) return;
   const int step = gridDim.y * blockDim.y;
   for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < n_out; r += step) {
-    const size_t tile = (size_t)(r >> 4) * kt + (b >> 2);
     const int lane = (r & 15) + 16 * (b & 3);
     const uint4 c = *reinterpret_cast<const uint4*>(p.codes + (size_t)r * p.ldc + (size_t)b * 16);
-    *reinterpret_cast<uint4*>(codes + tile * 1024 + lane * 16) = c;
-    scales[mx_scale_off(r >> 4, b >> 2, kt, lane)] = p.scales[(size_t)r * p.lds + b];
+    *reinterpret_cast<uint4*>(w + mx_code_off(r >> 4, b >> 2, kt) + lane * 16) = c;
+    w[mx_scale_off(r >> 4, b >> 2, kt, lane)] = p.scales[(size_t)r * p.lds + b];
   }
 }
 
-__global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict__ codes,
-                                                      const uint8_t* __restrict__ scales, int row0, int rows, int units,
-                                                      int kt, float* __restrict__ out) {
+__global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict__ w, int row0, int rows, int units, int kt,
+                                                      float* __restrict__ out) {
   const int u = blockIdx.x * blockDim.x + threadIdx.x;
   if (u >= units) return;
   const int step = gridDim.y * blockDim.y;
   for (int i = blockIdx.y * blockDim.y + threadIdx.y; i < rows; i += step) {
     const int r = row0 + i, b = u >> 2;
-    const size_t tile = (size_t)(r >> 4) * kt + (b >> 2);
     const int lane = (r & 15) + 16 * (b & 3);
-    const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + tile * 1024 + lane * 16 + (u & 3) * 4);
+    const uint32_t c = *reinterpret_cast<const uint32_t*>(w + mx_code_off(r >> 4, b >> 2, kt) + lane * 16 + (u & 3) * 4);
     float o[8];
-    fp4_unpack8(c, e8m0_f32(scales[mx_scale_off(r >> 4, b >> 2, kt, lane)]), o);
+    fp4_unpack8(c, e8m0_f32(w[mx_scale_off(r >> 4, b >> 2, kt, lane)]), o);
     float* d = out + (size_t)i * units * 8 + (size_t)u * 8;
     reinterpret_cast<float4*>(d)[0] = make_float4(o[0], o[1], o[2], o[3]);
     reinterpret_cast<float4*>(d)[1] = make_float4(o[4], o[5], o[6], o[7]);
@@ -199,12 +195,8 @@ __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x
 
 Args make_args(const QMat& w, const QMat* up, int rows, const MxOut& o) {
   Args a{};
-  a.wc = w.p0;
-  a.ws = w.p1;
-  if (up) {
-    a.uc = up->p0;
-    a.us = up->p1;
-  }
+  a.w = w.p0;
+  a.up = up ? up->p0 : nullptr;
   a.n_out = w.n_out;
   a.nt = mx_row_tiles(w.n_out);
   a.kt = mx_k_tiles(w.n_in);
@@ -274,7 +266,7 @@ void mx_quantize(const void* x, int type, int ldx, int rows, int k, uint8_t* cod
 void mx_tile(QMat& m, const MxPlanes& p, hipStream_t s) {
   const int nblk = m.n_in / kMxBlock;
   const RowGrid g(nblk, m.n_out);
-  hipLaunchKernelGGL(tile_kernel, g.grid, g.block, 0, s, p, m.n_out, nblk, mx_k_tiles(m.n_in), m.p0, m.p1);
+  hipLaunchKernelGGL(tile_kernel, g.grid, g.block, 0, s, p, m.n_out, nblk, mx_k_tiles(m.n_in), m.p0);
   PGD_HIP(hipGetLastError());
 }
 
@@ -282,7 +274,7 @@ void mx_dequant(const QMat& m, int row0, int rows, float* out, hipStream_t s) {
   if (rows == 0) return;
   const int units = m.n_in / 8;
   const RowGrid g(units, rows);
-  hipLaunchKernelGGL(dequant_kernel, g.grid, g.block, 0, s, m.p0, m.p1, row0, rows, units, mx_k_tiles(m.n_in), out);
+  hipLaunchKernelGGL(dequant_kernel, g.grid, g.block, 0, s, m.p0, row0, rows, units, mx_k_tiles(m.n_in), out);
   PGD_HIP(hipGetLastError());
 }
 

@@ -13,7 +13,7 @@
 //                                hdr   16B [n_out][nsb]         d, dmin (f16) + 12 packed scale bytes
 //   Q6K (GGML block_q6_K):       ql, qh, sc, d planes, tiled by 32 rows
 //                                (q6k_*_off below); rows padded with zeros
-//   MXFP4 (OCP MX, 32-element    codes, scales, tiled by 16 rows x 128 columns
+//   MXFP4 (OCP MX, 32-element    codes and scales of 64 rows x 128 columns together
 //    blocks, e8m0 scales):       (mxfp4.h)
 //
 // The planes hold exactly the bytes of the source blocks (144 B / 210 B per
@@ -39,7 +39,7 @@ struct QMat {
   uint8_t* base = nullptr;  // owning device allocation
   size_t bytes = 0;
   // plane pointers (into base)
-  // (MXFP4: p0 codes, p1 scales)
+  // (MXFP4: p0 the whole matrix)
   uint8_t* p0 = nullptr;  // A8 codes | Q4K qs | Q6K ql | Q8_0 int8 q [n_out][n_in] | Q5_0 qs [n_out][n_in / 2]
   uint8_t* p1 = nullptr;  // A8 sb    | Q4K hdr | Q6K qh | Q8_0 f16 d [n_out][nsb] | Q5_0 u32 qh [n_out][nsb]
   uint8_t* p2 = nullptr;  //                      Q6K sc |                        | Q5_0 f16 d [n_out][nsb]
