@@ -215,11 +215,18 @@ int pgd_matrix_upload_q5_0(pgd_dev* dev, const void* blocks, int n_out, int n_in
   return upload_kq(dev, FMT_Q5_0, blocks, n_out, n_in, out);
 }
 
+// (the kernels hold row and column numbers, rounded up to whole tiles, in an int)
+static void mx_dims(int n_out, int n_in) {
+  PGD_CHECK(n_out > 0 && n_in > 0 && n_out <= 1 << 30 && n_in <= 1 << 30, kErrShape, "matrix dims must be in 1..2^30");
+  PGD_CHECK(n_in % kMxBlock == 0, kErrShape, "MXFP4 n_in must be a multiple of 32");
+}
+
 int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* scales, int n_out, int n_in,
                             pgd_matrix** out) {
   pgd_matrix* held = nullptr;
   int rc = guard([&] {
     PGD_CHECK(codes && scales, kErrArg, "null argument");
+    mx_dims(n_out, n_in);
     DeviceScope scope(dev);
     new_matrix(dev, FMT_MXFP4, n_out, n_in, out, &held);
     const size_t nc = (size_t)n_out * (n_in / 2), ns = (size_t)n_out * (n_in / kMxBlock);
@@ -250,7 +257,7 @@ int pgd_matrix_from_mxfp4_dev(pgd_dev* dev, const uint8_t* codes, int ldc, const
                               int n_in, pgd_matrix** out) {
   pgd_matrix* held = nullptr;
   int rc = guard([&] {
-    PGD_CHECK(n_out > 0 && n_in > 0, kErrShape, "matrix dims must be positive");
+    mx_dims(n_out, n_in);
     const MxPlanes p = planes(codes, ldc, scales, lds, n_in);
     DeviceScope scope(dev);
     new_matrix(dev, FMT_MXFP4, n_out, n_in, out, &held);

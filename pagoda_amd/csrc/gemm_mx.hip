@@ -418,8 +418,8 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS outlives the workgroup
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
-    const int r = m0 + (wm * MF + m) * 16 + i16;
-    if (r >= a.rows) continue;
+    const uint32_t r = (uint32_t)m0 + (wm * MF + m) * 16 + i16;
+    if (r >= (uint32_t)a.rows) continue;
 #pragma unroll
     for (int n = 0; n < NW; ++n) {
       const int o = (nt0 + wn * NW + n) * 16 + q * 4;
@@ -445,7 +445,7 @@ template <int EPI>
 __global__ __launch_bounds__(256) void join_kernel(Args a, bool vec) {
   const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (n >= a.n_out) return;
-  for (int r = blockIdx.y; r < a.rows; r += gridDim.y) {
+  for (uint32_t r = blockIdx.y; r < (uint32_t)a.rows; r += gridDim.y) {
     const float* p = a.part + (size_t)r * (a.nt * 16) + n;
     f4 v = {}, u = {};
 #pragma unroll 4
@@ -536,7 +536,7 @@ constexpr Cost kDigits[] = {{32, 256, 6.56f, 1.218f, 2.22f, 0.796f, 0.78f, 2.19f
 
 double cost_us(const Cost& c, const Args& a, int splits) {
   const int pair = a.up ? 2 : 1;
-  const long long blocks = (long long)((a.rows + c.bm - 1) / c.bm) * ((a.nt * 16ll * pair + c.bn - 1) / c.bn) * splits;
+  const long long blocks = (((long long)a.rows + c.bm - 1) / c.bm) * ((a.nt * 16ll * pair + c.bn - 1) / c.bn) * splits;
   const long long per_cu = (blocks + 255) / 256;
   const double stages = (a.kt + splits - 1) / splits * (a.kind == TERMS ? a.terms : 1);
   double us = c.launch + (double)(per_cu / 2) * (stages * c.stage2 + c.block2);

@@ -339,7 +339,7 @@ double few_us(const Args& a) {
                                          {3.45f, 0.400f, 0.0f, 0.0060f, 0.0f, 0.0050f}};
   const int terms = a.kind == PLANES ? 1 : a.terms, chunk = std::min(a.rows, 64 / terms), x = chunk * terms, mt = (x + 15) / 16;
   const int tiles = a.up ? 1 : mt > 2 ? 1 : 2;
-  const double wg = (double)((a.nt + tiles - 1) / tiles) * ((a.rows + chunk - 1) / chunk) / 256.0;
+  const double wg = (double)((a.nt + tiles - 1) / tiles) * ((a.rows - 1) / chunk + 1) / 256.0;
   const float* c = a.kind == PLANES ? kPlanes[mt - 1] : kTerms[mt - 1];
   return c[0] + wg * (c[1] + a.kt * (c[2] * tiles * (a.up ? 2 : 1) + c[3] * x)) + a.kt * (c[4] + c[5] * x);
 }

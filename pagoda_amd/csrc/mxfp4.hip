@@ -45,7 +45,7 @@ struct RowGrid {
     int bx = 1;
     while (bx < units && bx < 256) bx *= 2;
     block = dim3(bx, 256 / bx);
-    grid = dim3((units + bx - 1) / bx, std::min((rows + (int)block.y - 1) / (int)block.y, 65535));
+    grid = dim3((units + bx - 1) / bx, std::min(((uint32_t)rows + block.y - 1) / block.y, 65535u));
   }
 };
 
@@ -54,14 +54,14 @@ struct RowGrid {
 // and saturate at 6: the conversion instruction's own rounding. Four threads
 // share a block. Bound by HBM: each element is read once and written once.
 template <int TYPE>
-__global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ x, int ldx, int rows, int units,
+__global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ x, int ldx, uint32_t rows, int units,
                                                        uint8_t* __restrict__ codes, int ldc,
                                                        uint8_t* __restrict__ scales, int lds,
                                                        float* __restrict__ values, int ldv) {
   const int u = blockIdx.x * blockDim.x + threadIdx.x;
   if (u >= units) return;  // (units is a multiple of 4: a block's threads stay together)
-  const int step = gridDim.y * blockDim.y;
-  for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += step) {
+  const uint32_t step = gridDim.y * blockDim.y;
+  for (uint32_t r = blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += step) {
     float v[8];
     load8<TYPE>(x, (size_t)r * ldx + (size_t)u * 8, v);
     // magnitudes as bits: a NaN's exceed an infinity's, so nothing is lost to a maximum
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ 
 __global__ __launch_bounds__(256) void tile_kernel(MxPlanes p, int n_out, int nblk, int kt, uint8_t* __restrict__ w) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= nblk) return;
-  const int step = gridDim.y * blockDim.y;
+  const uint32_t step = gridDim.y * blockDim.y;
   for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < n_out; r += step) {
     const int lane = (r & 15) + 16 * (b & 3);
     const uint4 c = *reinterpret_cast<const uint4*>(p.codes + (size_t)r * p.ldc + (size_t)b * 16);
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict_
                                                       float* __restrict__ out) {
   const int u = blockIdx.x * blockDim.x + threadIdx.x;
   if (u >= units) return;
-  const int step = gridDim.y * blockDim.y;
+  const uint32_t step = gridDim.y * blockDim.y;
   for (int i = blockIdx.y * blockDim.y + threadIdx.y; i < rows; i += step) {
     const int r = row0 + i, b = u >> 2;
     const int lane = (r & 15) + 16 * (b & 3);
@@ -120,12 +120,12 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict_
 // Rows as TERMS planes of bf16 terms (split_terms2). Columns [k, ldt) are zeros,
 // which the last k tile reads.
 template <int TYPE, int TERMS>
-__global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, int ldx, int rows, int units,
+__global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, int ldx, uint32_t rows, int units,
                                                     uint16_t* __restrict__ out, int ldt, size_t term_stride) {
   const int u = blockIdx.x * blockDim.x + threadIdx.x;
   if (u * 8 >= ldt) return;
-  const int step = gridDim.y * blockDim.y;
-  for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += step) {
+  const uint32_t step = gridDim.y * blockDim.y;
+  for (uint32_t r = blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += step) {
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (u < units) load8<TYPE>(x, (size_t)r * ldx + (size_t)u * 8, v);
     uint32_t t[4][TERMS];
@@ -308,7 +308,7 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   const int ldt = a.kt * kMxTileK;
   a.ldx = ldt;
   Plan p = plan(a, true);
-  if (type == X_F32 && rows > 16) {
+  if (type == X_F32 && rows > 16 && a.kt < (1 << 17)) {  // (lanes hold offsets in two of their row tiles in 32 bits)
     // digits: 8.5 bytes of each value read and written instead of 10, and half the matrix instructions' time
     Args d = a;
     d.kind = DIGITS;
@@ -317,7 +317,7 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   }
   std::lock_guard<std::mutex> lock(g_terms);
   if (a.kind == DIGITS) {
-    const long long tiles = (long long)((rows + 15) / 16) * a.kt;
+    const long long tiles = (long long)((rows - 1) / 16 + 1) * a.kt;
     auto* d = static_cast<uint8_t*>(gemv::gemv_scratch(s, (size_t)tiles * (kMxDigitTile + 64), 8));
     auto* ds = d + (size_t)tiles * kMxDigitTile;
     a.d = d;

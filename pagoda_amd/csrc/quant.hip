@@ -545,7 +545,6 @@ void qmat_alloc(QMat& m, int fmt, int n_out, int n_in, hipStream_t s) {
     place(1, rows * m.nsb * 4);
     place(2, rows * m.nsb * 2);
   } else if (fmt == FMT_MXFP4) {
-    PGD_CHECK(n_in % kMxBlock == 0, kErrShape, "MXFP4 n_in must be a multiple of 32");
     place(0, mx_bytes(n_out, n_in));
   } else {
     throw Error{kErrFormat, "unknown matrix format"};

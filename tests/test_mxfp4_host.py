@@ -88,6 +88,12 @@ def test_pair_of_planes_refuses(gate, up, want):
     ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 16, 0, 32), SHAPE),
     ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 16, 16, 0), SHAPE),
     ("pgd_matrix_from_mxfp4_dev", (None, A, 16, A, 16, 16, 32), ARG),
+    ("pgd_matrix_from_mxfp4_dev", (A, A, 32, A, 16, 16, 48), SHAPE),
+    ("pgd_matrix_from_mxfp4_dev", (A, A, 16, A, 16, (1 << 30) + 1, 32), SHAPE),
+    ("pgd_matrix_from_mxfp4_dev", (A, A, 1 << 30, A, 1 << 26, 16, (1 << 30) + 32), SHAPE),
+    ("pgd_matrix_upload_mxfp4", (A, A, A, 16, 48), SHAPE),
+    ("pgd_matrix_upload_mxfp4", (A, A, A, 0, 32), SHAPE),
+    ("pgd_matrix_upload_mxfp4", (A, A, A, (1 << 30) + 1, 32), SHAPE),
 ])
 def test_matrix_from_planes_refuses(name, args, want):
     out = C.c_void_p()
@@ -118,3 +124,12 @@ def test_definition_at_the_ends_of_the_range():
     v = mx.values(c, s)
     assert not v[0].any() and not v[1].any() and v[2, 5] == 6 * 2.0 ** 125
     assert np.isnan(v[3]).all() and np.isnan(v[4]).all()
+
+
+def test_other_activations_refuse_mxfp4():
+    """Prepared A8 rows and paired quantized rows are for other formats."""
+    m = handle()
+    p = C.byref(m)
+    assert code("pgd_matrix_gemv_act_dev", p, A, 1, A, 48, None, 0) == FORMAT
+    assert code("pgd_matrix_gemv_act_dev_noalloc", p, A, 1, A, 48, None, 0) == FORMAT
+    assert code("pgd_matrix_gemv_q8act_pair_dev", p, A, p, A, A, 64, 1, 48) == FORMAT
