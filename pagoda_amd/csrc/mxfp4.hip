@@ -146,51 +146,60 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
 // its values are exact to the last of their 24 where they are above 1/64 of the
 // largest, and within 2^-30 of it elsewhere (f32 sums of its products keep 24).
 // Digits -16..15 of that whole number, the top one to 16, are e2m3 codes (u / 8 is
-// code u up to 16), digit i scaled by 2^(e - 127 - 5 i). A wave takes one tile of 16
-// rows by 128 columns, lane l block l / 16 of row l % 16. A block with an infinity
-// or NaN is NaN. Rows and columns past the matrix are zeros.
+// code u up to 16), digit i scaled by 2^(e - 127 - 5 i). A tile of 16 rows by 128
+// columns goes to 128 threads, half a block each (of lane l: block l / 16 of row l %
+// 16). A block with an infinity or NaN is NaN. Rows and columns past the matrix are
+// zeros.
 __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x, int ldx, int rows, int nblk, int kt,
                                                      long long tiles, uint8_t* __restrict__ d,
                                                      uint8_t* __restrict__ ds) {
-  const long long tile = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long tile = (long long)blockIdx.x * 2 + (threadIdx.x >> 7);
   if (tile >= tiles) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = (threadIdx.x & 127) >> 1, half = threadIdx.x & 1;
   const int row = (int)(tile / kt) * 16 + (lane & 15), b = (int)(tile % kt) * 4 + (lane >> 4);
-  float v[4][8] = {};
+  float v[2][8] = {};
   if (row < rows && b < nblk) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load8<X_F32>(x, (size_t)row * ldx + (size_t)b * kMxBlock + j * 8, v[j]);
+    for (int j = 0; j < 2; ++j) load8<X_F32>(x, (size_t)row * ldx + (size_t)b * kMxBlock + half * 16 + j * 8, v[j]);
   }
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i >> 3][i & 7]) & 0x7fffffffu);
+  for (int i = 0; i < 16; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i >> 3][i & 7]) & 0x7fffffffu);
+  top = max(top, (uint32_t)__shfl_xor((int)top, 1));
   const int e = max((int)(top >> 23), 25);
-  uint32_t q[6][6] = {};  // [digit][dword]
+  uint32_t q[6][3] = {};  // [digit][dword]
   if (e != 255) {
     // (2^(155 - e) in two factors: it may pass the largest f32)
     const float up = __builtin_bit_cast(float, (uint32_t)(127 + (155 - e) / 2) << 23);
     const float up2 = __builtin_bit_cast(float, (uint32_t)(127 + (155 - e) - (155 - e) / 2) << 23);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      int n = __float2int_rn(v[i >> 3][i & 7] * up * up2);
+    for (int i = 0; i < 16; ++i) {
+      // (16 more in each of the lower five digits: their bits are then the digits plus 16)
+      const int n = __float2int_rn(v[i >> 3][i & 7] * up * up2) + 0x1084210;
 #pragma unroll
-      for (int k = 5; k >= 0; --k) {
-        const int u = k ? ((n + 16) & 31) - 16 : n;
-        n = (n - u) >> 5;
-        const uint32_t code = (uint32_t)abs(u) | (u < 0 ? 32u : 0u);
+      for (int k = 0; k < 6; ++k) {
+        const int u = k ? n >> (25 - 5 * k) & 31 : n >> 25;
+        const uint32_t code = k ? (u & 16 ? u & 15 : 48 - u) : (uint32_t)abs(u) | (u < 0 ? 32u : 0u);
         const int bit = 6 * i, w = bit >> 5, o = bit & 31;
         q[k][w] |= code << o;
         if (o > 26) q[k][w + 1] |= code >> (32 - o);
       }
     }
   }
-  uint8_t* out = d + (size_t)tile * kMxDigitTile + lane * 16;
+  uint8_t* out = d + (size_t)tile * kMxDigitTile;
 #pragma unroll
   for (int k = 0; k < 6; ++k) {
-    *reinterpret_cast<uint4*>(out + k * 1024) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
-    *reinterpret_cast<uint2*>(out + 6144 + k * 512 - lane * 8) = make_uint2(q[k][4], q[k][5]);
+    uint32_t* lo = reinterpret_cast<uint32_t*>(out + k * 1024 + lane * 16);
+    if (half == 0) {
+      lo[0] = q[k][0];
+      lo[1] = q[k][1];
+      lo[2] = q[k][2];
+    } else {
+      lo[3] = q[k][0];
+      *reinterpret_cast<uint2*>(out + 6144 + k * 512 + lane * 8) = make_uint2(q[k][1], q[k][2]);
+    }
   }
-  ds[(size_t)tile * 64 + lane] = (uint8_t)e;
+  if (half == 0) ds[(size_t)tile * 64 + lane] = (uint8_t)e;
 }
 
 Args make_args(const QMat& w, const QMat* up, int rows, const MxOut& o) {
@@ -322,7 +331,7 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
     auto* ds = d + (size_t)tiles * kMxDigitTile;
     a.d = d;
     a.ds = ds;
-    hipLaunchKernelGGL(digits_kernel, dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, s, static_cast<const float*>(x), ldx,
+    hipLaunchKernelGGL(digits_kernel, dim3((unsigned)((tiles + 1) / 2)), dim3(256), 0, s, static_cast<const float*>(x), ldx,
                        rows, a.nblk, a.kt, tiles, d, ds);
   } else {
     a.term_stride = (size_t)rows * ldt;

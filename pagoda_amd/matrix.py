@@ -31,8 +31,8 @@ def act_prep_dev(dev: Device, x_ptr: int, ldx: int, nrows: int, k: int, act_ptr:
 def mxfp4_quantize_dev(dev: Device, x_ptr: int, x_type: int, ldx: int, nrows: int, k: int, codes_ptr: int, ldc: int,
                        scales_ptr: int, lds: int, values_ptr: int = 0, ldv: int = 0) -> None:
     """Rows of f32 / f16 / bf16 (x_type) to MXFP4 planes; values_ptr also receives the values they stand for."""
-    call("pgd_mxfp4_quantize_dev", dev.handle, C.c_void_p(x_ptr), x_type, ldx, nrows, k, C.c_void_p(codes_ptr), ldc,
-         C.c_void_p(scales_ptr), lds, C.c_void_p(values_ptr or None), ldv)
+    call("pgd_mxfp4_quantize_dev", dev.handle, x_ptr, x_type, ldx, nrows, k, codes_ptr, ldc, scales_ptr, lds,
+         values_ptr, ldv)
 
 
 class Matrix:
@@ -123,8 +123,7 @@ class Matrix:
     def gemv_dev(self, x_ptr: int, ldx: int, nrows: int, y_ptr: int, ldy: int, x_f16: int = False,
                  res_ptr: int = 0, ldres: int = 0) -> None:
         """x_f16: f32 rows (False), f16 (True), or for MXFP4 matrices X_F32 / X_F16 / X_BF16."""
-        call("pgd_matrix_gemv_dev", self.handle, C.c_void_p(x_ptr), int(x_f16), ldx, nrows, C.c_void_p(y_ptr), ldy,
-             C.c_void_p(res_ptr or None), ldres)
+        call("pgd_matrix_gemv_dev", self.handle, x_ptr, int(x_f16), ldx, nrows, y_ptr, ldy, res_ptr, ldres)
 
     def gemv_q8act_dev(self, x_ptr: int, ldx: int, nrows: int, y_ptr: int, ldy: int, res_ptr: int = 0,
                        ldres: int = 0) -> None:
@@ -148,16 +147,14 @@ class Matrix:
 
     @staticmethod
     def gemv_swiglu_dev(gate: "Matrix", up: "Matrix", x_ptr: int, ldx: int, nrows: int, mid_ptr: int, ldm: int):
-        call("pgd_matrix_gemv_swiglu_dev", gate.handle, up.handle, C.c_void_p(x_ptr), ldx, nrows, C.c_void_p(mid_ptr), ldm)
+        call("pgd_matrix_gemv_swiglu_dev", gate.handle, up.handle, x_ptr, ldx, nrows, mid_ptr, ldm)
 
     def gemv_mx_dev(self, codes_ptr: int, ldc: int, scales_ptr: int, lds: int, nrows: int, y_ptr: int, ldy: int,
                     res_ptr: int = 0, ldres: int = 0) -> None:
         """MXFP4 rows (planes) times this MXFP4 matrix."""
-        call("pgd_matrix_gemv_mx_dev", self.handle, C.c_void_p(codes_ptr), ldc, C.c_void_p(scales_ptr), lds, nrows,
-             C.c_void_p(y_ptr), ldy, C.c_void_p(res_ptr or None), ldres)
+        call("pgd_matrix_gemv_mx_dev", self.handle, codes_ptr, ldc, scales_ptr, lds, nrows, y_ptr, ldy, res_ptr, ldres)
 
     @staticmethod
     def gemv_swiglu_mx_dev(gate: "Matrix", up: "Matrix", codes_ptr: int, ldc: int, scales_ptr: int, lds: int,
                            nrows: int, mid_ptr: int, ldm: int):
-        call("pgd_matrix_gemv_swiglu_mx_dev", gate.handle, up.handle, C.c_void_p(codes_ptr), ldc,
-             C.c_void_p(scales_ptr), lds, nrows, C.c_void_p(mid_ptr), ldm)
+        call("pgd_matrix_gemv_swiglu_mx_dev", gate.handle, up.handle, codes_ptr, ldc, scales_ptr, lds, nrows, mid_ptr, ldm)
