@@ -90,8 +90,9 @@ int pgd_matrix_upload_q5_0(pgd_dev* dev, const void* blocks, int n_out, int n_in
  * 0 .5 1 1.5 2 3 4 6) and one scale byte s that stands for 2^(s - 127); s = 255
  * makes the block NaN. Row-major planes: codes, element 2 i of a row in the low
  * nibble of byte i, and one scale byte per block. Format id 5 in
- * pgd_matrix_info; pgd_matrix_dequant and the pgd_matrix_gemv* entry points that
- * take f32 / f16 rows take these matrices too. n_in is a multiple of 32.
+ * pgd_matrix_info; pgd_matrix_dequant, pgd_matrix_gemv, pgd_matrix_gemv_dev and
+ * pgd_matrix_gemv_swiglu_dev take these matrices too. n_in is a multiple of 32, both
+ * sides are at most 2^30.
  *
  * upload: host planes, codes [n_out][n_in / 2], scales [n_out][n_in / 32]. */
 int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* scales, int n_out, int n_in,
@@ -130,8 +131,15 @@ int pgd_matrix_gemv(const pgd_matrix* m, const float* x, int nrows, float* y);
 /* Device form. x f32 (x_f16 = 0) or IEEE f16 (x_f16 = 1), row stride ldx
  * elements (multiple of 8); y row stride ldy; res (nullable) adds a residual
  * y = res + W.x (replaces affine_gemv_res, qwen3_gemv.rs:289-306).
- * MXFP4 matrices also take bf16 rows (x_f16 = 2), and x must be 16-byte
- * aligned; every x enters the products exactly, sums are f32. */
+ * MXFP4 matrices also take bf16 rows (x_f16 = 2; to the other formats any nonzero
+ * x_f16 is f16), and x must be 16-byte aligned. Sums are f32. f16 and bf16 rows and
+ * up to 16 f32 rows enter the products exactly. More f32 rows may be held, block of
+ * 32 by block, to 2^-30 of the power of two above the block's largest magnitude
+ * (2^-131 at the finest), and an infinity among them makes its row NaN. The order of
+ * the sums depends on the number of rows and on whether the stream is captured, on
+ * nothing else. In a stream capture, rows that would need scratch memory are PGD_ERR_STATE and queue
+ * nothing: all but up to 5 f32, 8 f16 or 4 bf16 rows and bf16 rows of n_in % 128 ==
+ * 0 (the same holds for pgd_matrix_gemv_swiglu_dev; MXFP4 rows are never refused). */
 int pgd_matrix_gemv_dev(const pgd_matrix* m, const void* x, int x_f16, int ldx, int nrows, float* y,
                         int ldy, const float* res, int ldres);
 /* mid = silu(gate . x) * (up . x); replaces affine_gemv2_silu
@@ -141,7 +149,9 @@ int pgd_matrix_gemv_swiglu_dev(const pgd_matrix* gate, const pgd_matrix* up, con
 /* Products of MXFP4 rows (planes as pgd_mxfp4_quantize_dev writes them, strides
  * as there; each plane nrows rows) with MXFP4 matrices, on the scaled 4-bit
  * matrix instructions with f32 sums: y = W.x, plus res (nullable) as in
- * pgd_matrix_gemv_dev, and mid = silu(gate.x) * (up.x). Any nrows >= 0. */
+ * pgd_matrix_gemv_dev, and mid = silu(gate.x) * (up.x). Any nrows >= 0. A plane's
+ * row is read to its whole strides: whatever lies past its codes and scales does not
+ * reach the results. */
 int pgd_matrix_gemv_mx_dev(const pgd_matrix* m, const uint8_t* codes, int ldc, const uint8_t* scales, int lds, int nrows,
                            float* y, int ldy, const float* res, int ldres);
 int pgd_matrix_gemv_swiglu_mx_dev(const pgd_matrix* gate, const pgd_matrix* up, const uint8_t* codes, int ldc,

@@ -7,9 +7,30 @@
 // loads of a stage, then one barrier per stage publishes it, and the slot that
 // the barrier retires is filled with the stage S - 1 ahead.
 //
-// Rows of several bf16 terms take one stage per term and k tile: all terms of a
-// row add to the same f32 sums. Rows in digits (mxfp4.hip) take six matrix
-// instructions of the 4-bit rate instead of three terms' twelve of the bf16 rate.
+// y[r][n] = sum over 32-element blocks b of 2^(sx[r][b] + sw[n][b]) sum x w of the
+// codes: the 4-bit instruction's own formula, for MXFP4 rows. Weights for bf16 rows
+// are turned into bf16 (exactly) in registers, under the matrix instructions. Rows
+// of several bf16 terms take one stage per term and k tile: all terms of a row add to
+// the same f32 sums. Rows in digits (mxfp4.hip) take six matrix instructions of the
+// 4-bit rate instead of three terms' twelve of the bf16 rate.
+//
+// Measured, weights from HBM (17408 x 5120 unless given; MFMA: share of cycles the
+// matrix units are busy):
+//   4096 MXFP4 rows          247 us  2.95 PFLOP/s  MFMA 38%   blocks of 128 x 256
+//   2048 MXFP4 rows, pair    230 us  3.17 PFLOP/s       42%   128 x 256
+//   48 MXFP4 rows, pair       30 us  3.2 TB/s            14%  64 x 128
+//   1999 bf16 rows of 6144 to 5120   112 us  1.13 PFLOP/s  61%   64 x 256
+//   333 f32 rows, pair       188 us  digits: 0.63 PFLOP/s of the result, 57%   32 x 256
+//   32 bf16 rows of 17408 to 5120    16 us  3.1 TB/s     21%  32 x 128, 12 ranges of k tiles
+// Large MXFP4 products are bound by getting operands to the matrix units: a CU takes
+// 43 B a clock from L2 into LDS at best (35 where rows give 64 B pieces) and needs 24
+// KiB a stage of 512 clocks, and LDS serves a stage's 48 KiB of reads in 400 clocks
+// besides. Small ones by the 3 TB/s that such loads reach from HBM: the loads alone
+// take as long. bf16 rows run at 93% of what a large library product of bf16 reaches.
+// Not taken, each at equal or longer times: weights straight into registers without
+// LDS (equal for bf16 and digits; 5% slower for 4096 MXFP4 rows, 12 to 20% for pairs:
+// the compiler's waits for them also wait for later LDS loads); longer rings (up to 8
+// stages: the bytes in flight do not limit); blocks starting at different k tiles.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -504,7 +525,12 @@ void launch(Args a, int splits, hipStream_t s) {
   PGD_HIP(hipGetLastError());
 }
 
-// The shapes, largest first.
+// The shapes, largest first: wide ones read activations and weights fewer times from
+// L2 and LDS per matrix instruction (4096 MXFP4 rows, 17408 x 5120: 32 x 128 blocks
+// 606 us, 64 x 128 386, 128 x 128 333, 128 x 256 273); small ones give few rows blocks
+// for all CUs (32 bf16 rows, 5120 x 17408, no ranges: 64 x 256 118, 64 x 128 77, 32 x
+// 128 57; ranges of k tiles then bring it to 16). Two blocks share a CU, so that one
+// computes while the other waits.
 using P0 = Shape<PLANES, 128, 256, 1, 4, 3, 2>;
 using P1 = Shape<PLANES, 128, 128, 2, 2, 4, 2>;
 using P2 = Shape<PLANES, 64, 128, 1, 4, 4, 2>;

@@ -10,6 +10,13 @@
 // Activation rows held as several bf16 terms take one matrix row per term and
 // batch row (term t of row r is row t * rows + r), and the terms' sums are added
 // at the end: a single f32 row costs one matrix instruction per 32 columns, not 3.
+//
+// Bound by HBM: the weights are read once, 4.25 bits each. Measured, weights from HBM:
+// a 2 x 17408 x 5120 pair and one f32 row 21 us (4.5 TB/s; a large copy moves 4.75),
+// 5120 x 17408 and 8 MXFP4 rows 10.3 us (4.6), 151936 x 896 and 5 f16 rows 18 us
+// (4.2, with the launch that splits them). Past about 16 rows of terms every
+// workgroup's reads of all activations from L2 weigh more than the weights (32 bf16
+// rows of 17408: 41 us, 16 in blocks that share them through LDS, gemm_mx.hip).
 #include <algorithm>
 
 #include "common.h"

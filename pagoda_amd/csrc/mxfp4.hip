@@ -52,7 +52,9 @@ struct RowGrid {
 // A block's scale byte is the exponent of its largest magnitude less 2 (6 = 1.5
 // 2^2 is the largest code), codes are rounded to nearest, ties to the even code,
 // and saturate at 6: the conversion instruction's own rounding. Four threads
-// share a block. Bound by HBM: each element is read once and written once.
+// share a block, so that a wave's loads and stores are runs of whole lines. Bound by
+// HBM: each element is read once, its code and value written once. 2048 x 17408 f32 with
+// values: 57 us, 5.35 TB/s.
 template <int TYPE>
 __global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ x, int ldx, uint32_t rows, int units,
                                                        uint8_t* __restrict__ codes, int ldc,
@@ -118,7 +120,8 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict_
 }
 
 // Rows as TERMS planes of bf16 terms (split_terms2). Columns [k, ldt) are zeros,
-// which the last k tile reads.
+// which the last k tile reads. Bound by latency at the row counts that take it: 2 us
+// for 5 f16 rows of 896.
 template <int TYPE, int TERMS>
 __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, int ldx, uint32_t rows, int units,
                                                     uint16_t* __restrict__ out, int ldt, size_t term_stride) {
@@ -149,7 +152,7 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
 // code u up to 16), digit i scaled by 2^(e - 127 - 5 i). A tile of 16 rows by 128
 // columns goes to 128 threads, half a block each (of lane l: block l / 16 of row l %
 // 16). A block with an infinity or NaN is NaN. Rows and columns past the matrix are
-// zeros.
+// zeros. 333 rows of 5120: 8.4 us, latency (420 workgroups; one thread a block 8.8).
 __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x, int ldx, int rows, int nblk, int kt,
                                                      long long tiles, uint8_t* __restrict__ d,
                                                      uint8_t* __restrict__ ds) {
