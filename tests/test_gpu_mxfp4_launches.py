@@ -122,7 +122,10 @@ def test_host_rows(dev, rows):
 
 
 def hip(name, *args):
-    assert getattr(C.CDLL("libamdhip64.so"), name)(*args) == 0, name
+    """A HIP call in the runtime that the backend library is linked to (another copy may be loaded)."""
+    from pagoda_amd import lib
+
+    assert getattr(lib(), name)(*args) == 0, name
 
 
 class Graph:
