@@ -49,7 +49,7 @@ __device__ inline bf8 fp4_bf16x8(uint32_t c, float scale) {
 
 // x = t0 + t1 + t2 exactly: each term is the truncation to bf16 (8 significant
 // bits) of what is left, so 3 terms hold the 24 bits of an f32, 2 the 11 of an
-// f16. An infinity or NaN is its first term alone (a NaN stays one: its bits
+// f16 (but for bits below 2^-133, the smallest bf16 number). An infinity or NaN is its first term alone (a NaN stays one: its bits
 // below bf16 are or-ed in). Two values, the terms packed low first.
 template <int TERMS>
 __device__ inline void split_terms2(float (&v)[2], uint32_t (&t)[TERMS]) {

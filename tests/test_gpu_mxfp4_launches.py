@@ -94,6 +94,43 @@ def test_f32_rows_beside_an_outlier(dev, buf, rows):
     assert (np.abs(got - xd @ wv.T) <= bound).all()
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 4, 12, 40, 300])
+def test_values_below_the_normal_range(dev, buf, t, rows):
+    """Subnormal activations under large weights, and weights of the smallest scales under large
+    activations, one product per output: f32 rows past 16 are held to steps of 2^-130 (so within
+    2^-131), fewer lose what is below 2^-133, the smallest bf16 number, which their last term
+    (the truncation of what the others leave) cannot hold. bf16 rows lose nothing."""
+    rng = np.random.default_rng(rows + t)
+    n, k = 40, 256
+    x = np.zeros((rows, k), np.float32)
+    at = rng.integers(0, k, rows)
+    x[np.arange(rows), at] = (rng.uniform(1, 2, rows) * 2.0 ** rng.integers(-140, -105, rows)).astype(np.float32)
+    codes = rng.integers(0, 256, (n, k // 2), dtype=np.uint8)
+    for scale, rows_x in ((127 + 100, x), (0, np.where(x != 0, np.float32(1.25 * 2.0 ** 100), np.float32(0)))):
+        w = codes, np.full((n, k // 32), scale, np.uint8)
+        raw, xv = mx.rows_of(rows_x, t)
+        wv, xd = mx.values(*w), xv.astype(np.float64)
+        want = xd @ wv.T
+        step = 0 if t == BF16 else 2.0 ** -131 if rows > 16 else 2.0 ** -133
+        got = run_rows(dev, buf, matrix(dev, w), raw, t)
+        assert (np.abs(got - want) <= 4 * 2.0 ** -23 * np.abs(want) + step * np.abs(wv[:, at].T)).all()
+
+
+def test_residual_of_another_stride(dev, buf):
+    rng = np.random.default_rng(12)
+    n, k, ldres = 100, 160, 131
+    w = weights(rng, n, k)
+    m, wv = matrix(dev, w), mx.values(*w)
+    for rows in (1, 30, 200):
+        x, res = rng.normal(0, 1, (rows, k)).astype(np.float32), rng.normal(0, 1, (rows, ldres)).astype(np.float32)
+        py = buf.up(np.zeros((rows, n), np.float32))
+        m.gemv_dev(buf.up(x), k, rows, py, n, F32, buf.up(res), ldres)
+        want = res[:, :n] + x.astype(np.float64) @ wv.T
+        got = buf.down(py, np.zeros((rows, n), np.float32))
+        assert (np.abs(got - want) <= mx.product_bound(x.astype(np.float64), wv) + 2.0 ** -23 * np.abs(want)).all()
+
+
 def test_no_rows(dev, buf):
     """Nothing is written, and null rows are as good as any."""
     from pagoda_amd import Matrix
