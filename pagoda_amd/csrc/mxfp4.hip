@@ -144,6 +144,13 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
   }
 }
 
+// The 6-bit codes of three digits at once: digit plus 16 in bits 0..4, 10..14 and 20..24
+// (others ignored) to a sign over a magnitude of 0..16 in bits 0..5, 10..15 and 20..25.
+__device__ __forceinline__ uint32_t digit_codes(uint32_t b) {
+  const uint32_t neg = ~(b >> 4) & 0x100401;
+  return (((b & 0xf03c0f) ^ neg * 15) + neg) | neg << 5;  // (below 16: 16 less the low bits)
+}
+
 // f32 rows in six base-32 digits. A block with largest magnitude below 2^(e - 126) (e
 // the biased exponent, 25 at least) is held in steps of 2^(e - 155): 30 bits, so
 // its values are exact to the last of their 24 where they are above 1/64 of the
@@ -152,16 +159,18 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
 // code u up to 16), digit i scaled by 2^(e - 127 - 5 i). A tile of 16 rows by 128
 // columns goes to 128 threads, half a block each (of lane l: block l / 16 of row l %
 // 16). A block with an infinity or NaN is NaN. Rows and columns past the matrix are
-// zeros. 333 rows of 5120: 8.4 us, latency (420 workgroups; one thread a block 8.8).
+// zeros. 333 rows of 5120: 7.8 us, latency (420 workgroups; one thread a block 8.8);
+// 868 rows of 3008: 11.6.
 __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x, int ldx, int rows, int nblk, int kt,
-                                                     long long tiles, uint8_t* __restrict__ d,
+                                                     uint32_t tiles, uint8_t* __restrict__ d,
                                                      uint8_t* __restrict__ ds) {
-  const long long tile = (long long)blockIdx.x * 2 + (threadIdx.x >> 7);
+  const uint32_t tile = blockIdx.x * 2 + (threadIdx.x >> 7);
   if (tile >= tiles) return;
   const int lane = (threadIdx.x & 127) >> 1, half = threadIdx.x & 1;
-  const int row = (int)(tile / kt) * 16 + (lane & 15), b = (int)(tile % kt) * 4 + (lane >> 4);
+  const uint32_t rt = tile / (uint32_t)kt, row = rt * 16 + (lane & 15);
+  const int b = (int)(tile - rt * kt) * 4 + (lane >> 4);
   float v[2][8] = {};
-  if (row < rows && b < nblk) {
+  if (row < (uint32_t)rows && b < nblk) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) load8<X_F32>(x, (size_t)row * ldx + (size_t)b * kMxBlock + half * 16 + j * 8, v[j]);
   }
@@ -179,10 +188,12 @@ __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x
     for (int i = 0; i < 16; ++i) {
       // (16 more in each of the lower five digits: their bits are then the digits plus 16)
       const int n = __float2int_rn(v[i >> 3][i & 7] * up * up2) + 0x1084210;
+      const int u = n >> 25;
+      const uint32_t c5 = digit_codes((uint32_t)n), c4 = digit_codes((uint32_t)n >> 5);
 #pragma unroll
       for (int k = 0; k < 6; ++k) {
-        const int u = k ? n >> (25 - 5 * k) & 31 : n >> 25;
-        const uint32_t code = k ? (u & 16 ? u & 15 : 48 - u) : (uint32_t)abs(u) | (u < 0 ? 32u : 0u);
+        const uint32_t code = k ? (k & 1 ? c5 : c4) >> (k < 2 ? 20 : k < 4 ? 10 : 0) & 63
+                                : (uint32_t)abs(u) | (u < 0 ? 32u : 0u);
         const int bit = 6 * i, w = bit >> 5, o = bit & 31;
         q[k][w] |= code << o;
         if (o > 26) q[k][w + 1] |= code >> (32 - o);
@@ -192,15 +203,9 @@ __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x
   uint8_t* out = d + (size_t)tile * kMxDigitTile;
 #pragma unroll
   for (int k = 0; k < 6; ++k) {
-    uint32_t* lo = reinterpret_cast<uint32_t*>(out + k * 1024 + lane * 16);
-    if (half == 0) {
-      lo[0] = q[k][0];
-      lo[1] = q[k][1];
-      lo[2] = q[k][2];
-    } else {
-      lo[3] = q[k][0];
-      *reinterpret_cast<uint2*>(out + 6144 + k * 512 + lane * 8) = make_uint2(q[k][1], q[k][2]);
-    }
+    const uint32_t fourth = (uint32_t)__shfl_xor((int)q[k][0], 1);  // (the second half's first dword)
+    if (half == 0) *reinterpret_cast<uint4*>(out + k * 1024 + lane * 16) = make_uint4(q[k][0], q[k][1], q[k][2], fourth);
+    else *reinterpret_cast<uint2*>(out + 6144 + k * 512 + lane * 8) = make_uint2(q[k][1], q[k][2]);
   }
   if (half == 0) ds[(size_t)tile * 64 + lane] = (uint8_t)e;
 }
@@ -332,12 +337,13 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   std::lock_guard<std::mutex> lock(g_terms);
   if (a.kind == DIGITS) {
     const long long tiles = (long long)((rows - 1) / 16 + 1) * a.kt;
+    PGD_CHECK(tiles < (1ll << 25), kErrShape, "too many activations for one MXFP4 product");
     auto* d = static_cast<uint8_t*>(gemv::gemv_scratch(s, (size_t)tiles * (kMxDigitTile + 64), 8));
     auto* ds = d + (size_t)tiles * kMxDigitTile;
     a.d = d;
     a.ds = ds;
     hipLaunchKernelGGL(digits_kernel, dim3((unsigned)((tiles + 1) / 2)), dim3(256), 0, s, static_cast<const float*>(x), ldx,
-                       rows, a.nblk, a.kt, tiles, d, ds);
+                       rows, a.nblk, a.kt, (uint32_t)tiles, d, ds);
   } else {
     a.term_stride = (size_t)rows * ldt;
     auto* t = static_cast<uint16_t*>(gemv::gemv_scratch(s, a.terms * a.term_stride * sizeof(uint16_t), 8));
