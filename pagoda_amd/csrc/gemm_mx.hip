@@ -560,8 +560,8 @@ constexpr Cost kTerms[] = {{64, 256, 6.22f, 1.311f, 1.13f, 0.813f, 0.00f, 1.85f,
 constexpr Cost kDigits[] = {{32, 256, 6.56f, 1.218f, 2.22f, 0.796f, 0.78f, 2.19f, 0.293f},
                             {32, 128, 5.73f, 0.757f, 2.58f, 0.526f, 1.24f, 2.14f, 0.278f}};
 
-double cost_us(const Cost& c, const Args& a, int splits) {
-  const int pair = a.up ? 2 : 1;
+double cost_us(const Cost& c, const Sizes& a, int splits) {
+  const int pair = a.pair ? 2 : 1;
   const long long blocks = (((long long)a.rows + c.bm - 1) / c.bm) * ((a.nt * 16ll * pair + c.bn - 1) / c.bn) * splits;
   const long long per_cu = (blocks + 255) / 256;
   const double stages = (a.kt + splits - 1) / splits * (a.kind == TERMS ? a.terms : 1);
@@ -573,15 +573,15 @@ double cost_us(const Cost& c, const Args& a, int splits) {
 
 }  // namespace
 
-Many plan_many(const Args& a, bool scratch) {
-  Many best{0, 1, 1e30};
+Many plan_many(const Sizes& a, bool scratch) {
+  Many best{0, 1, 0, 0, 1e30};
   const Cost* costs = a.kind == PLANES ? kPlanes : a.kind == TERMS ? kTerms : kDigits;
   const int shapes = a.kind == PLANES ? 4 : a.kind == TERMS ? 3 : 2;
   for (int i = 0; i < shapes; ++i)
     for (int splits : {1, 2, 3, 4, 6, 8, 10, 12, 16, 24}) {
       if (splits > 1 && (!scratch || splits * 2 > a.kt)) break;
       const double us = cost_us(costs[i], a, splits);
-      if (us < best.us) best = Many{i, splits, us};
+      if (us < best.us) best = Many{i, splits, costs[i].bm, costs[i].bn, us};
     }
   return best;
 }

@@ -326,16 +326,16 @@ void launch_rows(const Args& a, hipStream_t s) {
 // of a wave: measured for 1, 2, 4, 5 and 8 rows over 12 matrices from 300 x 17408
 // to 151936 x 896, where more than 5 workgroups per CU always lose.
 bool few_split_ok(int rows, int type) { return rows <= (type == X_F32 ? 5 : type == X_F16 ? 8 : 4); }
-bool few_split_pays(const Args& a, int type) {
+bool few_split_pays(const Sizes& a, int type) {
   const int terms = type == X_F32 ? 3 : type == X_F16 ? 2 : 1;
-  return few_split_ok(a.rows, type) && (a.up ? a.nt : (a.nt + 1) / 2) <= 1280 &&
+  return few_split_ok(a.rows, type) && (a.pair ? a.nt : (a.nt + 1) / 2) <= 1280 &&
          (a.kt + 7) / 8 * (0.05 + 0.03 * a.rows * terms) <= 2.2;
 }
 
 // Microseconds of a launch; per 256 workgroups, their weight tiles and their
 // activation tiles; per k tile, and row of terms of it (1..4 row tiles of rows).
 // Fitted with the costs in gemm_mx.hip: 10 to 15% rms off.
-double few_us(const Args& a) {
+double few_us(const Sizes& a) {
   static constexpr float kPlanes[4][6] = {{5.16f, 0.066f, 0.0257f, 0.00017f, 0.0005f, 0.0020f},
                                           {4.54f, 0.296f, 0.0188f, 0.0013f, 0.020f, 0.0024f},
                                           {4.04f, 0.384f, 0.0173f, 0.0018f, 0.0f, 0.0032f},
@@ -345,10 +345,10 @@ double few_us(const Args& a) {
                                          {3.15f, 0.142f, 0.0f, 0.0072f, 0.0f, 0.0053f},
                                          {3.45f, 0.400f, 0.0f, 0.0060f, 0.0f, 0.0050f}};
   const int terms = a.kind == PLANES ? 1 : a.terms, chunk = std::min(a.rows, 64 / terms), x = chunk * terms, mt = (x + 15) / 16;
-  const int tiles = a.up ? 1 : mt > 2 ? 1 : 2;
+  const int tiles = a.pair ? 1 : mt > 2 ? 1 : 2;
   const double wg = (double)((a.nt + tiles - 1) / tiles) * ((a.rows - 1) / chunk + 1) / 256.0;
   const float* c = a.kind == PLANES ? kPlanes[mt - 1] : kTerms[mt - 1];
-  return c[0] + wg * (c[1] + a.kt * (c[2] * tiles * (a.up ? 2 : 1) + c[3] * x)) + a.kt * (c[4] + c[5] * x);
+  return c[0] + wg * (c[1] + a.kt * (c[2] * tiles * (a.pair ? 2 : 1) + c[3] * x)) + a.kt * (c[4] + c[5] * x);
 }
 
 void run_few(const Args& a, hipStream_t s) {

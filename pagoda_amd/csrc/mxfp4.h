@@ -82,16 +82,20 @@ constexpr int kMxDigitTile = 9216;  // 6 digits of 24 B a lane
 //   ROWS    raw: rows of an XType with stride ldx, split by the launch itself
 enum Kind : int { PLANES = 0, TERMS = 1, DIGITS = 2, ROWS = 3 };
 
-// One product launch.
-struct Args {
-  const uint8_t *w, *up;  // the matrix, and the up matrix (SwiGLU) or null
+// What the choice of a kernel goes by, and
+struct Sizes {
   int n_out, nt, kt, nblk;  // outputs; row tiles, k tiles, 32-element blocks of a row
   int rows;
+  bool pair;  // gate and up
   Kind kind;
+  int terms;
+};
+// one product launch.
+struct Args : Sizes {
+  const uint8_t *w, *up;  // the matrix, and the up matrix (SwiGLU) or null
   MxPlanes p;
   const uint16_t* x;
   size_t ldx, term_stride;
-  int terms;
   const void* raw;
   int raw_type;
   const uint8_t *d, *ds;
@@ -106,17 +110,29 @@ struct Args {
 // estimated microseconds; whether it can split that many rows of a type itself, and
 // whether that beats splitting them first.
 void run_few(const Args& a, hipStream_t s);
-double few_us(const Args& a);
+double few_us(const Sizes& a);
 bool few_split_ok(int rows, int type);
-bool few_split_pays(const Args& a, int type);
+bool few_split_pays(const Sizes& a, int type);
 // Many rows (gemm_mx.hip; planes, terms or digits): the block shape and ranges of k tiles estimated
 // fastest (more than one range only if scratch memory may be used).
 struct Many {
   int shape, splits;
+  int block_rows, block_outs;  // (outputs of both matrices for a pair)
   double us;
 };
-Many plan_many(const Args& a, bool scratch);
+Many plan_many(const Sizes& a, bool scratch);
 void run_many(const Args& a, const Many& m, hipStream_t s);
+
+// What a product takes, from its sizes, type (an XType or X_PLANES), the stride of
+// its rows in bytes (planes: the larger one) and whether scratch memory may be used.
+struct Choice {
+  Kind kind;
+  bool prep;  // rows are split into scratch memory first
+  bool few;   // run_few, or run_many by
+  Many many;
+};
+constexpr int X_PLANES = 3;
+Choice choose(int n_out, int n_in, bool pair, int type, long long stride, int rows, bool scratch);
 
 }  // namespace mx
 }  // namespace pgd

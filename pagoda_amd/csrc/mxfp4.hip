@@ -210,18 +210,26 @@ __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x
   if (half == 0) ds[(size_t)tile * 64 + lane] = (uint8_t)e;
 }
 
+Sizes sizes_of(int n_out, int n_in, bool pair, int rows) {
+  Sizes a{};
+  a.n_out = n_out;
+  a.nt = mx_row_tiles(n_out);
+  a.kt = mx_k_tiles(n_in);
+  a.nblk = n_in / kMxBlock;
+  a.rows = rows;
+  a.pair = pair;
+  return a;
+}
+
 Args make_args(const QMat& w, const QMat* up, int rows, const MxOut& o) {
-  Args a{};
+  Args a{sizes_of(w.n_out, w.n_in, up != nullptr, rows)};
   a.w = w.p0;
   a.up = up ? up->p0 : nullptr;
-  a.n_out = w.n_out;
-  a.nt = mx_row_tiles(w.n_out);
-  a.kt = mx_k_tiles(w.n_in);
-  a.nblk = w.n_in / kMxBlock;
-  a.rows = rows;
   a.o = o;
   return a;
 }
+
+int terms_of(int type) { return type == X_F32 ? 3 : type == X_F16 ? 2 : 1; }
 
 // A captured graph would keep the address of scratch memory, which a later call
 // may replace: captured launches use none.
@@ -231,26 +239,20 @@ bool scratch_allowed(hipStream_t s) {
   return cap == hipStreamCaptureStatusNone;
 }
 
-// The plan of a launch: few, or many with their plan.
-struct Plan {
-  bool few;
-  Many many;
-  double us() const { return many.us; }
-};
-Plan plan(const Args& a, bool scratch) {
+// Few or many rows' kernel, for rows of a kind.
+Choice plan(const Sizes& a, size_t stride, bool scratch) {
   // (the many-row kernel's lanes hold offsets in 128 rows, and 16 row tiles of the matrix, in 32 bits)
-  const size_t stride = a.kind == PLANES ? std::max(a.p.ldc, a.p.lds) : a.ldx * 2;
-  Plan p{true, Many{0, 1, 1e30}};
-  if (a.kind == DIGITS || stride < ((size_t)1 << 24)) p = Plan{false, plan_many(a, scratch)};
-  if (a.kind == DIGITS) return p;
+  Choice c{a.kind, false, true, Many{0, 1, 0, 0, 1e30}};
+  if (a.kind == DIGITS || stride < ((size_t)1 << 24)) c.many = plan_many(a, scratch), c.few = false;
+  if (a.kind == DIGITS) return c;
   const double few = few_us(a);
-  if (few <= p.many.us) p = Plan{true, Many{0, 1, few}};
-  return p;
+  if (few <= c.many.us) c.few = true, c.many = Many{0, 1, 0, 0, few};
+  return c;
 }
 
-void run(const Args& a, const Plan& p, hipStream_t s) {
-  if (p.few) run_few(a, s);
-  else run_many(a, p.many, s);
+void run(const Args& a, const Choice& c, hipStream_t s) {
+  if (c.few) run_few(a, s);
+  else run_many(a, c.many, s);
 }
 
 void check(const QMat& w, const QMat* up, int rows) {
@@ -295,28 +297,47 @@ void mx_dequant(const QMat& m, int row0, int rows, float* out, hipStream_t s) {
   PGD_HIP(hipGetLastError());
 }
 
+Choice mx::choose(int n_out, int n_in, bool pair, int type, long long stride, int rows, bool scratch) {
+  Sizes a = sizes_of(n_out, n_in, pair, rows);
+  if (type == X_PLANES) {
+    a.kind = PLANES;
+    return plan(a, stride, scratch);
+  }
+  a.terms = terms_of(type);
+  a.kind = TERMS;
+  if (type == X_BF16 && n_in % kMxTileK == 0) return plan(a, stride, scratch);  // the rows are their own term
+  if (few_split_pays(a, type) || (!scratch && few_split_ok(rows, type))) return Choice{ROWS, false, true, Many{}};
+  const size_t ldt = (size_t)a.kt * kMxTileK;
+  Choice c = plan(a, ldt * 2, true);
+  if (type == X_F32 && rows > 16 && a.kt < (1 << 17)) {  // (lanes hold offsets in two of their row tiles in 32 bits)
+    // digits: 8.5 bytes of each value read and written instead of 10, and half the matrix
+    // instructions' time (333 rows to a pair of 17408 x 5120: 192 us, as terms 256). 16
+    // rows or fewer stay exact: reading the weights is their time either way.
+    a.kind = DIGITS;
+    const Choice d = plan(a, 0, true);
+    if (d.many.us + 8.5 / 4.5e6 * rows * ldt < c.many.us + 10 / 4.5e6 * rows * ldt) c = d;
+  }
+  c.prep = true;
+  return c;
+}
+
 void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, int rows, const MxOut& o, hipStream_t s) {
   check(w, up, rows);
   PGD_CHECK(type >= X_F32 && type <= X_BF16, kErrArg, "activations are f32 (0), f16 (1) or bf16 (2)");
   PGD_CHECK(ldx >= w.n_in && ldx % 8 == 0, kErrShape, "gemv ldx must be >= n_in and a multiple of 8");
   PGD_CHECK(reinterpret_cast<uintptr_t>(x) % 16 == 0, kErrArg, "MXFP4 activations must be 16-byte aligned");
   if (rows == 0) return;
-  Args a = make_args(w, up, rows, o);
-  a.terms = type == X_F32 ? 3 : type == X_F16 ? 2 : 1;
-  a.kind = TERMS;
   const bool scratch = scratch_allowed(s);
-  if (type == X_BF16 && w.n_in % kMxTileK == 0) {  // the rows are their own term
+  const Choice c = choose(w.n_out, w.n_in, up, type, (long long)ldx * xtype_bytes(type), rows, scratch);
+  Args a = make_args(w, up, rows, o);
+  a.kind = c.kind;
+  a.terms = terms_of(type);
+  a.ldx = ldx;
+  if (!c.prep) {  // TERMS: bf16 rows as they are, or ROWS
     a.x = static_cast<const uint16_t*>(x);
-    a.ldx = ldx;
-    run(a, plan(a, scratch), s);
-    return;
-  }
-  if (few_split_pays(a, type) || (!scratch && few_split_ok(rows, type))) {
-    a.kind = ROWS;
     a.raw = x;
     a.raw_type = type;
-    a.ldx = ldx;
-    run_few(a, s);
+    run(a, c, s);
     return;
   }
   PGD_CHECK(scratch, kErrState,
@@ -324,16 +345,6 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
             "rows, any bf16 rows of whole 128-column tiles, or MXFP4 rows");
   const int ldt = a.kt * kMxTileK;
   a.ldx = ldt;
-  Plan p = plan(a, true);
-  if (type == X_F32 && rows > 16 && a.kt < (1 << 17)) {  // (lanes hold offsets in two of their row tiles in 32 bits)
-    // digits: 8.5 bytes of each value read and written instead of 10, and half the matrix
-    // instructions' time (333 rows to a pair of 17408 x 5120: 192 us, as terms 256). 16
-    // rows or fewer stay exact: reading the weights is their time either way.
-    Args d = a;
-    d.kind = DIGITS;
-    const Plan pd = plan(d, true);
-    if (pd.us() + 8.5 / 4.5e6 * rows * ldt < p.us() + 10 / 4.5e6 * rows * ldt) a = d, p = pd;
-  }
   std::lock_guard<std::mutex> lock(g_terms);
   if (a.kind == DIGITS) {
     const long long tiles = (long long)((rows - 1) / 16 + 1) * a.kt;
@@ -357,7 +368,7 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
     else go(terms_kernel<X_BF16, 1>);
   }
   PGD_HIP(hipGetLastError());
-  run(a, p, s);
+  run(a, c, s);
 }
 
 void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, const MxOut& o, hipStream_t s) {
@@ -366,7 +377,7 @@ void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, 
   Args a = make_args(w, up, rows, o);
   a.p = x;
   a.kind = PLANES;
-  run(a, plan(a, scratch_allowed(s)), s);
+  run(a, choose(w.n_out, w.n_in, up, X_PLANES, std::max(x.ldc, x.lds), rows, scratch_allowed(s)), s);
 }
 
 }  // namespace pgd

@@ -1,0 +1,85 @@
+"""MXFP4 products of special values at sizes that take the many-row kernel (asserted):
+rounding of f32 rows held in digits, infinities and NaN, NaN blocks of weights."""
+import numpy as np
+import pytest
+
+import mxfp4 as mx
+from mxfp4_choice import BF16, F16, F32, MANY, PLANES, taken
+from test_gpu_mxfp4 import buf, matrix, run_planes, run_rows, weights  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def sizes(want):
+    """The sizes of MANY whose entry passes."""
+    return [c for c, v in MANY.items() if want(c, v)]
+
+
+def product(dev, buf, m, t, raw, up=None):
+    return run_planes(dev, buf, m, raw, up=up) if t == PLANES else run_rows(dev, buf, m, raw, t, up=up)
+
+
+@pytest.mark.parametrize("case", sizes(lambda c, v: v[0] == "digits" and not c[4]))
+def test_digits_round_to_their_step(dev, buf, case):
+    """One value a row whose weights are not zero, 2^8 to 2^29 below its block's largest,
+    1.5 2^e: rows are held within 2^-30 of the power of two above that one, and the product with
+    a weight of 2 bits is exact in f32, so outputs are off by 2^(e + 1 - 30) times the weight at
+    most. (30 bits with the sign: |x| < 2^(e + 1) as whole numbers up to 2^29 makes steps of
+    2^(e - 28), half of one 2^(e - 29). Three digits less are 2^15 times as far off.)"""
+    assert taken(*case) == MANY[case]
+    t, n, k, rows, _ = case
+    rng = np.random.default_rng(n + k)
+    codes, scales = weights(rng, n, k)
+    codes[:, 0::16] &= 0xF0  # each block's first element
+    wv = mx.values(codes, scales)
+    r = np.arange(rows)
+    col = rng.integers(0, k // 32, rows) * 32 + rng.integers(1, 32, rows)
+    e = rng.integers(-30, 30, rows)
+    x = np.zeros((rows, k), np.float32)
+    x[r, col // 32 * 32] = 1.5 * 2.0 ** e
+    x[r, col] = rng.uniform(-2, 2, rows) * 2.0 ** (e - rng.integers(8, 30, rows))
+    want = x[r, col].astype(np.float64)[:, None] * wv[:, col].T
+    got = run_rows(dev, buf, matrix(dev, (codes, scales)), x, t)
+    assert (np.abs(got - want) <= 2.0 ** (e - 29.0)[:, None] * np.abs(wv[:, col].T)).all()
+
+
+@pytest.mark.parametrize("case", sizes(lambda c, v: True))
+def test_nonfinite_stays_in_its_row_and_column(dev, buf, case):
+    """A NaN in a row's first block, an infinity in another's last and a NaN block of weights:
+    NaN for the first (and for f32 rows in digits the second), an infinity by the weight's sign
+    (NaN where the weight is zero) for the second otherwise, NaN in the weights' column. All
+    other outputs keep the bits that they have when the bad values are ordinary ones."""
+    assert taken(*case) == MANY[case]
+    t, n, k, rows, pair = case
+    rng = np.random.default_rng(n + k + rows)
+    w, u = weights(rng, n, k), weights(rng, n, k) if pair else None
+    w[1][n - 5, k // 32 - 1] = 255  # in the last k tile
+    wv = mx.values(*w)
+    m, up = matrix(dev, w), matrix(dev, u) if pair else None
+    nan_row, inf_row = rows // 2, rows - 1
+    if t == PLANES:
+        raw = weights(rng, rows, k, spread=5)
+        good = product(dev, buf, m, t, raw, up)
+        raw[1][nan_row, 0] = raw[1][inf_row, k // 32 - 1] = 255
+    else:
+        x = rng.normal(0, 1, (rows, k)).astype(np.float32)
+        raw, _ = mx.rows_of(x, t)
+        good = product(dev, buf, m, t, raw, up)
+        raw = raw.copy()
+        raw[nan_row, 3] = 0x7FC0 if t == BF16 else np.nan
+        raw[inf_row, k - 1] = 0x7F80 if t == BF16 else np.inf
+    got = product(dev, buf, m, t, raw, up)
+    assert np.isnan(good[:, n - 5]).all() and np.isnan(got[:, n - 5]).all()
+    live = np.arange(n) != n - 5
+    assert np.isfinite(good[:, live]).all()
+    assert np.isnan(got[nan_row]).all()
+    if t == PLANES or MANY[case][0] == "digits":
+        assert np.isnan(got[inf_row]).all()
+    elif not pair:
+        with np.errstate(invalid="ignore"):
+            assert np.array_equal(got[inf_row, live], (np.inf * wv[:, k - 1])[live], equal_nan=True)
+    else:  # (silu of minus infinity is NaN, as are products of infinities with zeros)
+        assert not np.isfinite(got[inf_row]).any()
+    rest = np.ones(rows, bool)
+    rest[[nan_row, inf_row]] = False
+    assert np.array_equal(got[rest][:, live].view(np.uint32), good[rest][:, live].view(np.uint32))
