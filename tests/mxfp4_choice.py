@@ -85,6 +85,11 @@ MANY = {
     (PLANES, 40, 4128, 47, True): ("planes", (32, 128), "+"),
 }
 
+# The few-row kernel: rows split inside the launch, terms and planes in 1 to 4 row tiles.
+FEW = [(F32, 333, 416, 1, False), (F32, 333, 416, 5, True), (F32, 100, 896, 16, False), (F32, 100, 160, 40, True),
+       (F16, 333, 416, 8, False), (F16, 100, 160, 20, False), (F16, 100, 160, 70, False), (BF16, 333, 416, 4, False),
+       (BF16, 100, 160, 40, False), (PLANES, 333, 416, 9, False), (PLANES, 100, 160, 40, True), (PLANES, 100, 160, 70, False)]
+
 
 def taken(t: int, n: int, k: int, rows: int, pair: bool) -> tuple:
     c = choice(t, n, k, rows, pair)

@@ -5,7 +5,7 @@ from pathlib import Path
 
 import pytest
 
-from mxfp4_choice import BF16, F16, F32, MANY, PLANES, choice, taken
+from mxfp4_choice import BF16, F16, F32, FEW, MANY, PLANES, choice, taken
 from test_gpu_mxfp4_launches import LAUNCHES
 
 # block shapes of the many-row kernel
@@ -45,6 +45,11 @@ def test_few_rows_and_captures():
     for rows in (1, 16, 47, 333, 4000):
         c = choice(PLANES, 5120, 4096, rows, scratch=False)
         assert c.ranges == 1 and not c.prep
+
+
+def test_few_sizes_take_the_few_row_kernel():
+    got = [choice(*c) for c in FEW]
+    assert all(not c.block for c in got) and {c.kind for c in got} == {"rows", "terms", "planes"}
 
 
 def test_f32_rows_are_exact_up_to_16():
