@@ -135,12 +135,13 @@ int pgd_matrix_gemv(const pgd_matrix* m, const float* x, int nrows, float* y);
  * x_f16 is f16), and x must be 16-byte aligned. Sums are f32. f16 and bf16 rows and
  * up to 16 f32 rows enter the products exactly (f32 but for bits below 2^-133). More
  * f32 rows may be held, block of 32 by block, to 2^-30 of the power of two above the
- * block's largest magnitude (2^-131 at the finest), and an infinity among them makes
- * its row NaN. The order of the sums depends on the matrix, the number and type of
- * rows and whether the stream is captured, on nothing else. In a stream capture, rows
- * that would need scratch memory are PGD_ERR_STATE and queue nothing: all but up to 5
- * f32, 8 f16 or 4 bf16 rows and bf16 rows of n_in % 128 == 0 (the same holds for
- * pgd_matrix_gemv_swiglu_dev; MXFP4 rows are never refused). */
+ * block's largest magnitude (2^-130 at the finest); an infinity among them makes
+ * its row NaN, and a result past the largest f32 is an infinity or NaN. A caller who
+ * needs f32 rows exact passes at most 16 a call. The order of the sums depends on the
+ * matrix, the number and type of rows and whether the stream is captured, on nothing
+ * else. In a stream capture, rows that would need scratch memory are PGD_ERR_STATE and
+ * queue nothing: all but up to 5 f32, 8 f16 or 4 bf16 rows and bf16 rows of n_in % 128
+ * == 0 (the same holds for pgd_matrix_gemv_swiglu_dev; MXFP4 rows are never refused). */
 int pgd_matrix_gemv_dev(const pgd_matrix* m, const void* x, int x_f16, int ldx, int nrows, float* y,
                         int ldy, const float* res, int ldres);
 /* mid = silu(gate . x) * (up . x); replaces affine_gemv2_silu

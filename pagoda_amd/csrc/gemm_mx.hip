@@ -437,6 +437,12 @@ __global__ __launch_bounds__(64 * T::W, T::W * T::OCC / 4) void gemm_kernel(Args
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS outlives the workgroup
+  if constexpr (T::DIG) {  // (digits are held at half their worth)
+#pragma unroll
+    for (int n = 0; n < NF; ++n)
+#pragma unroll
+      for (int m = 0; m < MF; ++m) acc[n][m] *= 2.0f;
+  }
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
     const uint32_t r = (uint32_t)m0 + (wm * MF + m) * 16 + i16;

@@ -144,19 +144,22 @@ __global__ __launch_bounds__(256) void terms_kernel(const void* __restrict__ x, 
   }
 }
 
-// The 6-bit codes of three digits at once: digit plus 16 in bits 0..4, 10..14 and 20..24
-// (others ignored) to a sign over a magnitude of 0..16 in bits 0..5, 10..15 and 20..25.
+// The 6-bit codes of three digits at once: 16 less the digit in bits 0..4, 10..14 and 20..24
+// (others ignored) to a sign over a magnitude of 0..16 in bits 0..5, 10..15 and 20..25 (0 is -0).
 __device__ __forceinline__ uint32_t digit_codes(uint32_t b) {
-  const uint32_t neg = ~(b >> 4) & 0x100401;
-  return (((b & 0xf03c0f) ^ neg * 15) + neg) | neg << 5;  // (below 16: 16 less the low bits)
+  const uint32_t minus = (b >> 4) & 0x100401, plus = minus ^ 0x100401;
+  return (((b & 0xf03c0f) ^ plus * 15) + plus) | minus << 5;  // (below 16: 16 less the low bits)
 }
 
 // f32 rows in six base-32 digits. A block with largest magnitude below 2^(e - 126) (e
-// the biased exponent, 25 at least) is held in steps of 2^(e - 155): 30 bits, so
+// the biased exponent, 26 at least) is held in steps of 2^(e - 155): 30 bits, so
 // its values are exact to the last of their 24 where they are above 1/64 of the
 // largest, and within 2^-30 of it elsewhere (f32 sums of its products keep 24).
-// Digits -16..15 of that whole number, the top one to 16, are e2m3 codes (u / 8 is
-// code u up to 16), digit i scaled by 2^(e - 127 - 5 i). A tile of 16 rows by 128
+// Digits -15..16 of that whole number, the top one from -16, are e2m3 codes (u / 8 is
+// code u up to 16), digit i scaled by 2^(e - 128 - 5 i): half its worth, the products'
+// kernel doubles its sums. Leading digits are up to 31/16 of their value (the others add up
+// to less than 32^i 16/31 in digit i's unit), so halves stay below 2^128 whatever digits are
+// still to come, wherever the magnitudes of the products add up to less. A tile of 16 rows by 128
 // columns goes to 128 threads, half a block each (of lane l: block l / 16 of row l %
 // 16). A block with an infinity or NaN is NaN. Rows and columns past the matrix are
 // zeros. 333 rows of 5120: 7.8 us, latency (420 workgroups; one thread a block 8.8);
@@ -178,7 +181,7 @@ __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x
 #pragma unroll
   for (int i = 0; i < 16; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i >> 3][i & 7]) & 0x7fffffffu);
   top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-  const int e = max((int)(top >> 23), 25);
+  const int e = max((int)(top >> 23), 26);
   uint32_t q[6][3] = {};  // [digit][dword]
   if (e != 255) {
     // (2^(155 - e) in two factors: it may pass the largest f32)
@@ -186,14 +189,15 @@ __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x
     const float up2 = __builtin_bit_cast(float, (uint32_t)(127 + (155 - e) - (155 - e) / 2) << 23);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      // (16 more in each of the lower five digits: their bits are then the digits plus 16)
-      const int n = __float2int_rn(v[i >> 3][i & 7] * up * up2) + 0x1084210;
+      // (of the negative, whose digits are -16..15; 16 more in each of the lower five: their
+      // bits are then 16 less the value's digits)
+      const int n = 0x1084210 - __float2int_rn(v[i >> 3][i & 7] * up * up2);
       const int u = n >> 25;
       const uint32_t c5 = digit_codes((uint32_t)n), c4 = digit_codes((uint32_t)n >> 5);
 #pragma unroll
       for (int k = 0; k < 6; ++k) {
         const uint32_t code = k ? (k & 1 ? c5 : c4) >> (k < 2 ? 20 : k < 4 ? 10 : 0) & 63
-                                : (uint32_t)abs(u) | (u < 0 ? 32u : 0u);
+                                : (uint32_t)abs(u) | (u > 0 ? 32u : 0u);
         const int bit = 6 * i, w = bit >> 5, o = bit & 31;
         q[k][w] |= code << o;
         if (o > 26) q[k][w + 1] |= code >> (32 - o);
@@ -207,7 +211,7 @@ __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x
     if (half == 0) *reinterpret_cast<uint4*>(out + k * 1024 + lane * 16) = make_uint4(q[k][0], q[k][1], q[k][2], fourth);
     else *reinterpret_cast<uint2*>(out + 6144 + k * 512 + lane * 8) = make_uint2(q[k][1], q[k][2]);
   }
-  if (half == 0) ds[(size_t)tile * 64 + lane] = (uint8_t)e;
+  if (half == 0) ds[(size_t)tile * 64 + lane] = (uint8_t)(e == 255 ? 255 : e - 1);
 }
 
 Sizes sizes_of(int n_out, int n_in, bool pair, int rows) {

@@ -83,3 +83,66 @@ def test_nonfinite_stays_in_its_row_and_column(dev, buf, case):
     rest = np.ones(rows, bool)
     rest[[nan_row, inf_row]] = False
     assert np.array_equal(got[rest][:, live].view(np.uint32), good[rest][:, live].view(np.uint32))
+
+
+DIGITS = sizes(lambda c, v: v[0] == "digits" and not c[4])
+
+
+@pytest.mark.parametrize("case", DIGITS)
+def test_digits_near_the_largest_number(dev, buf, case):
+    """Products just below 2^128, exact in f32: no leading digits of a value, rounded up, may
+    carry a sum past it. Rows in turn: a value of all ones (the digits of its leading half are
+    2^128 with the weight); the same far below the largest f32, under large weights; three
+    values beside an outlier whose top digit is 1.9375 times each; negated."""
+    assert taken(*case) == MANY[case]
+    t, n, k, rows, _ = case
+    rng = np.random.default_rng(n + k)
+    # each block: a zero weight, then ones of the output's sign; scales 1, 2^20 and 8 in turn
+    sign = rng.integers(0, 2, n).astype(np.uint8) * 0x88
+    codes = np.tile((0x22 | sign)[:, None], (1, k // 2)).astype(np.uint8)
+    codes[:, 0::16] &= 0xF0
+    scales = np.tile(np.resize(np.array([127, 147, 130], np.uint8), k // 32), (n, 1))
+    x = np.zeros((rows, k), np.float32)
+    r = np.arange(rows)
+    block = rng.integers(0, k // 96, rows) * 3 + r % 3
+    big = 2.0 ** 128 - 2.0 ** 104  # the largest f32
+    col = block * 32 + rng.integers(1, 28, rows)
+    x[r, col] = np.where(r % 3 == 1, big * 2.0 ** -20, big)
+    far = r[r % 3 == 2]
+    x[far, col[far]] = 0
+    x[far, block[far] * 32] = 2.0 ** 127  # steps of 2^99
+    for i in range(3):  # in those steps 32^5 / 1.9375, so a top digit of 1: 2^124, times 8 and thrice
+        x[far, col[far] + i] = float.fromhex("0x1084212p99")
+    x[r % 2 == 1] *= -1
+    w = mx.values(codes, scales)
+    want = x.astype(np.float64) @ w.T
+    assert np.abs(want).max() < 2.0 ** 128 and (np.abs(want) > 2.0 ** 127).all()
+    got = run_rows(dev, buf, matrix(dev, (codes, scales)), x, t)
+    # (three values: two additions of numbers below 2^128, each at most 2^-23 of the sum off, per digit)
+    assert (np.abs(got - want) <= 12 * 2.0 ** -23 * np.abs(want)).all()
+    one = r % 3 < 2
+    assert np.array_equal(got[one], want[one])
+
+
+@pytest.mark.parametrize("case", DIGITS)
+def test_digits_below_the_normal_range(dev, buf, case):
+    """One value a row, 2^-140 to 2^-95, under weights of 2^100 times their codes: blocks below
+    2^-100 are held in steps of 2^-129. Then large values under weights of the smallest scale,
+    whose products are exact."""
+    assert taken(*case) == MANY[case]
+    t, n, k, rows, _ = case
+    rng = np.random.default_rng(n + k)
+    r, col = np.arange(rows), rng.integers(0, k, rows)
+    x = np.zeros((rows, k), np.float32)
+    x[r, col] = rng.uniform(-2, 2, rows) * 2.0 ** rng.integers(-140, -95, rows)
+    codes = rng.integers(0, 256, (n, k // 2), dtype=np.uint8)
+    w = codes, np.full((n, k // 32), 227, np.uint8)
+    wv = mx.values(*w)[:, col].T
+    want = x[r, col].astype(np.float64)[:, None] * wv
+    got = run_rows(dev, buf, matrix(dev, w), x, t)
+    # (five additions of digits of up to 24 bits)
+    assert (np.abs(got - want) <= 2.0 ** -130 * np.abs(wv) + 10 * 2.0 ** -23 * np.abs(want)).all()
+    x = np.where(x != 0, np.float32(1.25 * 2.0 ** 100), np.float32(0))
+    w = codes, np.zeros((n, k // 32), np.uint8)
+    want = x[r, col].astype(np.float64)[:, None] * mx.values(*w)[:, col].T
+    assert np.array_equal(run_rows(dev, buf, matrix(dev, w), x, t), want)
