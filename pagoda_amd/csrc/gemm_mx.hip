@@ -492,7 +492,7 @@ template <class T, int EPI>
 void launch_blocks(const Args& a, hipStream_t s) {
   const int nb = EPI == MX_SWIGLU || EPI == MX_PART2 ? T::BN / 32 : T::BN / 16;
   const long long nmb = (a.rows + (long long)T::BM - 1) / T::BM, nnb = (a.nt + nb - 1) / nb;
-  PGD_CHECK(nmb * nnb * a.splits < (1ll << 30), kErrShape, "too many outputs for one MXFP4 product");
+  PGD_CHECK(nmb * nnb * a.splits <= kMaxGroups, kErrShape, "too many outputs for one MXFP4 product");
   const int per_xcd = (int)((nmb * nnb * a.splits + 7) / 8);
   PGD_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, EPI>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS));
@@ -569,6 +569,7 @@ constexpr Cost kDigits[] = {{32, 256, 6.56f, 1.218f, 2.22f, 0.796f, 0.78f, 2.19f
 double cost_us(const Cost& c, const Sizes& a, int splits) {
   const int pair = a.pair ? 2 : 1;
   const long long blocks = (((long long)a.rows + c.bm - 1) / c.bm) * ((a.nt * 16ll * pair + c.bn - 1) / c.bn) * splits;
+  if (blocks > kMaxGroups) return 1e30;
   const long long per_cu = (blocks + 255) / 256;
   const double stages = (a.kt + splits - 1) / splits * (a.kind == TERMS ? a.terms : 1);
   double us = c.launch + (double)(per_cu / 2) * (stages * c.stage2 + c.block2);

@@ -275,8 +275,23 @@ __global__ __launch_bounds__(64 * KW) void few_kernel(Args a, int chunk, bool ve
 }
 
 template <int KIND, int MT, int EPI>
-void launch(const Args& a, int chunk, hipStream_t s) {
+void launch(Args a, int chunk, hipStream_t s) {
   constexpr int NT = EPI == MX_SWIGLU || MT > 2 ? 1 : 2;
+  // (a grid has kMaxGroups workgroups in x: the row tiles past them go to a launch of their
+  // own; a multiple of 32 of them, so that steps and 16-byte stores stay whole)
+  constexpr int kTiles = (int)(kMaxGroups / 32 * 32) * NT;
+  if (a.nt > kTiles) {
+    Args rest = a;
+    rest.nt -= kTiles;
+    rest.n_out -= kTiles * kMxTileN;
+    rest.w += mx_code_off(kTiles, 0, a.kt);
+    if (a.up) rest.up += mx_code_off(kTiles, 0, a.kt);
+    rest.o.y += (size_t)kTiles * kMxTileN;
+    if (a.o.res) rest.o.res += (size_t)kTiles * kMxTileN;
+    launch<KIND, MT, EPI>(rest, chunk, s);
+    a.nt = kTiles;
+    a.n_out = kTiles * kMxTileN;
+  }
   // (grid y is at most 65535: the rest goes to further launches)
   Args b = a;
   for (long long r0 = 0; r0 < a.rows; r0 += b.rows) {

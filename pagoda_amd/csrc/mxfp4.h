@@ -72,6 +72,9 @@ void mx_gemv_planes(const QMat& w, const QMat* up, const MxPlanes& x, int rows, 
 namespace mx {
 
 constexpr int kMxDigitTile = 9216;  // 6 digits of 24 B a lane
+// Workgroups of 256 threads of one launch, a multiple of 64: HIP takes grid sizes of less
+// than 2^32 threads.
+constexpr long long kMaxGroups = (1 << 24) - 64;
 
 // How a launch holds its activation rows:
 //   PLANES  p: the MXFP4 planes

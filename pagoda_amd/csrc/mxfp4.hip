@@ -233,6 +233,8 @@ Args make_args(const QMat& w, const QMat* up, int rows, const MxOut& o) {
   return a;
 }
 
+long long digit_tiles(const Sizes& a) { return (long long)((a.rows - 1) / 16 + 1) * a.kt; }
+
 int terms_of(int type) { return type == X_F32 ? 3 : type == X_F16 ? 2 : 1; }
 
 // A captured graph would keep the address of scratch memory, which a later call
@@ -313,7 +315,8 @@ Choice mx::choose(int n_out, int n_in, bool pair, int type, long long stride, in
   if (few_split_pays(a, type) || (!scratch && few_split_ok(rows, type))) return Choice{ROWS, false, true, Many{}};
   const size_t ldt = (size_t)a.kt * kMxTileK;
   Choice c = plan(a, ldt * 2, true);
-  if (type == X_F32 && rows > 16 && a.kt < (1 << 17)) {  // (lanes hold offsets in two of their row tiles in 32 bits)
+  // (lanes hold offsets in two of the digits' row tiles in 32 bits, and two tiles go to a workgroup)
+  if (type == X_F32 && rows > 16 && a.kt < (1 << 17) && digit_tiles(a) <= 2 * kMaxGroups) {
     // digits: 8.5 bytes of each value read and written instead of 10, and half the matrix
     // instructions' time (333 rows to a pair of 17408 x 5120: 192 us, as terms 256). 16
     // rows or fewer stay exact: reading the weights is their time either way.
@@ -351,8 +354,7 @@ void mx_gemv(const QMat& w, const QMat* up, const void* x, int type, int ldx, in
   a.ldx = ldt;
   std::lock_guard<std::mutex> lock(g_terms);
   if (a.kind == DIGITS) {
-    const long long tiles = (long long)((rows - 1) / 16 + 1) * a.kt;
-    PGD_CHECK(tiles < (1ll << 25), kErrShape, "too many activations for one MXFP4 product");
+    const long long tiles = digit_tiles(a);
     auto* d = static_cast<uint8_t*>(gemv::gemv_scratch(s, (size_t)tiles * (kMxDigitTile + 64), 8));
     auto* ds = d + (size_t)tiles * kMxDigitTile;
     a.d = d;

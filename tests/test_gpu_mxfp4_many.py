@@ -4,8 +4,9 @@ import numpy as np
 import pytest
 
 import mxfp4 as mx
-from mxfp4_choice import BF16, F16, F32, MANY, PLANES, taken
+from mxfp4_choice import BF16, F16, F32, MANY, PLANES, choice, taken
 from test_gpu_mxfp4 import buf, matrix, run_planes, run_rows, weights  # noqa: F401
+from test_gpu_mxfp4_launches import big, fill, put  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -146,3 +147,58 @@ def test_digits_below_the_normal_range(dev, buf, case):
     w = codes, np.zeros((n, k // 32), np.uint8)
     want = x[r, col].astype(np.float64)[:, None] * mx.values(*w)[:, col].T
     assert np.array_equal(run_rows(dev, buf, matrix(dev, w), x, t), want)
+
+
+@pytest.mark.parametrize("t", [F32, PLANES])
+@pytest.mark.parametrize("n,pair", [((1 << 28) + 77, True), ((1 << 29) + 77, False)])
+def test_outputs_past_one_launch(big, t, n, pair):
+    """Row tiles of a matrix that need more workgroups of the few-row kernel than a grid
+    holds (one or two of them each): most weights are zeros, the others lie at both ends and
+    around the place where the second launch begins."""
+    from pagoda_amd import Matrix
+
+    dev, buf = big
+    rng = np.random.default_rng(n + t)
+    k, rows, ld = 32, 2, 16
+    assert not choice(t, n, k, rows, pair).block
+    pc, ps, py = dev.alloc(n * ld), dev.alloc(n * ld), dev.alloc(rows * n * 4)
+    buf.ptrs += [pc, ps, py]
+    fill(dev, pc, 0, n * ld)
+    fill(dev, ps, 127, n * ld)
+    cut = ((1 << 24) - 64) * (1 if pair else 2) * 16
+    ws = []
+    for r0 in (0, cut - 100, n - 200):
+        codes, _ = weights(rng, 200, k)
+        ws.append((r0, codes))
+        put(dev, pc + r0 * ld, codes)
+    m = Matrix.from_mxfp4_dev(dev, pc, ld, ps, ld, n, k)
+    if t == PLANES:
+        raw = weights(rng, rows, k)
+        x = mx.values(*raw)
+        xs = buf.up(mx.padded(raw[0], ld, np.uint8(0))), ld, buf.up(mx.padded(raw[1], ld, np.uint8(0))), ld
+        if pair:
+            Matrix.gemv_swiglu_mx_dev(m, m, *xs, rows, py, n)
+        else:
+            m.gemv_mx_dev(*xs, rows, py, n)
+    else:
+        x = rng.normal(0, 1, (rows, k)).astype(np.float32)
+        px = buf.up(x)
+        x = x.astype(np.float64)
+        if pair:
+            Matrix.gemv_swiglu_dev(m, m, px, k, rows, py, n)
+        else:
+            m.gemv_dev(px, k, rows, py, n)
+    for r in range(rows):
+        for r0, codes in ws:
+            at = max(r0 - 100, 0)
+            got = dev.download(py + (r * n + at) * 4, (min(500, n - at),), np.float32)
+            live = got[r0 - at:r0 - at + 200]
+            wv = mx.values(codes, np.full((200, 1), 127, np.uint8))
+            y, xr = x[r] @ wv.T, x[r:r + 1]
+            if pair:
+                assert (np.abs(live - mx.silu(y) * y) <= mx.swiglu_bound(xr, wv, wv)[0]).all()
+            else:
+                assert (np.abs(live - y) <= mx.product_bound(xr, wv)[0]).all()
+            assert not got[:r0 - at].any() and not got[r0 - at + 200:].any()
+    m.free()
+    buf.close()

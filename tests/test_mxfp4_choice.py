@@ -64,3 +64,21 @@ def test_long_strides_stay_in_the_few_row_kernel():
     assert choice(BF16, 2100, 512, 1100, stride=(1 << 24) - 16).block
     assert not choice(BF16, 2100, 512, 1100, stride=1 << 24).block
     assert not choice(PLANES, 5008, 160, 1300, stride=1 << 24).block
+
+
+def test_launches_stay_below_2_32_threads():
+    """The largest matrices and most rows: the many-row kernel's workgroups of 256 threads, and
+    the digits' (two tiles of 16 rows by 128 columns each), fit one launch of HIP."""
+    for n, k, rows in ((1 << 30, 32, 65), (1 << 30, 32, 129), (1 << 30, 128, 4096), (1 << 24, 64, 1 << 20),
+                       (4096, 128, (1 << 31) - 1), (151936, 896, 1 << 26), (32, 1 << 24, 4096), (32, 1 << 23, 8192)):
+        for t in (F32, F16, BF16, PLANES):
+            for pair in (False, True):
+                if pair and t in (F16, BF16):
+                    continue
+                c = choice(t, n, k, rows, pair)
+                if c.block:
+                    outs = -(-n // 16) * 16 * (2 if pair else 1)
+                    blocks = -(-rows // c.block[0]) * -(-outs // c.block[1]) * c.ranges
+                    assert -(-blocks // 8) * 8 * 256 < 1 << 32, (t, n, k, rows, pair, c)
+                if c.kind == "digits":
+                    assert -(-rows // 16) * -(-k // 128) // 2 * 256 < (1 << 32) - 256, (n, k, rows)
