@@ -53,13 +53,18 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 // 64 lanes' 16 (4) bytes from base + off to consecutive places from the LDS
 // address `to` on. Written in assembly (no output registers) because the
 // compiler would otherwise let later LDS reads wait for these loads to land;
-// the waits are the kernel's own.
+// the waits are the kernel's own. m0 is named as written: the compiler would
+// else use a value it put there before (it warns that m0 is reserved: it keeps
+// no variable there, which is what an m0 to be preserved would be).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(to)), "v"(off), "s"(uniform(base)) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(to)), "v"(off), "s"(uniform(base)) : "memory", "m0");
 }
 __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(uniform(to)), "v"(off), "s"(uniform(base)) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(uniform(to)), "v"(off), "s"(uniform(base)) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 template <int KIND_, int BM_, int BN_, int WM_, int WN_, int S_, int OCC_ = 1>
 struct Shape {
