@@ -92,7 +92,7 @@ int pgd_matrix_upload_q5_0(pgd_dev* dev, const void* blocks, int n_out, int n_in
  * nibble of byte i, and one scale byte per block. Format id 5 in
  * pgd_matrix_info; pgd_matrix_dequant, pgd_matrix_gemv, pgd_matrix_gemv_dev and
  * pgd_matrix_gemv_swiglu_dev take these matrices too. n_in is a multiple of 32, both
- * sides are at most 2^30.
+ * sides are at most 2^30. In a stream capture no matrix is made (PGD_ERR_STATE).
  *
  * upload: host planes, codes [n_out][n_in / 2], scales [n_out][n_in / 32]. */
 int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* scales, int n_out, int n_in,

@@ -221,6 +221,11 @@ static void mx_dims(int n_out, int n_in) {
   PGD_CHECK(n_in % kMxBlock == 0, kErrShape, "MXFP4 n_in must be a multiple of 32");
 }
 
+// (a capture would record the filling of a new matrix, a memset among it, for replays to run)
+static void mx_not_captured(const pgd_dev* dev) {
+  PGD_CHECK(!capturing(dev->stream), kErrState, "an MXFP4 matrix cannot be made in a stream capture");
+}
+
 int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* scales, int n_out, int n_in,
                             pgd_matrix** out) {
   pgd_matrix* held = nullptr;
@@ -228,6 +233,7 @@ int pgd_matrix_upload_mxfp4(pgd_dev* dev, const uint8_t* codes, const uint8_t* s
     PGD_CHECK(codes && scales, kErrArg, "null argument");
     mx_dims(n_out, n_in);
     DeviceScope scope(dev);
+    mx_not_captured(dev);
     new_matrix(dev, FMT_MXFP4, n_out, n_in, out, &held);
     const size_t nc = (size_t)n_out * (n_in / 2), ns = (size_t)n_out * (n_in / kMxBlock);
     DevBuf c(nc), sc(ns);
@@ -260,6 +266,7 @@ int pgd_matrix_from_mxfp4_dev(pgd_dev* dev, const uint8_t* codes, int ldc, const
     mx_dims(n_out, n_in);
     const MxPlanes p = planes(codes, ldc, scales, lds, n_in);
     DeviceScope scope(dev);
+    mx_not_captured(dev);
     new_matrix(dev, FMT_MXFP4, n_out, n_in, out, &held);
     mx_tile(held->m, p, dev->stream);
     *out = held;

@@ -45,6 +45,13 @@ struct Error {
     if (!(cond)) throw ::pgd::Error{(code), (msg)};  \
   } while (0)
 
+// Whether what is queued on s is recorded into a graph.
+inline bool capturing(hipStream_t s) {
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  PGD_HIP(hipStreamIsCapturing(s, &cap));
+  return cap != hipStreamCaptureStatusNone;
+}
+
 // ---------------------------------------------------------------------------
 // exact conversions (bit level, identical on host and device)
 // ---------------------------------------------------------------------------

@@ -239,11 +239,7 @@ int terms_of(int type) { return type == X_F32 ? 3 : type == X_F16 ? 2 : 1; }
 
 // A captured graph would keep the address of scratch memory, which a later call
 // may replace: captured launches use none.
-bool scratch_allowed(hipStream_t s) {
-  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-  PGD_HIP(hipStreamIsCapturing(s, &cap));
-  return cap == hipStreamCaptureStatusNone;
-}
+bool scratch_allowed(hipStream_t s) { return !capturing(s); }
 
 // Few or many rows' kernel, for rows of a kind.
 Choice plan(const Sizes& a, size_t stride, bool scratch) {

@@ -6,7 +6,7 @@ import pytest
 import mxfp4 as mx
 from mxfp4_choice import BF16, F16, F32, MANY, PLANES, choice, taken
 from test_gpu_mxfp4 import buf, matrix, run_planes, run_rows, weights  # noqa: F401
-from test_gpu_mxfp4_launches import big, fill, put  # noqa: F401
+from test_gpu_mxfp4_launches import Graph, big, fill, put  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -202,3 +202,34 @@ def test_outputs_past_one_launch(big, t, n, pair):
             assert not got[:r0 - at].any() and not got[r0 - at + 200:].any()
     m.free()
     buf.close()
+
+
+def test_capture_refuses_to_make_a_matrix(dev, buf):
+    """Its filling would be recorded, a memset among it. Refused before anything is queued: the
+    capture goes on, its replays run what else it holds, and the same calls work after it."""
+    from pagoda_amd import Matrix, PagodaError
+
+    rng = np.random.default_rng(3)
+    w = weights(rng, 48, 96)
+    m, wv = matrix(dev, w), mx.values(*w)
+    x = rng.normal(0, 1, (4, 96)).astype(np.float32)
+    px, py, pc, ps = buf.up(x), buf.up(np.zeros((4, 48), np.float32)), buf.up(w[0]), buf.up(mx.padded(w[1], 16, np.uint8(0)))
+    made = []
+
+    def calls():
+        for make in (lambda: Matrix.from_mxfp4_dev(dev, pc, 48, ps, 16, 48, 96), lambda: matrix(dev, w)):
+            with pytest.raises(PagodaError) as e:
+                made.append(make())
+            assert e.value.code == -5
+        m.gemv_dev(px, 96, 4, py, 48, F32)
+
+    g = Graph(dev, calls)
+    assert not made
+    want, bound = x.astype(np.float64) @ wv.T, mx.product_bound(x.astype(np.float64), wv)
+    for _ in range(3):
+        put(dev, py, np.zeros((4, 48), np.float32))
+        g.replay()
+        assert (np.abs(buf.down(py, np.zeros((4, 48), np.float32)) - want) <= bound).all()
+        for again in (Matrix.from_mxfp4_dev(dev, pc, 48, ps, 16, 48, 96), matrix(dev, w)):
+            assert np.array_equal(again.dequant(), wv.astype(np.float32))
+    g.close()
