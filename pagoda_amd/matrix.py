@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+from operator import index
 
 import numpy as np
 
@@ -18,6 +19,10 @@ def _ptr(a: np.ndarray) -> C.c_void_p:
     return a.ctypes.data_as(C.c_void_p)
 
 
+# Device addresses go to the library as index(p or 0): whole numbers, or None for none. (ctypes
+# would also take bytes, strings and arrays, as the addresses of host memory.)
+
+
 def act_bytes(nrows: int, k: int) -> int:
     from ._lib import lib
 
@@ -31,8 +36,8 @@ def act_prep_dev(dev: Device, x_ptr: int, ldx: int, nrows: int, k: int, act_ptr:
 def mxfp4_quantize_dev(dev: Device, x_ptr: int, x_type: int, ldx: int, nrows: int, k: int, codes_ptr: int, ldc: int,
                        scales_ptr: int, lds: int, values_ptr: int = 0, ldv: int = 0) -> None:
     """Rows of f32 / f16 / bf16 (x_type) to MXFP4 planes; values_ptr also receives the values they stand for."""
-    call("pgd_mxfp4_quantize_dev", dev.handle, x_ptr, x_type, ldx, nrows, k, codes_ptr, ldc, scales_ptr, lds,
-         values_ptr, ldv)
+    call("pgd_mxfp4_quantize_dev", dev.handle, index(x_ptr or 0), x_type, ldx, nrows, k, index(codes_ptr or 0), ldc,
+         index(scales_ptr or 0), lds, index(values_ptr or 0), ldv)
 
 
 class Matrix:
@@ -123,7 +128,8 @@ class Matrix:
     def gemv_dev(self, x_ptr: int, ldx: int, nrows: int, y_ptr: int, ldy: int, x_f16: int = False,
                  res_ptr: int = 0, ldres: int = 0) -> None:
         """x_f16: f32 rows (False), f16 (True), or for MXFP4 matrices X_F32 / X_F16 / X_BF16."""
-        call("pgd_matrix_gemv_dev", self.handle, x_ptr, int(x_f16), ldx, nrows, y_ptr, ldy, res_ptr, ldres)
+        call("pgd_matrix_gemv_dev", self.handle, index(x_ptr or 0), int(x_f16), ldx, nrows, index(y_ptr or 0), ldy,
+             index(res_ptr or 0), ldres)
 
     def gemv_q8act_dev(self, x_ptr: int, ldx: int, nrows: int, y_ptr: int, ldy: int, res_ptr: int = 0,
                        ldres: int = 0) -> None:
@@ -147,14 +153,16 @@ class Matrix:
 
     @staticmethod
     def gemv_swiglu_dev(gate: "Matrix", up: "Matrix", x_ptr: int, ldx: int, nrows: int, mid_ptr: int, ldm: int):
-        call("pgd_matrix_gemv_swiglu_dev", gate.handle, up.handle, x_ptr, ldx, nrows, mid_ptr, ldm)
+        call("pgd_matrix_gemv_swiglu_dev", gate.handle, up.handle, index(x_ptr or 0), ldx, nrows, index(mid_ptr or 0), ldm)
 
     def gemv_mx_dev(self, codes_ptr: int, ldc: int, scales_ptr: int, lds: int, nrows: int, y_ptr: int, ldy: int,
                     res_ptr: int = 0, ldres: int = 0) -> None:
         """MXFP4 rows (planes) times this MXFP4 matrix."""
-        call("pgd_matrix_gemv_mx_dev", self.handle, codes_ptr, ldc, scales_ptr, lds, nrows, y_ptr, ldy, res_ptr, ldres)
+        call("pgd_matrix_gemv_mx_dev", self.handle, index(codes_ptr or 0), ldc, index(scales_ptr or 0), lds, nrows,
+             index(y_ptr or 0), ldy, index(res_ptr or 0), ldres)
 
     @staticmethod
     def gemv_swiglu_mx_dev(gate: "Matrix", up: "Matrix", codes_ptr: int, ldc: int, scales_ptr: int, lds: int,
                            nrows: int, mid_ptr: int, ldm: int):
-        call("pgd_matrix_gemv_swiglu_mx_dev", gate.handle, up.handle, codes_ptr, ldc, scales_ptr, lds, nrows, mid_ptr, ldm)
+        call("pgd_matrix_gemv_swiglu_mx_dev", gate.handle, up.handle, index(codes_ptr or 0), ldc, index(scales_ptr or 0),
+             lds, nrows, index(mid_ptr or 0), ldm)
