@@ -14,19 +14,22 @@
 // the same f32 sums. Rows in digits (mxfp4.hip) take six matrix instructions of the
 // 4-bit rate instead of three terms' twelve of the bf16 rate.
 //
-// Measured, weights from HBM (17408 x 5120 unless given; MFMA: share of cycles the
+// Measured, inputs from HBM (17408 x 5120 unless given; MFMA: share of cycles the
 // matrix units are busy):
-//   4096 MXFP4 rows          247 us  2.95 PFLOP/s  MFMA 38%   blocks of 128 x 256
-//   2048 MXFP4 rows, pair    230 us  3.17 PFLOP/s       42%   128 x 256
-//   48 MXFP4 rows, pair       30 us  3.2 TB/s            14%  64 x 128
-//   1999 bf16 rows of 6144 to 5120   112 us  1.13 PFLOP/s  61%   64 x 256
-//   333 f32 rows, pair       188 us  digits: 0.63 PFLOP/s of the result, 57%   32 x 256
-//   32 bf16 rows of 17408 to 5120    16 us  3.1 TB/s     21%  32 x 128, 12 ranges of k tiles
+//   4096 MXFP4 rows          252 us  2.90 PFLOP/s  MFMA 38%   blocks of 128 x 256
+//   2048 MXFP4 rows, pair    235 us  3.10 PFLOP/s       42%   128 x 256
+//   48 MXFP4 rows, pair       34 us  2.9 TB/s            14%  64 x 128
+//   1999 bf16 rows of 6144 to 5120   117 us  1.08 PFLOP/s  61%   64 x 256
+//   333 f32 rows, pair       193 us  digits: 0.62 PFLOP/s of the result, 57%   32 x 256
+//   32 bf16 rows of 17408 to 5120    20 us  2.5 TB/s     21%  32 x 128, 6 ranges of k tiles
 // Large MXFP4 products are bound by getting operands to the matrix units: a CU takes
 // 43 B a clock from L2 into LDS at best (35 where rows give 64 B pieces) and needs 24
-// KiB a stage of 512 clocks, and LDS serves a stage's 48 KiB of reads in 400 clocks
-// besides. Small ones by the 3 TB/s that such loads reach from HBM: the loads alone
-// take as long. bf16 rows run at 93% of what a large library product of bf16 reaches.
+// KiB a stage of 512 clocks (585 to 700 of loads), and LDS serves a stage's 48 KiB of
+// reads in 400. A CU's two blocks take about 2390 clocks for a stage of each, which is the
+// sum of loads and matrix instructions and not the larger: they do not overlap as two
+// blocks a CU should make them, and which wait keeps them apart is not known. Small ones
+// are bound by the 2.5 to 3 TB/s that such loads reach from HBM: the loads alone take as
+// long. bf16 rows run at nine tenths of what a large library product of bf16 reaches.
 // Not taken, each at equal or longer times: weights straight into registers without
 // LDS (equal for bf16 and digits; 5% slower for 4096 MXFP4 rows, 12 to 20% for pairs:
 // the compiler's waits for them also wait for later LDS loads); longer rings (up to 8
@@ -555,8 +558,11 @@ using D1 = Shape<DIGITS, 32, 128, 2, 2, 3, 2>;
 // Microseconds of a launch, of a stage and of the rest of a block where a CU runs
 // two blocks and where it runs one, and of joining ranges (a launch, and each MB of
 // their sums). Least squares over 11 matrices from 300 x 8192 to 151936 x 896 with
-// 2..4000 rows, 1..24 ranges: 4 to 8% rms off. What they choose takes 1.008 times the
-// fastest choice on the average of those, 1.19 at most.
+// 2..4000 rows, 1..24 ranges, weights from the last-level cache: 4 to 8% rms off. What they
+// choose takes 1.008 times the fastest choice on the average of those, 1.19 at most. With
+// inputs from HBM products take longer than estimated: 32 bf16 rows, 5120 x 17408, 20.1 us
+// (16.5 here); 48 MXFP4 rows of a 17408 x 5120 pair 34 (22.9); 4096 to one matrix 252 (209);
+// 333 f32 rows of the pair 193 with 8 us of digits (159).
 struct Cost {
   int bm, bn;
   float launch, stage2, block2, stage1, block1, join, mb;

@@ -449,7 +449,7 @@ void run_q6k_mma(const GemvArgs& a, int nrows, int x_f16, int epi, hipStream_t s
 // before a buffer is replaced). Slots are independent buffers: 0 for prepared
 // activations and small reductions, 1 for split-K partial sums, 2 for Q8_K
 // activation operands, 3 for stream-K partial sums, 4 for attention chunk states, 5 for per-row scales,
-// 8 for the bf16 terms of MXFP4 products' activations, 9 for their partial sums.
+// 8 for the activations of MXFP4 products as bf16 terms or digits, 9 for their partial sums.
 void* gemv_scratch(hipStream_t s, size_t bytes, int slot = 0);
 // device scratch bytes (with per-slot alignment) one prepared-activation A8
 // GEMV of `rows` rows takes through run_a8_mma (epi EPI_STORE or EPI_RES, no

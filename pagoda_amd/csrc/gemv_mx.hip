@@ -11,12 +11,15 @@
 // batch row (term t of row r is row t * rows + r), and the terms' sums are added
 // at the end: a single f32 row costs one matrix instruction per 32 columns, not 3.
 //
-// Bound by HBM: the weights are read once, 4.25 bits each. Measured, weights from HBM:
-// a 2 x 17408 x 5120 pair and one f32 row 21 us (4.5 TB/s; a large copy moves 4.75),
-// 5120 x 17408 and 8 MXFP4 rows 10.3 us (4.6), 151936 x 896 and 5 f16 rows 18 us
-// (4.2, with the launch that splits them). Past about 16 rows of terms every
-// workgroup's reads of all activations from L2 weigh more than the weights (32 bf16
-// rows of 17408: 41 us, 16 in blocks that share them through LDS, gemm_mx.hip).
+// Bound by HBM: the weights are read once, 4.25 bits each. Measured, weights from HBM (in
+// brackets: from the last-level cache, where 2 to 5 matrices in turn fit it): a 2 x 17408 x
+// 5120 pair and one f32 row 22.9 us, 4.15 TB/s (19.9; a large copy moves 4.85), 5120 x 17408
+// and 8 MXFP4 rows 15.7 us, 3.05 TB/s (10.4), 151936 x 896 and 5 f16 rows 22.1 us, 3.4 TB/s
+// with the launch that splits them (18.3). The first has 1088 workgroups, the second 160 of
+// 8 waves: few bytes in flight. Past about 16 rows of terms every workgroup's reads of all
+// activations from L2 weigh more than the weights (32 bf16 rows of 17408: 59 us in a
+// graph, which takes no ranges of k tiles; 20 in blocks that share them through LDS with 6
+// ranges, gemm_mx.hip).
 #include <algorithm>
 
 #include "common.h"
@@ -349,7 +352,9 @@ bool few_split_pays(const Sizes& a, int type) {
 
 // Microseconds of a launch; per 256 workgroups, their weight tiles and their
 // activation tiles; per k tile, and row of terms of it (1..4 row tiles of rows).
-// Fitted with the costs in gemm_mx.hip: 10 to 15% rms off.
+// Fitted with the costs in gemm_mx.hip: 10 to 15% rms off, with weights from the last-level
+// cache. From HBM a few rows take up to 1.5 times as long (one f32 row, 5120 x 17408: 19.3
+// us, 12.3 here and 3 of the split); 8 f32 rows of a 17408 x 5120 pair take 73, 36 here.
 double few_us(const Sizes& a) {
   static constexpr float kPlanes[4][6] = {{5.16f, 0.066f, 0.0257f, 0.00017f, 0.0005f, 0.0020f},
                                           {4.54f, 0.296f, 0.0188f, 0.0013f, 0.020f, 0.0024f},

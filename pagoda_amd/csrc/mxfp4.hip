@@ -54,7 +54,7 @@ struct RowGrid {
 // and saturate at 6: the conversion instruction's own rounding. Four threads
 // share a block, so that a wave's loads and stores are runs of whole lines. Bound by
 // HBM: each element is read once, its code and value written once. 2048 x 17408 f32 with
-// values: 57 us, 5.35 TB/s.
+// values: 57 us, 5.35 TB/s; without them 28, 5.7 TB/s.
 template <int TYPE>
 __global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ x, int ldx, uint32_t rows, int units,
                                                        uint8_t* __restrict__ codes, int ldc,
@@ -162,8 +162,8 @@ __device__ __forceinline__ uint32_t digit_codes(uint32_t b) {
 // still to come, wherever the magnitudes of the products add up to less. A tile of 16 rows by 128
 // columns goes to 128 threads, half a block each (of lane l: block l / 16 of row l %
 // 16). A block with an infinity or NaN is NaN. Rows and columns past the matrix are
-// zeros. 333 rows of 5120: 7.8 us, latency (420 workgroups; one thread a block 8.8);
-// 868 rows of 3008: 11.6.
+// zeros. 333 rows of 5120: 8 us, latency (420 workgroups; one thread a block 1 us more);
+// 868 rows of 3008: 11.5.
 __global__ __launch_bounds__(256) void digits_kernel(const float* __restrict__ x, int ldx, int rows, int nblk, int kt,
                                                      uint32_t tiles, uint8_t* __restrict__ d,
                                                      uint8_t* __restrict__ ds) {
@@ -314,8 +314,9 @@ Choice mx::choose(int n_out, int n_in, bool pair, int type, long long stride, in
   // (lanes hold offsets in two of the digits' row tiles in 32 bits, and two tiles go to a workgroup)
   if (type == X_F32 && rows > 16 && a.kt < (1 << 17) && digit_tiles(a) <= 2 * kMaxGroups) {
     // digits: 8.5 bytes of each value read and written instead of 10, and half the matrix
-    // instructions' time (333 rows to a pair of 17408 x 5120: 192 us, as terms 256). 16
-    // rows or fewer stay exact: reading the weights is their time either way.
+    // instructions' time (333 rows to a pair of 17408 x 5120: 193 us, as terms 256). 16
+    // rows or fewer stay exact, so that a caller can have exact rows at any count; it costs
+    // them time (5120 x 17408: 16 rows 30.8 us, 17 in digits 25.3; the pair: 57, 35).
     a.kind = DIGITS;
     const Choice d = plan(a, 0, true);
     if (d.many.us + 8.5 / 4.5e6 * rows * ldt < c.many.us + 10 / 4.5e6 * rows * ldt) c = d;
