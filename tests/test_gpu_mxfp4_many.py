@@ -126,6 +126,26 @@ def test_digits_near_the_largest_number(dev, buf, case):
 
 
 @pytest.mark.parametrize("case", DIGITS)
+def test_results_past_the_largest_number(dev, buf, case):
+    """Never a finite number: an infinity, or a NaN where the digits' products pass it with both
+    signs. The other rows keep their bits."""
+    assert taken(*case) == MANY[case]
+    t, n, k, rows, _ = case
+    rng = np.random.default_rng(n + k)
+    w = np.where(rng.random((n, k // 2)) < 0.5, 0x66, 0xEE).astype(np.uint8), np.full((n, k // 32), 127, np.uint8)  # +-4
+    m = matrix(dev, w)
+    x = rng.normal(0, 1, (rows, k)).astype(np.float32)
+    good = run_rows(dev, buf, m, x, t)
+    past = np.arange(0, rows, 3)
+    x[past] = 0
+    x[past, rng.integers(0, k, past.size)] = rng.uniform(1, 2, past.size) * 2.0 ** rng.integers(126, 128, past.size)
+    got = run_rows(dev, buf, m, x, t)
+    assert not np.isfinite(got[past]).any()
+    rest = np.arange(rows) % 3 > 0
+    assert np.array_equal(got[rest].view(np.uint32), good[rest].view(np.uint32))
+
+
+@pytest.mark.parametrize("case", DIGITS)
 def test_digits_below_the_normal_range(dev, buf, case):
     """One value a row, 2^-140 to 2^-95, under weights of 2^100 times their codes: blocks below
     2^-100 are held in steps of 2^-129. Then large values under weights of the smallest scale,
