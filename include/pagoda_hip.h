@@ -234,6 +234,94 @@ int pgd_attn_decode_dev(pgd_dev* dev, int heads, int kv_heads, int head_dim, int
                         const float* gate, const float* k_pool, const float* v_pool, const int* seq_of_row,
                         const int* pos_of_row, const int* block_tables, int max_blocks, int rows, float* out);
 
+/* ---- 8-bit paged KV cache (no reference counterpart) --------------------------
+ * K and V in a quarter of the bytes of the f32 pages, written, addressed and read by
+ * calls that take everything of a step from device memory: no host plan, no
+ * wait, no allocation, so a whole step can be captured in a HIP graph.
+ *
+ * A pool is n_pages pages of pgd_kv8_page_bytes(kv_heads, head_dim) bytes each, caller's
+ * memory, 16-byte aligned (256 is faster). head_dim is 64, 128 or 256. A page holds 16
+ * positions of every KV head; a position's slot is page * 16 + place. A (page, KV head)
+ * holds its keys as e4m3 codes (OCP 8-bit floating point: 4 exponent and 3 mantissa bits,
+ * largest 448) times one power of two, and its values as codes times another:
+ * the smallest 2^e, e >= -126, with which the largest magnitude written fits. A page is
+ * copied by copying its bytes (pgd_device_copy_dev); nothing in it names its place.
+ * No page needs clearing before its first use. In every call here a slot or page
+ * number outside the pool is never followed. Element types: f32 (0), f16 (1), bf16 (2).
+ * Row strides (ld*) are in elements and multiples of 8 (of 4 in pgd_kv8_read_dev); rows,
+ * pools and workspaces are 16-byte aligned. */
+size_t pgd_kv8_page_bytes(int kv_heads, int head_dim);
+/* A step's bookkeeping, for these pages or any others of `block` positions. Sequence i
+ * has lens[i] positions, in the pages tables[i * max_blocks + p / block], and brings
+ * counts[i] rows. Pages it needs beyond those it has come from free_pages[taken[0]..n_free) in
+ * sequence order, and are entered into its table. Written: new_lens (lens + counts), new_taken
+ * (both may be the input array), row_start [nseq + 1] (sequence i's rows, sequence after
+ * sequence), and for each of `rows` rows seq_of_row, pos_of_row and slots (page * block +
+ * place); -1 in all three for rows behind the last sequence's. status[i]: 0; or why the
+ * sequence got nothing (its rows are -1, its length and table stay): 1 too few free
+ * pages, 2 more positions than max_blocks pages hold, 3 rows past `rows`, 4 a negative length or
+ * count. A sequence that needs no page is not refused for those that do. A table entry that is
+ * negative makes slots -1. */
+int pgd_kv_tables_dev(pgd_dev* dev, int block, int nseq, const int* lens, const int* counts, int* tables,
+                      int max_blocks, const int* free_pages, int n_free, const int* taken, int rows, int* new_lens,
+                      int* new_taken, int* row_start, int* seq_of_row, int* pos_of_row, int* slots, int* status);
+/* Rows k, v [rows, kv_heads * head_dim] into the slots slots[row] (negative, or past the
+ * pool: the row is left out). The rows of one page follow each other, in
+ * place order without gaps, as pgd_kv_tables_dev lays them out, and no other row of the call has
+ * their page. A row at place 0 starts its page anew; otherwise the page holds the
+ * places before the first row written, and places behind the last one become empty. If a row
+ * needs a larger power of two than its page has, the codes there are rounded again to the larger
+ * one; it never falls while the page fills. Rounding is to nearest, ties to the even code (a
+ * value within half a step of 2^128 reads as an infinity).
+ * A (row, KV head) with an infinity or NaN in k or v reads as NaN, and makes NaN
+ * what attends it; its page's other positions are not affected. */
+int pgd_kv8_append_dev(pgd_dev* dev, void* pool, int n_pages, int kv_heads, int head_dim, const void* k, int ldk,
+                       const void* v, int ldv, int type, const int* slots, int rows);
+/* The f32 values at slots[row]: k, v [rows, kv_heads * head_dim]. Rows of a slot outside the pool
+ * are left as they were. */
+int pgd_kv8_read_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, int head_dim, const int* slots,
+                     int rows, float* k, int ldk, float* v, int ldv);
+/* Causal GQA attention. Sequence i owns the rows [row_start[i], row_start[i + 1]) (clamped to
+ * rows), the latest of its lens[i] positions, and row j of its n attends to positions
+ * [0, lens[i] - n + j]: softmax(q k^T / sqrt(head_dim)) v, times sigmoid(gate) if
+ * there is one. q, gate, out [rows, heads * head_dim] of one type; heads is a multiple of
+ * kv_heads. Positions past max_blocks pages do not exist. A row that attends to nothing
+ * gets zeros; rows of no sequence are left as they were; attending a position of a page outside the pool
+ * gives NaN. f32 rows lose nothing beyond f32 sums; the softmax weights of f16 and bf16 rows are
+ * held to 2^-16 before they meet the values. max_rows: the largest
+ * number of rows of a sequence, or any bound on it (it selects kernels, results are
+ * right with any value). ws: pgd_attn_kv8_ws_bytes bytes that no other stream uses
+ * meanwhile (a captured graph's included); its contents do not matter. The order of the sums
+ * depends on the sizes, row_start and lens, on nothing else. */
+size_t pgd_attn_kv8_ws_bytes(int heads, int kv_heads, int head_dim, int nseq, int max_blocks, int rows);
+int pgd_attn_kv8_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, int head_dim, int heads, const void* q,
+                     int ldq, int type, int nseq, const int* row_start, const int* lens, const int* block_tables,
+                     int max_blocks, int rows, int max_rows, void* out, int ldo, const void* gate, int ldg, void* ws,
+                     size_t ws_bytes);
+/* Per (row, KV head) the `top` pages of the row's context with the highest scores, as places in its
+ * block table: sel [rows, kv_heads, top], ascending, -1 behind the count[row, kv_heads] =
+ * min(top, pages) entries. The first `sinks` and the last `recent` pages are always among
+ * them (sinks + recent <= top). The score bounds q.k over the page: q in signed 8 bits (q8 =
+ * q / 2^e to nearest, ties to even, 2^e the smallest power of two that keeps the
+ * group's heads within 127; non-finite entries count as 0), the page's key codes bounded per
+ * channel by whole numbers hi and lo (the largest and smallest code over 4, rounded outward; the
+ * append keeps them): score = 2^(key exponent) max over the group's heads of
+ * sum(max(q8 hi, q8 lo)), exact in f32; ties go to the lower page. A page outside the pool scores
+ * lowest. Rows of no sequence are left as they were; a row that attends to nothing selects nothing.
+ * ws as above, of pgd_kv8_sparse_ws_bytes bytes, which serves both calls, one after the other. */
+size_t pgd_kv8_sparse_ws_bytes(int heads, int kv_heads, int head_dim, int rows, int max_blocks, int top);
+int pgd_kv8_select_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, int head_dim, int heads,
+                       const void* q, int ldq, int type, int nseq, const int* row_start, const int* lens,
+                       const int* block_tables, int max_blocks, int rows, int top, int sinks, int recent, int* sel,
+                       int* count, void* ws, size_t ws_bytes);
+/* pgd_attn_kv8_dev over the pages sel[row, kv head, 0..count) alone (count is taken within
+ * 0..top; entries outside the table are skipped, a page named twice counts twice). */
+int pgd_attn_kv8_sparse_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, int head_dim, int heads,
+                            const void* q, int ldq, int type, int nseq, const int* row_start, const int* lens,
+                            const int* block_tables, int max_blocks, int rows, int top, const int* sel,
+                            const int* count, void* out, int ldo, const void* gate, int ldg, void* ws,
+                            size_t ws_bytes);
+
 /* ---- models and sessions ---------------------------------------------------
  * Architecture of a model handle. arch 0 is the hybrid Qwen3.5 tower
  * (Gated-DeltaNet + gated full attention, MLX affine-8 weights; Qwen35::load

@@ -8,6 +8,7 @@ and the model/session surface of the reference's ModelEngine/ModelSession
 """
 from ._lib import LIB_PATH, PagodaError, lib  # noqa: F401
 from .device import Device, Event, device_from_env  # noqa: F401
+from .kv8 import Kv8Pool  # noqa: F401
 from .matrix import Matrix  # noqa: F401
 
-__all__ = ["LIB_PATH", "PagodaError", "lib", "Device", "device_from_env", "Matrix"]
+__all__ = ["LIB_PATH", "PagodaError", "lib", "Device", "device_from_env", "Kv8Pool", "Matrix"]

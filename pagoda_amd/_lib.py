@@ -54,6 +54,22 @@ SIGNATURES: dict[str, tuple] = {
     "pgd_gdn_step_dev": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 10 + [c_int, c_void_p]),
     "pgd_gdn_prefill_dev": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 10 + [c_int, c_int, c_int, c_void_p]),
     "pgd_attn_decode_dev": (c_int, [c_void_p, c_int, c_int, c_int, c_int] + [c_void_p] * 7 + [c_int, c_int, c_void_p]),
+    "pgd_kv8_page_bytes": (c_size_t, [c_int, c_int]),
+    "pgd_kv_tables_dev": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                                  c_int] + [c_void_p] * 7),
+    "pgd_kv8_append_dev": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int,
+                                   c_void_p, c_int]),
+    "pgd_kv8_read_dev": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                                 c_int]),
+    "pgd_attn_kv8_ws_bytes": (c_size_t, [c_int] * 6),
+    "pgd_attn_kv8_dev": (c_int, [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_int, c_int] + [c_void_p] * 3 +
+                         [c_int] * 3 + [c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t]),
+    "pgd_kv8_sparse_ws_bytes": (c_size_t, [c_int] * 6),
+    "pgd_kv8_select_dev": (c_int, [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_int, c_int] +
+                           [c_void_p] * 3 + [c_int] * 5 + [c_void_p, c_void_p, c_void_p, c_size_t]),
+    "pgd_attn_kv8_sparse_dev": (c_int, [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_int, c_int] +
+                                [c_void_p] * 3 + [c_int] * 3 + [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                                                c_void_p, c_size_t]),
     "pgd_act_bytes": (c_size_t, [c_int, c_int]),
     "pgd_act_prep_dev": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "pgd_matrix_gemv_act_dev": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int]),

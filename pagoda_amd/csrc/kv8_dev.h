@@ -1,0 +1,78 @@
+// kv8_dev.h — device helpers shared by the kernels over the 8-bit KV cache.
+#pragma once
+
+#include "common.h"
+#include "kv8.h"
+
+namespace pgd {
+namespace kv8 {
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+// 2^e for e in [-126, 127], from its bits
+__device__ inline float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+
+// Four values of magnitude up to 448 to e4m3 codes, to nearest, ties to even (the
+// instruction's rounding; nothing here reaches its overflow).
+__device__ inline uint32_t to_codes(float a, float b, float c, float d) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+}
+__device__ inline f4 of_codes(uint32_t c) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  return f4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// The smallest exponent e >= -126 with top <= 448 * 2^e; 448 is 1.75 * 2^8.
+__device__ inline int holds(float top) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, top);
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return e > kExpMin ? e : kExpMin;
+}
+
+// Eight elements of a row of type T as f32.
+template <int T>
+__device__ inline void load8(const void* p, int64_t i, float (&x)[8]) {
+  if constexpr (T == F32) {
+    const f4* q = reinterpret_cast<const f4*>(static_cast<const float*>(p) + i);
+    const f4 a = q[0], b = q[1];
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = a[j], x[4 + j] = b[j];
+  } else if constexpr (T == F16) {
+    const h8 a = *reinterpret_cast<const h8*>(static_cast<const _Float16*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = (float)a[j];
+  } else {
+    const u4 a = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = __builtin_bit_cast(float, (j & 1 ? a[j / 2] & 0xffff0000u : a[j / 2] << 16));
+  }
+}
+
+// v combined with the values of the other lanes l ^ 16, l ^ 32, l ^ 48 (by two lane swaps,
+// whose two results hold each lane's own value and its partner's).
+template <class F>
+__device__ inline float over_quads(float v, F f) {
+  uint32_t b = __builtin_bit_cast(uint32_t, v);
+  auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  v = f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+  b = __builtin_bit_cast(uint32_t, v);
+  r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ inline float quads_max(float v) {
+  return over_quads(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ inline float quads_sum(float v) {
+  return over_quads(v, [](float a, float b) { return a + b; });
+}
+
+}  // namespace kv8
+}  // namespace pgd
