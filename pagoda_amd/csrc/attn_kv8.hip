@@ -4,27 +4,32 @@
 // For a query q of a row at position p:  o = sum_j w_j v_j / sum_j w_j over j <= p,
 // w_j = exp(q.k_j / sqrt(hd)), with k_j = 2^ek codes, v_j = 2^ev codes per page and head.
 // Per two pages (32 positions) and a tile of 16 queries (rows x group heads):
-//   S[pos][query]  = K codes . q        16x16x32 bf16 products over hd / 32 steps
-//   t = S 2^ek log2(e) / sqrt(hd), running maximum m and sum l in f32
-//   O[dim][query] += V codes^T . (2^(t - m) 2^ev)   the same products over the 32 positions
-// Codes convert to bf16 exactly. q enters exactly as bf16 terms (f32 three, f16 two,
-// bf16 itself); the weights enter as three (f32) or two: each term leaves at most 2^-8 of what it
-// is given, so f32 rows lose nothing that f32 sums keep, and the weights of f16 and bf16
-// rows are held to 2^-16, well below what their results round to (one term would add as much
-// error to bf16 results as their own rounding).
+//   S[pos][query]  = K codes . q        16x16x32 f16 products over hd / 32 steps
+//   t = S 2^ek log2(e) / sqrt(hd), its running maximum m and the sum l of 2^(t - m) in f32
+//   O[dim][query] += V codes^T . 2^(t + ev - M)   the same products over the 32 positions
+// with M the running maximum of t + ev, so that the largest weight of a value's code is
+// about one whatever the pages' powers of two. Codes convert to f16 exactly. Queries are
+// scaled by a power of two into f16's range and enter as f16 terms: f32 rows two (22 bits and
+// at least 2^-40 of the row's largest), f16 rows themselves, bf16 rows one (exact to 2^-40 of the
+// largest). The weights, times 2^15, enter as two terms (bf16 rows: one; its 2^-11 is an
+// eighth of their own rounding). bf16 terms would need no scaling but half as many more
+// products: three for f32 where f16 takes two.
 // The lane that holds a score holds it as the operand of the second product: lane
 // (query n = l % 16, kq = l / 16) has positions 4 kq .. 4 kq + 3 of both pages, which
 // are the 8 that a lane of the second product's operand takes, and its results are
-// columns n too, so m, l and the rescaling stay in the lane but for one maximum
+// columns n too, so m, M, l and the rescaling stay in the lane but for two maxima
 // over the four kq.
 //
-// Split: work is one list of (sequence, chunk of pages, KV head, tile) that every
+// Split: work is a list of (sequence, chunk of pages, KV head, tile of queries) that every
 // workgroup derives for itself from the row starts and lengths on the device, so a call
-// needs no plan from the host. The chunk length makes about kItems items of all.
-// In an item the four waves take pairs of pages in turn, each with its own m, l and O,
-// joined in LDS. Items of a context of one chunk write results, the others partial sums that the merge kernel
-// adds in chunk order.
+// needs no plan from the host. Sequences of few queries take item_kernel: tiles of 16
+// queries, four waves on pairs of pages in turn, each with its own maxima, sum and O, joined
+// in LDS. The others take prompt_kernel: the four waves of a workgroup have
+// queries of their own and walk the same pages, staged in LDS for all. Contexts of one chunk
+// write results, the others partial sums that merge_kernel adds in chunk order.
+#include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "kv8_dev.h"
 
@@ -33,69 +38,79 @@ namespace kv8 {
 
 namespace {
 
-constexpr int kItems = 1024;   // items that contexts are cut into, about
-constexpr int kMinChunk = 16;  // pages: fewer would be more joining than reading
+// Items that contexts are cut into, about. kFew: the workgroups that run at once (two on a CU at hd 256), less the
+// rest chunks of the contexts; kMany: prompts' tiles are mostly enough by themselves.
+constexpr int kFewItems = 448, kManyItems = 1024;
+constexpr int kMinChunk = 16;    // pages: fewer would be more joining than reading
+constexpr int kFewQueries = 32;  // of a sequence and KV head: calls of up to these are item_kernel's alone
 
 template <int T>
-constexpr int kTerms = T == F32 ? 3 : T == F16 ? 2 : 1;  // of a query
+constexpr int kTerms = T == F32 ? 2 : 1;  // f16 terms of a query
 template <int T>
-constexpr int kWeightTerms = T == F32 ? 3 : 2;
+constexpr int kWeightTerms = T == BF16 ? 1 : 2;
+constexpr float kWeightExp = 15;  // weights enter times 2^15: f16 holds 2^-24 to 65504
 
-// x as T terms of 8 bits, each the truncation of what is left (exact for what T is chosen for).
-template <int T>
-__device__ inline void split_trunc(const float (&x)[8], b8 (&out)[kTerms<T>]) {
+// x as f16 terms to nearest, each of what the ones before leave.
+template <int N>
+__device__ inline void split(const float (&x)[8], h8 (&out)[N]) {
   float r[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) r[j] = x[j];
 #pragma unroll
-  for (int k = 0; k < kTerms<T>; k++) {
-    u4 w;
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const uint32_t a = __builtin_bit_cast(uint32_t, r[j]), b = __builtin_bit_cast(uint32_t, r[j + 1]);
-      w[j / 2] = (a >> 16) | (b & 0xffff0000u);
-      r[j] -= __builtin_bit_cast(float, a & 0xffff0000u);
-      r[j + 1] -= __builtin_bit_cast(float, b & 0xffff0000u);
-    }
-    out[k] = __builtin_bit_cast(b8, w);
-  }
-}
-
-// x as terms rounded to nearest.
-template <int T>
-__device__ inline void split_near(const float (&x)[8], b8 (&out)[kWeightTerms<T>]) {
-  float r[8];
-#pragma unroll
-  for (int j = 0; j < 8; j++) r[j] = x[j];
-#pragma unroll
-  for (int k = 0; k < kWeightTerms<T>; k++) {
+  for (int k = 0; k < N; k++) {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      out[k][j] = (__bf16)r[j];
-      if (k + 1 < kWeightTerms<T>) r[j] -= (float)out[k][j];
+      out[k][j] = (_Float16)r[j];
+      if (k + 1 < N) r[j] -= (float)out[k][j];
     }
   }
 }
 
-// Eight codes as bf16.
-__device__ inline b8 of_codes8(uint32_t lo, uint32_t hi) {
-  const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
-  const b2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-  const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
-  const b2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
-  return b8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+// Eight codes as f16.
+__device__ inline h8 of_codes8(uint32_t lo, uint32_t hi) {
+  const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+  const h2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+  const h2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // ---- the list of items ------------------------------------------------------------
+
+// Sums over the lanes before and with a lane, and over all lanes (identical in every lane).
+template <int CTRL, int ROWS>
+__device__ inline int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ inline int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes of 16 up
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // lane 15 of a row to the next row, then lane 31 to the upper half
+  return dpp_add<0x143, 0xc>(v);
+}
+template <int CTRL, int ROWS>
+__device__ inline float dpp_addf(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+__device__ inline float wave_total(float v) {
+  v = dpp_addf<0x111, 0xf>(v);
+  v = dpp_addf<0x112, 0xf>(v);
+  v = dpp_addf<0x114, 0xf>(v);
+  v = dpp_addf<0x118, 0xf>(v);
+  v = dpp_addf<0x142, 0xa>(v);
+  v = dpp_addf<0x143, 0xc>(v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 
 struct Seq {
   int row0, n;      // its rows
   int len;          // positions as given
   int ctx, pages;   // positions that the table holds, and their pages
-  int tiles;        // query tiles of a KV head
 };
 
-__device__ inline Seq seq_at(const Rows& r, int group, int tile_queries, int i) {
+__device__ inline Seq seq_at(const Rows& r, int i) {
   Seq s;
   const int a = min(max(r.row_start[i], 0), r.rows), b = min(max(r.row_start[i + 1], 0), r.rows);
   s.row0 = a;
@@ -103,72 +118,84 @@ __device__ inline Seq seq_at(const Rows& r, int group, int tile_queries, int i) 
   s.len = r.lens[i];
   const long long most = (long long)r.max_blocks * kPage;
   s.ctx = (int)min((long long)max(s.len, 0), most);
-  s.pages = (int)(((long long)s.ctx + kPage - 1) / kPage);
-  s.tiles = (int)(((long long)s.n * group + tile_queries - 1) / tile_queries);
+  s.pages = (s.ctx + kPage - 1) / kPage;
   return s;
 }
 
+// A kernel's share of a call: sequences of at least `least` and at most `most` queries a KV head, in tiles.
+struct Share {
+  int least, most;
+  int tile;   // queries
+  int items;  // that contexts are cut into, about
+};
+
+struct Class {
+  int group;
+  Share sh;
+  __device__ int tiles(int n) const {
+    const long long q = (long long)n * group;
+    return q < sh.least || q > sh.most ? 0 : (int)((q + sh.tile - 1) / sh.tile);
+  }
+  // partial sums are of 16 queries, whatever the tile
+  __device__ int tiles16(int n) const { return (int)(((long long)n * group + 15) / 16); }
+};
+
+// The workspace's partial sums: how many it has, and a launch's own.
+struct Slots {
+  int all, first, end;
+};
+
 __device__ inline int chunks_of(int pages, int chunk) { return pages > 0 ? (pages + chunk - 1) / chunk : 1; }
 
-__device__ inline long long wave_sum64(long long v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-__device__ inline long long wave_scan64(long long v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
-}
-
-// Pages of a chunk: a multiple of 8 (a pair for each of four waves) that cuts all tiles' pages into at most kItems
-// full chunks.
-__device__ inline int chunk_of(long long tile_pages) {
-  const long long c = (tile_pages + kItems - 1) / kItems;
-  return (int)min(max((c + 7) & ~7ll, (long long)kMinChunk), (long long)INT_MAX / 2);
+// Pages of a chunk: a multiple of 8 (a pair for each of four waves) that cuts all tiles' pages into at most
+// `items` full chunks (of sums in f32, so about).
+__device__ inline int chunk_of(float tile_pages, int items) {
+  const float c = fminf(ceilf(tile_pages / (float)items), 1e9f);
+  return max(((int)c + 7) & ~7, kMinChunk);
 }
 
 struct Found {
   Seq s;
-  int seq;
-  int chunk;       // pages of a chunk
-  int item, slot;  // the sequence's first item, and its first partial sum if it has several chunks
+  int seq, tiles, chunk;
+  int local;  // the item among the sequence's
+  int slot;   // the sequence's first partial sum
 };
 
-// The sequence of an item (BY_ROW: of a row), as every wave works it out for itself, 64 sequences
-// at a time. Returns false past the last.
-template <bool BY_ROW>
-__device__ inline bool find(const Rows& r, int kv_heads, int group, int tile_queries, int key, Found& f) {
+// The sequence of a workgroup's item, as every wave works it out for itself, 64 sequences at a time.
+// Returns false for the workgroups past the list.
+__device__ inline bool find(const Rows& r, int kv_heads, const Class& cl, int key, Found& f) {
   const int lane = threadIdx.x & 63;
-  long long all = 0;
+  const bool strip = r.nseq <= 64;  // one strip: nothing is loaded twice
+  Seq s{};
+  int tiles = 0;
+  float all = 0;
   for (int base = 0; base < r.nseq; base += 64) {
     const int i = base + lane;
+    tiles = 0;
     if (i < r.nseq) {
-      const Seq s = seq_at(r, group, tile_queries, i);
-      all += (long long)s.tiles * s.pages;
+      s = seq_at(r, i);
+      tiles = cl.tiles(s.n);
     }
+    all += (float)tiles * (float)s.pages;
   }
-  f.chunk = chunk_of(wave_sum64(all) * kv_heads);
-  long long before = 0;  // items in the low half, partial sums in the high one
-  for (int base = 0; base < r.nseq; base += 64) {
-    const int i = base + lane;
-    Seq s{};
-    long long mine = 0;
-    if (i < r.nseq) {
-      s = seq_at(r, group, tile_queries, i);
-      const int chunks = chunks_of(s.pages, f.chunk);
-      const long long items = (long long)s.tiles * chunks * kv_heads;
-      mine = items | (chunks > 1 ? items << 32 : 0);
+  f.chunk = chunk_of(wave_total(all) * kv_heads, cl.sh.items);
+  auto items_of = [&](int base) {
+    if (!strip) {
+      tiles = 0;
+      if (base + lane < r.nseq) {
+        s = seq_at(r, base + lane);
+        tiles = cl.tiles(s.n);
+      }
     }
-    const long long upto = wave_scan64(mine) + before;
-    const long long from = upto - mine;
-    const int lo = (int)(uint32_t)from, hi = (int)(uint32_t)upto;
-    const bool here = BY_ROW ? key >= s.row0 && key < s.row0 + s.n : key >= lo && key < hi;
-    const uint64_t hit = __ballot(here);
+    return tiles * chunks_of(s.pages, f.chunk) * kv_heads;
+  };
+  int before = 0, split_before = 0;
+  for (int base = 0; base < r.nseq; base += 64) {
+    const int mine = items_of(base), upto = before + wave_scan(mine);
+    const int chunks = chunks_of(s.pages, f.chunk);
+    const int slots = chunks > 1 && tiles > 0 ? cl.tiles16(s.n) * kv_heads * chunks : 0;
+    const int slots_upto = split_before + wave_scan(slots);
+    const uint64_t hit = __ballot(key < upto && key >= upto - mine);
     if (hit) {
       const int src = __builtin_ctzll(hit);
       f.s.row0 = __builtin_amdgcn_readlane(s.row0, src);
@@ -176,14 +203,14 @@ __device__ inline bool find(const Rows& r, int kv_heads, int group, int tile_que
       f.s.len = __builtin_amdgcn_readlane(s.len, src);
       f.s.ctx = __builtin_amdgcn_readlane(s.ctx, src);
       f.s.pages = __builtin_amdgcn_readlane(s.pages, src);
-      f.s.tiles = __builtin_amdgcn_readlane(s.tiles, src);
-      f.item = __builtin_amdgcn_readlane(lo, src);
-      f.slot = __builtin_amdgcn_readlane((int)(from >> 32), src);
+      f.tiles = __builtin_amdgcn_readlane(tiles, src);
+      f.local = key - __builtin_amdgcn_readlane(upto - mine, src);
+      f.slot = __builtin_amdgcn_readlane(slots_upto - slots, src);
       f.seq = base + src;
       return true;
     }
-    before = ((long long)__builtin_amdgcn_readlane((int)(upto >> 32), 63) << 32) |
-             (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)upto, 63);
+    before = __builtin_amdgcn_readlane(upto, 63);
+    split_before = __builtin_amdgcn_readlane(slots_upto, 63);
   }
   return false;
 }
@@ -197,6 +224,17 @@ __device__ inline int seq_of(const Rows& r, int row) {
     if (hit) return base + __builtin_ctzll(hit);
   }
   return -1;
+}
+
+// Positions that row j of a sequence sees.
+__device__ inline int seen_by(const Seq& s, int j) {
+  return (int)max(min((long long)s.len - s.n + j + 1, (long long)s.ctx), 0ll);
+}
+
+// Pages that the last row of a tile sees.
+__device__ inline int tile_pages(const Seq& s, int group, int tile_queries, int tile) {
+  const int last = (int)min(((long long)(tile + 1) * tile_queries - 1) / group, (long long)s.n - 1);
+  return (seen_by(s, last) + kPage - 1) / kPage;
 }
 
 // ---- results ------------------------------------------------------------------------
@@ -242,37 +280,217 @@ __device__ inline void store4(const Out& o, int64_t row, int64_t col, f4 x) {
   }
 }
 
-// Partial sums: per slot and query O[hd], and behind all slots' O the pairs (m, l).
+// What merge_kernel needs to know of a row's sequence, left by the first item of the row's tile.
+struct RowPart {
+  int slot, chunk, row0, n, len, tile_queries, pad[2];
+};
+
+// Workspace: RowPart of every row, then per slot (16 queries of a chunk and head) O [16][hd], then their
+// (m, M, l).
 struct Partials {
+  RowPart* rows;
   float* o;
-  f2* ml;
+  f4* st;
 };
 template <int HD>
-__device__ __host__ inline Partials partials_at(void* ws, int slots, int queries) {
-  float* o = static_cast<float*>(ws);
-  return Partials{o, reinterpret_cast<f2*>(o + (size_t)slots * queries * HD)};
+__device__ __host__ inline Partials partials_at(void* ws, int rows, int slots) {
+  Partials p;
+  p.rows = static_cast<RowPart*>(ws);
+  p.o = reinterpret_cast<float*>(p.rows + rows);
+  p.st = reinterpret_cast<f4*>(p.o + (size_t)slots * 16 * HD);
+  return p;
 }
+
+// What several runs over parts of a context leave, joined: maxima and the sum.
+struct State {
+  float m = -INFINITY, mv = -INFINITY, l = 0;
+  // The factor of a part's O (a part that attended nothing has zeros, or NaN, to keep).
+  __device__ float of_part(f4 s) const { return s[1] > -INFINITY ? __builtin_amdgcn_exp2f(s[1] - mv) : 1.0f; }
+  __device__ float sum_of_part(f4 s) const { return (s[0] > -INFINITY ? __builtin_amdgcn_exp2f(s[0] - m) : 1.0f) * s[2]; }
+  template <int N, class F>
+  __device__ void join(F part, float (&by)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) m = fmaxf(m, part(i)[0]), mv = fmaxf(mv, part(i)[1]);
+#pragma unroll
+    for (int i = 0; i < N; i++) by[i] = of_part(part(i)), l += sum_of_part(part(i));
+  }
+  // From O to results; nothing attended gives zero.
+  __device__ float factor() const {
+    if (l == 0) return 0.0f;
+    return (m > -INFINITY ? __builtin_amdgcn_exp2f(mv - m - kWeightExp) : 1.0f) / l;
+  }
+};
 
 struct List {
   const int *sel, *count;
   int top, chunk, chunks;  // pages of a chunk and chunks of a full list
 };
 
-// ---- the item kernel ----------------------------------------------------------------
+// The RowParts of the rows whose first query a tile has.
+__device__ inline void leave_row_parts(const Partials& part, const Seq& s, int group, int tile, int tile_queries,
+                                       const Found& f, const Slots& slots) {
+  const int j = (int)(((int64_t)tile * tile_queries + group - 1) / group) + (int)threadIdx.x;
+  if ((int)threadIdx.x < tile_queries && j < s.n && (int64_t)j * group < (int64_t)(tile + 1) * tile_queries)
+    part.rows[s.row0 + j] = RowPart{slots.first + f.slot, f.chunk, s.row0, s.n, s.len, tile_queries, {0, 0}};
+}
 
-template <int HD, int T, int NT, bool LIST>
-__global__ __launch_bounds__(256) void item_kernel(Pool p, Rows r, Out out, List list, void* ws, int slots) {
-  constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kQueries = 16 * NT, kN = kTerms<T>,
-                kW = kWeightTerms<T>;
-  constexpr int kQBytes = NT * kN * kSteps * 1024, kJoinBytes = 4 * kTiles * 1024;
-  __shared__ __align__(16) uint8_t lds[kQBytes > kJoinBytes ? kQBytes : kJoinBytes];
-  __shared__ f2 lds_ml[4][kQueries];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// ---- 16 queries and two pages ---------------------------------------------------------
+
+// The next 64 pages of a walk, one a lane: places in the table and page numbers.
+// number: -1 for no page, -2 for one outside the pool (attending it makes NaN).
+struct Walk {
+  int index = -1, id = -1;
+  __device__ void set(int at, const int* table, int max_blocks, int n_pages) {
+    index = at;
+    id = -1;
+    if (at >= 0 && at < max_blocks) {
+      const int p = table[at];
+      id = p >= 0 && p < n_pages ? p : -2;
+    } else {
+      index = -1;
+    }
+  }
+};
+
+struct Page {
+  int index, id;
+  uint32_t meta;
+  const uint8_t* at;
+};
+
+struct PoolAt {
+  const uint8_t* base;
+  size_t page_bytes, head, meta;
+  __device__ PoolAt(const Pool& p, int h)
+      : base(p.base), page_bytes(p.at.page_bytes()), head((size_t)h * p.at.head_bytes()), meta(p.at.meta_at() + (size_t)h * 4) {}
+  __device__ Page page(const Walk& w, int lane) const {
+    Page g;
+    g.index = __builtin_amdgcn_readlane(w.index, lane);
+    g.id = __builtin_amdgcn_readlane(w.id, lane);
+    const uint8_t* p = base + (size_t)max(g.id, 0) * page_bytes;
+    g.at = p + head;
+    g.meta = *reinterpret_cast<const uint32_t*>(p + meta);
+    return g;
+  }
+};
+
+// A query's running maxima, sum (of this lane's positions) and scaling, as its column of lanes holds them.
+struct Query {
+  float m = -INFINITY, mv = -INFINITY, l = 0;
+  int exp = 0, lim = 0;  // power of two of its terms; positions it sees
+};
+
+// Scores of two pages' positions to weights: s[w][i] is position 16 index + 4 kq + i of page w.
+template <int KW, int N>
+__device__ inline void weigh(const f4 (&s)[2], const Page (&pg)[2], float scale, bool whole, Query& q, f4 (&o)[N],
+                             h8 (&out)[KW]) {
+  const int kq = threadIdx.x >> 4 & 3;
+  float x[8], ev[2];
+#pragma unroll
+  for (int w = 0; w < 2; w++) {
+    const float by = __builtin_ldexpf(scale, q.exp + Meta::ek(pg[w].meta));
+    ev[w] = (float)Meta::ev(pg[w].meta);
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[4 * w + i] = s[w][i] * by;
+  }
+  if (!whole) {
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+      const uint32_t nan = pg[w].id >= 0 ? Meta::nan(pg[w].meta) : pg[w].id == -2 ? 0xffffu : 0u;
+      // (a page of no index lies behind every position)
+      const int first = pg[w].index >= 0 ? pg[w].index * kPage + 4 * kq : INT_MAX - kPage;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float v = nan >> (4 * kq + i) & 1 ? NAN : x[4 * w + i];
+        x[4 * w + i] = first + i < q.lim ? v : -INFINITY;
+      }
+    }
+  }
+  const float x0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), x1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]));
+  const float top = fmaxf(q.m, quads_max(fmaxf(x0, x1)));
+  const float top_v = fmaxf(q.mv, quads_max(fmaxf(x0 + ev[0], x1 + ev[1])));
+  if (__any(top > q.m || top_v > q.mv)) {
+    q.l *= top > q.m ? __builtin_amdgcn_exp2f(q.m - top) : 1.0f;
+    const float down = top_v > q.mv ? __builtin_amdgcn_exp2f(q.mv - top_v) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) o[i] *= down;
+    q.m = top;
+    q.mv = top_v;
+  }
+  const float at = top > -INFINITY ? top : 0.0f, at_v = top > -INFINITY ? top_v - kWeightExp : 0.0f;
+  const float g0 = at - at_v + ev[0], g1 = at - at_v + ev[1];
+  float w[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    w[i] = __builtin_amdgcn_exp2f(x[i] - at);
+    q.l += w[i];
+  }
+  if (__any(fmaxf(g0, g1) > 100.0f)) {
+    // pages so far apart that 2^(t - m) underflows where the weight does not
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(x[i] + ev[i / 4] - at_v);
+  } else {
+    const float f0 = __builtin_amdgcn_exp2f(g0), f1 = __builtin_amdgcn_exp2f(g1);
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] *= i < 4 ? f0 : f1;
+  }
+  split<KW>(w, out);
+}
+
+// Whether all of two pages' positions count for every query of a wave that sees at least `least`.
+__device__ inline bool whole_pages(const Page (&pg)[2], int least) {
+  return pg[0].id >= 0 && pg[1].id >= 0 && (Meta::nan(pg[0].meta) | Meta::nan(pg[1].meta)) == 0 &&
+         (max(pg[0].index, pg[1].index) + 1) * kPage <= least;
+}
+
+// Eight dims of a query as f16 terms; x is scaled to [2^14, 2^15) for the largest magnitude of the HD / 8 lanes
+// that hold the query. Returns the power of two it was divided by.
+template <int T, int HD, int N>
+__device__ inline int query_terms(float (&x)[8], h8 (&t)[N]) {
+  int e = 0;
+  if constexpr (T != F16) {
+    float most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(x[j]));
+#pragma unroll
+    for (int w = 1; w < HD / 8; w <<= 1) most = fmaxf(most, __shfl_xor(most, w));
+    e = max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14, -112);
+    const float down = pow2(-e);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] *= down;
+  }
+  split<N>(x, t);
+  return e;
+}
+
+// ---- few queries a sequence ------------------------------------------------------------
+
+// NQ tiles of 16 queries, four waves each, side by side over the same pages: what one loads the other finds in the
+// caches.
+template <int HD, int T, int NQ, bool LIST>
+__global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out out, List list, Share share, void* ws,
+                                                           Slots slots) {
+  constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms<T>;
+  constexpr int kJoinTiles = kTiles < 8 ? kTiles : 8;  // tiles of O joined at a time
+  constexpr int kQBytes = kN * kSteps * 1024, kJoinBytes = 4 * kJoinTiles * 1024;
+  constexpr int kTileBytes = kQBytes > kJoinBytes ? kQBytes : kJoinBytes;
+  constexpr int kUnits = 16 * HD / 8;  // of 8 dims of a query
+  constexpr int kRounds = kUnits > 256 ? kUnits / 256 : 1;
+  __shared__ __align__(16) uint8_t lds_all[NQ * kTileBytes];
+  __shared__ f4 lds_st_all[NQ][4][16];
+  __shared__ int lds_exp_all[NQ][16];  // of the queries' powers of two
+  const int sub = NQ > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint8_t* const lds = lds_all + sub * kTileBytes;
+  f4(*const lds_st)[16] = lds_st_all[sub];
+  int* const lds_exp = lds_exp_all[sub];
   const int n16 = lane & 15, kq = lane >> 4;
   const int kv_heads = p.at.kv_heads, group = r.heads / kv_heads;
+  const Partials part = partials_at<HD>(ws, LIST ? 0 : r.rows, slots.all);
 
   // which pages, head and queries
-  int seq_table = 0, head, tile, page0, page1, row0, nrows, len, ctx, slot;
+  Seq s;
+  int seq, head, tile, page0, page1, slot;
   const int* pages_list = nullptr;
   if constexpr (LIST) {
     const int tiles = (group + 15) / 16;
@@ -283,234 +501,144 @@ __global__ __launch_bounds__(256) void item_kernel(Pool p, Rows r, Out out, List
     b /= tiles;
     head = b % kv_heads;
     const int row = b / kv_heads;
-    const int seq = seq_of(r, row);
-    if (seq < 0) return;
     const int count = min(max(list.count[(int64_t)row * kv_heads + head], 0), list.top);
     const int have = chunks_of(count, list.chunk);
     if (c >= have) return;
+    seq = seq_of(r, row);
+    if (seq < 0) return;
     page0 = c * list.chunk;
     page1 = min(page0 + list.chunk, count);
     pages_list = list.sel + ((int64_t)row * kv_heads + head) * list.top;
-    seq_table = seq;
-    row0 = row;
-    nrows = 1;
     // (as the last of the rows up to this one)
-    len = r.lens[seq] - (r.row_start[seq + 1] - 1 - row);
-    ctx = (int)min((long long)max(len, 0), (long long)r.max_blocks * kPage);
-    slot = have > 1 ? blockIdx.x : -1;
+    s.row0 = row;
+    s.n = 1;
+    s.len = r.lens[seq] - (r.row_start[seq + 1] - 1 - row);
+    s.ctx = (int)min((long long)max(s.len, 0), (long long)r.max_blocks * kPage);
+    slot = have > 1 ? (int)blockIdx.x : -1;
   } else {
     Found f;
-    if (!find<false>(r, kv_heads, group, kQueries, blockIdx.x, f)) return;
-    int local = blockIdx.x - f.item;
-    const int chunks = chunks_of(f.s.pages, f.chunk);
-    slot = chunks > 1 ? f.slot + local : -1;
-    if (slot >= slots) return;  // (rows that belong to several sequences)
-    tile = local % f.s.tiles;
-    local /= f.s.tiles;
+    const Class cl{group, share};
+    if (!find(r, kv_heads, cl, blockIdx.x, f)) return;
+    s = f.s;
+    seq = f.seq;
+    int local = f.local;
+    const int tile_of = local % f.tiles;
+    local /= f.tiles;
     head = local % kv_heads;
-    const int c = local / kv_heads;
+    const int c = local / kv_heads, pages = tile_pages(s, group, 16 * NQ, tile_of), have = chunks_of(pages, f.chunk);
+    if (c == 0 && head == 0 && slots.all > 0) leave_row_parts(part, s, group, tile_of, share.tile, f, slots);
+    if (c >= have) return;
     page0 = c * f.chunk;
-    page1 = min(page0 + f.chunk, f.s.pages);
-    row0 = f.s.row0;
-    nrows = f.s.n;
-    len = f.s.len;
-    ctx = f.s.ctx;
-    seq_table = f.seq;
+    page1 = min(page0 + f.chunk, pages);
+    tile = tile_of * NQ + sub;
+    slot = have > 1 ? slots.first + f.slot + (c * kv_heads + head) * cl.tiles16(s.n) + tile : -1;
+    if (slot >= slots.end) slot = INT_MAX;  // (row starts that do not ascend)
   }
-  const int* table = r.block_tables + (int64_t)seq_table * r.max_blocks;
+  const int* table = r.block_tables + (int64_t)seq * r.max_blocks;
 
-  // the tile's queries as operands: per (query tile, term, step) lane l's 16 bytes at 16 l
-  for (int u = tid; u < kQueries * HD / 8; u += 256) {
-    const int g8 = u % (HD / 8), q = u / (HD / 8);  // 8 dims of one query
-    const int qi = tile * kQueries + q;
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (qi < nrows * group) load8<T>(r.q, (int64_t)(row0 + qi / group) * r.ldq + (head * group + qi % group) * HD + g8 * 8, x);
-    b8 t[kN];
-    split_trunc<T>(x, t);
-    // dims 64 seg + 16 kq + 8 half
-    const int step = (g8 >> 3) * 2 + (g8 & 1), k4 = g8 >> 1 & 3;
-#pragma unroll
-    for (int k = 0; k < kN; k++)
-      reinterpret_cast<b8*>(lds)[(((q >> 4) * kN + k) * kSteps + step) * 64 + k4 * 16 + (q & 15)] = t[k];
-  }
-  // positions that a lane's queries see
-  int lim[NT];
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const int qi = tile * kQueries + t * 16 + n16;
-    lim[t] = qi < nrows * group ? (int)min((long long)len - nrows + qi / group + 1, (long long)ctx) : 0;
-  }
-  __syncthreads();
-
-  const float scale = 1.44269504088896340736f / sqrtf((float)HD);
-  float m[NT], l[NT];
-  f4 o[NT][kTiles];
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    m[t] = -INFINITY;
-    l[t] = 0;
-#pragma unroll
-    for (int i = 0; i < kTiles; i++) o[t][i] = f4{0, 0, 0, 0};
-  }
-
-  // This wave's pairs are pages page0 + 2 (wave + 4 it) and the next; a lane holds one of its next 64 pages.
+  // This wave's pairs are pages page0 + 2 (wave + 4 it) and the next.
   const int pairs = (page1 - page0 - 2 * wave + 7) / 8;
-  int my_index = 0, my_id = 0;
+  Walk walk;
   auto refill = [&](int it) {
     const int i = page0 + 2 * (wave + 4 * (it + (lane >> 1))) + (lane & 1);
-    my_index = -1;
-    my_id = -1;
-    if (i < page1) {
-      my_index = LIST ? pages_list[i] : i;
-      if (my_index >= 0 && my_index < r.max_blocks) {
-        const int id = table[my_index];
-        my_id = id >= 0 && id < p.n_pages ? id : -2;  // -2: attending it makes NaN
-      } else {
-        my_index = -1;
-      }
-    }
+    walk.set(i < page1 ? (LIST ? pages_list[i] : i) : -1, table, r.max_blocks, p.n_pages);
   };
-  struct Page {
-    int index, id;
-    uint32_t meta;
-    const uint8_t* at;
-  };
-  const size_t page_bytes = p.at.page_bytes(), head_at = (size_t)head * p.at.head_bytes(),
-               meta_at = p.at.meta_at() + (size_t)head * 4;
-  auto page_of = [&](int it, int which) {
-    Page g;
-    const int j = 2 * (it & 31) + which;
-    g.index = __builtin_amdgcn_readlane(my_index, j);
-    g.id = __builtin_amdgcn_readlane(my_id, j);
-    const uint8_t* base = p.base + (size_t)max(g.id, 0) * page_bytes;
-    g.at = base + head_at;
-    g.meta = *reinterpret_cast<const uint32_t*>(base + meta_at);
-    return g;
-  };
+  if (pairs > 0) refill(0);
+  float x[kRounds][8];
+#pragma unroll
+  for (int i = 0; i < kRounds; i++) {
+    const int u = tid + i * 256, qi = tile * 16 + u / (HD / 8);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[i][j] = 0;
+    if (u < kUnits && qi < s.n * group)
+      load8<T>(r.q, (int64_t)(s.row0 + qi / group) * r.ldq + (head * group + qi % group) * HD + u % (HD / 8) * 8, x[i]);
+  }
+  const PoolAt pool(p, head);
   u4 kc[2][kSegs], vc[2][kSegs];
   auto load_k = [&](const Page (&g)[2]) {
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-      for (int s = 0; s < kSegs; s++) kc[w][s] = reinterpret_cast<const u4*>(g[w].at)[s * 64 + lane];
+      for (int i = 0; i < kSegs; i++) kc[w][i] = reinterpret_cast<const u4*>(g[w].at)[i * 64 + lane];
   };
   auto load_v = [&](const Page (&g)[2]) {
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-      for (int s = 0; s < kSegs; s++) vc[w][s] = reinterpret_cast<const u4*>(g[w].at + kPage * HD)[s * 64 + lane];
+      for (int i = 0; i < kSegs; i++) vc[w][i] = reinterpret_cast<const u4*>(g[w].at + kPage * HD)[i * 64 + lane];
   };
-
   Page cur[2], next[2];
   if (pairs > 0) {
-    refill(0);
-    cur[0] = page_of(0, 0);
-    cur[1] = page_of(0, 1);
+    cur[0] = pool.page(walk, 0);
+    cur[1] = pool.page(walk, 1);
     load_k(cur);
     load_v(cur);
   }
+
+  // the tile's queries as operands: per (term, step) lane l's 16 bytes at 16 l
+#pragma unroll
+  for (int i = 0; i < kRounds; i++) {
+    const int u = tid + i * 256, g8 = u % (HD / 8), q = u / (HD / 8);
+    h8 t[kN];
+    const int e = query_terms<T, HD>(x[i], t);
+    if (u < kUnits) {
+      if (g8 == 0) lds_exp[q] = e;
+      // dims 64 seg + 16 kq + 8 half
+      const int step = (g8 >> 3) * 2 + (g8 & 1), k4 = g8 >> 1 & 3;
+#pragma unroll
+      for (int k = 0; k < kN; k++) reinterpret_cast<h8*>(lds)[(k * kSteps + step) * 64 + k4 * 16 + q] = t[k];
+    }
+  }
+  __syncthreads();
+
+  const float scale = 1.44269504088896340736f / sqrtf((float)HD);
+  const int qi = tile * 16 + n16;
+  const bool live = qi < s.n * group;
+  Query q;
+  q.exp = lds_exp[n16];
+  q.lim = live ? seen_by(s, qi / group) : 0;
+  const int least = seen_by(s, min(tile * 16, s.n * group - 1) / group);  // (rows see more and more)
+  const bool full = (tile + 1) * 16 <= s.n * group;                       // no query without a row
+  f4 o[kTiles];
+#pragma unroll
+  for (int i = 0; i < kTiles; i++) o[i] = f4{0, 0, 0, 0};
+
   for (int it = 0; it < pairs; it++) {
     const bool more = it + 1 < pairs;
     if (more) {
       if (((it + 1) & 31) == 0) refill(it + 1);
-      next[0] = page_of(it + 1, 0);
-      next[1] = page_of(it + 1, 1);
+      next[0] = pool.page(walk, 2 * ((it + 1) & 31));
+      next[1] = pool.page(walk, 2 * ((it + 1) & 31) + 1);
     }
-    f4 sc[NT][2];
-    {
-      f4 acc[NT][2][kN];
+    f4 sc[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+    for (int step = 0; step < kSteps; step++) {
+      const int i = step >> 1, h = step & 1;
+      const h8 a0 = of_codes8(kc[0][i][2 * h], kc[0][i][2 * h + 1]);
+      const h8 a1 = of_codes8(kc[1][i][2 * h], kc[1][i][2 * h + 1]);
 #pragma unroll
-        for (int w = 0; w < 2; w++)
-#pragma unroll
-          for (int k = 0; k < kN; k++) acc[t][w][k] = f4{0, 0, 0, 0};
-#pragma unroll
-      for (int step = 0; step < kSteps; step++) {
-        const int s = step >> 1, h = step & 1;
-        const b8 a0 = of_codes8(kc[0][s][2 * h], kc[0][s][2 * h + 1]);
-        const b8 a1 = of_codes8(kc[1][s][2 * h], kc[1][s][2 * h + 1]);
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-          for (int k = 0; k < kN; k++) {
-            const b8 q = reinterpret_cast<const b8*>(lds)[((t * kN + k) * kSteps + step) * 64 + lane];
-            acc[t][0][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, q, acc[t][0][k], 0, 0, 0);
-            acc[t][1][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, q, acc[t][1][k], 0, 0, 0);
-          }
+      for (int k = 0; k < kN; k++) {
+        const h8 b = reinterpret_cast<const h8*>(lds)[(k * kSteps + step) * 64 + lane];
+        sc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b, sc[0], 0, 0, 0);
+        sc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b, sc[1], 0, 0, 0);
       }
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-          sc[t][w] = acc[t][w][kN - 1];
-#pragma unroll
-          for (int k = kN - 2; k >= 0; k--) sc[t][w] += acc[t][w][k];
-        }
     }
     if (more) load_k(next);
-
-    uint32_t nan[2];
-    float kscale[2], vscale[2];
-    int first[2];
 #pragma unroll
-    for (int w = 0; w < 2; w++) {
-      const bool ok = cur[w].id >= 0;
-      nan[w] = ok ? Meta::nan(cur[w].meta) : cur[w].id == -2 ? 0xffffu : 0u;
-      kscale[w] = scale * pow2(ok ? Meta::ek(cur[w].meta) : 0);
-      vscale[w] = pow2(ok ? Meta::ev(cur[w].meta) : 0);
-      // (a page of no index lies behind every position)
-      first[w] = cur[w].index >= 0 ? cur[w].index * kPage + 4 * kq : INT_MAX - kPage;
-      if (!ok)
+    for (int w = 0; w < 2; w++)
+      if (cur[w].id < 0)
 #pragma unroll
-        for (int s = 0; s < kSegs; s++) vc[w][s] = u4{0, 0, 0, 0};
-    }
-    b8 wt[NT][kW];
+        for (int i = 0; i < kSegs; i++) vc[w][i] = u4{0, 0, 0, 0};
+    h8 wt[kW];
+    weigh<kW>(sc, cur, scale, full && whole_pages(cur, least), q, o, wt);
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      float x[8];
+    for (int i = 0; i < kSegs; i++)
 #pragma unroll
-      for (int w = 0; w < 2; w++)
+      for (int j = 0; j < 4; j++) {
+        const h8 a = of_codes8(vc[0][i][j], vc[1][i][j]);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          x[4 * w + i] = first[w] + i < lim[t] ? sc[t][w][i] * kscale[w] : -INFINITY;
-      if (nan[0] | nan[1]) {
-#pragma unroll
-        for (int w = 0; w < 2; w++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (first[w] + i < lim[t] && (nan[w] >> (4 * kq + i) & 1)) x[4 * w + i] = NAN;
-      }
-      float top = x[0];
-#pragma unroll
-      for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
-      top = fmaxf(m[t], quads_max(top));
-      if (__any(top > m[t])) {
-        const float down = top > -INFINITY ? __builtin_amdgcn_exp2f(m[t] - top) : 1.0f;
-        l[t] *= down;
-#pragma unroll
-        for (int i = 0; i < kTiles; i++) o[t][i] *= down;
-        m[t] = top;
-      }
-      const float at = top > -INFINITY ? top : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - at);
-        l[t] += x[i];
-        x[i] *= vscale[i / 4];
-      }
-      split_near<T>(x, wt[t]);
-    }
-#pragma unroll
-    for (int s = 0; s < kSegs; s++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const b8 a = of_codes8(vc[0][s][i], vc[1][s][i]);
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-          for (int k = kW - 1; k >= 0; k--)
-            o[t][4 * s + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, wt[t][k], o[t][4 * s + i], 0, 0, 0);
+        for (int k = kW - 1; k >= 0; k--)
+          o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wt[k], o[4 * i + j], 0, 0, 0);
       }
     if (more) {
       load_v(next);
@@ -520,135 +648,372 @@ __global__ __launch_bounds__(256) void item_kernel(Pool p, Rows r, Out out, List
   }
 
   // the four waves' states, joined in wave order
+  q.l = quads_sum(q.l);
+  if (kq == 0) lds_st[wave][n16] = f4{q.m, q.mv, q.l, 0};
+  State st;
+  float by[4], inv = 0;
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    l[t] = quads_sum(l[t]);
-    if (kq == 0) lds_ml[wave][t * 16 + n16] = f2{m[t], l[t]};
+  for (int t0 = 0; t0 < kTiles; t0 += kJoinTiles) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kJoinTiles; i++) reinterpret_cast<f4*>(lds)[(wave * kJoinTiles + i) * 64 + lane] = o[t0 + i];
+    __syncthreads();
+    if (t0 == 0) {
+      st.join<4>([&](int w) { return lds_st[w][n16]; }, by);
+      inv = st.factor();
+      if (live && slot >= 0 && slot < INT_MAX && wave == 0 && kq == 0) part.st[(int64_t)slot * 16 + n16] = f4{st.m, st.mv, st.l, 0};
+    }
+    if (live) {
+      const int row = s.row0 + qi / group, col = (head * group + qi % group) * HD;
+#pragma unroll
+      for (int i = wave; i < kJoinTiles; i += 4) {
+        f4 v = reinterpret_cast<const f4*>(lds)[i * 64 + lane] * by[0];
+#pragma unroll
+        for (int w = 1; w < 4; w++) v += reinterpret_cast<const f4*>(lds)[(w * kJoinTiles + i) * 64 + lane] * by[w];
+        const int d = (t0 + i) * 16 + kq * 4;
+        if (slot == INT_MAX) continue;
+        if (slot >= 0) *reinterpret_cast<f4*>(part.o + ((int64_t)slot * 16 + n16) * HD + d) = v;
+        else store4<T>(out, row, col + d, v * inv);
+      }
+    }
   }
-  const Partials part = partials_at<HD>(ws, slots, kQueries);
+}
+
+// ---- many queries a sequence -------------------------------------------------------------
+
+// Workgroup: 64 NT queries, 16 NT a wave, over the pages of a chunk, two at a time through LDS (two buffers, one
+// barrier a pair). A wave keeps its queries' terms in registers.
+template <int HD, int T, int NT>
+__global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out, Share share, void* ws, Slots slots) {
+  constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms<T>;
+  constexpr int kHead = 2 * kPage * HD;            // bytes of a page and head
+  constexpr int kRounds = 2 * kHead / 4096;        // 16 bytes a thread each, of a pair
+  constexpr int kQueries = 64 * NT;
+  constexpr int kQBytes = 16 * HD * 2;             // 16 queries' operands of one term
+  constexpr int kLds = 2 * 2 * kHead > 4 * kQBytes ? 2 * 2 * kHead : 4 * kQBytes;
+  __shared__ __align__(16) uint8_t lds[kLds];
+  __shared__ int lds_exp[kQueries];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n16 = lane & 15, kq = lane >> 4;
+  const int kv_heads = p.at.kv_heads, group = r.heads / kv_heads;
+  const Partials part = partials_at<HD>(ws, r.rows, slots.all);
+
+  Found f;
+  const Class cl{group, share};
+  if (!find(r, kv_heads, cl, blockIdx.x, f)) return;
+  const Seq s = f.s;
+  // The last tiles, which see most, first. KV heads in turn: workgroups go to the 8 XCDs in turn, so an L2
+  // holds the pages of one or two heads where there are 4 or 8.
+  int local = f.local;
+  const int head = local % kv_heads;
+  local /= kv_heads;
+  const int tile = f.tiles - 1 - local % f.tiles, c = local / f.tiles;
+  const int pages = tile_pages(s, group, kQueries, tile), have = chunks_of(pages, f.chunk);
+  if (c == 0 && head == 0 && slots.all > 0) leave_row_parts(part, s, group, tile, kQueries, f, slots);
+  if (c >= have) return;
+  const int page0 = c * f.chunk, page1 = min(page0 + f.chunk, pages), pairs = (page1 - page0 + 1) / 2;
+  const int* table = r.block_tables + (int64_t)f.seq * r.max_blocks;
+  Walk walk;
+  auto refill = [&](int it) {
+    const int i = page0 + 2 * it + lane;
+    walk.set(i < page1 ? i : -1, table, r.max_blocks, p.n_pages);
+  };
+  if (pairs > 0) refill(0);
+
+  // The wave's queries, 16 at a time: loaded as rows, turned into operands through LDS.
+  h8 qt[NT][kN][kSteps];
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kTiles; i++) reinterpret_cast<f4*>(lds)[(wave * kTiles + i) * 64 + lane] = o[t][i];
-    __syncthreads();
-    const int q = t * 16 + n16, qi = tile * kQueries + q;
-    if (qi < nrows * group) {
-      float top = -INFINITY, sum = 0, by[4];
+    for (int k = 0; k < kN; k++) {
+      if (t + k > 0) __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 4; w++) top = fmaxf(top, lds_ml[w][q][0]);
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        by[w] = lds_ml[w][q][0] > -INFINITY ? __builtin_amdgcn_exp2f(lds_ml[w][q][0] - top) : 1.0f;
-        sum += by[w] * lds_ml[w][q][1];
+      for (int u0 = 0; u0 < 16 * HD / 8; u0 += 64) {
+        const int u = u0 + lane, g8 = u % (HD / 8), q = u / (HD / 8);
+        const int ql = (wave * NT + t) * 16 + q, qi = tile * kQueries + ql;
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (qi < s.n * group)
+          load8<T>(r.q, (int64_t)(s.row0 + qi / group) * r.ldq + (head * group + qi % group) * HD + g8 * 8, x);
+        h8 terms[kN];
+        const int e = query_terms<T, HD>(x, terms);
+        if (g8 == 0) lds_exp[ql] = e;
+        const int step = (g8 >> 3) * 2 + (g8 & 1), k4 = g8 >> 1 & 3;
+        reinterpret_cast<h8*>(lds + wave * kQBytes)[step * 64 + k4 * 16 + q] = terms[k];
       }
-      const int row = row0 + qi / group, col = (head * group + qi % group) * HD;
-      const float inv = sum == 0 ? 0.0f : 1.0f / sum;  // (nothing attended: zero)
-      if (slot >= 0 && wave == 0 && kq == 0) part.ml[(int64_t)slot * kQueries + q] = f2{top, sum};
-      for (int i = wave; i < kTiles; i += 4) {
-        f4 x = reinterpret_cast<const f4*>(lds)[i * 64 + lane] * by[0];
+      __syncthreads();
 #pragma unroll
-        for (int w = 1; w < 4; w++) x += reinterpret_cast<const f4*>(lds)[(w * kTiles + i) * 64 + lane] * by[w];
-        if (slot >= 0) *reinterpret_cast<f4*>(part.o + ((int64_t)slot * kQueries + q) * HD + i * 16 + kq * 4) = x;
-        else store4<T>(out, row, col + i * 16 + kq * 4, x * inv);
+      for (int i = 0; i < kSteps; i++) qt[t][k][i] = reinterpret_cast<const h8*>(lds + wave * kQBytes)[i * 64 + lane];
+    }
+  }
+  __syncthreads();
+
+  Query q[NT];
+  int least = INT_MAX, most = 0;
+  bool full = true;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int ql = (wave * NT + t) * 16, qi = tile * kQueries + ql, end = s.n * group;
+    q[t].exp = lds_exp[ql + n16];
+    q[t].lim = qi + n16 < end ? seen_by(s, (qi + n16) / group) : 0;
+    full &= qi + 16 <= end;
+    if (qi < end) {
+      least = min(least, seen_by(s, qi / group));
+      most = max(most, seen_by(s, min(qi + 15, end - 1) / group));
+    }
+  }
+  const PoolAt pool(p, head);
+  u4 next[kRounds];
+  auto load = [&](const Page (&g)[2]) {
+#pragma unroll
+    for (int i = 0; i < kRounds; i++) {
+      const int at = (i * 256 + tid) * 16;  // a page of the pair takes whole rounds, or half of one
+      const int w = at / kHead;
+      const uint8_t* from = kRounds > 1 ? g[i * 4096 / kHead].at : (w ? g[1].at : g[0].at);
+      next[i] = *reinterpret_cast<const u4*>(from + (at - w * kHead));
+      const int id = kRounds > 1 ? g[i * 4096 / kHead].id : (w ? g[1].id : g[0].id);
+      if (id < 0) next[i] = u4{0, 0, 0, 0};
+    }
+  };
+  auto put = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < kRounds; i++) reinterpret_cast<u4*>(lds + b * 2 * kHead)[i * 256 + tid] = next[i];
+  };
+  const float scale = 1.44269504088896340736f / sqrtf((float)HD);
+  f4 o[NT][kTiles];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int i = 0; i < kTiles; i++) o[t][i] = f4{0, 0, 0, 0};
+  Page cur[2], nxt[2];
+  if (pairs > 0) {
+    cur[0] = pool.page(walk, 0);
+    cur[1] = pool.page(walk, 1);
+    load(cur);
+    put(0);
+  }
+  __syncthreads();
+  for (int it = 0; it < pairs; it++) {
+    const bool more = it + 1 < pairs;
+    if (more) {
+      if (((it + 1) & 31) == 0) refill(it + 1);
+      nxt[0] = pool.page(walk, 2 * ((it + 1) & 31));
+      nxt[1] = pool.page(walk, 2 * ((it + 1) & 31) + 1);
+      load(nxt);
+    }
+    if (cur[0].index * kPage < most) {  // (the pair is not behind all of the wave's queries)
+      const u4* kv = reinterpret_cast<const u4*>(lds + (it & 1) * 2 * kHead) + lane;
+      f4 sc[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; t++) sc[t][0] = sc[t][1] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kSegs; i++) {
+        const u4 c0 = kv[i * 64], c1 = kv[kHead / 16 + i * 64];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const h8 a0 = of_codes8(c0[2 * h], c0[2 * h + 1]), a1 = of_codes8(c1[2 * h], c1[2 * h + 1]);
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int k = 0; k < kN; k++) {
+              sc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, qt[t][k][2 * i + h], sc[t][0], 0, 0, 0);
+              sc[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, qt[t][k][2 * i + h], sc[t][1], 0, 0, 0);
+            }
+        }
       }
+      const bool whole = full && whole_pages(cur, least);
+      h8 wt[NT][kW];
+#pragma unroll
+      for (int t = 0; t < NT; t++) weigh<kW>(sc[t], cur, scale, whole, q[t], o[t], wt[t]);
+#pragma unroll
+      for (int i = 0; i < kSegs; i++) {
+        const u4 c0 = kv[kHead / 32 + i * 64], c1 = kv[kHead / 16 + kHead / 32 + i * 64];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const h8 a = of_codes8(c0[j], c1[j]);
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int k = kW - 1; k >= 0; k--)
+              o[t][4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wt[t][k], o[t][4 * i + j], 0, 0, 0);
+        }
+      }
+    }
+    if (more) {
+      put((it + 1) & 1);
+      cur[0] = nxt[0];
+      cur[1] = nxt[1];
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const float l = quads_sum(q[t].l);
+    const int qi = tile * kQueries + (wave * NT + t) * 16 + n16;
+    if (qi >= s.n * group) continue;
+    const int row = s.row0 + qi / group, col = (head * group + qi % group) * HD;
+    if (have > 1) {
+      const int64_t slot = slots.first + f.slot + ((int64_t)c * kv_heads + head) * cl.tiles16(s.n) + qi / 16;
+      if (slot >= slots.end) continue;
+      if (kq == 0) part.st[slot * 16 + n16] = f4{q[t].m, q[t].mv, l, 0};
+#pragma unroll
+      for (int i = 0; i < kTiles; i++)
+        *reinterpret_cast<f4*>(part.o + (slot * 16 + n16) * HD + i * 16 + kq * 4) = o[t][i];
+    } else {
+      State st;
+      st.m = q[t].m;
+      st.mv = q[t].mv;
+      st.l = l;
+      const float inv = st.factor();
+#pragma unroll
+      for (int i = 0; i < kTiles; i++) store4<T>(out, row, col + i * 16 + kq * 4, o[t][i] * inv);
     }
   }
 }
 
 // ---- joining the chunks ---------------------------------------------------------------
 
-// A wave per (row, head): the partial sums of its chunks in order.
-template <int HD, int T, int NT, bool LIST>
+// WAVES waves per (row, head): the partial sums of its chunks, each wave's in order, then the waves' in order.
+template <int HD, int T, bool LIST, int WAVES>
 __global__ __launch_bounds__(256) void merge_kernel(Rows r, Out out, List list, int kv_heads, void* ws, int slots) {
-  constexpr int kQueries = 16 * NT, kLanes = HD / 4;  // lanes with 4 dims each
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int kLanes = HD / 4, kSub = 64 / kLanes;  // lanes with 4 dims each, and chunks that a wave takes at once
+  constexpr int kParts = WAVES * kSub;
+  __shared__ f4 lds_o[4][kLanes];
+  __shared__ f4 lds_st[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = WAVES == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   const int row = __builtin_amdgcn_readfirstlane((int)(id / r.heads)), h = __builtin_amdgcn_readfirstlane((int)(id % r.heads));
+  const int first = (WAVES == 4 ? wave * kSub : 0) + lane / kLanes;  // this lane's first chunk
   if (row >= r.rows) return;
   const int group = r.heads / kv_heads, head = h / group;
-  int chunks, slot, step, q;
+  const Partials part = partials_at<HD>(ws, LIST ? 0 : r.rows, slots);
+  int chunks, q;
+  int64_t slot, step;
   if constexpr (LIST) {
-    const int seq = seq_of(r, row);
-    if (seq < 0) return;
     const int count = min(max(list.count[(int64_t)row * kv_heads + head], 0), list.top), tiles = (group + 15) / 16;
     chunks = chunks_of(count, list.chunk);
     q = h % group;
-    slot = ((row * kv_heads + head) * tiles + q / 16) * list.chunks;
+    slot = (((int64_t)row * kv_heads + head) * tiles + q / 16) * list.chunks;
     step = 1;
-    q %= 16;
+    if (chunks == 1 || seq_of(r, row) < 0) return;
   } else {
-    Found f;
-    if (!find<true>(r, kv_heads, group, kQueries, row, f)) return;
-    chunks = chunks_of(f.s.pages, f.chunk);
-    q = (row - f.s.row0) * group + h % group;
-    slot = f.slot + head * f.s.tiles + q / kQueries;
-    step = kv_heads * f.s.tiles;
-    q %= kQueries;
+    const RowPart rp = part.rows[row];
+    if (row < r.row_start[0] || row >= r.row_start[r.nseq]) return;
+    Seq s;
+    s.row0 = rp.row0;
+    s.n = rp.n;
+    s.len = rp.len;
+    s.ctx = (int)min((long long)max(s.len, 0), (long long)r.max_blocks * kPage);
+    q = (row - rp.row0) * group + h % group;
+    const int tiles = (int)(((int64_t)rp.n * group + 15) / 16);
+    if (rp.chunk < kMinChunk || rp.tile_queries < 16) return;
+    chunks = chunks_of(tile_pages(s, group, rp.tile_queries, q / rp.tile_queries), rp.chunk);
+    slot = rp.slot + (int64_t)head * tiles + q / 16;
+    step = (int64_t)kv_heads * tiles;
+    if (chunks == 1) return;
   }
-  if (chunks == 1 || slot < 0 || (int64_t)slot + (int64_t)(chunks - 1) * step >= slots) return;
-  const Partials part = partials_at<HD>(ws, slots, kQueries);
-  float top = -INFINITY;
-  for (int c = lane; c < chunks; c += 64) top = fmaxf(top, part.ml[((int64_t)slot + (int64_t)c * step) * kQueries + q][0]);
-  top = wave_max(top);
-  float sum = 0;
+  if (slot < 0 || step < 0 || slot + (chunks - 1) * step >= slots) return;  // (row starts that do not ascend)
+  q &= 15;
+  State j;
+  auto state_of = [&](int c) { return part.st[(slot + c * step) * 16 + q]; };
+  for (int c = lane; c < chunks; c += 64) {
+    const f4 st = state_of(c);
+    j.m = fmaxf(j.m, st[0]);
+    j.mv = fmaxf(j.mv, st[1]);
+  }
+  j.m = wave_max(j.m);
+  j.mv = wave_max(j.mv);
   f4 x{0, 0, 0, 0};
-  for (int c0 = 0; c0 < chunks; c0 += 64) {
-    f2 ml{-INFINITY, 0};
-    if (c0 + lane < chunks) ml = part.ml[((int64_t)slot + (int64_t)(c0 + lane) * step) * kQueries + q];
-    const float by = ml[0] > -INFINITY ? __builtin_amdgcn_exp2f(ml[0] - top) : 1.0f;
-    sum += by * ml[1];
-    const int many = min(chunks - c0, 64);
-    const float* from = part.o + (((int64_t)slot + (int64_t)c0 * step) * kQueries + q) * HD + (lane % kLanes) * 4;
 #pragma unroll 8
-    for (int c = 0; c < many; c++)
-      x += *reinterpret_cast<const f4*>(from + (int64_t)c * step * kQueries * HD) *
-           __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, by), c));
+  for (int c = first; c < chunks; c += kParts) {
+    const f4 st = state_of(c);
+    x += *reinterpret_cast<const f4*>(part.o + ((slot + c * step) * 16 + q) * HD + (lane % kLanes) * 4) * j.of_part(st);
+    j.l += j.sum_of_part(st);
   }
-  sum = wave_sum(sum);
-  if (lane < kLanes) store4<T>(out, row, (int64_t)h * HD + lane * 4, x * (sum == 0 ? 0.0f : 1.0f / sum));
+  // lanes of the same dims, then waves
+#pragma unroll
+  for (int o = kLanes; o < 64; o <<= 1) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] += __shfl_xor(x[i], o);
+    j.l += __shfl_xor(j.l, o);
+  }
+  if constexpr (WAVES == 4) {
+    if (lane < kLanes) lds_o[wave][lane] = x;
+    if (lane == 0) lds_st[wave][0] = j.l;
+    __syncthreads();
+    if (wave > 0) return;
+    if (lane < kLanes)
+#pragma unroll
+      for (int w = 1; w < 4; w++) x += lds_o[w][lane];
+#pragma unroll
+    for (int w = 1; w < 4; w++) j.l += lds_st[w][0];
+  }
+  if (lane < kLanes) store4<T>(out, row, (int64_t)h * HD + lane * 4, x * j.factor());
 }
 
 // ---- launches ---------------------------------------------------------------------------
 
-// Tiles of `queries` over all rows, at most.
-int64_t tiles_most(int group, int nseq, int rows, int queries) {
-  return (int64_t)rows * group / queries + (nseq < rows ? nseq : rows);
-}
-
 struct Grid {
   int64_t items, slots;
 };
-Grid grid_of(const Layout& at, int heads, int nseq, int max_blocks, int rows, int queries) {
-  const int64_t tiles = tiles_most(heads / at.kv_heads, nseq, rows, queries) * at.kv_heads;
-  const int64_t cut = tiles * ((max_blocks + kMinChunk - 1) / kMinChunk);
-  // contexts longer than a chunk of c pages make at most twice (all tiles' pages) / c items, the rest one each
-  return Grid{cut < tiles + kItems ? cut : tiles + kItems, cut < 2 * kItems ? cut : 2 * kItems};
+
+// Items and partial sums that a share may have. Tiles of all rows' queries: at most a full
+// one for every `tile` and a last one for every sequence. A context of p pages in chunks of c makes
+// up to p / c + 1 items of a tile, and 2 p / c if it is cut at all; c is at least all tiles' pages
+// over share.items (but for the rounding of sums in f32: an eighth more).
+Grid grid_of(const Layout& at, int heads, int nseq, int max_blocks, int rows, const Share& sh) {
+  const int64_t group = heads / at.kv_heads, seqs = nseq < rows ? nseq : rows;
+  int64_t tiles = rows * group / sh.tile + seqs;
+  if (sh.most < INT_MAX) tiles = std::min(tiles, seqs * ((sh.most + sh.tile - 1) / sh.tile));
+  tiles *= at.kv_heads;
+  const int64_t per = (max_blocks + kMinChunk - 1) / kMinChunk, cut = tiles * per, most = sh.items + sh.items / 8;
+  return Grid{std::min(cut, tiles + most), per > 1 ? std::min(cut, 2 * most) * (sh.tile / 16) : 0};
+}
+
+constexpr int prompt_tiles(int hd) { return hd == 256 ? 1 : 2; }
+
+// How a call is shared out: by the largest number of queries that a sequence has for a KV head. Up to 16 and up to 32
+// are item_kernel's alone, one or two tiles side by side; past that it keeps the sequences of up to 16.
+struct Plan {
+  Share few, many;
+  bool two;   // tiles side by side
+  bool both;  // prompt_kernel has a share
+};
+Plan plan_of(int hd, int group, int64_t max_rows) {
+  const int64_t most = max_rows * group;
+  Plan p{};
+  p.both = most > kFewQueries;
+  p.two = most > 16 && !p.both;
+  p.few = Share{1, p.both ? 16 : INT_MAX, p.two ? 32 : 16, kFewItems};
+  p.many = Share{17, INT_MAX, 64 * prompt_tiles(hd), kManyItems};
+  return p;
 }
 
 int sparse_chunk(const Layout& at, int heads, int rows, int top) {
   const int64_t all = (int64_t)rows * at.kv_heads * ((heads / at.kv_heads + 15) / 16) * top;
-  const int64_t c = ((all + kItems - 1) / kItems + 7) & ~7ll;
+  const int64_t c = ((all + kFewItems - 1) / kFewItems + 7) & ~7ll;
   return (int)(c > kMinChunk ? (c < 1 << 20 ? c : 1 << 20) : kMinChunk);
 }
 
-template <int HD, int T, int NT, bool LIST>
-void launch(const Pool& p, const Rows& r, const Out& o, const List& list, void* ws, int64_t items, int64_t slots,
-            bool merge, hipStream_t s) {
-  item_kernel<HD, T, NT, LIST><<<(unsigned)items, 256, 0, s>>>(p, r, o, list, ws, (int)slots);
-  PGD_HIP(hipGetLastError());
-  if (!merge) return;
-  const int64_t waves = (int64_t)r.rows * r.heads;
-  merge_kernel<HD, T, NT, LIST><<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(r, o, list, p.at.kv_heads, ws, (int)slots);
+template <int HD, int T>
+void merge(const Rows& r, const Out& o, const List* list, int kv_heads, void* ws, int64_t slots, hipStream_t s) {
+  const int64_t outs = (int64_t)r.rows * r.heads;
+  const List l = list ? *list : List{};
+  // Four waves a result where there are few; measured at <>.
+  auto go = [&](auto is_list, auto waves) {
+    const unsigned blocks = (unsigned)(waves == 4 ? outs : (outs + 3) / 4);
+    merge_kernel<HD, T, is_list, waves><<<blocks, 256, 0, s>>>(r, o, l, kv_heads, ws, (int)slots);
+  };
+  const bool wide = outs <= 4096;
+  using W4 = std::integral_constant<int, 4>;
+  using W1 = std::integral_constant<int, 1>;
+  if (list) wide ? go(std::true_type(), W4()) : go(std::true_type(), W1());
+  else wide ? go(std::false_type(), W4()) : go(std::false_type(), W1());
   PGD_HIP(hipGetLastError());
 }
 
-template <int NT, bool LIST>
-void launch_of(const Pool& p, const Rows& r, const Out& o, const List& list, void* ws, int64_t items, int64_t slots,
-               bool merge, hipStream_t s) {
-  auto go = [&](auto hd, auto type) {
-    launch<decltype(hd)::value, decltype(type)::value, NT, LIST>(p, r, o, list, ws, items, slots, merge, s);
-  };
+template <class F>
+void with_types(const Pool& p, const Rows& r, F&& go) {
   auto typed = [&](auto hd) {
     if (r.type == F32) go(hd, std::integral_constant<int, F32>());
     else if (r.type == F16) go(hd, std::integral_constant<int, F16>());
@@ -659,30 +1024,58 @@ void launch_of(const Pool& p, const Rows& r, const Out& o, const List& list, voi
   else typed(std::integral_constant<int, 256>());
 }
 
-size_t partial_bytes(const Layout& at, int64_t slots, int queries) { return (size_t)slots * queries * (at.hd + 2) * 4; }
+size_t partial_bytes(const Layout& at, int64_t slots) { return (size_t)slots * 16 * (at.hd + 4) * 4; }
 
 }  // namespace
 
 size_t attn_ws_bytes(const Layout& at, int heads, int nseq, int max_blocks, int rows) {
-  return partial_bytes(at, grid_of(at, heads, nseq, max_blocks, rows, 16).slots, 16);
+  // whatever max_rows the call will name
+  int64_t slots = 0;
+  for (int64_t max_rows : {(int64_t)0, (int64_t)kFewQueries / (heads / at.kv_heads), (int64_t)rows + kFewQueries}) {
+    const Plan p = plan_of(at.hd, heads / at.kv_heads, max_rows);
+    slots = std::max(slots, grid_of(at, heads, nseq, max_blocks, rows, p.few).slots +
+                                (p.both ? grid_of(at, heads, nseq, max_blocks, rows, p.many).slots : 0));
+  }
+  return slots ? (size_t)rows * sizeof(RowPart) + partial_bytes(at, slots) : 0;
 }
 
 void attn(const Pool& p, const Rows& r, int max_rows, const Out& o, void* ws, hipStream_t s) {
-  const Grid g = grid_of(p.at, r.heads, r.nseq, r.max_blocks, r.rows, 16);
-  launch_of<1, false>(p, r, o, List{}, ws, g.items, g.slots, r.max_blocks > kMinChunk, s);
+  const Plan pl = plan_of(p.at.hd, r.heads / p.at.kv_heads, max_rows);
+  const Grid few = grid_of(p.at, r.heads, r.nseq, r.max_blocks, r.rows, pl.few);
+  const Grid many = pl.both ? grid_of(p.at, r.heads, r.nseq, r.max_blocks, r.rows, pl.many) : Grid{};
+  const int all = (int)(few.slots + many.slots);
+  with_types(p, r, [&](auto hd, auto type) {
+    constexpr int HD = decltype(hd)::value, T = decltype(type)::value;
+    if (pl.both) {
+      prompt_kernel<HD, T, prompt_tiles(HD)><<<(unsigned)many.items, 256, 0, s>>>(p, r, o, pl.many, ws,
+                                                                                 Slots{all, (int)few.slots, all});
+      PGD_HIP(hipGetLastError());
+    }
+    const Slots own{all, 0, (int)few.slots};
+    if (pl.two) item_kernel<HD, T, 2, false><<<(unsigned)few.items, 512, 0, s>>>(p, r, o, List{}, pl.few, ws, own);
+    else item_kernel<HD, T, 1, false><<<(unsigned)few.items, 256, 0, s>>>(p, r, o, List{}, pl.few, ws, own);
+    PGD_HIP(hipGetLastError());
+    if (all > 0) merge<HD, T>(r, o, nullptr, p.at.kv_heads, ws, all, s);
+  });
 }
 
 size_t attn_sparse_ws_bytes(const Layout& at, int heads, int rows, int top) {
   const int c = sparse_chunk(at, heads, rows, top), chunks = (top + c - 1) / c;
   if (chunks <= 1) return 0;
-  return partial_bytes(at, (int64_t)rows * at.kv_heads * ((heads / at.kv_heads + 15) / 16) * chunks, 16);
+  return partial_bytes(at, (int64_t)rows * at.kv_heads * ((heads / at.kv_heads + 15) / 16) * chunks);
 }
 
 void attn_sparse(const Pool& p, const Rows& r, int top, const int* sel, const int* count, const Out& o, void* ws,
                  hipStream_t s) {
   const int c = sparse_chunk(p.at, r.heads, r.rows, top), chunks = (top + c - 1) / c;
   const int64_t items = (int64_t)r.rows * p.at.kv_heads * ((r.heads / p.at.kv_heads + 15) / 16) * chunks;
-  launch_of<1, true>(p, r, o, List{sel, count, top, c, chunks}, ws, items, items, chunks > 1, s);
+  const List list{sel, count, top, c, chunks};
+  with_types(p, r, [&](auto hd, auto type) {
+    constexpr int HD = decltype(hd)::value, T = decltype(type)::value;
+    item_kernel<HD, T, 1, true><<<(unsigned)items, 256, 0, s>>>(p, r, o, list, Share{}, ws, Slots{(int)items, 0, (int)items});
+    PGD_HIP(hipGetLastError());
+    if (chunks > 1) merge<HD, T>(r, o, &list, p.at.kv_heads, ws, items, s);
+  });
 }
 
 }  // namespace kv8

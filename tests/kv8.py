@@ -157,15 +157,17 @@ class Step:
                 yield int(self.row_start[s]) + j, s, max(c - n + j + 1, 0)
 
 
-def attend(q, k, v, t):
+def attend(q, k, v, t, unit=0.0):
     """One query [hd] over positions k, v [n, hd] (float64): the result and the bound on what a kernel with f32
-    sums may be off, with r the softmax weights' own rounding.
+    sums may be off. unit: the power of two of each position's value codes.
 
     A score of hd exact products in at most three terms, summed in any order: (3 hd + 4) 2^-23 of
     sum |q k|, and one rounding of the scaled score, of its maximum's difference and
     of the exponent's argument, each 2^-24 of its magnitude, 2^-22 for exp2 itself. Weights then
-    are off by the factor exp(2 d). They enter as bf16 terms, three for f32 and two for the others: a
-    significand of 8 bits is half a step, 2^-8, off at most, so k terms leave 2^-8k. The sums of n weights and n products by n 2^-23 each."""
+    are off by the factor exp(2 d). They enter as f16 terms, two (bf16 rows: one): a significand of
+    11 bits is half a step, 2^-11, off at most, so k terms leave 2^-11k, and no
+    less than f16's smallest half step, 2^-25, which is 2^-40 of the largest weight of a code; codes are up to
+    448. The sums of n weights and n products by n 2^-23 each."""
     if len(k) == 0:
         return np.zeros(v.shape[1]), np.zeros(v.shape[1])
     hd = k.shape[1]
@@ -176,9 +178,10 @@ def attend(q, k, v, t):
          + 4 * 2.0 ** -24 * 1.5 * np.abs(s).max() + 2.0 ** -22)
     w = np.exp(s - s.max())
     w /= w.sum()
-    held = {F32: 2.0 ** -24, F16: 2.0 ** -16, BF16: 2.0 ** -16}[t]
+    held = {F32: 2.0 ** -22, F16: 2.0 ** -22, BF16: 2.0 ** -11}[t]
     mass = w @ np.abs(v)
-    return w @ v, mass * (2 * np.expm1(2 * d) + held + (2 * len(k) + 16) * 2.0 ** -23)
+    small = len(k) * 448 * 2.0 ** -40 * (w * unit).max()
+    return w @ v, mass * (2 * np.expm1(2 * d) + held + (2 * len(k) + 16) * 2.0 ** -23) + small
 
 
 def sigmoid(x):
@@ -199,7 +202,8 @@ def attention(step, q, t, heads, gate=None, picked=None):
             at = (places[:, None] * PAGE + np.arange(PAGE)).reshape(-1)
             use = at < seen
             kk, vv = (x[step.tables[s, places], head].reshape(-1, c.hd)[use] for x in kv)
-            o, b = attend(q[row, h], kk, vv, t)
+            unit = 2.0 ** c.exps[1, step.tables[s, places], head].astype(float).repeat(PAGE)[use]
+            o, b = attend(q[row, h], kk, vv, t, unit)
             if gate is not None:
                 sg = sigmoid(gate[row, h])
                 # sigmoid: exp2 of a rounded product, a sum, a quotient; then the product
