@@ -66,6 +66,30 @@ __device__ inline void split(const float (&x)[8], h8 (&out)[N]) {
   }
 }
 
+// The same for weights, in fewer instructions: all terms but the last truncated, two at a time (what is left is
+// exact), the last to nearest.
+template <int N>
+__device__ inline void split_weights(const float (&x)[8], h8 (&out)[N]) {
+  float r[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) r[j] = x[j];
+#pragma unroll
+  for (int k = 0; k < N; k++)
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      if (k + 1 < N) {
+        const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(r[j], r[j + 1]));
+        out[k][j] = h[0];
+        out[k][j + 1] = h[1];
+        r[j] -= (float)h[0];
+        r[j + 1] -= (float)h[1];
+      } else {
+        out[k][j] = (_Float16)r[j];
+        out[k][j + 1] = (_Float16)r[j + 1];
+      }
+    }
+}
+
 // Eight codes as f16.
 __device__ inline h8 of_codes8(uint32_t lo, uint32_t hi) {
   const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
@@ -76,33 +100,6 @@ __device__ inline h8 of_codes8(uint32_t lo, uint32_t hi) {
 }
 
 // ---- the list of items ------------------------------------------------------------
-
-// Sums over the lanes before and with a lane, and over all lanes (identical in every lane).
-template <int CTRL, int ROWS>
-__device__ inline int dpp_add(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ inline int wave_scan(int v) {
-  v = dpp_add<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes of 16 up
-  v = dpp_add<0x112, 0xf>(v);
-  v = dpp_add<0x114, 0xf>(v);
-  v = dpp_add<0x118, 0xf>(v);
-  v = dpp_add<0x142, 0xa>(v);  // lane 15 of a row to the next row, then lane 31 to the upper half
-  return dpp_add<0x143, 0xc>(v);
-}
-template <int CTRL, int ROWS>
-__device__ inline float dpp_addf(float v) {
-  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
-}
-__device__ inline float wave_total(float v) {
-  v = dpp_addf<0x111, 0xf>(v);
-  v = dpp_addf<0x112, 0xf>(v);
-  v = dpp_addf<0x114, 0xf>(v);
-  v = dpp_addf<0x118, 0xf>(v);
-  v = dpp_addf<0x142, 0xa>(v);
-  v = dpp_addf<0x143, 0xc>(v);
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
 
 struct Seq {
   int row0, n;      // its rows
@@ -125,7 +122,7 @@ __device__ inline Seq seq_at(const Rows& r, int i) {
 // A kernel's share of a call: sequences of at least `least` and at most `most` queries a KV head, in tiles.
 struct Share {
   int least, most;
-  int tile;   // queries
+  int tile;   // queries, a power of two
   int items;  // that contexts are cut into, about
 };
 
@@ -133,11 +130,11 @@ struct Class {
   int group;
   Share sh;
   __device__ int tiles(int n) const {
-    const long long q = (long long)n * group;
-    return q < sh.least || q > sh.most ? 0 : (int)((q + sh.tile - 1) / sh.tile);
+    const int q = n * group;  // (rows * heads stay below 2^26)
+    return q < sh.least || q > sh.most ? 0 : (q + sh.tile - 1) >> __builtin_ctz(sh.tile);
   }
   // partial sums are of 16 queries, whatever the tile
-  __device__ int tiles16(int n) const { return (int)(((long long)n * group + 15) / 16); }
+  __device__ int tiles16(int n) const { return (n * group + 15) >> 4; }
 };
 
 // The workspace's partial sums: how many it has, and a launch's own.
@@ -233,7 +230,7 @@ __device__ inline int seen_by(const Seq& s, int j) {
 
 // Pages that the last row of a tile sees.
 __device__ inline int tile_pages(const Seq& s, int group, int tile_queries, int tile) {
-  const int last = (int)min(((long long)(tile + 1) * tile_queries - 1) / group, (long long)s.n - 1);
+  const int last = min(((tile + 1) * tile_queries - 1) / group, s.n - 1);
   return (seen_by(s, last) + kPage - 1) / kPage;
 }
 
@@ -258,7 +255,7 @@ __device__ inline void store4(const Out& o, int64_t row, int64_t col, f4 x) {
   if (o.gate) {
     const f4 g = load4<T>(o.gate, row * o.ldg + col);
 #pragma unroll
-    for (int j = 0; j < 4; j++) x[j] = x[j] / (1.0f + __builtin_amdgcn_exp2f(g[j] * -1.44269504088896f));
+    for (int j = 0; j < 4; j++) x[j] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g[j] * -1.44269504088896f));
   }
   if constexpr (T == F32) {
     *reinterpret_cast<f4*>(static_cast<float*>(o.out) + row * o.ldo + col) = x;
@@ -329,8 +326,8 @@ struct List {
 // The RowParts of the rows whose first query a tile has.
 __device__ inline void leave_row_parts(const Partials& part, const Seq& s, int group, int tile, int tile_queries,
                                        const Found& f, const Slots& slots) {
-  const int j = (int)(((int64_t)tile * tile_queries + group - 1) / group) + (int)threadIdx.x;
-  if ((int)threadIdx.x < tile_queries && j < s.n && (int64_t)j * group < (int64_t)(tile + 1) * tile_queries)
+  const int j = (tile * tile_queries + group - 1) / group + (int)threadIdx.x;
+  if ((int)threadIdx.x < tile_queries && j < s.n && j * group < (tile + 1) * tile_queries)
     part.rows[s.row0 + j] = RowPart{slots.first + f.slot, f.chunk, s.row0, s.n, s.len, tile_queries, {0, 0}};
 }
 
@@ -385,13 +382,14 @@ template <int KW, int N>
 __device__ inline void weigh(const f4 (&s)[2], const Page (&pg)[2], float scale, bool whole, Query& q, f4 (&o)[N],
                              h8 (&out)[KW]) {
   const int kq = threadIdx.x >> 4 & 3;
-  float x[8], ev[2];
+  float x[8], by[2], ev[2];
 #pragma unroll
   for (int w = 0; w < 2; w++) {
-    const float by = __builtin_ldexpf(scale, q.exp + Meta::ek(pg[w].meta));
+    // (not below the normal range: the scores of masked positions are infinite)
+    by[w] = fmaxf(__builtin_ldexpf(scale, q.exp + Meta::ek(pg[w].meta)), 1.17549435e-38f);
     ev[w] = (float)Meta::ev(pg[w].meta);
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[4 * w + i] = s[w][i] * by;
+    for (int i = 0; i < 4; i++) x[4 * w + i] = s[w][i];
   }
   if (!whole) {
 #pragma unroll
@@ -406,7 +404,8 @@ __device__ inline void weigh(const f4 (&s)[2], const Page (&pg)[2], float scale,
       }
     }
   }
-  const float x0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), x1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]));
+  const float x0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * by[0];
+  const float x1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])) * by[1];
   const float top = fmaxf(q.m, quads_max(fmaxf(x0, x1)));
   const float top_v = fmaxf(q.mv, quads_max(fmaxf(x0 + ev[0], x1 + ev[1])));
   if (__any(top > q.m || top_v > q.mv)) {
@@ -422,19 +421,19 @@ __device__ inline void weigh(const f4 (&s)[2], const Page (&pg)[2], float scale,
   float w[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    w[i] = __builtin_amdgcn_exp2f(x[i] - at);
+    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by[i / 4], -at));
     q.l += w[i];
   }
   if (__any(fmaxf(g0, g1) > 100.0f)) {
     // pages so far apart that 2^(t - m) underflows where the weight does not
 #pragma unroll
-    for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(x[i] + ev[i / 4] - at_v);
+    for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by[i / 4], ev[i / 4] - at_v));
   } else {
     const float f0 = __builtin_amdgcn_exp2f(g0), f1 = __builtin_amdgcn_exp2f(g1);
 #pragma unroll
     for (int i = 0; i < 8; i++) w[i] *= i < 4 ? f0 : f1;
   }
-  split<KW>(w, out);
+  split_weights<KW>(w, out);
 }
 
 // Whether all of two pages' positions count for every query of a wave that sees at least `least`.
@@ -488,9 +487,24 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
   const int kv_heads = p.at.kv_heads, group = r.heads / kv_heads;
   const Partials part = partials_at<HD>(ws, LIST ? 0 : r.rows, slots.all);
 
+  // This wave's pairs are pages page0 + 2 (wave + 4 it) and the next.
+  auto nth = [&](int it) { return 2 * (wave + 4 * (it + (lane >> 1))) + (lane & 1); };
+  float x[kRounds][8];
+  auto load_q = [&](const Seq& s, int head, int tile) {
+#pragma unroll
+    for (int i = 0; i < kRounds; i++) {
+      const int u = tid + i * 256, qi = tile * 16 + u / (HD / 8);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[i][j] = 0;
+      if (u < kUnits && qi < s.n * group)
+        load8<T>(r.q, (int64_t)(s.row0 + qi / group) * r.ldq + (head * group + qi % group) * HD + u % (HD / 8) * 8, x[i]);
+    }
+  };
+
   // which pages, head and queries
   Seq s;
   int seq, head, tile, page0, page1, slot;
+  int listed = -1;  // LIST: this lane's first page of the list
   const int* pages_list = nullptr;
   if constexpr (LIST) {
     const int tiles = (group + 15) / 16;
@@ -501,17 +515,19 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     b /= tiles;
     head = b % kv_heads;
     const int row = b / kv_heads;
-    const int count = min(max(list.count[(int64_t)row * kv_heads + head], 0), list.top);
-    const int have = chunks_of(count, list.chunk);
-    if (c >= have) return;
-    seq = seq_of(r, row);
-    if (seq < 0) return;
+    // what needs no other load is on its way together
     page0 = c * list.chunk;
-    page1 = min(page0 + list.chunk, count);
     pages_list = list.sel + ((int64_t)row * kv_heads + head) * list.top;
-    // (as the last of the rows up to this one)
+    if (nth(0) < list.chunk && page0 + nth(0) < list.top) listed = pages_list[page0 + nth(0)];
     s.row0 = row;
     s.n = 1;
+    load_q(s, head, tile);
+    const int count = min(max(list.count[(int64_t)row * kv_heads + head], 0), list.top);
+    seq = seq_of(r, row);
+    const int have = chunks_of(count, list.chunk);
+    if (c >= have || seq < 0) return;
+    page1 = min(page0 + list.chunk, count);
+    // (as the last of the rows up to this one)
     s.len = r.lens[seq] - (r.row_start[seq + 1] - 1 - row);
     s.ctx = (int)min((long long)max(s.len, 0), (long long)r.max_blocks * kPage);
     slot = have > 1 ? (int)blockIdx.x : -1;
@@ -536,23 +552,16 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
   }
   const int* table = r.block_tables + (int64_t)seq * r.max_blocks;
 
-  // This wave's pairs are pages page0 + 2 (wave + 4 it) and the next.
   const int pairs = (page1 - page0 - 2 * wave + 7) / 8;
   Walk walk;
   auto refill = [&](int it) {
-    const int i = page0 + 2 * (wave + 4 * (it + (lane >> 1))) + (lane & 1);
-    walk.set(i < page1 ? (LIST ? pages_list[i] : i) : -1, table, r.max_blocks, p.n_pages);
+    const int i = page0 + nth(it);
+    int at = -1;
+    if (i < page1) at = !LIST ? i : it == 0 ? listed : pages_list[i];
+    walk.set(at, table, r.max_blocks, p.n_pages);
   };
   if (pairs > 0) refill(0);
-  float x[kRounds][8];
-#pragma unroll
-  for (int i = 0; i < kRounds; i++) {
-    const int u = tid + i * 256, qi = tile * 16 + u / (HD / 8);
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[i][j] = 0;
-    if (u < kUnits && qi < s.n * group)
-      load8<T>(r.q, (int64_t)(s.row0 + qi / group) * r.ldq + (head * group + qi % group) * HD + u % (HD / 8) * 8, x[i]);
-  }
+  if constexpr (!LIST) load_q(s, head, tile);
   const PoolAt pool(p, head);
   u4 kc[2][kSegs], vc[2][kSegs];
   auto load_k = [&](const Page (&g)[2]) {
@@ -579,8 +588,9 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
 #pragma unroll
   for (int i = 0; i < kRounds; i++) {
     const int u = tid + i * 256, g8 = u % (HD / 8), q = u / (HD / 8);
-    h8 t[kN];
-    const int e = query_terms<T, HD>(x[i], t);
+    h8 t[kN] = {};
+    int e = 0;
+    if (tile * 16 + i * 256 / (HD / 8) < s.n * group) e = query_terms<T, HD>(x[i], t);  // (any live query among them)
     if (u < kUnits) {
       if (g8 == 0) lds_exp[q] = e;
       // dims 64 seg + 16 kq + 8 half
@@ -596,9 +606,9 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
   const bool live = qi < s.n * group;
   Query q;
   q.exp = lds_exp[n16];
-  q.lim = live ? seen_by(s, qi / group) : 0;
+  // (columns without a query, all zeros, go along with the last row)
+  q.lim = seen_by(s, min(qi, s.n * group - 1) / group);
   const int least = seen_by(s, min(tile * 16, s.n * group - 1) / group);  // (rows see more and more)
-  const bool full = (tile + 1) * 16 <= s.n * group;                       // no query without a row
   f4 o[kTiles];
 #pragma unroll
   for (int i = 0; i < kTiles; i++) o[i] = f4{0, 0, 0, 0};
@@ -630,7 +640,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
 #pragma unroll
         for (int i = 0; i < kSegs; i++) vc[w][i] = u4{0, 0, 0, 0};
     h8 wt[kW];
-    weigh<kW>(sc, cur, scale, full && whole_pages(cur, least), q, o, wt);
+    weigh<kW>(sc, cur, scale, whole_pages(cur, least), q, o, wt);
 #pragma unroll
     for (int i = 0; i < kSegs; i++)
 #pragma unroll
@@ -665,7 +675,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     }
     if (live) {
       const int row = s.row0 + qi / group, col = (head * group + qi % group) * HD;
-#pragma unroll
+#pragma unroll 1
       for (int i = wave; i < kJoinTiles; i += 4) {
         f4 v = reinterpret_cast<const f4*>(lds)[i * 64 + lane] * by[0];
 #pragma unroll
@@ -749,13 +759,11 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out,
 
   Query q[NT];
   int least = INT_MAX, most = 0;
-  bool full = true;
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     const int ql = (wave * NT + t) * 16, qi = tile * kQueries + ql, end = s.n * group;
     q[t].exp = lds_exp[ql + n16];
-    q[t].lim = qi + n16 < end ? seen_by(s, (qi + n16) / group) : 0;
-    full &= qi + 16 <= end;
+    q[t].lim = seen_by(s, min(qi + n16, end - 1) / group);
     if (qi < end) {
       least = min(least, seen_by(s, qi / group));
       most = max(most, seen_by(s, min(qi + 15, end - 1) / group));
@@ -820,7 +828,7 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out,
             }
         }
       }
-      const bool whole = full && whole_pages(cur, least);
+      const bool whole = whole_pages(cur, least);
       h8 wt[NT][kW];
 #pragma unroll
       for (int t = 0; t < NT; t++) weigh<kW>(sc[t], cur, scale, whole, q[t], o[t], wt[t]);
@@ -881,8 +889,8 @@ __global__ __launch_bounds__(256) void merge_kernel(Rows r, Out out, List list, 
   __shared__ f4 lds_o[4][kLanes];
   __shared__ f4 lds_st[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = WAVES == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  const int row = __builtin_amdgcn_readfirstlane((int)(id / r.heads)), h = __builtin_amdgcn_readfirstlane((int)(id % r.heads));
+  const int id = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + wave;  // (rows * heads stay below 2^26)
+  const int row = id / r.heads, h = id % r.heads;
   const int first = (WAVES == 4 ? wave * kSub : 0) + lane / kLanes;  // this lane's first chunk
   if (row >= r.rows) return;
   const int group = r.heads / kv_heads, head = h / group;
@@ -895,7 +903,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Rows r, Out out, List list, 
     q = h % group;
     slot = (((int64_t)row * kv_heads + head) * tiles + q / 16) * list.chunks;
     step = 1;
-    if (chunks == 1 || seq_of(r, row) < 0) return;
+    if (chunks == 1 || row < r.row_start[0] || row >= r.row_start[r.nseq]) return;
   } else {
     const RowPart rp = part.rows[row];
     if (row < r.row_start[0] || row >= r.row_start[r.nseq]) return;
@@ -905,7 +913,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Rows r, Out out, List list, 
     s.len = rp.len;
     s.ctx = (int)min((long long)max(s.len, 0), (long long)r.max_blocks * kPage);
     q = (row - rp.row0) * group + h % group;
-    const int tiles = (int)(((int64_t)rp.n * group + 15) / 16);
+    const int tiles = (rp.n * group + 15) >> 4;
     if (rp.chunk < kMinChunk || rp.tile_queries < 16) return;
     chunks = chunks_of(tile_pages(s, group, rp.tile_queries, q / rp.tile_queries), rp.chunk);
     slot = rp.slot + (int64_t)head * tiles + q / 16;

@@ -73,5 +73,32 @@ __device__ inline float quads_sum(float v) {
   return over_quads(v, [](float a, float b) { return a + b; });
 }
 
+// Sums over the lanes before and with a lane, and over all lanes (identical in every lane).
+template <int CTRL, int ROWS>
+__device__ inline int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ inline int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);  // 1, 2, 4, 8 lanes of 16 up
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // lane 15 of a row to the next row, then lane 31 to the upper half
+  return dpp_add<0x143, 0xc>(v);
+}
+template <int CTRL, int ROWS>
+__device__ inline float dpp_addf(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+__device__ inline float wave_total(float v) {
+  v = dpp_addf<0x111, 0xf>(v);
+  v = dpp_addf<0x112, 0xf>(v);
+  v = dpp_addf<0x114, 0xf>(v);
+  v = dpp_addf<0x118, 0xf>(v);
+  v = dpp_addf<0x142, 0xa>(v);
+  v = dpp_addf<0x143, 0xc>(v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 }  // namespace kv8
 }  // namespace pgd

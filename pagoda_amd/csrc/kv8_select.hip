@@ -16,7 +16,6 @@ namespace kv8 {
 
 namespace {
 
-constexpr int kScorePages = 256;  // pages of a scoring workgroup, 64 a wave
 
 // The sequence that owns a row and the pages of the row's context (0 for none).
 __device__ inline int row_pages(const Rows& r, int row, int& seq) {
@@ -44,51 +43,101 @@ __device__ inline int holds127(float top) {
   return e > kExpMin ? e : kExpMin;
 }
 
-// Workgroup: kScorePages pages of one (row, KV head).
-template <int HD, int T>
+// Workgroup: 64 TILES pages of one (row, KV head), 16 TILES a wave. The first bounds are on their way before q is
+// turned into operands.
+template <int HD, int T, int TILES>
 __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* scores) {
-  constexpr int kSegs = HD / 64;
+  constexpr int kSegs = HD / 64, kPages = 64 * TILES;
+  constexpr int kUnits = 16 * HD / 8, kRounds = kUnits > 256 ? kUnits / 256 : 1;
   __shared__ __align__(16) int8_t q8[2][kSegs][64][16];  // operand order: lane l = 16 kq + query
   __shared__ float tops[4];
   const int kv_heads = p.at.kv_heads, group = r.heads / kv_heads;
-  const int strips = (r.max_blocks + kScorePages - 1) / kScorePages, unit = blockIdx.x / strips;
+  const int strips = (r.max_blocks + kPages - 1) / kPages, unit = blockIdx.x / strips;
   const int row = unit / kv_heads, head = unit % kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kq = lane >> 4;
   int seq;
   const int pages = row_pages(r, row, seq);
-  const int page0 = (int)(blockIdx.x % strips) * kScorePages;
+  const int page0 = (int)(blockIdx.x % strips) * kPages;
   if (page0 >= pages) return;
 
+  const int* table = r.block_tables + (int64_t)seq * r.max_blocks;
+  int id[TILES];
+#pragma unroll
+  for (int i = 0; i < TILES; i++) {
+    const int page = page0 + (i * 4 + wave) * 16 + n16;
+    id[i] = page < pages ? table[page] : -1;
+  }
   auto finite = [](float v) { return fabsf(v) <= 3.402823466e38f ? v : 0.0f; };
   const int64_t q_at = (int64_t)row * r.ldq + (int64_t)head * group * HD;
-  float most = 0;
-  for (int i = tid; i < group * HD / 8; i += 256) {
-    float x[8];
-    load8<T>(r.q, q_at + i * 8, x);
+  auto load_q = [&](int q0, int i, float (&x)[8]) {
+    const int u = tid + i * 256;
 #pragma unroll
-    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(finite(x[j])));
-  }
+    for (int j = 0; j < 8; j++) x[j] = 0;
+    if (u < kUnits && q0 + u / (HD / 8) < group) {
+      load8<T>(r.q, q_at + (int64_t)q0 * HD + u * 8, x);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = finite(x[j]);
+    }
+  };
+  float x[kRounds][8];
+#pragma unroll
+  for (int i = 0; i < kRounds; i++) load_q(0, i, x[i]);
+  const size_t page_bytes = p.at.page_bytes(), bounds_at = p.at.bounds_at() + (size_t)head * 2 * HD + kq * 16,
+               meta_at = p.at.meta_at() + (size_t)head * 4;
+  i4 bound[2][kSegs];
+  uint32_t meta;
+  auto load_bounds = [&](int i) {
+    const uint8_t* b = p.base + (size_t)(id[i] >= 0 && id[i] < p.n_pages ? id[i] : 0) * page_bytes;
+#pragma unroll
+    for (int w = 0; w < 2; w++)
+#pragma unroll
+      for (int s = 0; s < kSegs; s++) bound[w][s] = *reinterpret_cast<const i4*>(b + bounds_at + w * HD + s * 64);
+    meta = *reinterpret_cast<const uint32_t*>(b + meta_at);
+  };
+  load_bounds(0);
+
+  float most = 0;
+#pragma unroll
+  for (int i = 0; i < kRounds; i++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(x[i][j]));
+  for (int q0 = 16; q0 < group; q0 += 16)
+    for (int i = 0; i < kRounds; i++) {
+      float more[8];
+      load_q(q0, i, more);
+#pragma unroll
+      for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(more[j]));
+    }
   most = wave_max(most);
   if (lane == 0) tops[wave] = most;
   __syncthreads();
   const float down = pow2(-holds127(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))));
 
-  int best[kScorePages / 64];
+  int best[TILES];
 #pragma unroll
-  for (int i = 0; i < kScorePages / 64; i++) best[i] = INT32_MIN;
-  const int* table = r.block_tables + (int64_t)seq * r.max_blocks;
+  for (int i = 0; i < TILES; i++) best[i] = INT32_MIN;
+  float scale[TILES];  // (a page outside the pool: -1)
   for (int q0 = 0; q0 < group; q0 += 16) {
-    __syncthreads();
-    for (int u = tid; u < 16 * HD / 8; u += 256) {
-      const int q = u / (HD / 8), g8 = u % (HD / 8);
-      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (q0 + q < group) load8<T>(r.q, q_at + (int64_t)(q0 + q) * HD + g8 * 8, x);
-      const int l = (g8 >> 1 & 3) * 16 + q;
+    if (q0 > 0) {
+      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int v = (int)rintf(finite(x[j]) * down);
-        q8[0][g8 >> 3][l][(g8 & 1) * 8 + j] = (int8_t)max(v, 0);
-        q8[1][g8 >> 3][l][(g8 & 1) * 8 + j] = (int8_t)min(v, 0);
+      for (int i = 0; i < kRounds; i++) load_q(q0, i, x[i]);
+      load_bounds(0);
+    }
+#pragma unroll
+    for (int i = 0; i < kRounds; i++) {
+      const int u = tid + i * 256, q = u / (HD / 8), g8 = u % (HD / 8);
+      if (u < kUnits) {
+        const int l = (g8 >> 1 & 3) * 16 + q;
+        uint32_t pos[2] = {0, 0}, neg[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int v = (int)rintf(x[i][j] * down);
+          pos[j / 4] |= (uint32_t)(max(v, 0) & 255) << (8 * (j & 3));
+          neg[j / 4] |= (uint32_t)(min(v, 0) & 255) << (8 * (j & 3));
+        }
+        *reinterpret_cast<u2*>(&q8[0][g8 >> 3][l][(g8 & 1) * 8]) = u2{pos[0], pos[1]};
+        *reinterpret_cast<u2*>(&q8[1][g8 >> 3][l][(g8 & 1) * 8]) = u2{neg[0], neg[1]};
       }
     }
     __syncthreads();
@@ -98,20 +147,14 @@ __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* score
 #pragma unroll
       for (int s = 0; s < kSegs; s++) qa[w][s] = *reinterpret_cast<const i4*>(q8[w][s][lane]);
 #pragma unroll
-    for (int i = 0; i < kScorePages / 64; i++) {
-      const int page = page0 + wave * 64 + i * 16 + n16;
-      const int id = page < pages ? table[page] : -1;
-      const bool ok = id >= 0 && id < p.n_pages;
-      const int8_t* b = reinterpret_cast<const int8_t*>(p.base + (size_t)(ok ? id : 0) * p.at.page_bytes() +
-                                                         p.at.bounds_at()) + (size_t)head * 2 * HD;
+    for (int i = 0; i < TILES; i++) {
       i4 acc{0, 0, 0, 0};
 #pragma unroll
       for (int w = 0; w < 2; w++)
 #pragma unroll
-        for (int s = 0; s < kSegs; s++) {
-          const i4 bound = *reinterpret_cast<const i4*>(b + w * HD + s * 64 + kq * 16);
-          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[w][s], bound, acc, 0, 0, 0);
-        }
+        for (int s = 0; s < kSegs; s++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[w][s], bound[w][s], acc, 0, 0, 0);
+      scale[i] = id[i] >= 0 && id[i] < p.n_pages ? pow2(Meta::ek(meta)) : -1.0f;
+      if (i + 1 < TILES) load_bounds(i + 1);
       // acc[j]: query q0 + 4 kq + j with this lane's page
 #pragma unroll
       for (int j = 0; j < 4; j++)
@@ -119,20 +162,13 @@ __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* score
     }
   }
 #pragma unroll
-  for (int i = 0; i < kScorePages / 64; i++) {
+  for (int i = 0; i < TILES; i++) {
     int v = best[i];
     v = max(v, __shfl_xor(v, 16));
     v = max(v, __shfl_xor(v, 32));
-    const int page = page0 + wave * 64 + i * 16 + n16;
-    if (kq == 0 && page < pages) {
-      const int id = table[page];
-      float score = -INFINITY;  // (a page outside the pool)
-      if (id >= 0 && id < p.n_pages) {
-        const uint32_t m = reinterpret_cast<const uint32_t*>(p.base + (size_t)id * p.at.page_bytes() + p.at.meta_at())[head];
-        score = (float)v * pow2(Meta::ek(m));
-      }
-      scores[((int64_t)row * kv_heads + head) * r.max_blocks + page] = score;
-    }
+    const int page = page0 + (i * 4 + wave) * 16 + n16;
+    if (kq == 0 && page < pages)
+      scores[((int64_t)row * kv_heads + head) * r.max_blocks + page] = scale[i] > 0 ? (float)v * scale[i] : -INFINITY;
   }
 }
 
@@ -144,14 +180,19 @@ __device__ inline uint32_t order_of(float s) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Workgroup per (row, KV head): the threshold by four rounds over the keys' bytes, highest first, then
-// the pages above it, and the lowest ones that equal it, in page order.
+// Workgroup per (row, KV head): the lowest key that is taken, then the pages in order. A round counts the keys of
+// a range in 2048 equal bins from its top and goes on with the bin that holds the last key taken; a bin
+// of at most kRank keys is settled by counting, per key, those before it. Scores lie close together, and
+// the first range is that of the keys themselves, so one round mostly does.
+constexpr int kBins = 2 * kPick, kBinBits = __builtin_ctz(kBins), kRank = kPick, kHeld = 8;
+
 __global__ __launch_bounds__(kPick) void pick_kernel(Rows r, int kv_heads, int top, int sinks, int recent,
                                                      const float* scores, int* sel, int* count) {
-  __shared__ int bins[256];
-  __shared__ int chosen, rest;
-  __shared__ int wave_gt[kPick / 64], wave_eq[kPick / 64];
-  const int row = blockIdx.x / kv_heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ uint32_t lds[kBins > 2 * kRank ? kBins : 2 * kRank];  // bins, then (key, page) of the last bin
+  __shared__ uint32_t part[2][kPick / 64];
+  __shared__ int counts[kHeld * kPick / 64];
+  __shared__ uint32_t chosen[4];  // bin, keys still to take, keys of the bin; keys listed
+  const int row = blockIdx.x / kv_heads, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int seq;
   const int pages = row_pages(r, row, seq);
   if (seq < 0) return;
@@ -164,66 +205,162 @@ __global__ __launch_bounds__(kPick) void pick_kernel(Rows r, int kv_heads, int t
     for (int i = tid; i < pages; i += kPick) to[i] = i;
     return;
   }
-  auto key = [&](int i) { return i < sinks || i >= pages - recent ? ~0u : order_of(s[i]); };
-  uint32_t prefix = 0;
-  int need = take;  // still to take among the keys that begin with prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) bins[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < pages; i += kPick) {
-      const uint32_t k = key(i);
-      if (shift == 24 || k >> (shift + 8) == prefix) atomicAdd(&bins[k >> shift & 255], 1);
-    }
-    __syncthreads();
-    if (wave == 0) {
-      // lane l holds the bins 255 - 4 l .. 252 - 4 l, highest first
-      int v[4], sum = 0;
+  // Pages that are taken anyway are none of the keys.
+  const int from = min(sinks, pages), until = max(pages - recent, from), forced = pages - (until - from);
+  uint32_t held[kHeld];
 #pragma unroll
-      for (int j = 0; j < 4; j++) sum += v[j] = bins[255 - 4 * lane - j];
-      int upto = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(upto, o);
-        if (lane >= o) upto += x;
-      }
-      int before = upto - sum;
-      if (before < need && need <= upto) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          if (before < need && need <= before + v[j]) chosen = 255 - 4 * lane - j, rest = need - before;
-          before += v[j];
-        }
-      }
-    }
-    __syncthreads();
-    prefix = prefix << 8 | (uint32_t)chosen;
-    need = rest;
+  for (int j = 0; j < kHeld; j++) {
+    const int i = from + j * kPick + tid;
+    held[j] = i < until ? order_of(s[i]) : 0;
   }
-  int at = 0, equal = 0;
-  for (int base = 0; base < pages; base += kPick) {
-    const int i = base + tid;
-    const uint32_t k = i < pages ? key(i) : 0;
-    const uint64_t gt = __ballot(i < pages && k > prefix), eq = __ballot(i < pages && k == prefix);
-    if (lane == 0) wave_gt[wave] = __popcll(gt), wave_eq[wave] = __popcll(eq);
+  // f(key, page) for this thread's keys
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < kHeld; j++) {
+      const int i = from + j * kPick + tid;
+      if (i < until) f(held[j], i);
+    }
+    for (int i = from + kHeld * kPick + tid; i < until; i += kPick) f(order_of(s[i]), i);
+  };
+  for (int i = tid; i < kBins; i += kPick) lds[i] = 0;
+  if (tid == 0) chosen[3] = 0;
+  uint32_t low = ~0u, high = 0;
+  each([&](uint32_t k, int) { low = min(low, k), high = max(high, k); });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    low = min(low, (uint32_t)__shfl_xor((int)low, o));
+    high = max(high, (uint32_t)__shfl_xor((int)high, o));
+  }
+  if (lane == 0) part[0][wave] = low, part[1][wave] = high;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPick / 64; w++) low = min(low, part[0][w]), high = max(high, part[1][w]);
+
+  int need = take - forced;  // still to take among the keys of [low, high]; those above are taken
+  int listed = 0;            // keys of the last bin, in lds
+  while (need > 0) {
+    const uint32_t span = high - low;
+    const int shift = max(0, 32 - kBinBits - (span ? __builtin_clz(span) : 32));  // span >> shift < kBins
+    each([&](uint32_t k, int) {
+      if (k >= low && k <= high) atomicAdd(&lds[(high - k) >> shift], 1u);
+    });
+    __syncthreads();
+    // thread t holds the bins 2 t and 2 t + 1
+    const uint32_t a = lds[2 * tid], b = lds[2 * tid + 1];
+    uint32_t upto = (uint32_t)wave_scan((int)(a + b));
+    if (lane == 63) part[0][wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) upto += part[0][w];
+    const uint32_t before = upto - a - b;
+    if (before < (uint32_t)need && (uint32_t)need <= upto) {
+      const bool first = (uint32_t)need <= before + a;
+      chosen[0] = 2 * tid + (first ? 0 : 1);
+      chosen[1] = need - (first ? before : before + a);
+      chosen[2] = first ? a : b;
+    }
+    __syncthreads();
+    const uint32_t bin = chosen[0];
+    need = (int)chosen[1];
+    const int many = (int)chosen[2];
+    high -= bin << shift;
+    low = high - low >= (1u << shift) ? high - ((1u << shift) - 1) : low;
+    if (many <= kRank || low == high) {
+      listed = many;
+      break;
+    }
+    for (int i = tid; i < kBins; i += kPick) lds[i] = 0;
+    __syncthreads();
+  }
+  // Which of the last bin's keys: by rank if they are few; else they are all equal and the lowest pages win.
+  const bool ranked = need > 0 && listed <= kRank;
+  if (ranked) {
+    each([&](uint32_t k, int i) {
+      if (k >= low && k <= high) {
+        const uint32_t at = atomicAdd(&chosen[3], 1u);
+        lds[2 * at] = k;
+        lds[2 * at + 1] = (uint32_t)i;
+      }
+    });
+    __syncthreads();
+  }
+  auto taken = [&](uint32_t k, int i) {  // 1: taken, 2: one of too many equal keys, by page
+    if (need == 0 || k < low) return 0;
+    if (k > high) return 1;
+    if (!ranked) return 2;
+    int rank = 0;
+    for (int j = 0; j < listed; j++) rank += lds[2 * j] > k || (lds[2 * j] == k && lds[2 * j + 1] < (uint32_t)i);
+    return rank < need ? 1 : 0;
+  };
+  for (int i = tid; i < from; i += kPick) to[i] = i;
+  for (int i = tid; i < pages - until; i += kPick) to[take - (pages - until) + i] = until + i;
+  if (ranked && until - from <= kHeld * kPick) {
+    // all keys are held: one count of every 64 pages, in page order
+    uint64_t mine[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; j++) {
+      const int i = from + j * kPick + tid;
+      mine[j] = __ballot(i < until && taken(held[j], i) == 1);
+      if (lane == 0) counts[j * (kPick / 64) + wave] = __popcll(mine[j]);
+    }
+    __syncthreads();
+    static_assert(kHeld * kPick / 64 == 128, "two counts a lane");
+    const int a = counts[2 * lane], b = counts[2 * lane + 1], upto = wave_scan(a + b);
+#pragma unroll
+    for (int j = 0; j < kHeld; j++) {
+      const int e = j * (kPick / 64) + wave;  // (the same for the whole wave)
+      const int pair_end = __builtin_amdgcn_readlane(upto, e >> 1), second = __builtin_amdgcn_readlane(b, e >> 1),
+                first = __builtin_amdgcn_readlane(a, e >> 1);
+      const int before = pair_end - second - (e & 1 ? 0 : first);
+      if (mine[j] >> lane & 1)
+        to[from + before + __popcll(mine[j] & ((1ull << lane) - 1))] = from + j * kPick + tid;
+    }
+    return;
+  }
+  int at = from, equal = 0;
+  for (int j = 0; from + j * kPick < until; j++) {
+    const int i = from + j * kPick + tid;
+    int how = 0;
+    if (i < until) {
+      uint32_t k = 0;
+      if (j < kHeld) {
+#pragma unroll
+        for (int h = 0; h < kHeld; h++) k = j == h ? held[h] : k;
+      } else {
+        k = order_of(s[i]);
+      }
+      how = taken(k, i);
+    }
+    const uint64_t sure = __ballot(how == 1), tie = __ballot(how == 2);
+    __syncthreads();
+    if (lane == 0) part[0][wave] = __popcll(sure), part[1][wave] = __popcll(tie);
     __syncthreads();
     int g = at, e = equal;
-    for (int w = 0; w < wave; w++) g += wave_gt[w], e += wave_eq[w];
+    for (int w = 0; w < kPick / 64; w++) {
+      if (w < wave) g += part[0][w], e += part[1][w];
+      at += part[0][w];
+      equal += part[1][w];
+    }
     const uint64_t below = (1ull << lane) - 1;
-    const int my_gt = g + __popcll(gt & below), my_eq = e + __popcll(eq & below);
-    const int place = my_gt + min(my_eq, need);
-    if ((gt >> lane & 1) || ((eq >> lane & 1) && my_eq < need)) to[place] = i;
-    for (int w = 0; w < kPick / 64; w++) at += wave_gt[w], equal += wave_eq[w];
-    __syncthreads();
+    g += __popcll(sure & below);
+    e += __popcll(tie & below);
+    if (how == 1 || (how == 2 && e < need)) to[g + min(e, ranked ? 0 : need)] = i;
   }
+}
+
+template <int HD, int TILES>
+void score_of(const Pool& p, const Rows& r, float* scores, hipStream_t s) {
+  const unsigned grid = (unsigned)(r.rows * p.at.kv_heads) * ((r.max_blocks + 64 * TILES - 1) / (64 * TILES));
+  if (r.type == F32) score_kernel<HD, F32, TILES><<<grid, 256, 0, s>>>(p, r, scores);
+  else if (r.type == F16) score_kernel<HD, F16, TILES><<<grid, 256, 0, s>>>(p, r, scores);
+  else score_kernel<HD, BF16, TILES><<<grid, 256, 0, s>>>(p, r, scores);
+  PGD_HIP(hipGetLastError());
 }
 
 template <int HD>
 void score_hd(const Pool& p, const Rows& r, float* scores, hipStream_t s) {
-  const unsigned grid = (unsigned)(r.rows * p.at.kv_heads) * ((r.max_blocks + kScorePages - 1) / kScorePages);
-  if (r.type == F32) score_kernel<HD, F32><<<grid, 256, 0, s>>>(p, r, scores);
-  else if (r.type == F16) score_kernel<HD, F16><<<grid, 256, 0, s>>>(p, r, scores);
-  else score_kernel<HD, BF16><<<grid, 256, 0, s>>>(p, r, scores);
-  PGD_HIP(hipGetLastError());
+  // 64 pages a workgroup while that makes few of them, 128 past that.
+  if ((int64_t)r.rows * p.at.kv_heads * r.max_blocks <= 64 * 2048) score_of<HD, 1>(p, r, scores, s);
+  else score_of<HD, 2>(p, r, scores, s);
 }
 
 }  // namespace

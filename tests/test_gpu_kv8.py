@@ -617,3 +617,58 @@ def test_lists_of_ones_own(dev, buf, t, heads, kv, hd):
     assert (np.abs(got - want) <= bound).all()
     count[:] = -3
     assert not call.sparse(sel, count).any()
+
+
+def test_selection_of_many_equal_scores(dev, buf):
+    """More pages of one score than are settled by rank, above and below others, past what threads hold of
+    keys: the lowest ones that fit."""
+    from pagoda_amd import Kv8Pool
+    from pagoda_amd.kv8 import page_bytes
+
+    rng = np.random.default_rng(35)
+    for pages, distinct in ((1500, 1), (3000, 3), (9100, 2), (9100, 5000), (20000, 40)):
+        # `distinct` pages of keys, named by the table many times over
+        d = min(distinct, 600)
+        k = np.repeat(rng.normal(0, 1, (d, 1, 64)), 16, 1).reshape(-1, 64).astype(np.float32)
+        slots = np.arange(16 * d, dtype=np.int32)
+        cache = kv8.Cache(d, 1, 64)
+        cache.append(k.astype(float), k.astype(float), slots)
+        pool = GpuPool(dev, buf, 1, 64, d)
+        pool.append(k, k, slots, F32)
+        table = rng.integers(0, d, pages).astype(np.int32)
+        q = rng.normal(0, 1, (1, 64)).astype(np.float32)
+        q8 = np.rint(q[0].astype(float) * 2.0 ** -kv8.holds(np.abs(q).max(), 127.0))
+        by_page = []
+        for p in range(d):
+            hi, lo = (b[0] for b in cache.bounds(p))
+            by_page.append(np.maximum(q8 * hi, q8 * lo).sum() * 2.0 ** cache.exps[0, p, 0])
+        score = np.array(by_page)[table]
+        ptrs = [buf.up(a) for a in (q, np.int32([0, 1]), np.int32([pages * 16]), table)]
+        for top, sinks, recent in ((1, 0, 0), (700, 0, 0), (1400, 5, 3), (pages - 1, 0, 1), (pages, 0, 0)):
+            sel, count = np.full(top, 9, np.int32), np.int32([9])
+            ps, pc = buf.up(sel), buf.up(count)
+            size = pool.pool.sparse_ws_bytes(1, 1, pages, top)
+            pool.pool.select_dev(1, ptrs[0], 64, F32, 1, *ptrs[1:], pages, 1, top, sinks, recent, ps, pc,
+                                 buf.up(np.zeros(size, np.uint8)), size)
+            forced = (np.arange(pages) < sinks) | (np.arange(pages) >= pages - recent)
+            want = np.sort(np.lexsort((np.arange(pages), -score, ~forced))[:top])
+            assert buf.down(pc, count)[0] == top
+            np.testing.assert_array_equal(buf.down(ps, sel), want, err_msg=str((pages, distinct, top)))
+
+
+@pytest.mark.parametrize("kv,hd", [(1, 64), (3, 128), (2, 256)])
+def test_read_of_many_rows(dev, buf, kv, hd):
+    """More rows than the call reads one by one: whole sequences, any order, runs across pages, slots
+    twice and outside the pool."""
+    rng = np.random.default_rng(40 + hd)
+    step = Step(rng, kv, hd, [400, 77, 5], [0, 0, 0], F32)
+    pool = pool_of(dev, buf, step)
+    same_as(step.cache, pool, step.slots)
+    some = np.concatenate([step.slots[3:200], rng.permutation(step.slots), step.slots[::-1][:100], np.repeat(step.slots[7], 19)])
+    same_as(step.cache, pool, some)
+    bad = rng.random(len(some)) < 0.2
+    some[bad] = rng.choice([-1, -2, -3, step.cache.n * 16, 2 ** 31 - 1, -2 ** 31], bad.sum())
+    k, v = pool.read(some, kv * hd + 4)
+    assert (k[bad] == -77).all() and (v[bad] == -77).all()
+    for got, w in ((k, 0), (v, 1)):
+        np.testing.assert_array_equal(got[~bad], step.cache.read(w, some[~bad]).astype(np.float32))
