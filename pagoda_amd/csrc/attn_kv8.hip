@@ -38,10 +38,13 @@ namespace kv8 {
 
 namespace {
 
-// Items that contexts are cut into, about. kFew: the workgroups that run at once (two on a CU at hd 256), less the
-// rest chunks of the contexts; kMany: prompts' tiles are mostly enough by themselves.
-constexpr int kFewItems = 448, kManyItems = 1024;
-constexpr int kMinChunk = 16;    // pages: fewer would be more joining than reading
+// Items that contexts are cut into, about: as many as run at once (item_kernel: workgroups of four waves that a
+// CU holds at a head_dim, over the 256 CUs; prompt_kernel: 512 run at once, more where a tile is long and
+// the rounds uneven).
+constexpr int few_items(int hd, int tiles) { return 256 * (hd == 256 ? 2 : hd == 128 ? 3 : 4) / tiles; }
+constexpr int many_items(int hd) { return hd == 128 ? 1024 : 1536; }
+constexpr int kMinChunk = 8;     // pages: a pair for each of four waves
+constexpr int kOneChunk = 16;    // pages of tables (and lists) that are never cut: the join would cost more
 constexpr int kFewQueries = 32;  // of a sequence and KV head: calls of up to these are item_kernel's alone
 
 template <int T>
@@ -144,11 +147,13 @@ struct Slots {
 
 __device__ inline int chunks_of(int pages, int chunk) { return pages > 0 ? (pages + chunk - 1) / chunk : 1; }
 
-// Pages of a chunk: a multiple of 8 (a pair for each of four waves) that cuts all tiles' pages into at most
-// `items` full chunks (of sums in f32, so about).
-__device__ inline int chunk_of(float tile_pages, int items) {
-  const float c = fminf(ceilf(tile_pages / (float)items), 1e9f);
-  return max(((int)c + 7) & ~7, kMinChunk);
+__device__ __host__ inline int least_chunk(int max_blocks) { return max_blocks <= kOneChunk ? kOneChunk : kMinChunk; }
+
+// Pages of a chunk of a context, where all contexts' tiles together are to be cut into chunks of about `each`
+// pages: contexts are cut evenly, into multiples of 8 pages (a pair for each of four waves).
+__device__ inline int chunk_of(int pages, float each, int least) {
+  const float n = fmaxf(floorf((float)pages / each + 0.25f), 1.0f);
+  return max(((int)ceilf((float)pages / n) + 7) & ~7, least);
 }
 
 struct Found {
@@ -175,7 +180,9 @@ __device__ inline bool find(const Rows& r, int kv_heads, const Class& cl, int ke
     }
     all += (float)tiles * (float)s.pages;
   }
-  f.chunk = chunk_of(wave_total(all) * kv_heads, cl.sh.items);
+  const float each = fmaxf(wave_total(all) * kv_heads / cl.sh.items, 1.0f);
+  const int least = least_chunk(r.max_blocks);
+  int chunk = 0;  // this lane's sequence's
   auto items_of = [&](int base) {
     if (!strip) {
       tiles = 0;
@@ -184,12 +191,13 @@ __device__ inline bool find(const Rows& r, int kv_heads, const Class& cl, int ke
         tiles = cl.tiles(s.n);
       }
     }
-    return tiles * chunks_of(s.pages, f.chunk) * kv_heads;
+    chunk = chunk_of(s.pages, each, least);
+    return tiles * chunks_of(s.pages, chunk) * kv_heads;
   };
   int before = 0, split_before = 0;
   for (int base = 0; base < r.nseq; base += 64) {
     const int mine = items_of(base), upto = before + wave_scan(mine);
-    const int chunks = chunks_of(s.pages, f.chunk);
+    const int chunks = chunks_of(s.pages, chunk);
     const int slots = chunks > 1 && tiles > 0 ? cl.tiles16(s.n) * kv_heads * chunks : 0;
     const int slots_upto = split_before + wave_scan(slots);
     const uint64_t hit = __ballot(key < upto && key >= upto - mine);
@@ -201,6 +209,7 @@ __device__ inline bool find(const Rows& r, int kv_heads, const Class& cl, int ke
       f.s.ctx = __builtin_amdgcn_readlane(s.ctx, src);
       f.s.pages = __builtin_amdgcn_readlane(s.pages, src);
       f.tiles = __builtin_amdgcn_readlane(tiles, src);
+      f.chunk = __builtin_amdgcn_readlane(chunk, src);
       f.local = key - __builtin_amdgcn_readlane(upto - mine, src);
       f.slot = __builtin_amdgcn_readlane(slots_upto - slots, src);
       f.seq = base + src;
@@ -377,37 +386,42 @@ struct Query {
   int exp = 0, lim = 0;  // power of two of its terms; positions it sees
 };
 
-// Scores of two pages' positions to weights: s[w][i] is position 16 index + 4 kq + i of page w.
-template <int KW, int N>
-__device__ inline void weigh(const f4 (&s)[2], const Page (&pg)[2], float scale, bool whole, Query& q, f4 (&o)[N],
-                             h8 (&out)[KW]) {
+// Scores of PG pages' positions to weights: s[w][i] is position 16 index + 4 kq + i of page w.
+template <int KW, int PG, int N>
+__device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scale, bool whole, Query& q, f4 (&o)[N],
+                             h8 (&out)[PG / 2][KW]) {
   const int kq = threadIdx.x >> 4 & 3;
-  float x[8], by[2], ev[2];
+  float x[PG][4], by[PG], ev[PG];
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
+  for (int w = 0; w < PG; w++) {
     // (not below the normal range: the scores of masked positions are infinite)
     by[w] = fmaxf(__builtin_ldexpf(scale, q.exp + Meta::ek(pg[w].meta)), 1.17549435e-38f);
     ev[w] = (float)Meta::ev(pg[w].meta);
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[4 * w + i] = s[w][i];
+    for (int i = 0; i < 4; i++) x[w][i] = s[w][i];
   }
   if (!whole) {
 #pragma unroll
-    for (int w = 0; w < 2; w++) {
+    for (int w = 0; w < PG; w++) {
       const uint32_t nan = pg[w].id >= 0 ? Meta::nan(pg[w].meta) : pg[w].id == -2 ? 0xffffu : 0u;
       // (a page of no index lies behind every position)
       const int first = pg[w].index >= 0 ? pg[w].index * kPage + 4 * kq : INT_MAX - kPage;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const float v = nan >> (4 * kq + i) & 1 ? NAN : x[4 * w + i];
-        x[4 * w + i] = first + i < q.lim ? v : -INFINITY;
+        const float v = nan >> (4 * kq + i) & 1 ? NAN : x[w][i];
+        x[w][i] = first + i < q.lim ? v : -INFINITY;
       }
     }
   }
-  const float x0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * by[0];
-  const float x1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])) * by[1];
-  const float top = fmaxf(q.m, quads_max(fmaxf(x0, x1)));
-  const float top_v = fmaxf(q.mv, quads_max(fmaxf(x0 + ev[0], x1 + ev[1])));
+  float top = -INFINITY, top_v = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < PG; w++) {
+    const float t = fmaxf(fmaxf(x[w][0], x[w][1]), fmaxf(x[w][2], x[w][3])) * by[w];
+    top = fmaxf(top, t);
+    top_v = fmaxf(top_v, t + ev[w]);
+  }
+  top = fmaxf(q.m, quads_max(top));
+  top_v = fmaxf(q.mv, quads_max(top_v));
   if (__any(top > q.m || top_v > q.mv)) {
     q.l *= top > q.m ? __builtin_amdgcn_exp2f(q.m - top) : 1.0f;
     const float down = top_v > q.mv ? __builtin_amdgcn_exp2f(q.mv - top_v) : 1.0f;
@@ -417,29 +431,45 @@ __device__ inline void weigh(const f4 (&s)[2], const Page (&pg)[2], float scale,
     q.mv = top_v;
   }
   const float at = top > -INFINITY ? top : 0.0f, at_v = top > -INFINITY ? top_v - kWeightExp : 0.0f;
-  const float g0 = at - at_v + ev[0], g1 = at - at_v + ev[1];
-  float w[8];
+  float far = -INFINITY, sum[PG];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by[i / 4], -at));
-    q.l += w[i];
+  for (int w = 0; w < PG; w++) far = fmaxf(far, ev[w]);
+  const bool apart = __any(at - at_v + far > 100.0f);
+#pragma unroll
+  for (int w = 0; w < PG; w++) {
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[w][i], by[w], -at));
+    sum[w] = (e[0] + e[1]) + (e[2] + e[3]);
+    if (apart) {
+      // pages so far apart that 2^(t - m) underflows where the weight does not
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[w][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[w][i], by[w], ev[w] - at_v));
+    } else {
+      const float f = __builtin_amdgcn_exp2f(at - at_v + ev[w]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[w][i] = e[i] * f;
+    }
   }
-  if (__any(fmaxf(g0, g1) > 100.0f)) {
-    // pages so far apart that 2^(t - m) underflows where the weight does not
 #pragma unroll
-    for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by[i / 4], ev[i / 4] - at_v));
-  } else {
-    const float f0 = __builtin_amdgcn_exp2f(g0), f1 = __builtin_amdgcn_exp2f(g1);
+  for (int w = 0; w < PG; w++) q.l += sum[w];
 #pragma unroll
-    for (int i = 0; i < 8; i++) w[i] *= i < 4 ? f0 : f1;
+  for (int w = 0; w < PG; w += 2) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = x[w + i / 4][i & 3];
+    split_weights<KW>(v, out[w / 2]);
   }
-  split_weights<KW>(w, out);
 }
 
-// Whether all of two pages' positions count for every query of a wave that sees at least `least`.
-__device__ inline bool whole_pages(const Page (&pg)[2], int least) {
-  return pg[0].id >= 0 && pg[1].id >= 0 && (Meta::nan(pg[0].meta) | Meta::nan(pg[1].meta)) == 0 &&
-         (max(pg[0].index, pg[1].index) + 1) * kPage <= least;
+// Whether all of some pages' positions count for every query of a wave that sees at least `least`.
+template <int PG>
+__device__ inline bool whole_pages(const Page (&pg)[PG], int least) {
+  bool whole = true;
+#pragma unroll
+  for (int w = 0; w < PG; w++)
+    whole &= pg[w].id >= 0 && Meta::nan(pg[w].meta) == 0 && (pg[w].index + 1) * kPage <= least;
+  return whole;
 }
 
 // Eight dims of a query as f16 terms; x is scaled to [2^14, 2^15) for the largest magnitude of the HD / 8 lanes
@@ -639,7 +669,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
       if (cur[w].id < 0)
 #pragma unroll
         for (int i = 0; i < kSegs; i++) vc[w][i] = u4{0, 0, 0, 0};
-    h8 wt[kW];
+    h8 wt[1][kW];
     weigh<kW>(sc, cur, scale, whole_pages(cur, least), q, o, wt);
 #pragma unroll
     for (int i = 0; i < kSegs; i++)
@@ -648,7 +678,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
         const h8 a = of_codes8(vc[0][i][j], vc[1][i][j]);
 #pragma unroll
         for (int k = kW - 1; k >= 0; k--)
-          o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wt[k], o[4 * i + j], 0, 0, 0);
+          o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wt[0][k], o[4 * i + j], 0, 0, 0);
       }
     if (more) {
       load_v(next);
@@ -691,16 +721,17 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
 
 // ---- many queries a sequence -------------------------------------------------------------
 
-// Workgroup: 64 NT queries, 16 NT a wave, over the pages of a chunk, two at a time through LDS (two buffers, one
-// barrier a pair). A wave keeps its queries' terms in registers.
-template <int HD, int T, int NT>
+// Workgroup: 64 queries, 16 a wave, over the pages of a chunk, PG at a time through LDS (two buffers, one
+// barrier a step). A wave keeps its queries' terms in registers. 32 queries a wave would share the codes' conversion
+// and measured slower, with a third fewer waves (<> against <> us).
+template <int HD, int T, int PG>
 __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out, Share share, void* ws, Slots slots) {
   constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms<T>;
   constexpr int kHead = 2 * kPage * HD;            // bytes of a page and head
-  constexpr int kRounds = 2 * kHead / 4096;        // 16 bytes a thread each, of a pair
-  constexpr int kQueries = 64 * NT;
+  constexpr int kRounds = PG * kHead / 4096;       // 16 bytes a thread each, of a step
+  constexpr int kQueries = 64;
   constexpr int kQBytes = 16 * HD * 2;             // 16 queries' operands of one term
-  constexpr int kLds = 2 * 2 * kHead > 4 * kQBytes ? 2 * 2 * kHead : 4 * kQBytes;
+  constexpr int kLds = 2 * PG * kHead > 4 * kQBytes ? 2 * PG * kHead : 4 * kQBytes;
   __shared__ __align__(16) uint8_t lds[kLds];
   __shared__ int lds_exp[kQueries];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -721,161 +752,159 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out,
   const int pages = tile_pages(s, group, kQueries, tile), have = chunks_of(pages, f.chunk);
   if (c == 0 && head == 0 && slots.all > 0) leave_row_parts(part, s, group, tile, kQueries, f, slots);
   if (c >= have) return;
-  const int page0 = c * f.chunk, page1 = min(page0 + f.chunk, pages), pairs = (page1 - page0 + 1) / 2;
+  const int page0 = c * f.chunk, page1 = min(page0 + f.chunk, pages), steps = (page1 - page0 + PG - 1) / PG;
   const int* table = r.block_tables + (int64_t)f.seq * r.max_blocks;
   Walk walk;
   auto refill = [&](int it) {
-    const int i = page0 + 2 * it + lane;
+    const int i = page0 + PG * it + lane;
     walk.set(i < page1 ? i : -1, table, r.max_blocks, p.n_pages);
   };
-  if (pairs > 0) refill(0);
+  if (steps > 0) refill(0);
 
   // The wave's queries, 16 at a time: loaded as rows, turned into operands through LDS.
-  h8 qt[NT][kN][kSteps];
+  h8 qt[kN][kSteps];
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
+  for (int k = 0; k < kN; k++) {
+    if (k > 0) __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kN; k++) {
-      if (t + k > 0) __syncthreads();
-#pragma unroll
-      for (int u0 = 0; u0 < 16 * HD / 8; u0 += 64) {
-        const int u = u0 + lane, g8 = u % (HD / 8), q = u / (HD / 8);
-        const int ql = (wave * NT + t) * 16 + q, qi = tile * kQueries + ql;
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (qi < s.n * group)
-          load8<T>(r.q, (int64_t)(s.row0 + qi / group) * r.ldq + (head * group + qi % group) * HD + g8 * 8, x);
-        h8 terms[kN];
-        const int e = query_terms<T, HD>(x, terms);
-        if (g8 == 0) lds_exp[ql] = e;
-        const int step = (g8 >> 3) * 2 + (g8 & 1), k4 = g8 >> 1 & 3;
-        reinterpret_cast<h8*>(lds + wave * kQBytes)[step * 64 + k4 * 16 + q] = terms[k];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kSteps; i++) qt[t][k][i] = reinterpret_cast<const h8*>(lds + wave * kQBytes)[i * 64 + lane];
+    for (int u0 = 0; u0 < 16 * HD / 8; u0 += 64) {
+      const int u = u0 + lane, g8 = u % (HD / 8), q = u / (HD / 8);
+      const int ql = wave * 16 + q, qi = tile * kQueries + ql;
+      float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (qi < s.n * group)
+        load8<T>(r.q, (int64_t)(s.row0 + qi / group) * r.ldq + (head * group + qi % group) * HD + g8 * 8, x);
+      h8 terms[kN];
+      const int e = query_terms<T, HD>(x, terms);
+      if (g8 == 0) lds_exp[ql] = e;
+      const int step = (g8 >> 3) * 2 + (g8 & 1), k4 = g8 >> 1 & 3;
+      reinterpret_cast<h8*>(lds + wave * kQBytes)[step * 64 + k4 * 16 + q] = terms[k];
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) qt[k][i] = reinterpret_cast<const h8*>(lds + wave * kQBytes)[i * 64 + lane];
   }
   __syncthreads();
 
-  Query q[NT];
-  int least = INT_MAX, most = 0;
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const int ql = (wave * NT + t) * 16, qi = tile * kQueries + ql, end = s.n * group;
-    q[t].exp = lds_exp[ql + n16];
-    q[t].lim = seen_by(s, min(qi + n16, end - 1) / group);
-    if (qi < end) {
-      least = min(least, seen_by(s, qi / group));
-      most = max(most, seen_by(s, min(qi + 15, end - 1) / group));
-    }
-  }
+  // (columns without a query, all zeros, go along with the last row)
+  const int q0 = tile * kQueries + wave * 16, end = s.n * group, qi = q0 + n16;
+  Query q;
+  q.exp = lds_exp[wave * 16 + n16];
+  q.lim = seen_by(s, min(qi, end - 1) / group);
+  const int least = seen_by(s, min(q0, end - 1) / group);
+  const int most = q0 < end ? seen_by(s, min(q0 + 15, end - 1) / group) : 0;
   const PoolAt pool(p, head);
   u4 next[kRounds];
-  auto load = [&](const Page (&g)[2]) {
+  auto load = [&](const Page (&g)[PG]) {
 #pragma unroll
     for (int i = 0; i < kRounds; i++) {
-      const int at = (i * 256 + tid) * 16;  // a page of the pair takes whole rounds, or half of one
-      const int w = at / kHead;
-      const uint8_t* from = kRounds > 1 ? g[i * 4096 / kHead].at : (w ? g[1].at : g[0].at);
-      next[i] = *reinterpret_cast<const u4*>(from + (at - w * kHead));
-      const int id = kRounds > 1 ? g[i * 4096 / kHead].id : (w ? g[1].id : g[0].id);
+      // a page takes whole rounds, or (hd 64) half of one
+      constexpr int kPer = kHead / 4096;
+      const Page* from = &g[kPer > 0 ? i / (kPer > 0 ? kPer : 1) : 2 * i];
+      const uint8_t* at = from->at;
+      int id = from->id;
+      if (kPer == 0 && tid >= 128) {
+        at = g[(2 * i + 1) % PG].at;
+        id = g[(2 * i + 1) % PG].id;
+      }
+      next[i] = *reinterpret_cast<const u4*>(at + (i * 4096 + tid * 16) % kHead);
       if (id < 0) next[i] = u4{0, 0, 0, 0};
     }
   };
   auto put = [&](int b) {
 #pragma unroll
-    for (int i = 0; i < kRounds; i++) reinterpret_cast<u4*>(lds + b * 2 * kHead)[i * 256 + tid] = next[i];
+    for (int i = 0; i < kRounds; i++) reinterpret_cast<u4*>(lds + b * PG * kHead)[i * 256 + tid] = next[i];
   };
   const float scale = 1.44269504088896340736f / sqrtf((float)HD);
-  f4 o[NT][kTiles];
+  f4 o[kTiles];
 #pragma unroll
-  for (int t = 0; t < NT; t++)
+  for (int i = 0; i < kTiles; i++) o[i] = f4{0, 0, 0, 0};
+  Page cur[PG], nxt[PG];
+  auto pages_at = [&](int it, Page (&g)[PG]) {
 #pragma unroll
-    for (int i = 0; i < kTiles; i++) o[t][i] = f4{0, 0, 0, 0};
-  Page cur[2], nxt[2];
-  if (pairs > 0) {
-    cur[0] = pool.page(walk, 0);
-    cur[1] = pool.page(walk, 1);
+    for (int w = 0; w < PG; w++) g[w] = pool.page(walk, PG * (it % (64 / PG)) + w);
+  };
+  if (steps > 0) {
+    pages_at(0, cur);
     load(cur);
     put(0);
   }
   __syncthreads();
-  for (int it = 0; it < pairs; it++) {
-    const bool more = it + 1 < pairs;
+  for (int it = 0; it < steps; it++) {
+    const bool more = it + 1 < steps;
     if (more) {
-      if (((it + 1) & 31) == 0) refill(it + 1);
-      nxt[0] = pool.page(walk, 2 * ((it + 1) & 31));
-      nxt[1] = pool.page(walk, 2 * ((it + 1) & 31) + 1);
+      if ((it + 1) % (64 / PG) == 0) refill(it + 1);
+      pages_at(it + 1, nxt);
       load(nxt);
     }
-    if (cur[0].index * kPage < most) {  // (the pair is not behind all of the wave's queries)
-      const u4* kv = reinterpret_cast<const u4*>(lds + (it & 1) * 2 * kHead) + lane;
-      f4 sc[NT][2];
+    if (cur[0].index * kPage < most) {  // (the step is not behind all of the wave's queries)
+      const u4* kv = reinterpret_cast<const u4*>(lds + (it & 1) * PG * kHead) + lane;
+      f4 sc[PG];
 #pragma unroll
-      for (int t = 0; t < NT; t++) sc[t][0] = sc[t][1] = f4{0, 0, 0, 0};
+      for (int w = 0; w < PG; w++) sc[w] = f4{0, 0, 0, 0};
+      __builtin_amdgcn_s_setprio(1);  // (the other wave of the SIMD weighs meanwhile)
 #pragma unroll
       for (int i = 0; i < kSegs; i++) {
-        const u4 c0 = kv[i * 64], c1 = kv[kHead / 16 + i * 64];
+        u4 code[PG];
+#pragma unroll
+        for (int w = 0; w < PG; w++) code[w] = kv[w * kHead / 16 + i * 64];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const h8 a0 = of_codes8(c0[2 * h], c0[2 * h + 1]), a1 = of_codes8(c1[2 * h], c1[2 * h + 1]);
+          h8 a[PG];
 #pragma unroll
-          for (int t = 0; t < NT; t++)
+          for (int w = 0; w < PG; w++) a[w] = of_codes8(code[w][2 * h], code[w][2 * h + 1]);
 #pragma unroll
-            for (int k = 0; k < kN; k++) {
-              sc[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, qt[t][k][2 * i + h], sc[t][0], 0, 0, 0);
-              sc[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, qt[t][k][2 * i + h], sc[t][1], 0, 0, 0);
-            }
+          for (int k = 0; k < kN; k++)
+#pragma unroll
+            for (int w = 0; w < PG; w++)
+              sc[w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[w], qt[k][2 * i + h], sc[w], 0, 0, 0);
         }
       }
-      const bool whole = whole_pages(cur, least);
-      h8 wt[NT][kW];
-#pragma unroll
-      for (int t = 0; t < NT; t++) weigh<kW>(sc[t], cur, scale, whole, q[t], o[t], wt[t]);
+      __builtin_amdgcn_s_setprio(0);
+      h8 wt[PG / 2][kW];
+      weigh<kW>(sc, cur, scale, whole_pages(cur, least), q, o, wt);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < kSegs; i++) {
-        const u4 c0 = kv[kHead / 32 + i * 64], c1 = kv[kHead / 16 + kHead / 32 + i * 64];
+        u4 code[PG];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const h8 a = of_codes8(c0[j], c1[j]);
+        for (int w = 0; w < PG; w++) code[w] = kv[w * kHead / 16 + kHead / 32 + i * 64];
 #pragma unroll
-          for (int t = 0; t < NT; t++)
+        for (int w = 0; w < PG; w += 2)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const h8 a = of_codes8(code[w][j], code[w + 1][j]);
 #pragma unroll
             for (int k = kW - 1; k >= 0; k--)
-              o[t][4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wt[t][k], o[t][4 * i + j], 0, 0, 0);
-        }
+              o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wt[w / 2][k], o[4 * i + j], 0, 0, 0);
+          }
       }
+      __builtin_amdgcn_s_setprio(0);
     }
     if (more) {
       put((it + 1) & 1);
-      cur[0] = nxt[0];
-      cur[1] = nxt[1];
+#pragma unroll
+      for (int w = 0; w < PG; w++) cur[w] = nxt[w];
     }
     __syncthreads();
   }
 
+  const float l = quads_sum(q.l);
+  if (qi >= end) return;
+  const int row = s.row0 + qi / group, col = (head * group + qi % group) * HD;
+  if (have > 1) {
+    const int64_t slot = slots.first + f.slot + ((int64_t)c * kv_heads + head) * cl.tiles16(s.n) + qi / 16;
+    if (slot >= slots.end) return;
+    if (kq == 0) part.st[slot * 16 + n16] = f4{q.m, q.mv, l, 0};
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const float l = quads_sum(q[t].l);
-    const int qi = tile * kQueries + (wave * NT + t) * 16 + n16;
-    if (qi >= s.n * group) continue;
-    const int row = s.row0 + qi / group, col = (head * group + qi % group) * HD;
-    if (have > 1) {
-      const int64_t slot = slots.first + f.slot + ((int64_t)c * kv_heads + head) * cl.tiles16(s.n) + qi / 16;
-      if (slot >= slots.end) continue;
-      if (kq == 0) part.st[slot * 16 + n16] = f4{q[t].m, q[t].mv, l, 0};
+    for (int i = 0; i < kTiles; i++) *reinterpret_cast<f4*>(part.o + (slot * 16 + n16) * HD + i * 16 + kq * 4) = o[i];
+  } else {
+    State st;
+    st.m = q.m;
+    st.mv = q.mv;
+    st.l = l;
+    const float inv = st.factor();
 #pragma unroll
-      for (int i = 0; i < kTiles; i++)
-        *reinterpret_cast<f4*>(part.o + (slot * 16 + n16) * HD + i * 16 + kq * 4) = o[t][i];
-    } else {
-      State st;
-      st.m = q[t].m;
-      st.mv = q[t].mv;
-      st.l = l;
-      const float inv = st.factor();
-#pragma unroll
-      for (int i = 0; i < kTiles; i++) store4<T>(out, row, col + i * 16 + kq * 4, o[t][i] * inv);
-    }
+    for (int i = 0; i < kTiles; i++) store4<T>(out, row, col + i * 16 + kq * 4, o[i] * inv);
   }
 }
 
@@ -966,19 +995,18 @@ struct Grid {
 };
 
 // Items and partial sums that a share may have. Tiles of all rows' queries: at most a full
-// one for every `tile` and a last one for every sequence. A context of p pages in chunks of c makes
-// up to p / c + 1 items of a tile, and 2 p / c if it is cut at all; c is at least all tiles' pages
-// over share.items (but for the rounding of sums in f32: an eighth more).
+// one for every `tile` and a last one for every sequence. A context of p pages makes at most p / each + 1 items of a
+// tile, and 8/7 p / each if it is cut at all; all tiles' pages over `each` are share.items (but for the rounding of
+// sums in f32: an eighth more).
 Grid grid_of(const Layout& at, int heads, int nseq, int max_blocks, int rows, const Share& sh) {
   const int64_t group = heads / at.kv_heads, seqs = nseq < rows ? nseq : rows;
   int64_t tiles = rows * group / sh.tile + seqs;
   if (sh.most < INT_MAX) tiles = std::min(tiles, seqs * ((sh.most + sh.tile - 1) / sh.tile));
   tiles *= at.kv_heads;
-  const int64_t per = (max_blocks + kMinChunk - 1) / kMinChunk, cut = tiles * per, most = sh.items + sh.items / 8;
+  const int64_t per = (max_blocks + least_chunk(max_blocks) - 1) / least_chunk(max_blocks), cut = tiles * per,
+                most = sh.items + sh.items / 8;
   return Grid{std::min(cut, tiles + most), per > 1 ? std::min(cut, 2 * most) * (sh.tile / 16) : 0};
 }
-
-constexpr int prompt_tiles(int hd) { return hd == 256 ? 1 : 2; }
 
 // How a call is shared out: by the largest number of queries that a sequence has for a KV head. Up to 16 and up to 32
 // are item_kernel's alone, one or two tiles side by side; past that it keeps the sequences of up to 16.
@@ -992,15 +1020,15 @@ Plan plan_of(int hd, int group, int64_t max_rows) {
   Plan p{};
   p.both = most > kFewQueries;
   p.two = most > 16 && !p.both;
-  p.few = Share{1, p.both ? 16 : INT_MAX, p.two ? 32 : 16, kFewItems};
-  p.many = Share{17, INT_MAX, 64 * prompt_tiles(hd), kManyItems};
+  p.few = Share{1, p.both ? 16 : INT_MAX, p.two ? 32 : 16, few_items(hd, p.two ? 2 : 1)};
+  p.many = Share{17, INT_MAX, 64, many_items(hd)};
   return p;
 }
 
 int sparse_chunk(const Layout& at, int heads, int rows, int top) {
   const int64_t all = (int64_t)rows * at.kv_heads * ((heads / at.kv_heads + 15) / 16) * top;
-  const int64_t c = ((all + kFewItems - 1) / kFewItems + 7) & ~7ll;
-  return (int)(c > kMinChunk ? (c < 1 << 20 ? c : 1 << 20) : kMinChunk);
+  const int64_t items = few_items(at.hd, 1), c = ((all + items - 1) / items + 7) & ~7ll;
+  return (int)std::max(std::min(c, (int64_t)1 << 20), (int64_t)least_chunk(top));
 }
 
 template <int HD, int T>
@@ -1055,7 +1083,7 @@ void attn(const Pool& p, const Rows& r, int max_rows, const Out& o, void* ws, hi
   with_types(p, r, [&](auto hd, auto type) {
     constexpr int HD = decltype(hd)::value, T = decltype(type)::value;
     if (pl.both) {
-      prompt_kernel<HD, T, prompt_tiles(HD)><<<(unsigned)many.items, 256, 0, s>>>(p, r, o, pl.many, ws,
+      prompt_kernel<HD, T, HD == 64 ? 2 : 4><<<(unsigned)many.items, 256, 0, s>>>(p, r, o, pl.many, ws,
                                                                                  Slots{all, (int)few.slots, all});
       PGD_HIP(hipGetLastError());
     }
