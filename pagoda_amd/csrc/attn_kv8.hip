@@ -723,7 +723,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
 
 // Workgroup: 64 queries, 16 a wave, over the pages of a chunk, PG at a time through LDS (two buffers, one
 // barrier a step). A wave keeps its queries' terms in registers. 32 queries a wave would share the codes' conversion
-// and measured slower, with a third fewer waves (<> against <> us).
+// and measured slower, with fewer waves (1500 bf16 rows on 3900 positions at head_dim 128 107 against 91 us).
 template <int HD, int T, int PG>
 __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out, Share share, void* ws, Slots slots) {
   constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms<T>;
@@ -1035,12 +1035,12 @@ template <int HD, int T>
 void merge(const Rows& r, const Out& o, const List* list, int kv_heads, void* ws, int64_t slots, hipStream_t s) {
   const int64_t outs = (int64_t)r.rows * r.heads;
   const List l = list ? *list : List{};
-  // Four waves a result where there are few; measured at <>.
+  // Four waves a result where there are few: 768 results 24.2 against 25.5 us with one wave each, 1536 the same.
   auto go = [&](auto is_list, auto waves) {
     const unsigned blocks = (unsigned)(waves == 4 ? outs : (outs + 3) / 4);
     merge_kernel<HD, T, is_list, waves><<<blocks, 256, 0, s>>>(r, o, l, kv_heads, ws, (int)slots);
   };
-  const bool wide = outs <= 4096;
+  const bool wide = outs <= 1024;
   using W4 = std::integral_constant<int, 4>;
   using W1 = std::integral_constant<int, 1>;
   if (list) wide ? go(std::true_type(), W4()) : go(std::true_type(), W1());

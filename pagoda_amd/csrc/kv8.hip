@@ -262,8 +262,9 @@ __device__ inline void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Inclusive sums over a workgroup of N threads of values in [0, 2^31), and the totals.
-template <int N>
+constexpr int kScan = 1024;  // threads of a workgroup, and sequences of a strip
+
+// Inclusive sums over a workgroup of values in [0, 2^31), and the totals.
 __device__ inline void block_scan2(long long (&v)[2], long long (&total)[2], long long (*part)[2]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (64 halves of 16 bits fit an int)
@@ -277,7 +278,7 @@ __device__ inline void block_scan2(long long (&v)[2], long long (&total)[2], lon
   long long before[2] = {0, 0};
   total[0] = total[1] = 0;
 #pragma unroll
-  for (int w = 0; w < N / 64; w++)
+  for (int w = 0; w < kScan / 64; w++)
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       total[i] += part[w][i];
@@ -287,13 +288,13 @@ __device__ inline void block_scan2(long long (&v)[2], long long (&total)[2], lon
   v[1] += before[1];
 }
 
-// Every workgroup goes over the sequences in strips of N: what each needs, running sums of rows and pages. The
+// Every workgroup goes over the sequences in strips of kScan: what each needs, running sums of rows and pages. The
 // first one writes what belongs to sequences (with `maps` row starts and status, with `lens` new lengths and
 // the pages taken); with `maps` all enter their share of the pages into the tables and place rows_per rows each. Nothing
 // is read that the call writes: a row's new page comes from the free list. The same input arrays as outputs
 // (lengths, taken) need one workgroup, or `lens` in a launch behind.
-template <int N>
-__global__ __launch_bounds__(N) void tables_kernel(Tables t, int rows_per, bool maps, bool lens) {
+__global__ __launch_bounds__(kScan) void tables_kernel(Tables t, int rows_per, bool maps, bool lens) {
+  constexpr int N = kScan;
   __shared__ long long part[N / 64][2];
   // the strip's rows and pages before each sequence, pages that it has (-1: gets none), its length (-1: refused)
   __shared__ int starts[N + 1], fresh[N + 1], have_of[N], len_of[N];
@@ -324,7 +325,7 @@ __global__ __launch_bounds__(N) void tables_kernel(Tables t, int rows_per, bool 
     // (Rows are laid out and pages counted for refused sequences too: whatever comes behind rows or
     // pages that do not fit has either none of its own or does not fit itself.)
     long long end[2] = {rows, need}, total[2];
-    block_scan2<N>(end, total, part);
+    block_scan2(end, total, part);
     const long long row_end = carry[0] + end[0], page_end = carry[1] + end[1];
     if (status == kFits && row_end > t.rows) status = kNoRows;
     if (status == kFits && need > 0 && page_end > avail) status = kNoPages;
@@ -404,7 +405,10 @@ void append_rows(const Pool& p, const void* k, int64_t ldk, const void* v, int64
 template <int HD>
 void append_hd(const Pool& p, const void* k, int64_t ldk, const void* v, int64_t ldv, int type, const int* slots,
                int rows, hipStream_t s) {
-  if (rows <= 512) append_rows<HD, 1>(p, k, ldk, v, ldv, type, slots, rows, s);
+  // 256 decode rows take 20.8 us with a workgroup a row (and head), 26.9 with one of four, which takes pages one
+  // after the other; 512 rows of a prompt, where most workgroups of a row have no page of their own, 19.0 and 12.9
+  // (with the read-back of 3 us and more, head_dim 256, 4 KV heads).
+  if (rows <= 256) append_rows<HD, 1>(p, k, ldk, v, ldv, type, slots, rows, s);
   else append_rows<HD, 4>(p, k, ldk, v, ldv, type, slots, rows, s);
 }
 
@@ -418,7 +422,9 @@ void append(const Pool& p, const void* k, int64_t ldk, const void* v, int64_t ld
 }
 
 void read(const Pool& p, const int* slots, int rows, float* k, int64_t ldk, float* v, int64_t ldv, hipStream_t s) {
-  if (rows > 256) {
+  // Runs of 9 rows (64 and 500 pages): one by one 10 and 22 us with their write, run by run 17 and 25; a prompt's 1000
+  // rows the same, 8600 rows 50 and 41.
+  if (rows > 4096) {
     const unsigned grid = (unsigned)(((int64_t)(rows + 15) / 16 * p.at.kv_heads + 3) / 4);
     if (p.at.hd == 64) read_runs_kernel<64><<<grid, 256, 0, s>>>(p, slots, rows, k, ldk, v, ldv);
     else if (p.at.hd == 128) read_runs_kernel<128><<<grid, 256, 0, s>>>(p, slots, rows, k, ldk, v, ldv);
@@ -431,13 +437,13 @@ void read(const Pool& p, const int* slots, int rows, float* k, int64_t ldk, floa
 }
 
 void tables(const Tables& t, hipStream_t s) {
-  // 256 threads' barriers cost less while one strip of them holds all sequences (one sequence: <> against <> us).
-  const bool small = t.nseq <= 256 && t.rows <= 1024;
   const bool in_place = t.new_lens == t.lens || t.new_taken == t.taken;
-  const int groups = small ? 1 : (t.rows + 511) / 512;
+  // 512 rows a workgroup: half its threads' worth, the rest enter pages meanwhile (29000 rows of 512 sequences 7.9
+  // us, with 1024 rows a workgroup 8.2).
+  constexpr int kRows = 512;
+  const int groups = (t.rows + kRows - 1) / kRows;
   auto go = [&](int n, bool maps, bool lens) {
-    if (small) tables_kernel<256><<<1, 256, 0, s>>>(t, t.rows, maps, lens);
-    else tables_kernel<1024><<<n, 1024, 0, s>>>(t, 512, maps, lens);
+    tables_kernel<<<n, kScan, 0, s>>>(t, kRows, maps, lens);
     PGD_HIP(hipGetLastError());
   };
   if (in_place && groups > 1) {

@@ -9,6 +9,7 @@ using namespace pgd::kv8;
 
 namespace {
 
+constexpr int kMaxSeqs = 1 << 24;
 constexpr int64_t kBlocks = 1 << 24;  // workgroups of 256 threads below a grid's 2^32 threads
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -37,6 +38,7 @@ void check_type(int type) { PGD_CHECK(type >= F32 && type <= BF16, kErrArg, "typ
 void check_sizes(const Layout& at, int heads, int nseq, int max_blocks, int rows) {
   PGD_CHECK(heads > 0 && heads % at.kv_heads == 0, kErrShape, "heads must be a multiple of kv_heads");
   PGD_CHECK(nseq >= 0 && rows >= 0, kErrArg, "nseq and rows must not be negative");
+  PGD_CHECK(nseq <= kMaxSeqs, kErrShape, "nseq must be at most 2^24");
   PGD_CHECK(max_blocks > 0 && max_blocks <= 1 << 26, kErrShape, "max_blocks must be 1..2^26");
   const int64_t group = heads / at.kv_heads, tiles = rows * group / 16 + (nseq < rows ? nseq : rows);
   PGD_CHECK((int64_t)rows * heads < kBlocks * 4 && tiles * at.kv_heads < kBlocks / 2, kErrShape,
@@ -71,7 +73,7 @@ void check_ws(const void* ws, size_t have, size_t need) {
 void check_list(const Layout& at, int heads, int rows, int max_blocks, int top) {
   PGD_CHECK(top > 0 && top <= 1 << 20, kErrShape, "top must be 1..2^20");
   const int64_t units = (int64_t)rows * at.kv_heads;
-  PGD_CHECK(units < kBlocks / 4 && units * ((max_blocks + 255) / 256) < kBlocks, kErrShape,
+  PGD_CHECK(units < kBlocks / 4 && units * ((max_blocks + 127) / 128) < kBlocks, kErrShape,
             "more rows and pages than one launch holds");
   PGD_CHECK(units * ((heads / at.kv_heads + 15) / 16) < kBlocks / 8, kErrShape, "more rows than one launch holds");
 }
@@ -102,6 +104,7 @@ int pgd_kv_tables_dev(pgd_dev* dev, int block, int nseq, const int* lens, const 
   return guard([&] {
     PGD_CHECK(dev, kErrArg, "null device");
     PGD_CHECK(block > 0 && max_blocks > 0 && nseq >= 0 && n_free >= 0 && rows >= 0, kErrArg, "bad sizes");
+    PGD_CHECK(nseq <= kMaxSeqs && rows <= 1 << 30, kErrShape, "nseq must be at most 2^24 and rows at most 2^30");
     PGD_CHECK(taken && new_taken && row_start, kErrArg, "null argument");
     PGD_CHECK(nseq == 0 || (lens && counts && tables_io && new_lens && status), kErrArg, "null argument");
     PGD_CHECK(n_free == 0 || free_pages, kErrArg, "null free list");

@@ -658,13 +658,14 @@ def test_selection_of_many_equal_scores(dev, buf):
 
 @pytest.mark.parametrize("kv,hd", [(1, 64), (3, 128), (2, 256)])
 def test_read_of_many_rows(dev, buf, kv, hd):
-    """More rows than the call reads one by one: whole sequences, any order, runs across pages, slots
+    """More rows than the call reads one by one (4096): whole sequences, any order, runs across pages, slots
     twice and outside the pool."""
     rng = np.random.default_rng(40 + hd)
     step = Step(rng, kv, hd, [400, 77, 5], [0, 0, 0], F32)
     pool = pool_of(dev, buf, step)
     same_as(step.cache, pool, step.slots)
-    some = np.concatenate([step.slots[3:200], rng.permutation(step.slots), step.slots[::-1][:100], np.repeat(step.slots[7], 19)])
+    some = np.concatenate([step.slots[3:200], rng.permutation(step.slots), step.slots[::-1][:100], np.repeat(step.slots[7], 19)] * 6)
+    assert len(some) > 4096
     same_as(step.cache, pool, some)
     bad = rng.random(len(some)) < 0.2
     some[bad] = rng.choice([-1, -2, -3, step.cache.n * 16, 2 ** 31 - 1, -2 ** 31], bad.sum())

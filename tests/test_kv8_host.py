@@ -81,10 +81,10 @@ POOL = [(dict(pool=0), ARG), (dict(pool=A + 8), ARG), (dict(n_pages=0), SHAPE), 
 QUERY = [(dict(heads=3), SHAPE), (dict(heads=0), SHAPE), (dict(q=0), ARG), (dict(q=A + 4), ARG), (dict(ldq=255), SHAPE),
          (dict(ldq=260), SHAPE), (dict(type=3), ARG), (dict(type=-1), ARG), (dict(nseq=-1), ARG), (dict(row_start=0), ARG),
          (dict(lens=0), ARG), (dict(tables=0), ARG), (dict(max_blocks=0), SHAPE), (dict(max_blocks=(1 << 26) + 1), SHAPE),
-         (dict(rows=1 << 24), SHAPE), (dict(ws=0), ARG), (dict(ws=A + 8), ARG), (dict(ws_bytes=16), SHAPE)]
+         (dict(rows=1 << 24), SHAPE), (dict(nseq=(1 << 24) + 1), SHAPE), (dict(ws=0), ARG), (dict(ws=A + 8), ARG), (dict(ws_bytes=16), SHAPE)]
 RESULT = [(dict(out=0), ARG), (dict(out=A + 8), ARG), (dict(ldo=248), SHAPE), (dict(ldo=258), SHAPE),
           (dict(gate=A + 8), ARG), (dict(ldg=248), SHAPE)]
-LIST = [(dict(top=0), SHAPE), (dict(top=(1 << 20) + 1), SHAPE), (dict(sel=0), ARG), (dict(count=0), ARG)]
+LIST = [(dict(rows=1 << 21, max_blocks=1 << 12), SHAPE), (dict(top=0), SHAPE), (dict(top=(1 << 20) + 1), SHAPE), (dict(sel=0), ARG), (dict(count=0), ARG)]
 REFUSED = (
     [("pgd_kv8_append_dev", c, e) for c, e in POOL + [
         (dict(k=0), ARG), (dict(v=0), ARG), (dict(k=A + 8), ARG), (dict(v=A + 2), ARG), (dict(ldk=127), SHAPE),
@@ -100,7 +100,8 @@ REFUSED = (
     + [("pgd_kv_tables_dev", c, ARG) for c in [
         dict(block=0), dict(block=-16), dict(nseq=-1), dict(max_blocks=0), dict(n_free=-1), dict(rows=-1), dict(lens=0),
         dict(counts=0), dict(tables=0), dict(free=0), dict(taken=0), dict(new_lens=0), dict(new_taken=0),
-        dict(row_start=0), dict(seq=0), dict(pos=0), dict(slots=0), dict(status=0)]])
+        dict(row_start=0), dict(seq=0), dict(pos=0), dict(slots=0), dict(status=0)]]
+    + [("pgd_kv_tables_dev", c, SHAPE) for c in [dict(rows=(1 << 30) + 1), dict(nseq=(1 << 24) + 1)]])
 
 
 @pytest.mark.parametrize("name,change,code", REFUSED, ids=[f"{n}-{c}" for n, c, _ in REFUSED])
