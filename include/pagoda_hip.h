@@ -257,7 +257,8 @@ size_t pgd_kv8_page_bytes(int kv_heads, int head_dim);
  * sequence order, and are entered into its table. Written: new_lens (lens + counts), new_taken
  * (both may be the input array), row_start [nseq + 1] (sequence i's rows, sequence after
  * sequence), and for each of `rows` rows seq_of_row, pos_of_row and slots (page * block +
- * place); -1 in all three for rows behind the last sequence's. status[i]: 0; or why the
+ * place); -1 in all three for rows behind the last sequence's. No other output overlaps an
+ * input. nseq is at most 2^24, rows at most 2^30. status[i]: 0; or why the
  * sequence got nothing (its rows are -1, its length and table stay): 1 too few free
  * pages, 2 more positions than max_blocks pages hold, 3 rows past `rows`, 4 a negative length or
  * count. A sequence that needs no page is not refused for those that do. A table entry that is
@@ -287,12 +288,13 @@ int pgd_kv8_read_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
  * there is one. q, gate, out [rows, heads * head_dim] of one type; heads is a multiple of
  * kv_heads. Positions past max_blocks pages do not exist. A row that attends to nothing
  * gets zeros; rows of no sequence are left as they were; attending a position of a page outside the pool
- * gives NaN. f32 rows lose nothing beyond f32 sums; the softmax weights of f16 and bf16 rows are
- * held to 2^-16 before they meet the values. max_rows: the largest
+ * gives NaN. Sums, maxima and the weights' sum are f32. Before the products on the matrix cores f32 rows of q are held
+ * to 2^-22 (f16 rows exactly, bf16 rows too but for what lies below 2^-40 of the head's largest), the
+ * softmax weights to 2^-21 and for bf16 rows to 2^-11, nothing finer than 2^-40 of the largest. max_rows: the largest
  * number of rows of a sequence, or any bound on it (it selects kernels, results are
- * right with any value). ws: pgd_attn_kv8_ws_bytes bytes that no other stream uses
- * meanwhile (a captured graph's included); its contents do not matter. The order of the sums
- * depends on the sizes, row_start and lens, on nothing else. */
+ * right with any value). row_start ascends. ws: pgd_attn_kv8_ws_bytes bytes (0 of sizes that the call refuses) that no
+ * other stream uses meanwhile (a captured graph's included); its contents do not matter. The order of the sums
+ * depends on the sizes, max_rows, row_start and lens, on nothing else. */
 size_t pgd_attn_kv8_ws_bytes(int heads, int kv_heads, int head_dim, int nseq, int max_blocks, int rows);
 int pgd_attn_kv8_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, int head_dim, int heads, const void* q,
                      int ldq, int type, int nseq, const int* row_start, const int* lens, const int* block_tables,

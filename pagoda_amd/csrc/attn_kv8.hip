@@ -11,7 +11,7 @@
 // about one whatever the pages' powers of two. Codes convert to f16 exactly. Queries are
 // scaled by a power of two into f16's range and enter as f16 terms: f32 rows two (22 bits and
 // at least 2^-40 of the row's largest), f16 rows themselves, bf16 rows one (exact to 2^-40 of the
-// largest). The weights, times 2^15, enter as two terms (bf16 rows: one; its 2^-11 is an
+// largest). The weights, times 2^15, enter as two terms, 2^-21 (bf16 rows: one; its 2^-11 is an
 // eighth of their own rounding). bf16 terms would need no scaling but half as many more
 // products: three for f32 where f16 takes two.
 // The lane that holds a score holds it as the operand of the second product: lane
@@ -558,8 +558,8 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     if (c >= have || seq < 0) return;
     page1 = min(page0 + list.chunk, count);
     // (as the last of the rows up to this one)
-    s.len = r.lens[seq] - (r.row_start[seq + 1] - 1 - row);
-    s.ctx = (int)min((long long)max(s.len, 0), (long long)r.max_blocks * kPage);
+    s.len = (int)max((long long)r.lens[seq] - (min(r.row_start[seq + 1], r.rows) - 1 - row), 0ll);
+    s.ctx = (int)min((long long)s.len, (long long)r.max_blocks * kPage);
     slot = have > 1 ? (int)blockIdx.x : -1;
   } else {
     Found f;

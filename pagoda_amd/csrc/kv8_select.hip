@@ -30,7 +30,7 @@ __device__ inline int row_pages(const Rows& r, int row, int& seq) {
     }
   }
   if (seq < 0) return 0;
-  const long long seen = (long long)r.lens[seq] - ((long long)r.row_start[seq + 1] - 1 - row);
+  const long long seen = (long long)r.lens[seq] - (min(r.row_start[seq + 1], r.rows) - 1 - row);
   if (seen <= 0) return 0;
   const long long pages = (seen + kPage - 1) / kPage;
   return (int)(pages < r.max_blocks ? pages : r.max_blocks);

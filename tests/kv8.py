@@ -161,11 +161,11 @@ def attend(q, k, v, t, unit=0.0):
     """One query [hd] over positions k, v [n, hd] (float64): the result and the bound on what a kernel with f32
     sums may be off. unit: the power of two of each position's value codes.
 
-    A score of hd exact products in at most three terms, summed in any order: (3 hd + 4) 2^-23 of
+    A score of hd products in at most two terms, summed in any order, q held to 2^-22: (3 hd + 4) 2^-23 of
     sum |q k|, and one rounding of the scaled score, of its maximum's difference and
     of the exponent's argument, each 2^-24 of its magnitude, 2^-22 for exp2 itself. Weights then
-    are off by the factor exp(2 d). They enter as f16 terms, two (bf16 rows: one): a significand of
-    11 bits is half a step, 2^-11, off at most, so k terms leave 2^-11k, and no
+    are off by the factor exp(2 d). They enter as f16 terms of 11 bits: one (bf16 rows) to nearest is 2^-11
+    off at most; of two the first is truncated, 2^-10, and the second to nearest, 2^-11 of that; and no
     less than f16's smallest half step, 2^-25, which is 2^-40 of the largest weight of a code; codes are up to
     448. The sums of n weights and n products by n 2^-23 each."""
     if len(k) == 0:
@@ -178,7 +178,7 @@ def attend(q, k, v, t, unit=0.0):
          + 4 * 2.0 ** -24 * 1.5 * np.abs(s).max() + 2.0 ** -22)
     w = np.exp(s - s.max())
     w /= w.sum()
-    held = {F32: 2.0 ** -22, F16: 2.0 ** -22, BF16: 2.0 ** -11}[t]
+    held = {F32: 2.0 ** -21, F16: 2.0 ** -21, BF16: 2.0 ** -11}[t]
     mass = w @ np.abs(v)
     small = len(k) * 448 * 2.0 ** -40 * (w * unit).max()
     return w @ v, mass * (2 * np.expm1(2 * d) + held + (2 * len(k) + 16) * 2.0 ** -23) + small

@@ -673,3 +673,39 @@ def test_read_of_many_rows(dev, buf, kv, hd):
     assert (k[bad] == -77).all() and (v[bad] == -77).all()
     for got, w in ((k, 0), (v, 1)):
         np.testing.assert_array_equal(got[~bad], step.cache.read(w, some[~bad]).astype(np.float32))
+
+
+@pytest.mark.parametrize("t,heads,kv,hd", [(F32, 14, 2, 64), (F16, 28, 4, 128), (BF16, 24, 4, 256), (F32, 17, 1, 64)])
+def test_selection_through_tables_of_any_width(dev, buf, t, heads, kv, hd):
+    """The pages do not hang on the width of the tables, which the scores are split by, nor on the size of a group."""
+    rng = np.random.default_rng(50 + hd)
+    step = Step(rng, kv, hd, [1000, 40, 530], [1, 2, 1], t)
+    pool = pool_of(dev, buf, step)
+    q, qv, _ = queries(rng, step, heads, t)
+    narrow = step.tables
+    for top, sinks, recent in ((5, 0, 0), (30, 1, 2)):
+        want = kv8.select(step, qv, heads, top, sinks, recent)
+        for width in (64, 1024, 1025, 5000):
+            step.tables = np.full((3, width), -1, np.int32)
+            step.tables[:, :min(width, narrow.shape[1])] = narrow[:, :width]
+            step.width = width
+            sel, count = Call(dev, buf, step, pool, heads, t, q).select(top, sinks, recent)
+            for row in range(step.rows):
+                for h in range(kv):
+                    assert sel[row, h].tolist() == want[row][h] + [-1] * (top - len(want[row][h])), (width, row, h)
+        step.tables, step.width = narrow, narrow.shape[1]
+
+
+def test_rows_end_where_the_call_says(dev, buf):
+    """Row starts past the number of rows: the rows that are there are their sequence's latest, to every call."""
+    rng = np.random.default_rng(60)
+    step = Step(rng, 1, 64, [200, 90], [2, 3], F32)
+    pool = pool_of(dev, buf, step)
+    q, qv, _ = queries(rng, step, 2, F32)
+    step.row_start = np.int32([0, 2, 9])
+    call = Call(dev, buf, step, pool, 2, F32, q)
+    want, bound = kv8.attention(step, qv, F32, 2)
+    assert (np.abs(call.attn() - want) <= bound).all()
+    sel, count = call.select(step.width, 0, 0)
+    assert count[:, 0].tolist() == [13, 13, 6, 6, 6]
+    assert (np.abs(call.sparse(sel, count) - want) <= bound).all()
