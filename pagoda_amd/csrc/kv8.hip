@@ -262,9 +262,8 @@ __device__ inline void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-constexpr int kScan = 1024;  // threads of a workgroup, and sequences of a strip
-
-// Inclusive sums over a workgroup of values in [0, 2^31), and the totals.
+// Inclusive sums over a workgroup of N threads of values in [0, 2^31), and the totals.
+template <int N>
 __device__ inline void block_scan2(long long (&v)[2], long long (&total)[2], long long (*part)[2]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (64 halves of 16 bits fit an int)
@@ -278,7 +277,7 @@ __device__ inline void block_scan2(long long (&v)[2], long long (&total)[2], lon
   long long before[2] = {0, 0};
   total[0] = total[1] = 0;
 #pragma unroll
-  for (int w = 0; w < kScan / 64; w++)
+  for (int w = 0; w < N / 64; w++)
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       total[i] += part[w][i];
@@ -288,13 +287,13 @@ __device__ inline void block_scan2(long long (&v)[2], long long (&total)[2], lon
   v[1] += before[1];
 }
 
-// Every workgroup goes over the sequences in strips of kScan: what each needs, running sums of rows and pages. The
+// Every workgroup goes over the sequences in strips of N: what each needs, running sums of rows and pages. The
 // first one writes what belongs to sequences (with `maps` row starts and status, with `lens` new lengths and
 // the pages taken); with `maps` all enter their share of the pages into the tables and place rows_per rows each. Nothing
 // is read that the call writes: a row's new page comes from the free list. The same input arrays as outputs
 // (lengths, taken) need one workgroup, or `lens` in a launch behind.
-__global__ __launch_bounds__(kScan) void tables_kernel(Tables t, int rows_per, bool maps, bool lens) {
-  constexpr int N = kScan;
+template <int N>
+__global__ __launch_bounds__(N) void tables_kernel(Tables t, int rows_per, bool maps, bool lens) {
   __shared__ long long part[N / 64][2];
   // the strip's rows and pages before each sequence, pages that it has (-1: gets none), its length (-1: refused)
   __shared__ int starts[N + 1], fresh[N + 1], have_of[N], len_of[N];
@@ -325,7 +324,7 @@ __global__ __launch_bounds__(kScan) void tables_kernel(Tables t, int rows_per, b
     // (Rows are laid out and pages counted for refused sequences too: whatever comes behind rows or
     // pages that do not fit has either none of its own or does not fit itself.)
     long long end[2] = {rows, need}, total[2];
-    block_scan2(end, total, part);
+    block_scan2<N>(end, total, part);
     const long long row_end = carry[0] + end[0], page_end = carry[1] + end[1];
     if (status == kFits && row_end > t.rows) status = kNoRows;
     if (status == kFits && need > 0 && page_end > avail) status = kNoPages;
@@ -443,7 +442,9 @@ void tables(const Tables& t, hipStream_t s) {
   constexpr int kRows = 512;
   const int groups = (t.rows + kRows - 1) / kRows;
   auto go = [&](int n, bool maps, bool lens) {
-    tables_kernel<<<n, kScan, 0, s>>>(t, kRows, maps, lens);
+    // (4.5 us of the kernel for one sequence with 256 threads, 5.8 with 1024; more rows than threads take longer)
+    if (t.nseq <= 256 && t.rows <= 256) tables_kernel<256><<<n, 256, 0, s>>>(t, kRows, maps, lens);
+    else tables_kernel<1024><<<n, 1024, 0, s>>>(t, kRows, maps, lens);
     PGD_HIP(hipGetLastError());
   };
   if (in_place && groups > 1) {
