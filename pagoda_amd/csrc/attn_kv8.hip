@@ -481,8 +481,7 @@ __device__ inline int query_terms(float (&x)[8], h8 (&t)[N]) {
     float most = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(x[j]));
-#pragma unroll
-    for (int w = 1; w < HD / 8; w <<= 1) most = fmaxf(most, __shfl_xor(most, w));
+    most = lanes_max<HD / 8>(most);
     e = max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14, -112);
     const float down = pow2(-e);
 #pragma unroll
@@ -958,8 +957,8 @@ __global__ __launch_bounds__(256) void merge_kernel(Rows r, Out out, List list, 
     j.m = fmaxf(j.m, st[0]);
     j.mv = fmaxf(j.mv, st[1]);
   }
-  j.m = wave_max(j.m);
-  j.mv = wave_max(j.mv);
+  j.m = lanes_max<64>(j.m);
+  j.mv = lanes_max<64>(j.mv);
   f4 x{0, 0, 0, 0};
 #pragma unroll 8
   for (int c = first; c < chunks; c += kParts) {

@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void append_kernel(Pool p, const void* k, int6
     }
 #pragma unroll
     for (int w = 0; w < 2; w++) {
-      most[w] = wave_max(most[w]);
+      most[w] = lanes_max<64>(most[w]);
       if (lane == 0) top[w][wave] = most[w];
     }
     __syncthreads();
@@ -437,7 +437,7 @@ void read(const Pool& p, const int* slots, int rows, float* k, int64_t ldk, floa
 
 void tables(const Tables& t, hipStream_t s) {
   const bool in_place = t.new_lens == t.lens || t.new_taken == t.taken;
-  // 512 rows a workgroup: half its threads' worth, the rest enter pages meanwhile (29000 rows of 512 sequences 7.9
+  // 512 rows a workgroup: half its threads' worth, the rest enter pages meanwhile (46000 rows of 512 sequences 7.9
   // us, with 1024 rows a workgroup 8.2).
   constexpr int kRows = 512;
   const int groups = (t.rows + kRows - 1) / kRows;

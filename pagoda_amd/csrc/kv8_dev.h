@@ -1,6 +1,8 @@
 // kv8_dev.h — device helpers shared by the kernels over the 8-bit KV cache.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 #include "kv8.h"
 
@@ -68,6 +70,42 @@ __device__ inline float over_quads(float v, F f) {
 }
 __device__ inline float quads_max(float v) {
   return over_quads(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ inline int quads_max(int v) {
+  return __builtin_bit_cast(int, over_quads(__builtin_bit_cast(float, v), [](float a, float b) {
+    return __builtin_bit_cast(float, max(__builtin_bit_cast(int, a), __builtin_bit_cast(int, b)));
+  }));
+}
+
+// f over aligned groups of N lanes, the result in every lane, without LDS: within 16 lanes by exchanging
+// neighbours, pairs, quads and halves, then by lane swaps.
+template <int N, class T, class F>
+__device__ inline T over_lanes(T v, F f) {
+  auto other = [](T x, auto ctrl) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  auto swapped = [&](auto r) { return f(__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1])); };
+  v = f(v, other(v, std::integral_constant<int, 0xb1>()));
+  v = f(v, other(v, std::integral_constant<int, 0x4e>()));
+  v = f(v, other(v, std::integral_constant<int, 0x141>()));
+  if constexpr (N >= 16) v = f(v, other(v, std::integral_constant<int, 0x140>()));
+  if constexpr (N >= 32) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    v = swapped(__builtin_amdgcn_permlane16_swap(b, b, false, false));
+  }
+  if constexpr (N >= 64) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    v = swapped(__builtin_amdgcn_permlane32_swap(b, b, false, false));
+  }
+  return v;
+}
+template <int N, class T>
+__device__ inline T lanes_max(T v) {
+  return over_lanes<N>(v, [](T a, T b) { return std::is_same<T, float>::value ? fmaxf(a, b) : max(a, b); });
+}
+template <int N, class T>
+__device__ inline T lanes_min(T v) {
+  return over_lanes<N>(v, [](T a, T b) { return min(a, b); });
 }
 __device__ inline float quads_sum(float v) {
   return over_quads(v, [](float a, float b) { return a + b; });

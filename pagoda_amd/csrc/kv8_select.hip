@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* score
 #pragma unroll
       for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(more[j]));
     }
-  most = wave_max(most);
+  most = lanes_max<64>(most);
   if (lane == 0) tops[wave] = most;
   __syncthreads();
   const float down = pow2(-holds127(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))));
@@ -163,9 +163,7 @@ __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* score
   }
 #pragma unroll
   for (int i = 0; i < TILES; i++) {
-    int v = best[i];
-    v = max(v, __shfl_xor(v, 16));
-    v = max(v, __shfl_xor(v, 32));
+    const int v = quads_max(best[i]);
     const int page = page0 + (i * 4 + wave) * 16 + n16;
     if (kq == 0 && page < pages)
       scores[((int64_t)row * kv_heads + head) * r.max_blocks + page] = scale[i] > 0 ? (float)v * scale[i] : -INFINITY;
@@ -226,11 +224,8 @@ __global__ __launch_bounds__(kPick) void pick_kernel(Rows r, int kv_heads, int t
   if (tid == 0) chosen[3] = 0;
   uint32_t low = ~0u, high = 0;
   each([&](uint32_t k, int) { low = min(low, k), high = max(high, k); });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    low = min(low, (uint32_t)__shfl_xor((int)low, o));
-    high = max(high, (uint32_t)__shfl_xor((int)high, o));
-  }
+  low = lanes_min<64>(low);
+  high = lanes_max<64>(high);
   if (lane == 0) part[0][wave] = low, part[1][wave] = high;
   __syncthreads();
 #pragma unroll
