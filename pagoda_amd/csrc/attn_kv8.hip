@@ -221,17 +221,6 @@ __device__ inline bool find(const Rows& r, int kv_heads, const Class& cl, int ke
   return false;
 }
 
-// The sequence that owns a row: its index, -1 without one.
-__device__ inline int seq_of(const Rows& r, int row) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < r.nseq; base += 64) {
-    const int i = base + lane;
-    const uint64_t hit = __ballot(i < r.nseq && r.row_start[i] <= row && row < r.row_start[i + 1]);
-    if (hit) return base + __builtin_ctzll(hit);
-  }
-  return -1;
-}
-
 // Positions that row j of a sequence sees.
 __device__ inline int seen_by(const Seq& s, int j) {
   return (int)max(min((long long)s.len - s.n + j + 1, (long long)s.ctx), 0ll);
@@ -552,12 +541,13 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     s.n = 1;
     load_q(s, head, tile);
     const int count = min(max(list.count[(int64_t)row * kv_heads + head], 0), list.top);
-    seq = seq_of(r, row);
+    const RowSeq rs = row_seq(r, row);
+    seq = rs.seq;
     const int have = chunks_of(count, list.chunk);
     if (c >= have || seq < 0) return;
     page1 = min(page0 + list.chunk, count);
     // (as the last of the rows up to this one)
-    s.len = (int)max((long long)r.lens[seq] - (min(r.row_start[seq + 1], r.rows) - 1 - row), 0ll);
+    s.len = rs.seen(row);
     s.ctx = (int)min((long long)s.len, (long long)r.max_blocks * kPage);
     slot = have > 1 ? (int)blockIdx.x : -1;
   } else {

@@ -138,5 +138,28 @@ __device__ inline float wave_total(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+// The sequence that owns a row (-1: none), with all that a row's context needs in one round of loads.
+struct RowSeq {
+  int seq, end, len;
+  // positions that the row sees
+  __device__ int seen(int row) const {
+    return (int)max((long long)len - (end - 1 - row), 0ll);
+  }
+};
+__device__ inline RowSeq row_seq(const Rows& r, int row) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < r.nseq; base += 64) {
+    const int i = base + lane;
+    int from = 0, end = 0, len = 0;
+    if (i < r.nseq) from = r.row_start[i], end = r.row_start[i + 1], len = r.lens[i];
+    const uint64_t hit = __ballot(i < r.nseq && from <= row && row < end);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      return RowSeq{base + src, min(__builtin_amdgcn_readlane(end, src), r.rows), __builtin_amdgcn_readlane(len, src)};
+    }
+  }
+  return RowSeq{-1, 0, 0};
+}
+
 }  // namespace kv8
 }  // namespace pgd

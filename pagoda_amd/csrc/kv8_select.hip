@@ -17,23 +17,11 @@ namespace kv8 {
 namespace {
 
 
-// The sequence that owns a row and the pages of the row's context (0 for none).
+// The pages of a row's context (0 for none).
 __device__ inline int row_pages(const Rows& r, int row, int& seq) {
-  const int lane = threadIdx.x & 63;
-  seq = -1;
-  for (int base = 0; base < r.nseq; base += 64) {
-    const int i = base + lane;
-    const uint64_t hit = __ballot(i < r.nseq && r.row_start[i] <= row && row < r.row_start[i + 1]);
-    if (hit) {
-      seq = base + __builtin_ctzll(hit);
-      break;
-    }
-  }
-  if (seq < 0) return 0;
-  const long long seen = (long long)r.lens[seq] - (min(r.row_start[seq + 1], r.rows) - 1 - row);
-  if (seen <= 0) return 0;
-  const long long pages = (seen + kPage - 1) / kPage;
-  return (int)(pages < r.max_blocks ? pages : r.max_blocks);
+  const RowSeq rs = row_seq(r, row);
+  seq = rs.seq;
+  return seq < 0 ? 0 : min((rs.seen(row) - 1) / kPage + (rs.seen(row) > 0 ? 1 : 0), r.max_blocks);
 }
 
 // Smallest exponent with top <= 127 * 2^e; 127 is 1.984375 * 2^6.
@@ -55,6 +43,17 @@ __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* score
   const int strips = (r.max_blocks + kPages - 1) / kPages, unit = blockIdx.x / strips;
   const int row = unit / kv_heads, head = unit % kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kq = lane >> 4;
+  auto finite = [](float v) { return fabsf(v) <= 3.402823466e38f ? v : 0.0f; };
+  const int64_t q_at = (int64_t)row * r.ldq + (int64_t)head * group * HD;
+  auto load_q = [&](int q0, int i, float (&x)[8]) {
+    const int u = tid + i * 256;
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = 0;
+    if (u < kUnits && q0 + u / (HD / 8) < group) load8<T>(r.q, q_at + (int64_t)q0 * HD + u * 8, x);
+  };
+  float x[kRounds][8];
+#pragma unroll
+  for (int i = 0; i < kRounds; i++) load_q(0, i, x[i]);
   int seq;
   const int pages = row_pages(r, row, seq);
   const int page0 = (int)(blockIdx.x % strips) * kPages;
@@ -67,21 +66,6 @@ __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* score
     const int page = page0 + (i * 4 + wave) * 16 + n16;
     id[i] = page < pages ? table[page] : -1;
   }
-  auto finite = [](float v) { return fabsf(v) <= 3.402823466e38f ? v : 0.0f; };
-  const int64_t q_at = (int64_t)row * r.ldq + (int64_t)head * group * HD;
-  auto load_q = [&](int q0, int i, float (&x)[8]) {
-    const int u = tid + i * 256;
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = 0;
-    if (u < kUnits && q0 + u / (HD / 8) < group) {
-      load8<T>(r.q, q_at + (int64_t)q0 * HD + u * 8, x);
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = finite(x[j]);
-    }
-  };
-  float x[kRounds][8];
-#pragma unroll
-  for (int i = 0; i < kRounds; i++) load_q(0, i, x[i]);
   const size_t page_bytes = p.at.page_bytes(), bounds_at = p.at.bounds_at() + (size_t)head * 2 * HD + kq * 16,
                meta_at = p.at.meta_at() + (size_t)head * 4;
   i4 bound[2][kSegs];
@@ -100,13 +84,13 @@ __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* score
 #pragma unroll
   for (int i = 0; i < kRounds; i++)
 #pragma unroll
-    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(x[i][j]));
+    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(finite(x[i][j])));
   for (int q0 = 16; q0 < group; q0 += 16)
     for (int i = 0; i < kRounds; i++) {
       float more[8];
       load_q(q0, i, more);
 #pragma unroll
-      for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(more[j]));
+      for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(finite(more[j])));
     }
   most = lanes_max<64>(most);
   if (lane == 0) tops[wave] = most;
@@ -132,7 +116,7 @@ __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* score
         uint32_t pos[2] = {0, 0}, neg[2] = {0, 0};
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const int v = (int)rintf(x[i][j] * down);
+          const int v = (int)rintf(finite(x[i][j]) * down);
           pos[j / 4] |= (uint32_t)(max(v, 0) & 255) << (8 * (j & 3));
           neg[j / 4] |= (uint32_t)(min(v, 0) & 255) << (8 * (j & 3));
         }
@@ -191,10 +175,17 @@ __global__ __launch_bounds__(kPick) void pick_kernel(Rows r, int kv_heads, int t
   __shared__ int counts[kHeld * kPick / 64];
   __shared__ uint32_t chosen[4];  // bin, keys still to take, keys of the bin; keys listed
   const int row = blockIdx.x / kv_heads, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // (scores of pages past the row's are whatever the workspace held, and not looked at)
+  const float* s = scores + (int64_t)blockIdx.x * r.max_blocks;
+  float early[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; j++) {
+    const int i = sinks + j * kPick + tid;
+    early[j] = i < r.max_blocks ? s[i] : 0.0f;
+  }
   int seq;
   const int pages = row_pages(r, row, seq);
   if (seq < 0) return;
-  const float* s = scores + (int64_t)blockIdx.x * r.max_blocks;
   int* to = sel + (int64_t)blockIdx.x * top;
   const int take = min(top, pages);
   if (tid == 0) count[blockIdx.x] = take;
@@ -209,7 +200,7 @@ __global__ __launch_bounds__(kPick) void pick_kernel(Rows r, int kv_heads, int t
 #pragma unroll
   for (int j = 0; j < kHeld; j++) {
     const int i = from + j * kPick + tid;
-    held[j] = i < until ? order_of(s[i]) : 0;
+    held[j] = i < until ? order_of(early[j]) : 0;  // (from is sinks, or no page is left)
   }
   // f(key, page) for this thread's keys
   auto each = [&](auto f) {
