@@ -8,11 +8,11 @@
 //   t = S 2^ek log2(e) / sqrt(hd), its running maximum m and the sum l of 2^(t - m) in f32
 //   O[dim][query] += V codes^T . 2^(t + ev - M)   the same products over the 32 positions
 // with M the running maximum of t + ev, so that the largest weight of a value's code is
-// about one whatever the pages' powers of two. Codes convert to f16 exactly. Queries are
+// about one whatever the pages' powers of two (both maxima may lag a factor of 2^4 behind). Codes convert to f16 exactly. Queries are
 // scaled by a power of two into f16's range and enter as f16 terms: f32 rows two (22 bits and
 // at least 2^-40 of the row's largest), f16 rows themselves, bf16 rows one (exact to 2^-40 of the
-// largest). The weights, times 2^15, enter as two terms, 2^-21 (bf16 rows: one; its 2^-11 is an
-// eighth of their own rounding). bf16 terms would need no scaling but half as many more
+// largest). The weights, times 2^11, enter as two terms, 2^-21 and 2^-36 of the largest (bf16 rows: one; its
+// 2^-11 is an eighth of their own rounding). bf16 terms would need no scaling but half as many more
 // products: three for f32 where f16 takes two.
 // The lane that holds a score holds it as the operand of the second product: lane
 // (query n = l % 16, kq = l / 16) has positions 4 kq .. 4 kq + 3 of both pages, which
@@ -51,7 +51,9 @@ template <int T>
 constexpr int kTerms = T == F32 ? 2 : 1;  // f16 terms of a query
 template <int T>
 constexpr int kWeightTerms = T == BF16 ? 1 : 2;
-constexpr float kWeightExp = 15;  // weights enter times 2^15: f16 holds 2^-24 to 65504
+// O and the sum are only brought to new maxima that are 2^kSlack times the old ones or more (and all of a wave's
+// with them), so weights reach 2^kSlack. They enter times 2^kWeightExp: f16 holds 2^-24 to 65504.
+constexpr float kSlack = 4, kWeightExp = 15 - kSlack;
 
 // x as f16 terms to nearest, each of what the ones before leave.
 template <int N>
@@ -409,9 +411,11 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
     top = fmaxf(top, t);
     top_v = fmaxf(top_v, t + ev[w]);
   }
-  top = fmaxf(q.m, quads_max(top));
-  top_v = fmaxf(q.mv, quads_max(top_v));
-  if (__any(top > q.m || top_v > q.mv)) {
+  top = quads_max(top);
+  top_v = quads_max(top_v);
+  if (__any(top > q.m + kSlack || top_v > q.mv + kSlack)) {
+    top = fmaxf(q.m, top);
+    top_v = fmaxf(q.mv, top_v);
     q.l *= top > q.m ? __builtin_amdgcn_exp2f(q.m - top) : 1.0f;
     const float down = top_v > q.mv ? __builtin_amdgcn_exp2f(q.mv - top_v) : 1.0f;
 #pragma unroll
@@ -419,7 +423,7 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
     q.m = top;
     q.mv = top_v;
   }
-  const float at = top > -INFINITY ? top : 0.0f, at_v = top > -INFINITY ? top_v - kWeightExp : 0.0f;
+  const float at = q.m > -INFINITY ? q.m : 0.0f, at_v = q.m > -INFINITY ? q.mv - kWeightExp : 0.0f;
   float far = -INFINITY, sum[PG];
 #pragma unroll
   for (int w = 0; w < PG; w++) far = fmaxf(far, ev[w]);
@@ -661,14 +665,17 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     h8 wt[1][kW];
     weigh<kW>(sc, cur, scale, whole_pages(cur, least), q, o, wt);
 #pragma unroll
-    for (int i = 0; i < kSegs; i++)
+    for (int i = 0; i < kSegs; i++) {
+      h8 a[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const h8 a = of_codes8(vc[0][i][j], vc[1][i][j]);
+      for (int j = 0; j < 4; j++) a[j] = of_codes8(vc[0][i][j], vc[1][i][j]);
+      // (terms outermost: a product on the same sums as the one before it would wait for it)
 #pragma unroll
-        for (int k = kW - 1; k >= 0; k--)
-          o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wt[0][k], o[4 * i + j], 0, 0, 0);
-      }
+      for (int k = kW - 1; k >= 0; k--)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], wt[0][k], o[4 * i + j], 0, 0, 0);
+    }
     if (more) {
       load_v(next);
       cur[0] = next[0];
@@ -858,14 +865,17 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out,
 #pragma unroll
         for (int w = 0; w < PG; w++) code[w] = kv[w * kHead / 16 + kHead / 32 + i * 64];
 #pragma unroll
-        for (int w = 0; w < PG; w += 2)
+        for (int w = 0; w < PG; w += 2) {
+          h8 a[4];
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const h8 a = of_codes8(code[w][j], code[w + 1][j]);
+          for (int j = 0; j < 4; j++) a[j] = of_codes8(code[w][j], code[w + 1][j]);
+          // (terms outermost: a product on the same sums as the one before it would wait for it)
 #pragma unroll
-            for (int k = kW - 1; k >= 0; k--)
-              o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wt[w / 2][k], o[4 * i + j], 0, 0, 0);
-          }
+          for (int k = kW - 1; k >= 0; k--)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              o[4 * i + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], wt[w / 2][k], o[4 * i + j], 0, 0, 0);
+        }
       }
       __builtin_amdgcn_s_setprio(0);
     }

@@ -166,8 +166,8 @@ def attend(q, k, v, t, unit=0.0):
     of the exponent's argument, each 2^-24 of its magnitude, 2^-22 for exp2 itself. Weights then
     are off by the factor exp(2 d). They enter as f16 terms of 11 bits: one (bf16 rows) to nearest is 2^-11
     off at most; of two the first is truncated, 2^-10, and the second to nearest, 2^-11 of that; and no
-    less than f16's smallest half step, 2^-25, which is 2^-40 of the largest weight of a code; codes are up to
-    448. The sums of n weights and n products by n 2^-23 each."""
+    less than f16's smallest half step, 2^-25, times 2^-11 the weights' scale: 2^-36 of a weight that is the
+    largest or up to 2^4 below; codes are up to 448. The sums of n weights and n products by n 2^-23 each."""
     if len(k) == 0:
         return np.zeros(v.shape[1]), np.zeros(v.shape[1])
     hd = k.shape[1]
@@ -180,7 +180,7 @@ def attend(q, k, v, t, unit=0.0):
     w /= w.sum()
     held = {F32: 2.0 ** -21, F16: 2.0 ** -21, BF16: 2.0 ** -11}[t]
     mass = w @ np.abs(v)
-    small = len(k) * 448 * 2.0 ** -40 * (w * unit).max()
+    small = len(k) * 448 * 2.0 ** -36 * (w * unit).max()
     return w @ v, mass * (2 * np.expm1(2 * d) + held + (2 * len(k) + 16) * 2.0 ** -23) + small
 
 
