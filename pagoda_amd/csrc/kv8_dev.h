@@ -101,7 +101,10 @@ __device__ inline T over_lanes(T v, F f) {
 }
 template <int N, class T>
 __device__ inline T lanes_max(T v) {
-  return over_lanes<N>(v, [](T a, T b) { return std::is_same<T, float>::value ? fmaxf(a, b) : max(a, b); });
+  return over_lanes<N>(v, [](T a, T b) {
+    if constexpr (std::is_same<T, float>::value) return fmaxf(a, b);
+    else return max(a, b);
+  });
 }
 template <int N, class T>
 __device__ inline T lanes_min(T v) {
