@@ -261,8 +261,10 @@ size_t pgd_kv8_page_bytes(int kv_heads, int head_dim);
  * input. nseq is at most 2^24, rows at most 2^30. status[i]: 0; or why the
  * sequence got nothing (its rows are -1, its length and table stay): 1 too few free
  * pages, 2 more positions than max_blocks pages hold, 3 rows past `rows`, 4 a negative length or
- * count. A sequence that needs no page is not refused for those that do. A table entry that is
- * negative makes slots -1. */
+ * count. A sequence that needs no page is not refused for those that do; of those that need some, all behind the
+ * first that is refused for want of pages are refused too. Refused rows keep their place in row_start, so
+ * an attention over it computes something for them, of the positions that the sequence has; it is to be ignored.
+ * A table entry that is negative makes slots -1. */
 int pgd_kv_tables_dev(pgd_dev* dev, int block, int nseq, const int* lens, const int* counts, int* tables,
                       int max_blocks, const int* free_pages, int n_free, const int* taken, int rows, int* new_lens,
                       int* new_taken, int* row_start, int* seq_of_row, int* pos_of_row, int* slots, int* status);
@@ -308,7 +310,7 @@ int pgd_attn_kv8_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
  * group's heads within 127; non-finite entries count as 0), the page's key codes bounded per
  * channel by whole numbers hi and lo (the largest and smallest code over 4, rounded outward; the
  * append keeps them): score = 2^(key exponent) max over the group's heads of
- * sum(max(q8 hi, q8 lo)), exact in f32; ties go to the lower page. A page outside the pool scores
+ * sum(max(q8 hi, q8 lo)), exact in f32 (an infinity from 2^128 on); ties go to the lower page. A page outside the pool scores
  * lowest. Rows of no sequence are left as they were; a row that attends to nothing selects nothing.
  * ws as above, of pgd_kv8_sparse_ws_bytes bytes, which serves both calls, one after the other. */
 size_t pgd_kv8_sparse_ws_bytes(int heads, int kv_heads, int head_dim, int rows, int max_blocks, int top);

@@ -139,6 +139,7 @@ int pgd_kv8_read_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
     PGD_CHECK(dev, kErrArg, "null device");
     const Pool p = pool_of(pool, n_pages, kv_heads, head_dim);
     PGD_CHECK(rows >= 0, kErrArg, "rows must not be negative");
+    PGD_CHECK((int64_t)rows * kv_heads < kBlocks * 32, kErrShape, "more rows than one launch holds");
     if (rows == 0) return;
     PGD_CHECK(slots, kErrArg, "null slots");
     check_rows(k, ldk, (int64_t)kv_heads * head_dim, 4, "k");

@@ -91,7 +91,8 @@ REFUSED = (
         (dict(ldk=120), SHAPE), (dict(ldv=132), SHAPE), (dict(type=3), ARG), (dict(slots=0), ARG),
         (dict(rows=1 << 23), SHAPE)]]
     + [("pgd_kv8_read_dev", c, e) for c, e in POOL + [
-        (dict(k=0), ARG), (dict(v=A + 4), ARG), (dict(ldk=126), SHAPE), (dict(ldv=130), SHAPE), (dict(slots=0), ARG)]]
+        (dict(k=0), ARG), (dict(v=A + 4), ARG), (dict(ldk=126), SHAPE), (dict(ldv=130), SHAPE), (dict(slots=0), ARG),
+        (dict(rows=1 << 28), SHAPE)]]
     + [("pgd_attn_kv8_dev", c, e) for c, e in POOL + QUERY + RESULT + [(dict(max_rows=-1), ARG)]]
     + [("pgd_kv8_select_dev", c, e) for c, e in POOL + QUERY + LIST + [
         (dict(sinks=-1), ARG), (dict(recent=-1), ARG), (dict(sinks=6, recent=3), ARG),
