@@ -411,10 +411,12 @@ void append_hd(const Pool& p, const void* k, int64_t ldk, const void* v, int64_t
                int rows, hipStream_t s) {
   // 256 decode rows take 13.7 us with a workgroup a row (and head), 18.7 with one of four, which takes pages one
   // after the other; 500 decode rows 21.2 and 24.9; 512 rows of a prompt, where most workgroups of a row have no page
-  // of their own, 16.7 and 11.9 (with the read-back of 3 us and more, head_dim 256, 4 KV heads). Eight rows: 1024 of
-  // a prompt 14.1 against 16.3, 500 decode rows 32.6.
+  // of their own, 16.7 and 11.9 (with the read-back of 3 us and more, head_dim 256, 4 KV heads). Four rows a
+  // workgroup or eight: 2048 and 4000 rows of a prompt 23.5 and 19.1, 37.0 and 29.5; 2000 decode rows 79 both, 4000
+  // 153 and 162; but 1000 decode rows 42 and 49.
   if (rows <= 256) append_rows<HD, 1>(p, k, ldk, v, ldv, type, slots, rows, s);
-  else append_rows<HD, 4>(p, k, ldk, v, ldv, type, slots, rows, s);
+  else if (rows < 2048) append_rows<HD, 4>(p, k, ldk, v, ldv, type, slots, rows, s);
+  else append_rows<HD, 8>(p, k, ldk, v, ldv, type, slots, rows, s);
 }
 
 }  // namespace
@@ -427,9 +429,9 @@ void append(const Pool& p, const void* k, int64_t ldk, const void* v, int64_t ld
 }
 
 void read(const Pool& p, const int* slots, int rows, float* k, int64_t ldk, float* v, int64_t ldv, hipStream_t s) {
-  // Runs of 9 rows (64 and 500 pages): one by one 10 and 22 us with their write, run by run 17 and 25; a prompt's 1000
-  // rows the same, 8600 rows 50 and 41.
-  if (rows > 4096) {
+  // Runs of 9 rows (64 pages): one by one 10 us with their write, run by run 17, of 200 pages and more the same; a
+  // prompt's 1000 rows the same, 2048 rows 19.2 and 17.5, 4000 rows 29.5 and 24.5.
+  if (rows >= 2048) {
     const unsigned grid = (unsigned)(((int64_t)(rows + 15) / 16 * p.at.kv_heads + 3) / 4);
     if (p.at.hd == 64) read_runs_kernel<64><<<grid, 256, 0, s>>>(p, slots, rows, k, ldk, v, ldv);
     else if (p.at.hd == 128) read_runs_kernel<128><<<grid, 256, 0, s>>>(p, slots, rows, k, ldk, v, ldv);

@@ -658,7 +658,7 @@ def test_selection_of_many_equal_scores(dev, buf):
 
 @pytest.mark.parametrize("kv,hd", [(1, 64), (3, 128), (2, 256)])
 def test_read_of_many_rows(dev, buf, kv, hd):
-    """More rows than the call reads one by one (4096): whole sequences, any order, runs across pages, slots
+    """More rows than the call reads one by one (2047): whole sequences, any order, runs across pages, slots
     twice and outside the pool."""
     rng = np.random.default_rng(40 + hd)
     step = Step(rng, kv, hd, [400, 77, 5], [0, 0, 0], F32)
@@ -673,6 +673,40 @@ def test_read_of_many_rows(dev, buf, kv, hd):
     assert (k[bad] == -77).all() and (v[bad] == -77).all()
     for got, w in ((k, 0), (v, 1)):
         np.testing.assert_array_equal(got[~bad], step.cache.read(w, some[~bad]).astype(np.float32))
+
+
+@pytest.mark.parametrize("t,kv,hd", [(F32, 1, 64), (F16, 2, 128), (BF16, 1, 256)])
+@pytest.mark.parametrize("rows", [255, 256, 257, 1000, 2047, 2048, 2049, 5000])
+def test_write_of_many_rows(dev, buf, t, kv, hd, rows):
+    """Calls of sizes that are shared out to workgroups and read in different ways: runs of one to many pages that
+    begin and end anywhere, single rows, and rows of no slot between them; then the pages' second halves."""
+    rng = np.random.default_rng(rows + hd)
+    slots, ends, page = [], [], 0
+    numbers = rng.permutation(rows + 8)
+    while len(slots) < rows:
+        kind = rng.integers(4)
+        if kind == 0:
+            slots += [-1, 2 ** 31 - 1, (rows + 8) * PAGE][: rng.integers(1, 4)]
+            continue
+        n = min(1 if kind == 1 else rng.integers(1, 17) if kind == 2 else rng.integers(17, 200), rows - len(slots))
+        if n <= 0:
+            break
+        place = np.arange(n)
+        slots += list(numbers[page + place // PAGE] * PAGE + place % PAGE)
+        page += -(-n // PAGE)
+        ends.append(slots[-1])
+    slots = np.array(slots[:rows])
+    cache, pool = kv8.Cache(rows + 8, kv, hd), GpuPool(dev, buf, kv, hd, rows + 8)
+    for _ in range(2):
+        size = 2.0 ** rng.integers(-12, 6, (2, len(slots), 1)) * rng.normal(0, 1, (2, len(slots), kv * hd))
+        (kr, k), (vr, v) = typed(size[0], t), typed(size[1], t)
+        pool.append(kr, vr, slots, t, kv * hd + 8, kv * hd)
+        cache.append(k, v, slots)
+        live = slots[(slots >= 0) & (slots < cache.n * PAGE)]
+        same_as(cache, pool, live)
+        # (go on behind the last rows of the runs, to their pages' ends)
+        slots = np.array([s for e in ends for s in range(e + 1, (e | (PAGE - 1)) + 1)], np.int64)
+    assert pool.untouched()
 
 
 @pytest.mark.parametrize("t,heads,kv,hd", [(F32, 14, 2, 64), (F16, 28, 4, 128), (BF16, 24, 4, 256), (F32, 17, 1, 64)])
