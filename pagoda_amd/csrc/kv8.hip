@@ -113,8 +113,9 @@ __global__ __launch_bounds__(256) void append_kernel(Pool p, const void* k, int6
       e[w] = max(need, w ? Meta::ev(m0) : Meta::ek(m0));
     }
 
-    // old codes at the new exponents, nothing at the places from s0 on
-    if (tid < HD) {
+    // old codes at the new exponents, nothing at the places from s0 on (which the rows of a full page cover)
+    const bool full = s0 == 0 && n == kPage;
+    if (!full && tid < HD) {
       const int place_k = tid & 15, place_v = tid >> 4 & 3;
       const float down[2] = {pow2(max(Meta::ek(m0) - e[0], kExpMin)), pow2(max(Meta::ev(m0) - e[1], kExpMin))};
       uint32_t keep_v = 0;
@@ -122,17 +123,17 @@ __global__ __launch_bounds__(256) void append_kernel(Pool p, const void* k, int6
       for (int j = 0; j < 4; j++) keep_v |= 4 * place_v + j < s0 ? 0xffu << (8 * j) : 0u;
 #pragma unroll
       for (int w = 0; w < 2; w++) {
-        const uint32_t keep = w ? keep_v : place_k < s0 ? ~0u : 0u;
-        u4 c;
+        u4 c = old[w] & (w ? keep_v : place_k < s0 ? ~0u : 0u);
+        if (s0 && e[w] != (w ? Meta::ev(m0) : Meta::ek(m0)))
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const f4 u = of_codes(old[w][j] & keep) * down[w];
-          c[j] = to_codes(u[0], u[1], u[2], u[3]);
-        }
+          for (int j = 0; j < 4; j++) {
+            const f4 u = of_codes(c[j]) * down[w];
+            c[j] = to_codes(u[0], u[1], u[2], u[3]);
+          }
         reinterpret_cast<u4*>(code[w])[tid] = c;
       }
     }
-    __syncthreads();
+    if (!full) __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPasses; i++) {
       const int j = r + i * kStep;
