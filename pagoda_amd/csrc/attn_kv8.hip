@@ -38,11 +38,16 @@ namespace kv8 {
 
 namespace {
 
-// Items that contexts are cut into, about: as many as run at once (item_kernel: workgroups of four waves that a
-// CU holds at a head_dim, over the 256 CUs; prompt_kernel: 512 run at once, more where a tile is long and
-// the rounds uneven).
+// Items that contexts are cut into, about. item_kernel: as many as run at once (workgroups of four waves that a
+// CU holds at a head_dim, over the 256 CUs).
 constexpr int few_items(int hd, int tiles) { return 256 * (hd == 256 ? 2 : hd == 128 ? 3 : 4) / tiles; }
 constexpr int many_items(int hd) { return hd == 128 ? 1024 : 1536; }
+// prompt_kernel: more, as contexts that are cut or not make uneven rounds (3 prompts of 2274 rows, head_dim 256: 277 us
+// against 346 with 512 items), but as many as run at once rather than chunks of less than kFullChunk pages, which the
+// way to their first page and their partial sums would make dear (236 rows on 3977 positions, head_dim 256: 74 us
+// against 97; 30 on 15000: 49 against 81; 500 on 3977: 122 against 130; with 32 pages 82, 49 and 131).
+constexpr int many_at_once(int hd) { return hd == 64 ? 1024 : 512; }
+constexpr int kFullChunk = 64;
 constexpr int kMinChunk = 8;     // pages: a pair for each of four waves
 constexpr int kOneChunk = 16;    // pages of tables (and lists) that are never cut: the join would cost more
 constexpr int kFewQueries = 32;  // of a sequence and KV head: calls of up to these are item_kernel's alone
@@ -129,6 +134,7 @@ struct Share {
   int least, most;
   int tile;   // queries, a power of two
   int items;  // that contexts are cut into, about
+  int fewest;  // as many, rather than chunks of less than kFullChunk pages
 };
 
 struct Class {
@@ -182,7 +188,8 @@ __device__ inline bool find(const Rows& r, int kv_heads, const Class& cl, int ke
     }
     all += (float)tiles * (float)s.pages;
   }
-  const float each = fmaxf(wave_total(all) * kv_heads / cl.sh.items, 1.0f);
+  const float total = wave_total(all) * kv_heads;
+  const float each = fmaxf(fmaxf(total / cl.sh.items, fminf(total / cl.sh.fewest, kFullChunk)), 1.0f);
   const int least = least_chunk(r.max_blocks);
   int chunk = 0;  // this lane's sequence's
   auto items_of = [&](int base) {
@@ -1025,8 +1032,8 @@ Plan plan_of(int hd, int group, int64_t max_rows) {
   Plan p{};
   p.both = most > kFewQueries;
   p.two = most > 16 && !p.both;
-  p.few = Share{1, p.both ? 16 : INT_MAX, p.two ? 32 : 16, few_items(hd, p.two ? 2 : 1)};
-  p.many = Share{17, INT_MAX, 64, many_items(hd)};
+  p.few = Share{1, p.both ? 16 : INT_MAX, p.two ? 32 : 16, few_items(hd, p.two ? 2 : 1), few_items(hd, p.two ? 2 : 1)};
+  p.many = Share{17, INT_MAX, 64, many_items(hd), many_at_once(hd)};
   return p;
 }
 

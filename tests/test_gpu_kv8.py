@@ -359,6 +359,28 @@ def test_attention_long(dev, buf, t, heads, kv, hd, ctx, new):
     check_attention(dev, buf, rng, Step(rng, kv, hd, ctx, new, t), heads, t)
 
 
+@pytest.mark.parametrize("t,heads,kv,hd,ctx,new", [
+    (F16, 24, 4, 256, [3977], [236]), (F32, 24, 4, 256, [7000], [30]), (BF16, 8, 4, 128, [4000, 150], [1500, 140]),
+    (F32, 8, 8, 128, [4000, 90], [2200, 90]), (F32, 14, 2, 64, [4000, 2000], [1300, 17]),
+    (BF16, 24, 8, 64, [4000, 4000], [1500, 1300]), (F32, 6, 2, 256, [5000, 700, 33], [2500, 600, 33])])
+def test_attention_of_prompts_on_long_contexts(dev, buf, t, heads, kv, hd, ctx, new):
+    """Contexts cut into as many chunks as run at once, into chunks of a fixed size, and into as few as balance: some
+    rows of each sequence against the definition, its first and last among them."""
+    rng = np.random.default_rng(ctx[0] + new[0] + hd)
+    step = Step(rng, kv, hd, ctx, new, t)
+    pool = pool_of(dev, buf, step)
+    q, qv, (g, gv) = queries(rng, step, heads, t, True)
+    rows = list(step.each_row())
+    ends = np.cumsum([0] + new)
+    some = sorted(set(rng.integers(0, step.rows, 25)) | set(ends[:-1]) | set(ends[1:] - 1))
+    step.each_row = lambda: [rows[i] for i in some]
+    want, bound = kv8.attention(step, qv, t, heads, gv)
+    got = Call(dev, buf, step, pool, heads, t, q, g).attn()
+    bad = ~(np.abs(got - want) <= bound)[some]
+    assert not bad.any(), (np.argwhere(bad)[:5], got[some][bad][:5], want[some][bad][:5])
+    assert np.isfinite(got).all()
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("max_rows", [0, 1, 7, 10 ** 6])
 def test_any_bound_on_the_rows(dev, buf, t, max_rows):
