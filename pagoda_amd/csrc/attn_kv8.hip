@@ -50,7 +50,10 @@ constexpr int many_at_once(int hd) { return hd == 64 ? 1024 : 512; }
 constexpr int kFullChunk = 64;
 constexpr int kMinChunk = 8;     // pages: a pair for each of four waves
 constexpr int kOneChunk = 16;    // pages of tables (and lists) that are never cut: the join would cost more
-constexpr int kFewQueries = 32;  // of a sequence and KV head: calls of up to these are item_kernel's alone
+// Queries of a sequence and KV head: calls of up to these are item_kernel's alone. 16 sequences of 100 to 6000
+// positions, 7 queries a row at head_dim 64 (f32) and 6 at 256 (f16), with this and with 32: 12 rows each 20 and 31 us,
+// 58 and 58; 1 to 20 rows 46 and 54 at 256; 20 rows 66 and 63, 30 rows (past both) the same.
+constexpr int kFewQueries = 128;
 
 template <int T>
 constexpr int kTerms = T == F32 ? 2 : 1;  // f16 terms of a query
@@ -1020,8 +1023,9 @@ Grid grid_of(const Layout& at, int heads, int nseq, int max_blocks, int rows, co
   return Grid{std::min(cut, tiles + most), per > 1 ? std::min(cut, 2 * most) * (sh.tile / 16) : 0};
 }
 
-// How a call is shared out: by the largest number of queries that a sequence has for a KV head. Up to 16 and up to 32
-// are item_kernel's alone, one or two tiles side by side; past that it keeps the sequences of up to 16.
+// How a call is shared out: by the largest number of queries that a sequence has for a KV head. Up to 16 and up to
+// kFewQueries are item_kernel's alone, one or two tiles side by side; past that it keeps the sequences of up to 16
+// (16 of 2 to 32 rows, 6 queries a row: 63 us; up to 32 or 64: 67 and 66).
 struct Plan {
   Share few, many;
   bool two;   // tiles side by side

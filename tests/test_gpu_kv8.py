@@ -381,6 +381,15 @@ def test_attention_of_prompts_on_long_contexts(dev, buf, t, heads, kv, hd, ctx, 
     assert np.isfinite(got).all()
 
 
+@pytest.mark.parametrize("t,heads,kv,hd", [(F32, 14, 2, 64), (F16, 24, 4, 256), (BF16, 28, 4, 128), (F32, 40, 1, 64)])
+@pytest.mark.parametrize("most", [3, 9, 18, 19, 21, 22])
+def test_attention_of_chunks_of_many_sizes(dev, buf, t, heads, kv, hd, most):
+    """Verify chunks of up to 4 tiles and past them, whose kernels differ, next to single rows and none."""
+    rng = np.random.default_rng(most + hd)
+    ctx = [most, 700, 150, 1, 333, 64]
+    check_attention(dev, buf, rng, Step(rng, kv, hd, ctx, [most, most, 2, 1, 0, most // 2], t), heads, t, gate=hd == 64)
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("max_rows", [0, 1, 7, 10 ** 6])
 def test_any_bound_on_the_rows(dev, buf, t, max_rows):
