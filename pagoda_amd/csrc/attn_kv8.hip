@@ -57,8 +57,7 @@ constexpr int kFewQueries = 128;
 
 template <int T>
 constexpr int kTerms = T == F32 ? 2 : 1;  // f16 terms of a query
-template <int T>
-constexpr int kWeightTerms = T == BF16 ? 1 : 2;
+constexpr int kWeightTerms = 2;
 // O and the sum are only brought to new maxima that are 2^kSlack times the old ones or more (and all of a wave's
 // with them), so weights reach 2^kSlack. They enter times 2^kWeightExp: f16 holds 2^-24 to 65504.
 constexpr float kSlack = 4, kWeightExp = 15 - kSlack;
@@ -388,9 +387,9 @@ struct Query {
 };
 
 // Scores of PG pages' positions to weights: s[w][i] is position 16 index + 4 kq + i of page w.
-template <int KW, int PG, int N>
+template <int PG, int N>
 __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scale, bool whole, Query& q, f4 (&o)[N],
-                             h8 (&out)[PG / 2][KW]) {
+                             h8 (&out)[PG / 2][kWeightTerms]) {
   const int kq = threadIdx.x >> 4 & 3;
   float x[PG][4], by[PG], ev[PG];
 #pragma unroll
@@ -461,7 +460,7 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = x[w + i / 4][i & 3];
-    split_weights<KW>(v, out[w / 2]);
+    split_weights(v, out[w / 2]);
   }
 }
 
@@ -503,7 +502,7 @@ __device__ inline int query_terms(float (&x)[8], h8 (&t)[N]) {
 template <int HD, int T, int NQ, bool LIST>
 __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out out, List list, Share share, void* ws,
                                                            Slots slots) {
-  constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms<T>;
+  constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms;
   constexpr int kJoinTiles = kTiles < 8 ? kTiles : 8;  // tiles of O joined at a time
   constexpr int kQBytes = kN * kSteps * 1024, kJoinBytes = 4 * kJoinTiles * 1024;
   constexpr int kTileBytes = kQBytes > kJoinBytes ? kQBytes : kJoinBytes;
@@ -675,7 +674,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
 #pragma unroll
         for (int i = 0; i < kSegs; i++) vc[w][i] = u4{0, 0, 0, 0};
     h8 wt[1][kW];
-    weigh<kW>(sc, cur, scale, whole_pages(cur, least), q, o, wt);
+    weigh(sc, cur, scale, whole_pages(cur, least), q, o, wt);
 #pragma unroll
     for (int i = 0; i < kSegs; i++) {
       h8 a[4];
@@ -737,7 +736,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
 // contexts.
 template <int HD, int T, int PG>
 __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out, Share share, void* ws, Slots slots) {
-  constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms<T>;
+  constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms;
   constexpr int kHead = 2 * kPage * HD;            // bytes of a page and head
   constexpr int kRounds = PG * kHead / 4096;       // 16 bytes a thread each, of a step
   constexpr int kQueries = 64;
@@ -872,7 +871,7 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out,
       }
       __builtin_amdgcn_s_setprio(0);
       h8 wt[PG / 2][kW];
-      weigh<kW>(sc, cur, scale, whole_pages(cur, least), q, o, wt);
+      weigh(sc, cur, scale, whole_pages(cur, least), q, o, wt);
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < kSegs; i++) {

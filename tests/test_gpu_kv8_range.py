@@ -1,0 +1,66 @@
+"""8-bit KV attention to the accuracy of its terms (kv8_close.py), and over the range of f32: the smallest and
+largest values, scores, queries and gates."""
+import numpy as np
+import pytest
+
+import kv8
+import kv8_close
+from kv8 import BF16, F16, F32, PAGE, Step, typed, value
+from kv8_close import assert_close
+from test_gpu_kv8 import HEADS, Call, GpuPool, pool_of, queries
+from test_gpu_mxfp4 import Buffers, buf  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# one chunk; several of them; verify rows; prompt rows; (last: attention over lists of all pages)
+FORMS = {"decode": ([37, 250], [1, 1]), "chunks": ([3000, 90], [1, 1]), "verify": ([400, 30], [4, 3]),
+         "prompt": ([150, 900], [70, 130]), "list": ([37, 800], [1, 2])}
+
+
+def with_rows(step, k=None, v=None):
+    """The step with other keys or values, f32 rows [positions, kv * hd] rounded to its type."""
+    if k is not None:
+        step.k_raw = typed(k, step.t)[0]
+    if v is not None:
+        step.v_raw = typed(v, step.t)[0]
+    step.cache = kv8.Cache(step.cache.n, step.cache.kv, step.cache.hd)
+    step.cache.append(value(step.k_raw, step.t), value(step.v_raw, step.t), step.slots)
+    return step
+
+
+def run(dev, buf, step, heads, t, q, gate=None, form="", pool=None):
+    """Raw queries and gates of type t to results."""
+    call = Call(dev, buf, step, pool or pool_of(dev, buf, step), heads, t, q, gate)
+    if form != "list":
+        return call.attn()
+    return call.sparse(*call.select(step.width, 0, 0))
+
+
+def some_rows(step, rng, most=40):
+    rows = range(step.rows)
+    return set(rows) if step.rows <= most else set(rng.choice(step.rows, most, replace=False)) | {0, step.rows - 1}
+
+
+def check(dev, buf, rng, step, heads, t, q, qv, form="", gate=(None, None)):
+    rows = some_rows(step, rng)
+    want, off = kv8_close.attention(step, qv, heads, gate[1], rows=rows)
+    assert np.isfinite(want[sorted(rows)]).all()
+    got = run(dev, buf, step, heads, t, q, gate[0], form)
+    rows = sorted(rows)
+    assert_close(got[rows], want[rows], off[rows], t)
+    return got, want
+
+
+# ---- accuracy -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("heads,kv,hd", HEADS)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+def test_results_are_the_definitions_rounded(dev, buf, t, form, heads, kv, hd):
+    """No result is another number of its type than one within the roundings of f32 sums and two f16 terms."""
+    rng = np.random.default_rng(heads + hd + t + len(form))
+    ctx, new = FORMS[form]
+    step = Step(rng, kv, hd, ctx, new, t)
+    q, qv, gate = queries(rng, step, heads, t, hd == 128)
+    check(dev, buf, rng, step, heads, t, q, qv, form, gate)
