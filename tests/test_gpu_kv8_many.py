@@ -1,0 +1,106 @@
+"""The 8-bit KV cache at more than 64 sequences (the lanes that look through them at once) with contexts that are cut, and the
+choice among many different scores."""
+import numpy as np
+import pytest
+
+import kv8
+import kv8_close
+from kv8 import BF16, F16, F32, PAGE, Step, typed
+from kv8_close import assert_close
+from test_gpu_kv8 import Call, GpuPool, pool_of, queries
+from test_gpu_mxfp4 import Buffers, buf  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def sequences(rng, n, most):
+    """Contexts of 1 to 600 positions, the longest on both sides of every 64th sequence, with up to `most` rows and
+    some with none."""
+    ctx = np.exp(rng.uniform(0, np.log(600), n)).astype(int) + 1
+    ctx[[0, 61, 62, 63, n - 2, n - 1]] = [500, 3, 1, 900, 700, 650]
+    new = np.where(rng.random(n) < 0.15, 0, np.where(rng.random(n) < 0.9, 1, rng.integers(1, most + 1, n)))
+    new[[63, n - 2, n - 1]] = [most, most, most]
+    return ctx.tolist(), np.minimum(new, ctx).tolist()
+
+
+@pytest.mark.parametrize("n", [65, 150, 257])
+@pytest.mark.parametrize("t,heads,kv,hd,most", [(F32, 6, 1, 64, 1), (BF16, 7, 1, 128, 4), (F16, 12, 2, 64, 15), (F32, 7, 1, 64, 60)])
+def test_cut_contexts_of_many_sequences(dev, buf, n, t, heads, kv, hd, most):
+    """Decode rows, verify rows, and rows of both kernels in one call."""
+    rng = np.random.default_rng(n + most)
+    ctx, new = sequences(rng, n, most)
+    step = Step(rng, kv, hd, ctx, new, t)
+    q, qv, (g, gv) = queries(rng, step, heads, t, True)
+    want, off = kv8_close.attention(step, qv, heads, gv)
+    call = Call(dev, buf, step, pool_of(dev, buf, step), heads, t, q, g)
+    got = call.attn()
+    assert_close(got, want, off, t)
+    assert np.array_equal(call.attn(), got)
+
+
+@pytest.mark.parametrize("n", [65, 150])
+@pytest.mark.parametrize("t,heads,kv,hd", [(F32, 6, 2, 64), (F16, 4, 1, 128)])
+def test_selection_of_many_sequences(dev, buf, n, t, heads, kv, hd):
+    rng = np.random.default_rng(n + hd)
+    ctx, new = sequences(rng, n, 3)
+    step = Step(rng, kv, hd, ctx, new, t)
+    q, qv, _ = queries(rng, step, heads, t)
+    call = Call(dev, buf, step, pool_of(dev, buf, step), heads, t, q)
+    for top in (5, 24):
+        picked = kv8.select(step, qv, heads, top, 1, 2 if top > 5 else 0)
+        sel, count = call.select(top, 1, 2 if top > 5 else 0)
+        for row in range(step.rows):
+            for h in range(kv):
+                assert sel[row, h].tolist() == picked[row][h] + [-1] * (top - len(picked[row][h])), (row, h)
+                assert count[row, h] == len(picked[row][h])
+        want, off = kv8_close.attention(step, qv, heads, None, picked)
+        assert_close(call.sparse(sel, count), want, off, t)
+
+
+def chosen(score, top, sinks, recent):
+    pages = np.arange(len(score))
+    forced = (pages < sinks) | (pages >= len(score) - recent)
+    return np.sort(np.lexsort((pages, -score, ~forced))[:top])
+
+
+@pytest.mark.parametrize("kind", ["spread", "crowded", "steps"])
+@pytest.mark.parametrize("pages", [5000, 9100])
+def test_selection_among_different_scores(dev, buf, kind, pages):
+    """Thousands of different scores, fewer and more than threads hold: spread over the bins that a round counts; nearly all
+    in one bin beside a few far out, so that its keys need a round of their own; and in steps of very different size."""
+    rng = np.random.default_rng(pages)
+    key = np.zeros((pages, 64))
+    channels = rng.integers(0, 450, (pages, 64))
+    if kind == "spread":
+        key[:] = channels
+    elif kind == "crowded":
+        # (the outliers make the range of scores' bits so wide that the others share a bin or two)
+        key[:] = 448
+        key[:, 48:] = 256 + 32 * (channels[:, 48:] % 7)
+        key[rng.choice(pages, 9, replace=False)] *= 2.0 ** 60
+        key[rng.choice(pages, 9, replace=False)] *= -1
+    else:
+        key[:] = channels * 2.0 ** rng.integers(-100, 100, (pages, 1))
+    k = key.repeat(PAGE, 0).astype(np.float32)
+    k[:, -1] = np.where(k[:, -1] == 0, k[:, 0], k[:, -1])
+    slots = np.arange(PAGE * pages, dtype=np.int32)
+    pool = GpuPool(dev, buf, 1, 64, pages)
+    pool.append(k, k, slots, F32)
+    q = np.abs(rng.normal(0, 1, (1, 64))).astype(np.float32)
+    # the definition, page by page at once: an exponent, codes, bounds in steps of 4, a sum of whole numbers
+    first = k[::PAGE].astype(float)
+    exps = np.array([kv8.holds(x) for x in np.abs(first).max(1)], float)
+    codes = kv8.round_e4m3(first * 2.0 ** -exps[:, None]) / 4
+    q8 = np.rint(q[0].astype(float) * 2.0 ** -kv8.holds(np.abs(q).max(), 127.0))
+    score = np.maximum(q8 * np.ceil(codes), q8 * np.floor(codes)).sum(1) * 2.0 ** exps
+    assert len(np.unique(score)) > 1024
+    table = rng.permutation(pages).astype(np.int32)
+    ptrs = [buf.up(a) for a in (q, np.int32([0, 1]), np.int32([pages * PAGE]), table)]
+    for top, sinks, recent in ((1, 0, 0), (40, 1, 2), (700, 0, 0), (2500, 5, 3), (pages - 1, 0, 1)):
+        sel, count = np.full(top, 9, np.int32), np.int32([9])
+        ps, pc = buf.up(sel), buf.up(count)
+        size = pool.pool.sparse_ws_bytes(1, 1, pages, top)
+        pool.pool.select_dev(1, ptrs[0], 64, F32, 1, *ptrs[1:], pages, 1, top, sinks, recent, ps, pc,
+                             buf.up(np.zeros(size, np.uint8)), size)
+        assert buf.down(pc, count)[0] == top
+        np.testing.assert_array_equal(buf.down(ps, sel), chosen(score[table], top, sinks, recent), err_msg=str(top))
