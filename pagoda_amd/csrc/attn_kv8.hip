@@ -320,10 +320,21 @@ struct State {
 #pragma unroll
     for (int i = 0; i < N; i++) by[i] = of_part(part(i)), l += sum_of_part(part(i));
   }
-  // From O to results; nothing attended gives zero.
-  __device__ float factor() const {
-    if (l == 0) return 0.0f;
-    return (m > -INFINITY ? __builtin_amdgcn_exp2f(mv - m - kWeightExp) : 1.0f) / l;
+  // O to results, x * by * 2^exp: the power of two may lie below the normal range where the result does not. Nothing
+  // attended gives zero.
+  struct Factor {
+    float by;
+    int exp;
+    __device__ f4 operator()(f4 x) const {
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = __builtin_ldexpf(x[i] * by, exp);
+      return x;
+    }
+  };
+  __device__ Factor factor() const {
+    if (l == 0) return Factor{0.0f, 0};
+    const float e = m > -INFINITY ? mv - m - kWeightExp : 0.0f, whole = floorf(e);
+    return Factor{__builtin_amdgcn_exp2f(e - whole) / l, (int)whole};
   }
 };
 
@@ -698,7 +709,8 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
   q.l = quads_sum(q.l);
   if (kq == 0) lds_st[wave][n16] = f4{q.m, q.mv, q.l, 0};
   State st;
-  float by[4], inv = 0;
+  State::Factor result{};
+  float by[4];
 #pragma unroll
   for (int t0 = 0; t0 < kTiles; t0 += kJoinTiles) {
     __syncthreads();
@@ -707,7 +719,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     __syncthreads();
     if (t0 == 0) {
       st.join<4>([&](int w) { return lds_st[w][n16]; }, by);
-      inv = st.factor();
+      result = st.factor();
       if (live && slot >= 0 && slot < INT_MAX && wave == 0 && kq == 0) part.st[(int64_t)slot * 16 + n16] = f4{st.m, st.mv, st.l, 0};
     }
     if (live) {
@@ -720,7 +732,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
         const int d = (t0 + i) * 16 + kq * 4;
         if (slot == INT_MAX) continue;
         if (slot >= 0) *reinterpret_cast<f4*>(part.o + ((int64_t)slot * 16 + n16) * HD + d) = v;
-        else store4<T>(out, row, col + d, v * inv);
+        else store4<T>(out, row, col + d, result(v));
       }
     }
   }
@@ -915,9 +927,9 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out,
     st.m = q.m;
     st.mv = q.mv;
     st.l = l;
-    const float inv = st.factor();
+    const State::Factor result = st.factor();
 #pragma unroll
-    for (int i = 0; i < kTiles; i++) store4<T>(out, row, col + i * 16 + kq * 4, o[i] * inv);
+    for (int i = 0; i < kTiles; i++) store4<T>(out, row, col + i * 16 + kq * 4, result(o[i]));
   }
 }
 
@@ -999,7 +1011,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Rows r, Out out, List list, 
 #pragma unroll
     for (int w = 1; w < 4; w++) j.l += lds_st[w][0];
   }
-  if (lane < kLanes) store4<T>(out, row, (int64_t)h * HD + lane * 4, x * j.factor());
+  if (lane < kLanes) store4<T>(out, row, (int64_t)h * HD + lane * 4, j.factor()(x));
 }
 
 // ---- launches ---------------------------------------------------------------------------

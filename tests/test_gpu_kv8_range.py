@@ -64,3 +64,20 @@ def test_results_are_the_definitions_rounded(dev, buf, t, form, heads, kv, hd):
     step = Step(rng, kv, hd, ctx, new, t)
     q, qv, gate = queries(rng, step, heads, t, hd == 128)
     check(dev, buf, rng, step, heads, t, q, qv, form, gate)
+
+
+# ---- the ends of the range -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("power", [-110, -118, -125])
+def test_the_smallest_values(dev, buf, t, form, power):
+    """Values whose pages have the lowest exponents come out as themselves."""
+    rng = np.random.default_rng(-power)
+    ctx, new = FORMS[form]
+    step = Step(rng, 2, 64, ctx, new, t)
+    with_rows(step, v=(rng.normal(0, 1, (len(step.slots), 128)) * 2.0 ** power).astype(np.float32))
+    q, qv, _ = queries(rng, step, 6, t)
+    got, want = check(dev, buf, rng, step, 6, t, q, qv, form)
+    assert np.abs(got).max() > 2.0 ** (power - 3)
