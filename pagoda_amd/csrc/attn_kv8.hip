@@ -403,13 +403,26 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
                              h8 (&out)[PG / 2][kWeightTerms]) {
   const int kq = threadIdx.x >> 4 & 3;
   float x[PG][4], by[PG], ev[PG];
+  int highest = INT_MIN;
 #pragma unroll
   for (int w = 0; w < PG; w++) {
     // (not below the normal range: the scores of masked positions are infinite)
     by[w] = fmaxf(__builtin_ldexpf(scale, q.exp + Meta::ek(pg[w].meta)), 1.17549435e-38f);
     ev[w] = (float)Meta::ev(pg[w].meta);
+    highest = max(highest, Meta::ek(pg[w].meta));
 #pragma unroll
     for (int i = 0; i < 4; i++) x[w][i] = s[w][i];
+  }
+  if (__any(q.exp + highest > 126)) {
+    // not above it either, where keys and queries that have no channel in common may be: a power of two goes to the
+    // product first
+#pragma unroll
+    for (int w = 0; w < PG; w++) {
+      const int exp = q.exp + Meta::ek(pg[w].meta), over = max(exp - 126, 0);
+      if (over > 0) by[w] = __builtin_ldexpf(scale, 126);
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[w][i] = __builtin_ldexpf(x[w][i], over);
+    }
   }
   if (!whole) {
 #pragma unroll

@@ -81,3 +81,23 @@ def test_the_smallest_values(dev, buf, t, form, power):
     q, qv, _ = queries(rng, step, 6, t)
     got, want = check(dev, buf, rng, step, 6, t, q, qv, form)
     assert np.abs(got).max() > 2.0 ** (power - 3)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_scores_of_large_queries_and_keys(dev, buf, t, form):
+    """Queries of 2^100 beside keys of 2^60 that they have no channel in common with, and beside keys of 2^-100 that
+    they do: all scores are small."""
+    rng = np.random.default_rng(12)
+    ctx, new = FORMS[form]
+    heads, kv, hd = 6, 2, 64
+    step = Step(rng, kv, hd, ctx, new, t)
+    k = np.zeros((len(step.slots), kv, hd), np.float32)
+    low = np.arange(len(k)) // PAGE % 2 == 0
+    k[low, :, 0] = rng.normal(0, 1, (low.sum(), kv)) * 2.0 ** -98
+    k[~low, :, 1:] = rng.normal(0, 1, ((~low).sum(), kv, hd - 1)) * 2.0 ** 60
+    with_rows(step, k=k.reshape(len(k), -1))
+    q = np.zeros((step.rows, heads, hd), np.float32)
+    q[..., 0] = rng.normal(0, 1, (step.rows, heads)) * 2.0 ** 100
+    q, qv = typed(q.reshape(step.rows, -1), t)
+    check(dev, buf, rng, step, heads, t, q, qv.reshape(-1, heads, hd), form)
