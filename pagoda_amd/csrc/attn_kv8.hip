@@ -6,18 +6,20 @@
 // Per two pages (32 positions) and a tile of 16 queries (rows x group heads):
 //   S[pos][query]  = K codes . q        16x16x32 f16 products over hd / 32 steps
 //   t = S 2^ek log2(e) / sqrt(hd), its running maximum m and the sum l of 2^(t - m) in f32
-//   O[dim][query] += V codes^T . 2^(t + ev - M)   the same products over the 32 positions
-// with M the running maximum of t + ev, so that the largest weight of a value's code is
-// about one whatever the pages' powers of two (both maxima may lag a factor of 2^4 behind).
+//   O[dim][query] += V codes^T . 2^(t - m + ev - d)   the same products over the 32 positions
+// with d the running maximum of t - m + ev, rounded up, so that the largest weight of a value's code is
+// about one whatever the pages' powers of two (both maxima may lag behind, m a factor of 2^4 and d one of 2^3). d is a
+// whole number near the pages' exponents: adding them to it and taking it back from results is exact, also where
+// scores are so large that t + ev would not be.
 // Codes convert to f16 exactly. Queries are scaled by a power of two into f16's range and enter as f16 terms: f32
 // rows two (22 bits and at least 2^-40 of the row's largest), f16 rows themselves, bf16 rows one (exact to 2^-40 of the
-// largest). The weights, times 2^11, enter as two terms, 2^-21 and 2^-36 of the largest (bf16 rows: one; its
+// largest). The weights, times 2^12, enter as two terms, 2^-21 and 2^-36 of the largest (bf16 rows: one; its
 // 2^-11 is an eighth of their own rounding). bf16 terms would need no scaling but half as many more
 // products: three for f32 where f16 takes two.
 // The lane that holds a score holds it as the operand of the second product: lane
 // (query n = l % 16, kq = l / 16) has positions 4 kq .. 4 kq + 3 of both pages, which
 // are the 8 that a lane of the second product's operand takes, and its results are
-// columns n too, so m, M, l and the rescaling stay in the lane but for two maxima
+// columns n too, so m, d, l and the rescaling stay in the lane but for two maxima
 // over the four kq.
 //
 // Split: work is a list of (sequence, chunk of pages, KV head, tile of queries) that every
@@ -58,9 +60,10 @@ constexpr int kFewQueries = 128;
 template <int T>
 constexpr int kTerms = T == F32 ? 2 : 1;  // f16 terms of a query
 constexpr int kWeightTerms = 2;
-// O and the sum are only brought to new maxima that are 2^kSlack times the old ones or more (and all of a wave's
-// with them), so weights reach 2^kSlack. They enter times 2^kWeightExp: f16 holds 2^-24 to 65504.
-constexpr float kSlack = 4, kWeightExp = 15 - kSlack;
+// O and the sum are only brought to new maxima that are 2^kSlack (of weights) or 2^kSlackV (of weights of codes) times
+// the old ones or more (and all of a wave's with them), so weights of codes reach 2^kSlackV. They enter times
+// 2^kWeightExp: f16 holds 2^-24 to 65504.
+constexpr float kSlack = 4, kSlackV = 3, kWeightExp = 15 - kSlackV;
 
 // x as f16 terms to nearest, each of what the ones before leave.
 template <int N>
@@ -292,7 +295,7 @@ struct RowPart {
 };
 
 // Workspace: RowPart of every row, then per slot (16 queries of a chunk and head) O [16][hd], then their
-// (m, M, l).
+// (m, d, l).
 struct Partials {
   RowPart* rows;
   float* o;
@@ -309,14 +312,18 @@ __device__ __host__ inline Partials partials_at(void* ws, int rows, int slots) {
 
 // What several runs over parts of a context leave, joined: maxima and the sum.
 struct State {
-  float m = -INFINITY, mv = -INFINITY, l = 0;
+  float m = -INFINITY, d = -INFINITY, l = 0;
+  // d of a part, from m on (-infinity of one that attended nothing).
+  __device__ float level(f4 s) const { return s[0] > -INFINITY ? ceilf(s[0] - m + s[1]) : -INFINITY; }
   // The factor of a part's O (a part that attended nothing has zeros, or NaN, to keep).
-  __device__ float of_part(f4 s) const { return s[1] > -INFINITY ? __builtin_amdgcn_exp2f(s[1] - mv) : 1.0f; }
+  __device__ float of_part(f4 s) const { return s[0] > -INFINITY ? __builtin_amdgcn_exp2f((s[0] - m) + (s[1] - d)) : 1.0f; }
   __device__ float sum_of_part(f4 s) const { return (s[0] > -INFINITY ? __builtin_amdgcn_exp2f(s[0] - m) : 1.0f) * s[2]; }
   template <int N, class F>
   __device__ void join(F part, float (&by)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; i++) m = fmaxf(m, part(i)[0]), mv = fmaxf(mv, part(i)[1]);
+    for (int i = 0; i < N; i++) m = fmaxf(m, part(i)[0]);
+#pragma unroll
+    for (int i = 0; i < N; i++) d = fmaxf(d, level(part(i)));
 #pragma unroll
     for (int i = 0; i < N; i++) by[i] = of_part(part(i)), l += sum_of_part(part(i));
   }
@@ -333,8 +340,7 @@ struct State {
   };
   __device__ Factor factor() const {
     if (l == 0) return Factor{0.0f, 0};
-    const float e = m > -INFINITY ? mv - m - kWeightExp : 0.0f, whole = floorf(e);
-    return Factor{__builtin_amdgcn_exp2f(e - whole) / l, (int)whole};
+    return Factor{1.0f / l, d > -INFINITY ? (int)(d - kWeightExp) : 0};
   }
 };
 
@@ -393,7 +399,7 @@ struct PoolAt {
 
 // A query's running maxima, sum (of this lane's positions) and scaling, as its column of lanes holds them.
 struct Query {
-  float m = -INFINITY, mv = -INFINITY, l = 0;
+  float m = -INFINITY, d = -INFINITY, l = 0;
   int exp = 0, lim = 0;  // power of two of its terms; positions it sees
 };
 
@@ -437,44 +443,62 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
       }
     }
   }
-  float top = -INFINITY, top_v = -INFINITY;
+  // This lane's largest t and t - m + ev. What its column's other lanes have need not be known while no lane of the
+  // wave is past what its column's maxima may lag.
+  float t[PG], top = -INFINITY, top_v = -INFINITY;
 #pragma unroll
   for (int w = 0; w < PG; w++) {
-    const float t = fmaxf(fmaxf(x[w][0], x[w][1]), fmaxf(x[w][2], x[w][3])) * by[w];
-    top = fmaxf(top, t);
-    top_v = fmaxf(top_v, t + ev[w]);
+    t[w] = fmaxf(fmaxf(x[w][0], x[w][1]), fmaxf(x[w][2], x[w][3])) * by[w];
+    top = fmaxf(top, t[w]);
+    top_v = fmaxf(top_v, t[w] - q.m + ev[w]);
   }
-  top = quads_max(top);
-  top_v = quads_max(top_v);
-  if (__any(top > q.m + kSlack || top_v > q.mv + kSlack)) {
-    top = fmaxf(q.m, top);
-    top_v = fmaxf(q.mv, top_v);
-    q.l *= top > q.m ? __builtin_amdgcn_exp2f(q.m - top) : 1.0f;
-    const float down = top_v > q.mv ? __builtin_amdgcn_exp2f(q.mv - top_v) : 1.0f;
+  if (__any(top > q.m + kSlack || top_v > q.d + kSlackV)) {
+    const float m = fmaxf(q.m, quads_max(top)), base = m > -INFINITY ? m : 0.0f;
+    top_v = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; i++) o[i] *= down;
-    q.m = top;
-    q.mv = top_v;
+    for (int w = 0; w < PG; w++) top_v = fmaxf(top_v, t[w] - base + ev[w]);
+    const float d = ceilf(fmaxf(quads_max(top_v), q.d + (q.m - base)));
+    if (q.m > -INFINITY) {  // (else O holds zeros, or NaN)
+      q.l *= __builtin_amdgcn_exp2f(q.m - base);
+      const float down = __builtin_amdgcn_exp2f((q.m - base) + (q.d - d));
+#pragma unroll
+      for (int i = 0; i < N; i++) o[i] *= down;
+    }
+    q.m = m;
+    q.d = d;
   }
-  const float at = q.m > -INFINITY ? q.m : 0.0f, at_v = q.m > -INFINITY ? q.mv - kWeightExp : 0.0f;
+  const float at = q.m > -INFINITY ? q.m : 0.0f, up = q.d > -INFINITY ? kWeightExp - q.d : 0.0f;
+  if (__any(fabsf(at) > 65536.0f)) {
+    // m is a rounded product: an exact one would lie past it by up to its half step, which may be many powers of two
+#pragma unroll
+    for (int w = 0; w < PG; w++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[w][i] *= by[w];
+      by[w] = 1.0f;
+    }
+  }
   float far = -INFINITY, sum[PG];
 #pragma unroll
   for (int w = 0; w < PG; w++) far = fmaxf(far, ev[w]);
-  const bool apart = __any(at - at_v + far > 100.0f);
+  const bool apart = __any(up + far > 100.0f);
 #pragma unroll
   for (int w = 0; w < PG; w++) {
     float e[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[w][i], by[w], -at));
-    sum[w] = (e[0] + e[1]) + (e[2] + e[3]);
+    for (int i = 0; i < 4; i++) e[i] = __builtin_fmaf(x[w][i], by[w], -at);
+    const float f = up + ev[w];
     if (apart) {
       // pages so far apart that 2^(t - m) underflows where the weight does not
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[w][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[w][i], by[w], ev[w] - at_v));
-    } else {
-      const float f = __builtin_amdgcn_exp2f(at - at_v + ev[w]);
+      for (int i = 0; i < 4; i++) x[w][i] = __builtin_amdgcn_exp2f(e[i] + f);
+    }
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[w][i] = e[i] * f;
+    for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(e[i]);
+    sum[w] = (e[0] + e[1]) + (e[2] + e[3]);
+    if (!apart) {
+      const float of_code = __builtin_amdgcn_exp2f(f);
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[w][i] = e[i] * of_code;
     }
   }
 #pragma unroll
@@ -720,7 +744,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
 
   // the four waves' states, joined in wave order
   q.l = quads_sum(q.l);
-  if (kq == 0) lds_st[wave][n16] = f4{q.m, q.mv, q.l, 0};
+  if (kq == 0) lds_st[wave][n16] = f4{q.m, q.d, q.l, 0};
   State st;
   State::Factor result{};
   float by[4];
@@ -733,7 +757,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     if (t0 == 0) {
       st.join<4>([&](int w) { return lds_st[w][n16]; }, by);
       result = st.factor();
-      if (live && slot >= 0 && slot < INT_MAX && wave == 0 && kq == 0) part.st[(int64_t)slot * 16 + n16] = f4{st.m, st.mv, st.l, 0};
+      if (live && slot >= 0 && slot < INT_MAX && wave == 0 && kq == 0) part.st[(int64_t)slot * 16 + n16] = f4{st.m, st.d, st.l, 0};
     }
     if (live) {
       const int row = s.row0 + qi / group, col = (head * group + qi % group) * HD;
@@ -932,13 +956,13 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out,
   if (have > 1) {
     const int64_t slot = slots.first + f.slot + ((int64_t)c * kv_heads + head) * cl.tiles16(s.n) + qi / 16;
     if (slot >= slots.end) return;
-    if (kq == 0) part.st[slot * 16 + n16] = f4{q.m, q.mv, l, 0};
+    if (kq == 0) part.st[slot * 16 + n16] = f4{q.m, q.d, l, 0};
 #pragma unroll
     for (int i = 0; i < kTiles; i++) *reinterpret_cast<f4*>(part.o + (slot * 16 + n16) * HD + i * 16 + kq * 4) = o[i];
   } else {
     State st;
     st.m = q.m;
-    st.mv = q.mv;
+    st.d = q.d;
     st.l = l;
     const State::Factor result = st.factor();
 #pragma unroll
@@ -992,13 +1016,13 @@ __global__ __launch_bounds__(256) void merge_kernel(Rows r, Out out, List list, 
   q &= 15;
   State j;
   auto state_of = [&](int c) { return part.st[(slot + c * step) * 16 + q]; };
-  for (int c = lane; c < chunks; c += 64) {
-    const f4 st = state_of(c);
-    j.m = fmaxf(j.m, st[0]);
-    j.mv = fmaxf(j.mv, st[1]);
-  }
+  const f4 own = lane < chunks ? state_of(lane) : f4{-INFINITY, -INFINITY, 0, 0};
+  j.m = own[0];
+  for (int c = lane + 64; c < chunks; c += 64) j.m = fmaxf(j.m, state_of(c)[0]);
   j.m = lanes_max<64>(j.m);
-  j.mv = lanes_max<64>(j.mv);
+  j.d = j.level(own);
+  for (int c = lane + 64; c < chunks; c += 64) j.d = fmaxf(j.d, j.level(state_of(c)));
+  j.d = lanes_max<64>(j.d);
   f4 x{0, 0, 0, 0};
 #pragma unroll 8
   for (int c = first; c < chunks; c += kParts) {

@@ -101,3 +101,45 @@ def test_scores_of_large_queries_and_keys(dev, buf, t, form):
     q[..., 0] = rng.normal(0, 1, (step.rows, heads)) * 2.0 ** 100
     q, qv = typed(q.reshape(step.rows, -1), t)
     check(dev, buf, rng, step, heads, t, q, qv.reshape(-1, heads, hd), form)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [16, 23, 26, 30, 60])
+def test_scores_past_whole_numbers(dev, buf, t, form, power, sign):
+    """Scores of about 2^power, all of one sign: nothing but the largest one's value is taken, whatever the spacing of
+    f32 numbers there, from pages of different exponents."""
+    rng = np.random.default_rng(power)
+    ctx, new = FORMS[form]
+    heads, kv, hd = 6, 2, 64
+    step = Step(rng, kv, hd, ctx, new, t)
+    n = len(step.slots)
+    size = 2.0 ** rng.integers(-30, 30, n).repeat(PAGE)[:n, None]
+    k = np.exp(rng.normal(0, 1, (n, 1)) + rng.normal(0, 0.1, (n, kv * hd)))
+    with_rows(step, k=k.astype(np.float32), v=(rng.normal(0, 1, (n, kv * hd)) * size).astype(np.float32))
+    q, qv = typed(np.abs(rng.normal(0, 1, (step.rows, heads * hd))) * sign * 2.0 ** (power - 3), t)
+    check(dev, buf, rng, step, heads, t, q, qv.reshape(-1, heads, hd), form)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("power", [0, 16, 24, 27, 31])
+def test_equal_scores_past_whole_numbers(dev, buf, form, power):
+    """Positions of one key, whatever its score: the mean of their values, which lie in pages of very different
+    exponents."""
+    rng = np.random.default_rng(power + 1)
+    ctx, new = FORMS[form]
+    heads, kv, hd = 4, 1, 64
+    step = Step(rng, kv, hd, ctx, new, F32)
+    n = len(step.slots)
+    key = np.abs(rng.normal(0, 1, (1, hd))) * 2.0 ** (power / 2)
+    size = 2.0 ** rng.integers(-60, 60, n).repeat(PAGE)[:n, None]
+    with_rows(step, k=np.repeat(key, n, 0).astype(np.float32), v=(rng.uniform(1, 2, (n, hd)) * size).astype(np.float32))
+    for sign in (1, -1):
+        q = (np.abs(rng.normal(0, 1, (step.rows, heads * hd))) * sign * 2.0 ** (power / 2)).astype(np.float32)
+        got = run(dev, buf, step, heads, F32, q, form=form)
+        v = step.cache.values(1)
+        for row, s, seen in step.each_row():
+            want = v[step.tables[s, :kv8.pages(seen)], 0].reshape(-1, hd)[:seen].mean(0)
+            # (all values are positive: sums of n of them, and terms of the weights)
+            assert (np.abs(got[row] - want) <= want * ((2 * seen + 16) * 2.0 ** -23 + 2.0 ** -20)).all()
