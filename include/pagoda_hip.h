@@ -313,7 +313,8 @@ int pgd_attn_kv8_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
  * append keeps them): score = 2^(key exponent) max over the group's heads of
  * sum(max(q8 hi, q8 lo)), exact in f32 (an infinity from 2^128 on); ties go to the lower page. A page outside the pool scores
  * lowest. Rows of no sequence are left as they were; a row that attends to nothing selects nothing.
- * ws as above, of pgd_kv8_sparse_ws_bytes bytes, which serves both calls, one after the other. */
+ * ws as above, of pgd_kv8_sparse_ws_bytes bytes, which serves both calls, one after the other, and those of fewer rows,
+ * narrower tables and lower top too. */
 size_t pgd_kv8_sparse_ws_bytes(int heads, int kv_heads, int head_dim, int rows, int max_blocks, int top);
 int pgd_kv8_select_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, int head_dim, int heads,
                        const void* q, int ldq, int type, int nseq, const int* row_start, const int* lens,

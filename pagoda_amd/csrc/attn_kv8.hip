@@ -1165,6 +1165,15 @@ size_t attn_sparse_ws_bytes(const Layout& at, int heads, int rows, int top) {
   return partial_bytes(at, (int64_t)rows * at.kv_heads * ((heads / at.kv_heads + 15) / 16) * chunks);
 }
 
+// Lists are cut only while there are fewer of them than items, then into at most top / c + 1 chunks of c pages, whose
+// top / c is at most items over lists; and no chunk is shorter than the least.
+size_t attn_sparse_ws_most(const Layout& at, int heads, int rows, int top) {
+  if (top <= kOneChunk) return 0;
+  const int64_t items = few_items(at.hd, 1), lists = (int64_t)rows * at.kv_heads * ((heads / at.kv_heads + 15) / 16),
+                cut = std::min(lists, items - 1), per = (top + least_chunk(top) - 1) / least_chunk(top);
+  return partial_bytes(at, std::min(cut * per, items + cut));
+}
+
 void attn_sparse(const Pool& p, const Rows& r, int top, const int* sel, const int* count, const Out& o, void* ws,
                  hipStream_t s) {
   const int c = sparse_chunk(p.at, r.heads, r.rows, top), chunks = (top + c - 1) / c;

@@ -96,7 +96,9 @@ void attn(const Pool& p, const Rows& r, int max_rows, const Out& o, void* ws, hi
 size_t select_ws_bytes(const Layout& at, int rows, int max_blocks);
 void select(const Pool& p, const Rows& r, int top, int sinks, int recent, int* sel, int* count, void* ws, hipStream_t s);
 
+// What a call needs, and the most that one of these or any smaller numbers of rows and pages needs.
 size_t attn_sparse_ws_bytes(const Layout& at, int heads, int rows, int top);
+size_t attn_sparse_ws_most(const Layout& at, int heads, int rows, int top);
 void attn_sparse(const Pool& p, const Rows& r, int top, const int* sel, const int* count, const Out& o, void* ws,
                  hipStream_t s);
 

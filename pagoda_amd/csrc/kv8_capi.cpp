@@ -79,7 +79,7 @@ void check_list(const Layout& at, int heads, int rows, int max_blocks, int top) 
 }
 
 size_t sparse_ws(const Layout& at, int heads, int rows, int max_blocks, int top) {
-  const size_t a = select_ws_bytes(at, rows, max_blocks), b = attn_sparse_ws_bytes(at, heads, rows, top);
+  const size_t a = select_ws_bytes(at, rows, max_blocks), b = attn_sparse_ws_most(at, heads, rows, top);
   return a > b ? a : b;
 }
 

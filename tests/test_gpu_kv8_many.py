@@ -104,3 +104,21 @@ def test_selection_among_different_scores(dev, buf, kind, pages):
                              buf.up(np.zeros(size, np.uint8)), size)
         assert buf.down(pc, count)[0] == top
         np.testing.assert_array_equal(buf.down(ps, sel), chosen(score[table], top, sinks, recent), err_msg=str(top))
+
+
+def test_a_workspace_of_the_largest_step_serves_smaller_ones(dev, buf):
+    rng = np.random.default_rng(70)
+    heads, kv, hd, top = 24, 4, 64, 128
+    width = 140
+    for rows in (1, 20, 96):
+        step = Step(rng, kv, hd, [width * PAGE] if rows < 20 else [2100, 40], [rows] if rows < 20 else [1, rows - 1], F16)
+        q, qv, _ = queries(rng, step, heads, F16)
+        pool = pool_of(dev, buf, step)
+        call = Call(dev, buf, step, pool, heads, F16, q)
+        size = max(pool.pool.sparse_ws_bytes(heads, 256, width + 9, t) for t in (top, top + 9))
+        call.workspace = lambda t: (buf.up(np.full(size, 0xFF, np.uint8)), size)
+        picked = kv8.select(step, qv, heads, top, 0, 1)
+        sel, count = call.select(top, 0, 1)
+        assert all(sel[r, h, :count[r, h]].tolist() == picked[r][h] for r in range(rows) for h in range(kv))
+        want, off = kv8_close.attention(step, qv, heads, None, picked)
+        assert_close(call.sparse(sel, count), want, off, F16)
