@@ -295,10 +295,13 @@ int pgd_kv8_read_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
  * softmax weights to 2^-21, nothing finer than 2^-36 of the largest. A score of magnitude 2^127 and more is an
  * infinity: a row with a positive one is NaN, one whose scores are all negative ones gets zeros. max_rows: the largest
  * number of rows of a sequence, or any bound on it (it selects kernels, results are
- * right with any value). row_start ascends. ws: pgd_attn_kv8_ws_bytes bytes (0 of sizes that the call refuses) that no
- * other stream uses meanwhile (a captured graph's included); its contents do not matter. The order of the sums
- * depends on the sizes, max_rows, row_start and lens, on nothing else. */
+ * right with any value). row_start ascends. ws: pgd_attn_kv8_rows_ws_bytes bytes, or pgd_attn_kv8_ws_bytes for any
+ * max_rows (0 of sizes that the call refuses), that no other stream uses meanwhile (a captured graph's included); its
+ * contents do not matter, and one that is large enough for a call is for every call of smaller numbers. The order of the
+ * sums depends on the sizes, max_rows, row_start and lens, on nothing else. */
 size_t pgd_attn_kv8_ws_bytes(int heads, int kv_heads, int head_dim, int nseq, int max_blocks, int rows);
+size_t pgd_attn_kv8_rows_ws_bytes(int heads, int kv_heads, int head_dim, int nseq, int max_blocks, int rows,
+                                  int max_rows);
 int pgd_attn_kv8_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, int head_dim, int heads, const void* q,
                      int ldq, int type, int nseq, const int* row_start, const int* lens, const int* block_tables,
                      int max_blocks, int rows, int max_rows, void* out, int ldo, const void* gate, int ldg, void* ws,

@@ -62,6 +62,7 @@ SIGNATURES: dict[str, tuple] = {
     "pgd_kv8_read_dev": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                  c_int]),
     "pgd_attn_kv8_ws_bytes": (c_size_t, [c_int] * 6),
+    "pgd_attn_kv8_rows_ws_bytes": (c_size_t, [c_int] * 7),
     "pgd_attn_kv8_dev": (c_int, [c_void_p, c_void_p] + [c_int] * 4 + [c_void_p, c_int, c_int, c_int] + [c_void_p] * 3 +
                          [c_int] * 3 + [c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t]),
     "pgd_kv8_sparse_ws_bytes": (c_size_t, [c_int] * 6),

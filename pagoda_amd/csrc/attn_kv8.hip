@@ -1128,11 +1128,12 @@ size_t partial_bytes(const Layout& at, int64_t slots) { return (size_t)slots * 1
 
 }  // namespace
 
-size_t attn_ws_bytes(const Layout& at, int heads, int nseq, int max_blocks, int rows) {
-  // whatever max_rows the call will name
+size_t attn_ws_bytes(const Layout& at, int heads, int nseq, int max_blocks, int rows, int max_rows) {
+  // the plans of all numbers up to max_rows
+  const int group = heads / at.kv_heads, most = std::min(max_rows, rows);
   int64_t slots = 0;
-  for (int64_t max_rows : {(int64_t)0, (int64_t)kFewQueries / (heads / at.kv_heads), (int64_t)rows + kFewQueries}) {
-    const Plan p = plan_of(at.hd, heads / at.kv_heads, max_rows);
+  for (int n : {0, std::min(kFewQueries / group, most), most}) {
+    const Plan p = plan_of(at.hd, group, n);
     slots = std::max(slots, grid_of(at, heads, nseq, max_blocks, rows, p.few).slots +
                                 (p.both ? grid_of(at, heads, nseq, max_blocks, rows, p.many).slots : 0));
   }
@@ -1140,7 +1141,7 @@ size_t attn_ws_bytes(const Layout& at, int heads, int nseq, int max_blocks, int 
 }
 
 void attn(const Pool& p, const Rows& r, int max_rows, const Out& o, void* ws, hipStream_t s) {
-  const Plan pl = plan_of(p.at.hd, r.heads / p.at.kv_heads, max_rows);
+  const Plan pl = plan_of(p.at.hd, r.heads / p.at.kv_heads, std::min(max_rows, r.rows));
   const Grid few = grid_of(p.at, r.heads, r.nseq, r.max_blocks, r.rows, pl.few);
   const Grid many = pl.both ? grid_of(p.at, r.heads, r.nseq, r.max_blocks, r.rows, pl.many) : Grid{};
   const int all = (int)(few.slots + many.slots);

@@ -90,7 +90,8 @@ struct Out {
   int64_t ldg;
 };
 
-size_t attn_ws_bytes(const Layout& at, int heads, int nseq, int max_blocks, int rows);
+// The most that a call of these or any smaller numbers needs.
+size_t attn_ws_bytes(const Layout& at, int heads, int nseq, int max_blocks, int rows, int max_rows);
 void attn(const Pool& p, const Rows& r, int max_rows, const Out& o, void* ws, hipStream_t s);
 
 size_t select_ws_bytes(const Layout& at, int rows, int max_blocks);

@@ -1,6 +1,8 @@
 // kv8_capi.cpp — C entry points of the 8-bit paged KV cache: argument checks, then the launches.
 #include "../../include/pagoda_hip.h"
 
+#include <algorithm>
+
 #include "device.h"
 #include "kv8.h"
 
@@ -150,10 +152,16 @@ int pgd_kv8_read_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
 }
 
 size_t pgd_attn_kv8_ws_bytes(int heads, int kv_heads, int head_dim, int nseq, int max_blocks, int rows) {
+  return pgd_attn_kv8_rows_ws_bytes(heads, kv_heads, head_dim, nseq, max_blocks, rows, std::max(rows, 0));
+}
+
+size_t pgd_attn_kv8_rows_ws_bytes(int heads, int kv_heads, int head_dim, int nseq, int max_blocks, int rows,
+                                  int max_rows) {
   return bytes_or_zero([&] {
     const Layout at = pool_of(reinterpret_cast<void*>(16), 1, kv_heads, head_dim).at;
     check_sizes(at, heads, nseq, max_blocks, rows);
-    return attn_ws_bytes(at, heads, nseq, max_blocks, rows);
+    PGD_CHECK(max_rows >= 0, kErrArg, "max_rows must not be negative");
+    return attn_ws_bytes(at, heads, nseq, max_blocks, rows, max_rows);
   });
 }
 
@@ -168,7 +176,7 @@ int pgd_attn_kv8_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
     PGD_CHECK(max_rows >= 0, kErrArg, "max_rows must not be negative");
     if (rows == 0 || nseq == 0) return;
     const Out o = out_of(r, p.at, out, ldo, gate, ldg);
-    check_ws(ws, ws_bytes, attn_ws_bytes(p.at, heads, nseq, max_blocks, rows));
+    check_ws(ws, ws_bytes, attn_ws_bytes(p.at, heads, nseq, max_blocks, rows, max_rows));
     DeviceScope scope(dev);
     attn(p, r, max_rows, o, ws, dev->stream);
   });

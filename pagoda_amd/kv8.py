@@ -65,8 +65,10 @@ class Kv8Pool:
         call("pgd_kv8_read_dev", *self._pool(), index(slots_ptr or 0), rows, index(k_ptr or 0), ldk, index(v_ptr or 0),
              ldv)
 
-    def attn_ws_bytes(self, heads: int, nseq: int, max_blocks: int, rows: int) -> int:
-        return int(lib().pgd_attn_kv8_ws_bytes(heads, self.kv_heads, self.head_dim, nseq, max_blocks, rows))
+    def attn_ws_bytes(self, heads: int, nseq: int, max_blocks: int, rows: int, max_rows: int | None = None) -> int:
+        """Workspace of attn_dev for calls of up to these numbers (max_rows None: whatever the call will say)."""
+        return int(lib().pgd_attn_kv8_rows_ws_bytes(heads, self.kv_heads, self.head_dim, nseq, max_blocks, rows,
+                                                    max(rows, 0) if max_rows is None else max_rows))
 
     def attn_dev(self, heads: int, q_ptr: int, ldq: int, x_type: int, nseq: int, row_start_ptr: int, lens_ptr: int,
                  tables_ptr: int, max_blocks: int, rows: int, max_rows: int, out_ptr: int, ldo: int, ws_ptr: int,

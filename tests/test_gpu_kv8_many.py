@@ -122,3 +122,24 @@ def test_a_workspace_of_the_largest_step_serves_smaller_ones(dev, buf):
         assert all(sel[r, h, :count[r, h]].tolist() == picked[r][h] for r in range(rows) for h in range(kv))
         want, off = kv8_close.attention(step, qv, heads, None, picked)
         assert_close(call.sparse(sel, count), want, off, F16)
+
+
+@pytest.mark.parametrize("t,heads,kv,hd", [(F32, 24, 4, 256), (BF16, 28, 4, 128), (F16, 14, 2, 64)])
+@pytest.mark.parametrize("ctx,new", [([6000, 300], [1, 1]), ([3000, 40], [4, 2]), ([2500, 300], [40, 1]), ([9000], [1])])
+def test_attention_stays_in_its_workspace(dev, buf, t, heads, kv, hd, ctx, new):
+    """Of the size that the call's largest number of rows needs, with the bytes behind it left as they were."""
+    rng = np.random.default_rng(ctx[0] + hd)
+    step = Step(rng, kv, hd, ctx, new, t)
+    q, qv, _ = queries(rng, step, heads, t)
+    call = Call(dev, buf, step, pool_of(dev, buf, step), heads, t, q)
+    p = call.pool.pool
+    rows = sorted({0, step.rows - 1} | set(rng.choice(step.rows, min(step.rows, 9), replace=False)))
+    want, off = kv8_close.attention(step, qv, heads, rows=rows)
+    for most in (max(new), 1):
+        size = p.attn_ws_bytes(heads, len(ctx), step.width, step.rows, most)
+        assert size <= p.attn_ws_bytes(heads, len(ctx), step.width, step.rows)
+        whole = np.full(size + 65536, 0xFF, np.uint8)
+        ws = buf.up(whole)
+        p.attn_dev(*call.args(), most, call.out, call.fresh.shape[1], ws, size)
+        assert_close(call.result()[rows], want[rows], off[rows], t)
+        assert (buf.down(ws, whole)[size:] == 0xFF).all()

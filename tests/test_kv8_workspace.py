@@ -32,3 +32,27 @@ def test_lists(heads, kv, hd):
             never_falls(lambda b: size(rows, b, top), BLOCKS)
     # the scores, and partial sums of at most twice as many pieces of lists as run at once
     assert size(32, 600, 128) <= max(32 * kv * 600 * 4, 2 * 1024 * 16 * (hd + 4) * 4)
+
+
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+def test_attention(heads, kv, hd):
+    size = lambda nseq, blocks, rows, most: lib().pgd_attn_kv8_rows_ws_bytes(heads, kv, hd, nseq, blocks, rows, most)
+    for nseq, blocks in ((1, 100), (7, 600), (64, 8200)):
+        for most in (0, 1, 3, 22, 100, 5000):
+            never_falls(lambda r: size(nseq, blocks, r, most), ROWS)
+        for rows in ROWS:
+            never_falls(lambda m: size(nseq, blocks, rows, m), [0] + ROWS)
+            assert size(nseq, blocks, rows, rows) == size(nseq, blocks, rows, 2 ** 31 - 1)
+            assert size(nseq, blocks, rows, rows) == lib().pgd_attn_kv8_ws_bytes(heads, kv, hd, nseq, blocks, rows)
+    for rows in ROWS:
+        never_falls(lambda n: size(n, 600, rows, 4), [1, 2, 31, 32, 33, 64, 65, 1000])
+        never_falls(lambda b: size(40, b, rows, 4), BLOCKS)
+    assert size(1, 100, 8, -1) == 0 == size(1, 100, -8, 1)
+
+
+def test_decode_steps_need_no_prompts_workspace():
+    """At most 2.25 partial sums (16 queries of a head, with their two maxima and sum) per workgroup that runs at once, 32 bytes
+    a row beside them: of one row, whatever max_rows says, and of more rows by max_rows."""
+    most = 2.25 * 512 * 16 * (256 + 4) * 4
+    assert 0 < lib().pgd_attn_kv8_ws_bytes(24, 4, 256, 1, 8200, 1) <= most + 32
+    assert 0 < lib().pgd_attn_kv8_rows_ws_bytes(24, 4, 256, 32, 8200, 32, 1) <= most + 32 * 32
