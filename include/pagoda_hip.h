@@ -324,7 +324,7 @@ int pgd_kv8_select_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads
                        const int* block_tables, int max_blocks, int rows, int top, int sinks, int recent, int* sel,
                        int* count, void* ws, size_t ws_bytes);
 /* pgd_attn_kv8_dev over the pages sel[row, kv head, 0..count) alone (count is taken within
- * 0..top; entries outside the table are skipped, a page named twice counts twice). */
+ * 0..top; entries outside the table or past the row's context are skipped, a page named twice counts twice). */
 int pgd_attn_kv8_sparse_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, int head_dim, int heads,
                             const void* q, int ldq, int type, int nseq, const int* row_start, const int* lens,
                             const int* block_tables, int max_blocks, int rows, int top, const int* sel,

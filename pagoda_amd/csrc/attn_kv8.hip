@@ -612,6 +612,7 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     // (as the last of the rows up to this one)
     s.len = rs.seen(row);
     s.ctx = (int)min((long long)s.len, (long long)r.max_blocks * kPage);
+    s.pages = (s.ctx + kPage - 1) / kPage;
     slot = have > 1 ? (int)blockIdx.x : -1;
   } else {
     Found f;
@@ -640,7 +641,8 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
     const int i = page0 + nth(it);
     int at = -1;
     if (i < page1) at = !LIST ? i : it == 0 ? listed : pages_list[i];
-    walk.set(at, table, r.max_blocks, p.n_pages);
+    // (what the table says past a row's context, and what such pages hold, may be anything)
+    walk.set(at, table, LIST ? s.pages : r.max_blocks, p.n_pages);
   };
   if (pairs > 0) refill(0);
   if constexpr (!LIST) load_q(s, head, tile);

@@ -143,3 +143,28 @@ def test_attention_stays_in_its_workspace(dev, buf, t, heads, kv, hd, ctx, new):
         p.attn_dev(*call.args(), most, call.out, call.fresh.shape[1], ws, size)
         assert_close(call.result()[rows], want[rows], off[rows], t)
         assert (buf.down(ws, whole)[size:] == 0xFF).all()
+
+
+@pytest.mark.parametrize("t,heads,kv,hd", [(F32, 6, 2, 64), (BF16, 20, 1, 128), (F16, 3, 3, 256)])
+def test_listed_pages_behind_a_rows_context(dev, buf, t, heads, kv, hd):
+    """Entries of the table past a row's context, which may name pages that hold anything, or nothing yet: a list that names
+    them gives what it gives without them."""
+    rng = np.random.default_rng(hd)
+    step = Step(rng, kv, hd, [300, 70, 40], [4, 1, 1], t, spare=9, widen=8)
+    pool = pool_of(dev, buf, step)  # (pages not written hold 0xFF, codes of no number)
+    used = set(step.slots // PAGE)
+    fresh = [p for p in range(step.cache.n) if p not in used]
+    for s, c in enumerate(step.ctx):
+        m = kv8.pages(c)
+        step.tables[s, m:] = rng.choice(fresh + [-1, step.cache.n], step.width - m)
+        step.tables[s, m:m + 4] = fresh[:4]
+    q, qv, _ = queries(rng, step, heads, t)
+    call = Call(dev, buf, step, pool, heads, t, q)
+    for top in (7, 60):
+        sel = rng.integers(0, step.width, (step.rows, kv, top)).astype(np.int32)
+        sel[..., -1] = step.width - 1
+        sel[..., 0] = 0
+        picked = {r: [[p for p in sel[r, h] if p * PAGE < seen] for h in range(kv)] for r, _, seen in step.each_row()}
+        got = call.sparse(sel, np.full((step.rows, kv), top, np.int32))
+        want, off = kv8_close.attention(step, qv, heads, None, picked)
+        assert_close(got, want, off, t)
