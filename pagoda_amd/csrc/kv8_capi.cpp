@@ -43,7 +43,8 @@ void check_sizes(const Layout& at, int heads, int nseq, int max_blocks, int rows
   PGD_CHECK(nseq <= kMaxSeqs, kErrShape, "nseq must be at most 2^24");
   PGD_CHECK(max_blocks > 0 && max_blocks <= 1 << 26, kErrShape, "max_blocks must be 1..2^26");
   const int64_t group = heads / at.kv_heads, tiles = rows * group / 16 + (nseq < rows ? nseq : rows);
-  PGD_CHECK((int64_t)rows * heads < kBlocks * 4 && tiles * at.kv_heads < kBlocks / 2, kErrShape,
+  // (the join has a workgroup for four results of a row and head)
+  PGD_CHECK((int64_t)rows * heads + 3 < kBlocks * 4 && tiles * at.kv_heads < kBlocks / 2, kErrShape,
             "more rows or sequences than one launch holds");
 }
 

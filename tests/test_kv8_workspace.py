@@ -56,3 +56,13 @@ def test_decode_steps_need_no_prompts_workspace():
     most = 2.25 * 512 * 16 * (256 + 4) * 4
     assert 0 < lib().pgd_attn_kv8_ws_bytes(24, 4, 256, 1, 8200, 1) <= most + 32
     assert 0 < lib().pgd_attn_kv8_rows_ws_bytes(24, 4, 256, 32, 8200, 32, 1) <= most + 32 * 32
+
+
+def test_the_most_rows_that_a_launch_holds():
+    """Four results of a row and head a workgroup of 256 threads, below 2^32 threads: the sizes past that are refused."""
+    for size in (lambda rows: lib().pgd_attn_kv8_ws_bytes(1, 1, 64, 2, 40, rows),
+                 lambda rows: lib().pgd_attn_kv8_ws_bytes(2, 1, 64, 2, 40, rows // 2)):
+        assert size(2 ** 26 - 4) > 0
+        for rows in (2 ** 26 - 2, 2 ** 26, 2 ** 26 + 2):
+            assert size(rows) == 0
+    assert lib().pgd_attn_kv8_ws_bytes(1, 1, 64, 2, 40, 2 ** 26 - 3) == 0 == lib().pgd_attn_kv8_ws_bytes(1, 1, 64, 2, 40, 2 ** 26 - 1)
