@@ -526,6 +526,9 @@ __device__ inline bool whole_pages(const Page (&pg)[PG], int least) {
 // that hold the query. Returns the power of two it was divided by.
 template <int T, int HD, int N>
 __device__ inline int query_terms(float (&x)[8], h8 (&t)[N]) {
+  // An infinity becomes NaN: scores of -infinity alone would be those of masked positions.
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = __builtin_fmaf(x[j], 0.0f, x[j]);
   int e = 0;
   if constexpr (T != F16) {
     float most = 0;

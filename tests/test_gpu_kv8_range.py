@@ -143,3 +143,21 @@ def test_equal_scores_past_whole_numbers(dev, buf, form, power):
             want = v[step.tables[s, :kv8.pages(seen)], 0].reshape(-1, hd)[:seen].mean(0)
             # (all values are positive: sums of n of them, and terms of the weights)
             assert (np.abs(got[row] - want) <= want * ((2 * seen + 16) * 2.0 ** -23 + 2.0 ** -20)).all()
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("form", ["decode", "chunks", "prompt", "list"])
+def test_infinite_queries_give_nan(dev, buf, t, form):
+    """Also where all scores are the infinity that would be a masked position's."""
+    rng = np.random.default_rng(14)
+    ctx, new = FORMS[form]
+    heads, kv, hd = 4, 2, 64
+    step = Step(rng, kv, hd, ctx, new, t)
+    k = np.abs(rng.normal(0, 1, (len(step.slots), kv * hd))) + 0.5
+    with_rows(step, k=k.astype(np.float32))
+    q, qv, _ = queries(rng, step, heads, t)
+    q[0, 5], q[step.rows - 1, 3 * hd + 60] = [{BF16: np.uint16(b)}.get(t, x) for b, x in ((0xFF80, -np.inf), (0x7F80, np.inf))]
+    got = run(dev, buf, step, heads, t, q, form=form)
+    hit = np.zeros((step.rows, heads), bool)
+    hit[0, 0] = hit[step.rows - 1, 3] = True
+    assert np.isnan(got[hit]).all() and np.isfinite(got[~hit]).all()
