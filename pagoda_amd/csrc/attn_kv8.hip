@@ -522,8 +522,8 @@ __device__ inline bool whole_pages(const Page (&pg)[PG], int least) {
   return whole;
 }
 
-// Eight dims of a query as f16 terms; x is scaled to [2^14, 2^15) for the largest magnitude of the HD / 8 lanes
-// that hold the query. Returns the power of two it was divided by.
+// Eight dims of a query as f16 terms; x is scaled to [2^14, 2^15) for the largest magnitude (below 2^-126: by 2^141) of
+// the HD / 8 lanes that hold the query. Returns the power of two it was divided by.
 template <int T, int HD, int N>
 __device__ inline int query_terms(float (&x)[8], h8 (&t)[N]) {
   // An infinity becomes NaN: scores of -infinity alone would be those of masked positions.
@@ -535,10 +535,11 @@ __device__ inline int query_terms(float (&x)[8], h8 (&t)[N]) {
 #pragma unroll
     for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(x[j]));
     most = lanes_max<HD / 8>(most);
-    e = max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14, -112);
-    const float down = pow2(-e);
+    e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14;
+    // (2^-e may lie past f32: two powers of two)
+    const float up = pow2(min(-e, 126)), more = pow2(max(-e - 126, 0));
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] *= down;
+    for (int j = 0; j < 8; j++) x[j] = x[j] * up * more;
   }
   split<N>(x, t);
   return e;

@@ -161,3 +161,18 @@ def test_infinite_queries_give_nan(dev, buf, t, form):
     hit = np.zeros((step.rows, heads), bool)
     hit[0, 0] = hit[step.rows - 1, 3] = True
     assert np.isnan(got[hit]).all() and np.isfinite(got[~hit]).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("power", [-100, -118, -127, -135])
+def test_the_smallest_queries(dev, buf, t, form, power):
+    """Queries down to the smallest numbers before keys that are as large."""
+    rng = np.random.default_rng(-power)
+    ctx, new = FORMS[form]
+    heads, kv, hd = 6, 2, 64
+    step = Step(rng, kv, hd, ctx, new, t)
+    size = 2.0 ** min(-power, 125)
+    with_rows(step, k=(rng.normal(0, 1, (len(step.slots), kv * hd)).clip(-3, 3) * size).astype(np.float32))
+    q, qv = typed(rng.normal(0, 1, (step.rows, heads * hd)) * 2.0 ** power, t)
+    check(dev, buf, rng, step, heads, t, q, qv.reshape(-1, heads, hd), form)
