@@ -310,8 +310,8 @@ int pgd_attn_kv8_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
  * block table: sel [rows, kv_heads, top], ascending, -1 behind the count[row, kv_heads] =
  * min(top, pages) entries. The first `sinks` and the last `recent` pages are always among
  * them (sinks + recent <= top). The score bounds q.k over the page: q in signed 8 bits (q8 =
- * q / 2^e to nearest, ties to even, 2^e the smallest power of two that keeps the
- * group's heads within 127; non-finite entries count as 0), the page's key codes bounded per
+ * q / 2^e to nearest, ties to even, 2^e the smallest power of two, e >= -126, that keeps
+ * the group's heads within 127; non-finite entries count as 0), the page's key codes bounded per
  * channel by whole numbers hi and lo (the largest and smallest code over 4, rounded outward; the
  * append keeps them): score = 2^(key exponent) max over the group's heads of
  * sum(max(q8 hi, q8 lo)), exact in f32 (an infinity from 2^128 on); ties go to the lower page. A page outside the pool scores

@@ -267,7 +267,7 @@ __device__ inline void store4(const Out& o, int64_t row, int64_t col, f4 x) {
   if (o.gate) {
     const f4 g = load4<T>(o.gate, row * o.ldg + col);
 #pragma unroll
-    for (int j = 0; j < 4; j++) x[j] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g[j] * -1.44269504088896f));
+    for (int j = 0; j < 4; j++) x[j] /= 1.0f + __builtin_amdgcn_exp2f(g[j] * -1.44269504088896f);
   }
   if constexpr (T == F32) {
     *reinterpret_cast<f4*>(static_cast<float*>(o.out) + row * o.ldo + col) = x;

@@ -176,3 +176,17 @@ def test_the_smallest_queries(dev, buf, t, form, power):
     with_rows(step, k=(rng.normal(0, 1, (len(step.slots), kv * hd)).clip(-3, 3) * size).astype(np.float32))
     q, qv = typed(rng.normal(0, 1, (step.rows, heads * hd)) * 2.0 ** power, t)
     check(dev, buf, rng, step, heads, t, q, qv.reshape(-1, heads, hd), form)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_gates_of_large_values(dev, buf, t, form):
+    """A gate whose reciprocal lies below the normal range, before values that bring the product back."""
+    rng = np.random.default_rng(15)
+    ctx, new = FORMS[form]
+    step = Step(rng, 2, 64, ctx, new, t)
+    with_rows(step, v=(rng.normal(0, 1, (len(step.slots), 128)) * 2.0 ** 110).astype(np.float32))
+    q, qv, _ = queries(rng, step, 6, t)
+    g, gv = typed(rng.uniform(-88.5, -86.5, (step.rows, 6 * 64)), t)
+    got, want = check(dev, buf, rng, step, 6, t, q, qv, form, (g, gv.reshape(-1, 6, 64)))
+    assert np.abs(got).max() > 2.0 ** -20
