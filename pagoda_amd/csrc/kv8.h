@@ -20,7 +20,6 @@ namespace kv8 {
 constexpr int kPage = 16;             // positions of a page
 constexpr int kMaxPages = 1 << 27;    // slots (page * 16 + place) are ints
 constexpr int kExpMin = -126;         // smallest exponent of a (page, head)
-constexpr float kCodeMax = 448.0f;
 
 enum Type { F32 = 0, F16 = 1, BF16 = 2 };
 
