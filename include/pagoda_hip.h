@@ -260,11 +260,13 @@ size_t pgd_kv8_page_bytes(int kv_heads, int head_dim);
  * place); -1 in all three for rows behind the last sequence's. No other output overlaps an
  * input. nseq is at most 2^24, rows at most 2^30. status[i]: 0; or why the
  * sequence got nothing (its rows are -1, its length and table stay): 1 too few free
- * pages, 2 more positions than max_blocks pages hold, 3 rows past `rows`, 4 a negative length or
+ * pages, 2 more positions than max_blocks pages hold, 3 rows past `rows` (all sequences behind one that has some,
+ * those without rows too), 4 a negative length or
  * count. A sequence that needs no page is not refused for those that do; of those that need some, all behind the
  * first that is refused for want of pages are refused too. Refused rows keep their place in row_start, so
  * an attention over it computes something for them, of the positions that the sequence has; it is to be ignored.
- * A table entry that is negative makes slots -1. */
+ * A table entry that is negative makes slots -1. Maps without a row of -1 serve pgd_attn_decode_dev, which refuses
+ * such rows. */
 int pgd_kv_tables_dev(pgd_dev* dev, int block, int nseq, const int* lens, const int* counts, int* tables,
                       int max_blocks, const int* free_pages, int n_free, const int* taken, int rows, int* new_lens,
                       int* new_taken, int* row_start, int* seq_of_row, int* pos_of_row, int* slots, int* status);

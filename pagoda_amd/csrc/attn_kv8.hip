@@ -47,14 +47,16 @@ constexpr int many_items(int hd) { return hd == 128 ? 1024 : 1536; }
 // prompt_kernel: more, as contexts that are cut or not make uneven rounds (3 prompts of 2274 rows, head_dim 256: 277 us
 // against 346 with 512 items), but as many as run at once rather than chunks of less than kFullChunk pages, which the
 // way to their first page and their partial sums would make dear (236 rows on 3977 positions, head_dim 256: 74 us
-// against 97; 30 on 15000: 49 against 81; 500 on 3977: 122 against 130; with 32 pages 82, 49 and 131).
+// against 97; 30 on 15000: 49 against 81; 500 on 3977: 122 against 130; with 32 pages 82, 49 and 131; but two prompts of
+// 1500 rows on 900 and 3000 at head_dim 64: 64 against 62).
 constexpr int many_at_once(int hd) { return hd == 64 ? 1024 : 512; }
 constexpr int kFullChunk = 64;
 constexpr int kMinChunk = 8;     // pages: a pair for each of four waves
 constexpr int kOneChunk = 16;    // pages of tables (and lists) that are never cut: the join would cost more
 // Queries of a sequence and KV head: calls of up to these are item_kernel's alone. 16 sequences of 100 to 6000
-// positions, 7 queries a row at head_dim 64 (f32) and 6 at 256 (f16), with this and with 32: 12 rows each 20 and 31 us,
-// 58 and 58; 1 to 20 rows 46 and 54 at 256; 20 rows 66 and 63, 30 rows (past both) the same.
+// positions, 7 queries a row at head_dim 64 (f32) and 128 (bf16), 6 at 256 (f16), with this and with 32: at 64 12 rows
+// each 20 and 31 us, 18 rows 23 and 33; at 128 8 rows 31 and 34, 12 rows 38 and 41, but 18 rows 45 and 42; at 256 12 rows
+// 57 and 59, 1 to 20 rows 46 and 54, but 20 rows 66 and 63. 30 rows (past both) the same.
 constexpr int kFewQueries = 128;
 
 template <int T>

@@ -168,3 +168,26 @@ def test_listed_pages_behind_a_rows_context(dev, buf, t, heads, kv, hd):
         got = call.sparse(sel, np.full((step.rows, kv), top, np.int32))
         want, off = kv8_close.attention(step, qv, heads, None, picked)
         assert_close(got, want, off, t)
+
+
+def test_the_f32_attention_refuses_rows_to_spare(dev, buf):
+    """Rows that a step's maps give to no sequence are an error there, before anything is read for them."""
+    import ctypes as C
+
+    from pagoda_amd import PagodaError
+    from pagoda_amd._lib import call
+    from pagoda_amd.kv8 import kv_tables_dev
+
+    ints = lambda *v: buf.up(np.int32(v))
+    tables, rows = buf.up(np.full((1, 4), -1, np.int32)), 5
+    outs = [buf.up(np.zeros(n, np.int32)) for n in (1, 1, 2, rows, rows, rows, 1)]
+    kv_tables_dev(dev, 16, 1, ints(0), ints(3), tables, 4, ints(1, 0), 2, ints(0), rows, *outs)
+    assert buf.down(outs[3], np.zeros(rows, np.int32)).tolist() == [0, 0, 0, -1, -1]
+    q = np.ones((rows, 2, 64), np.float32)
+    pool, out = buf.up(np.ones((2, 1, 16, 64), np.float32)), buf.up(q)
+    attend = lambda n: call("pgd_attn_decode_dev", dev.handle, 2, 1, 64, 16, C.c_void_p(buf.up(q)), None, C.c_void_p(pool),
+                            C.c_void_p(pool), C.c_void_p(outs[3]), C.c_void_p(outs[4]), C.c_void_p(tables), 4, n, C.c_void_p(out))
+    with pytest.raises(PagodaError):
+        attend(rows)
+    attend(3)
+    assert np.allclose(buf.down(out, q)[:3], 1)
