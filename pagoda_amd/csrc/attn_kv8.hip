@@ -447,18 +447,19 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
   }
   // This lane's largest t and t - m + ev. What its column's other lanes have need not be known while no lane of the
   // wave is past what its column's maxima may lag.
-  float t[PG], top = -INFINITY, top_v = -INFINITY;
+  auto largest = [&](int w) { return fmaxf(fmaxf(x[w][0], x[w][1]), fmaxf(x[w][2], x[w][3])) * by[w]; };
+  float top = -INFINITY, top_v = -INFINITY;
 #pragma unroll
   for (int w = 0; w < PG; w++) {
-    t[w] = fmaxf(fmaxf(x[w][0], x[w][1]), fmaxf(x[w][2], x[w][3])) * by[w];
-    top = fmaxf(top, t[w]);
-    top_v = fmaxf(top_v, t[w] - q.m + ev[w]);
+    const float t = largest(w);
+    top = fmaxf(top, t);
+    top_v = fmaxf(top_v, t - q.m + ev[w]);
   }
   if (__any(top > q.m + kSlack || top_v > q.d + kSlackV)) {
     const float m = fmaxf(q.m, quads_max(top)), base = m > -INFINITY ? m : 0.0f;
     top_v = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < PG; w++) top_v = fmaxf(top_v, t[w] - base + ev[w]);
+    for (int w = 0; w < PG; w++) top_v = fmaxf(top_v, largest(w) - base + ev[w]);
     const float d = ceilf(fmaxf(quads_max(top_v), q.d + (q.m - base)));
     if (q.m > -INFINITY) {  // (else O holds zeros, or NaN)
       q.l *= __builtin_amdgcn_exp2f(q.m - base);
@@ -485,19 +486,18 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
   const bool apart = __any(up + far > 100.0f);
 #pragma unroll
   for (int w = 0; w < PG; w++) {
+    const float f = up + ev[w];
     float e[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) e[i] = __builtin_fmaf(x[w][i], by[w], -at);
-    const float f = up + ev[w];
+    for (int i = 0; i < 4; i++) x[w][i] = __builtin_fmaf(x[w][i], by[w], -at);
+#pragma unroll
+    for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(x[w][i]);
+    sum[w] = (e[0] + e[1]) + (e[2] + e[3]);
     if (apart) {
       // pages so far apart that 2^(t - m) underflows where the weight does not
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[w][i] = __builtin_amdgcn_exp2f(e[i] + f);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(e[i]);
-    sum[w] = (e[0] + e[1]) + (e[2] + e[3]);
-    if (!apart) {
+      for (int i = 0; i < 4; i++) x[w][i] = __builtin_amdgcn_exp2f(x[w][i] + f);
+    } else {
       const float of_code = __builtin_amdgcn_exp2f(f);
 #pragma unroll
       for (int i = 0; i < 4; i++) x[w][i] = e[i] * of_code;
