@@ -551,8 +551,8 @@ __device__ inline int query_terms(float (&x)[8], h8 (&t)[N]) {
 
 // NQ tiles of 16 queries, four waves each, side by side over the same pages: what one loads the other finds in the
 // caches. Bound by HBM at long contexts (8 of 20000 to 130000 positions, 4 heads of 128, bf16: 98 us, 5.1 TB/s); at
-// short ones 5 us of the chain from row starts to pages go before it (32 of 40 to 4000, 4 heads of 256, f32: 18.5 us,
-// 3.3 TB/s).
+// short ones 5 us of the chain from row starts to pages go before it (32 of 40 to 4000, 4 heads of 256, f32: 18.8 us,
+// 3.2 TB/s).
 template <int HD, int T, int NQ, bool LIST>
 __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out out, List list, Share share, void* ws,
                                                            Slots slots) {
@@ -787,10 +787,11 @@ __global__ __launch_bounds__(256 * NQ, 2) void item_kernel(Pool p, Rows r, Out o
 
 // Workgroup: 64 queries, 16 a wave, over the pages of a chunk, PG at a time through LDS (two buffers, one
 // barrier a step). A wave keeps its queries' terms in registers. 32 queries a wave would share the codes' conversion
-// and measured slower, with fewer waves (1500 bf16 rows on 3900 positions at head_dim 128 107 against 91 us).
+// and measured slower, with fewer waves (1500 bf16 rows on 3900 positions at head_dim 128 107 against 91 us, with one
+// term of weights; with two this form takes 97).
 // Bound by issue: 5 VALU instructions (codes to f16, softmax) for each matrix instruction of 16 clocks, which are busy
-// 36% of the time. 2274 f32 rows on 500 to 4001 positions, 24 / 4 heads of 256: 177 to 322 us by how rows fall on
-// contexts.
+// 37% of the time. 2274 f32 rows on 500 to 4001 positions, 24 / 4 heads of 256: 174 to 330 us by how rows fall on
+// contexts. 1000 bf16 rows on 4000 positions 206 us.
 template <int HD, int T, int PG>
 __global__ __launch_bounds__(256, 2) void prompt_kernel(Pool p, Rows r, Out out, Share share, void* ws, Slots slots) {
   constexpr int kSegs = HD / 64, kSteps = HD / 32, kTiles = HD / 16, kN = kTerms<T>, kW = kWeightTerms;

@@ -30,7 +30,7 @@ __device__ inline void wave_lds_fence() {
 // takes the page and the rows that follow it there (up to 15 past the workgroup's own), the others are
 // passed over. The page is made in LDS and written whole: 32 hd bytes, whatever part is new.
 // Few rows: 4 us, one page's chain of slots, loads, maxima, codes and bounds. 8400 prompt rows (bf16, 4 heads of 256:
-// 34 MB in, 17 out) 21 us, 2.4 TB/s: all pages are in flight at once, so they load, compute and store together;
+// 34 MB in, 17 out) 20 us, 2.6 TB/s: all pages are in flight at once, so they load, compute and store together;
 // the bounds and the values' single bytes are 1.3 us of it each. A wave a page is slower (its ~2500 instructions).
 template <int HD, int T, int ROWS>
 __global__ __launch_bounds__(256) void append_kernel(Pool p, const void* k, int64_t ldk, const void* v, int64_t ldv,
