@@ -293,11 +293,11 @@ int pgd_kv8_read_dev(pgd_dev* dev, const void* pool, int n_pages, int kv_heads, 
  * kv_heads. Positions past max_blocks pages do not exist. A row that attends to nothing
  * gets zeros; rows of no sequence are left as they were; attending a position of a page outside the pool
  * gives NaN. Sums, maxima and the weights' sum are f32. Before the products on the matrix cores f32 rows of q are held
- * to 2^-22 (f16 rows exactly, bf16 rows too but for what lies below 2^-40 of the head's largest), the
- * softmax weights to 2^-21, nothing finer than 2^-36 of the largest. An infinity or NaN in a head of q makes that
- * head's result NaN. A score of magnitude 2^127 and more is an infinity: a row with a positive one is NaN, one whose
- * scores are all negative ones gets zeros. max_rows: the largest number of rows of a sequence, or any bound on it (it
- * selects kernels, results are right with any value). row_start ascends. ws: pgd_attn_kv8_rows_ws_bytes bytes, or pgd_attn_kv8_ws_bytes for any
+ * to 2^-22 and bf16 rows exactly, but to no less than 2^-39 of the head's largest entry, f16 rows exactly; the softmax
+ * weights to 2^-21, but to no less than 2^-36 of the largest. An infinity or NaN in a head of q makes that head's
+ * result NaN. A score of magnitude 2^127 and more is an infinity: a result whose largest score is one is NaN.
+ * max_rows: the largest number of rows of a sequence, or any bound on it (it selects kernels, results are right with
+ * any value). row_start ascends. ws: pgd_attn_kv8_rows_ws_bytes bytes, or pgd_attn_kv8_ws_bytes for any
  * max_rows (0 of sizes that the call refuses), that no other stream uses meanwhile (a captured graph's included); its
  * contents do not matter, and one that is large enough for a call is for every call of smaller numbers. The order of the
  * sums depends on the sizes, max_rows, row_start and lens, on nothing else. */

@@ -12,10 +12,10 @@
 // whole number near the pages' exponents: adding them to it and taking it back from results is exact, also where
 // scores are so large that t + ev would not be.
 // Codes convert to f16 exactly. Queries are scaled by a power of two into f16's range and enter as f16 terms: f32
-// rows two (22 bits and at least 2^-40 of the row's largest), f16 rows themselves, bf16 rows one (exact to 2^-40 of the
-// largest). The weights, times 2^12, enter as two terms, 2^-21 and 2^-36 of the largest (bf16 rows: one; its
-// 2^-11 is an eighth of their own rounding). bf16 terms would need no scaling but half as many more
-// products: three for f32 where f16 takes two.
+// rows two (22 bits), f16 rows themselves, bf16 rows one (exact): all to half of f16's smallest step, 2^-25 where the
+// largest entry is 2^14 or more. The weights, times 2^12, enter as two terms, 2^-21, and 2^-36 of the largest. With one
+// term, an eighth of bf16's own rounding, up to one bf16 result in 200 is a neighbour of the exact one's rounding. bf16
+// terms would need no scaling but half as many more products: three for f32 where f16 takes two.
 // The lane that holds a score holds it as the operand of the second product: lane
 // (query n = l % 16, kq = l / 16) has positions 4 kq .. 4 kq + 3 of both pages, which
 // are the 8 that a lane of the second product's operand takes, and its results are
@@ -66,6 +66,7 @@ constexpr int kWeightTerms = 2;
 // the old ones or more (and all of a wave's with them), so weights of codes reach 2^kSlackV. They enter times
 // 2^kWeightExp: f16 holds 2^-24 to 65504.
 constexpr float kSlack = 4, kSlackV = 3, kWeightExp = 15 - kSlackV;
+constexpr float kLowest = -3.402823466e38f;
 
 // x as f16 terms to nearest, each of what the ones before leave.
 template <int N>
@@ -342,6 +343,7 @@ struct State {
   };
   __device__ Factor factor() const {
     if (l == 0) return Factor{0.0f, 0};
+    if (m == kLowest) return Factor{NAN, 0};  // all scores lie below f32's range, who knows how far apart
     return Factor{1.0f / l, d > -INFINITY ? (int)(d - kWeightExp) : 0};
   }
 };
@@ -421,15 +423,17 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
 #pragma unroll
     for (int i = 0; i < 4; i++) x[w][i] = s[w][i];
   }
-  if (__any(q.exp + highest > 126)) {
-    // not above it either, where keys and queries that have no channel in common may be: a power of two goes to the
-    // product first
+  if (__any(q.exp + highest > 96)) {
+    // (s stays below 2^33.) The factor may be infinite where keys and queries have no channel in common, so its power of
+    // two comes last. A score below f32's range becomes its lowest number: -infinity is a masked position's.
 #pragma unroll
     for (int w = 0; w < PG; w++) {
-      const int exp = q.exp + Meta::ek(pg[w].meta), over = max(exp - 126, 0);
-      if (over > 0) by[w] = __builtin_ldexpf(scale, 126);
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[w][i] = __builtin_ldexpf(x[w][i], over);
+      for (int i = 0; i < 4; i++) {
+        const float t = __builtin_ldexpf(x[w][i] * scale, q.exp + Meta::ek(pg[w].meta));
+        x[w][i] = t < kLowest ? kLowest : t;
+      }
+      by[w] = 1.0f;
     }
   }
   if (!whole) {

@@ -190,3 +190,43 @@ def test_gates_of_large_values(dev, buf, t, form):
     g, gv = typed(rng.uniform(-88.5, -86.5, (step.rows, 6 * 64)), t)
     got, want = check(dev, buf, rng, step, 6, t, q, qv, form, (g, gv.reshape(-1, 6, 64)))
     assert np.abs(got).max() > 2.0 ** -20
+
+
+def held(q, t):
+    """Queries [rows, heads, hd] as the products take them: the head's largest entry brought to [2^14, 2^15) by a power of two,
+    in two f16 terms (bf16 rows: one)."""
+    e = np.frexp(np.abs(q).max(-1, keepdims=True))[1] - 15
+    x = np.ldexp(q, -e)
+    first = x.astype(np.float16).astype(float)
+    return np.ldexp(first + ((x - first).astype(np.float16).astype(float) if t == F32 else 0), e)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_scores_past_f32(dev, buf, t, form):
+    """A head whose largest score is infinite is NaN, of either sign; infinitely low scores beside others count nothing."""
+    rng = np.random.default_rng(16)
+    ctx, new = FORMS[form]
+    heads, kv, hd = 6, 2, 64
+    step = Step(rng, kv, hd, ctx, new, t)
+    n = len(step.slots)
+    k = np.zeros((n, kv, hd), np.float32)
+    k[..., 0] = rng.uniform(1, 2, (n, kv)) * 2.0 ** 60
+    k[:, 1, 1:] = np.where(np.arange(n) % 3 == 0, 1, 0)[:, None] * rng.normal(0, 1, (n, hd - 1)) * 2.0 ** 55
+    k[::3, 1, 0] = 0  # head 1: every third position has scores of its own
+    with_rows(step, k=k.reshape(n, -1))
+    q = np.zeros((step.rows, heads, hd), np.float32)
+    q[:, :3, 0] = np.where(np.arange(3) == 1, 1, -1) * 2.0 ** 100
+    q[:, 3:, 0] = -(2.0 ** 100)
+    q[:, 3:, 1:] = rng.normal(0, 1, (step.rows, 3, hd - 1)) * 2.0 ** 67  # (far apart, and far below 2^127 more)
+    q, qv = typed(q.reshape(step.rows, -1), t)
+    qv = qv.reshape(-1, heads, hd)
+    got = run(dev, buf, step, heads, t, q, form=form)
+    assert np.isnan(got[:, :3]).all()
+    rows = sorted(some_rows(step, rng))
+    # Entries of 2^67 beside 2^100 are held to 2^61, half of f16's smallest step times 2^86: scores of 2^122 move by
+    # 2^116 then, which may be more than the two largest lie apart.
+    largest = np.abs(qv).max(-1, keepdims=True)
+    assert (np.abs(held(qv, t) - qv) <= np.maximum(2.0 ** -22 * np.abs(qv), 2.0 ** -39 * largest)).all()
+    want, off = kv8_close.attention(step, held(qv, t), heads, rows=rows)
+    assert_close(got[rows, 3:], want[rows, 3:], off[rows, 3:], t)
