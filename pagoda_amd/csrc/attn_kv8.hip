@@ -413,13 +413,16 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
                              h8 (&out)[PG / 2][kWeightTerms]) {
   const int kq = threadIdx.x >> 4 & 3;
   float x[PG][4], by[PG], ev[PG];
-  int highest = INT_MIN;
+  int ek[PG], highest = INT_MIN;
 #pragma unroll
   for (int w = 0; w < PG; w++) {
+    // (for no page the pool's first one was loaded: what that holds must not show, be it in the rounding of results)
+    const uint32_t meta = pg[w].id >= 0 ? pg[w].meta : Meta::pack(kExpMin, kExpMin, 0);
+    ek[w] = Meta::ek(meta);
+    ev[w] = (float)Meta::ev(meta);
     // (not below the normal range: the scores of masked positions are infinite)
-    by[w] = fmaxf(__builtin_ldexpf(scale, q.exp + Meta::ek(pg[w].meta)), 1.17549435e-38f);
-    ev[w] = (float)Meta::ev(pg[w].meta);
-    highest = max(highest, Meta::ek(pg[w].meta));
+    by[w] = fmaxf(__builtin_ldexpf(scale, q.exp + ek[w]), 1.17549435e-38f);
+    highest = max(highest, ek[w]);
 #pragma unroll
     for (int i = 0; i < 4; i++) x[w][i] = s[w][i];
   }
@@ -430,7 +433,7 @@ __device__ inline void weigh(const f4 (&s)[PG], const Page (&pg)[PG], float scal
     for (int w = 0; w < PG; w++) {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const float t = __builtin_ldexpf(x[w][i] * scale, q.exp + Meta::ek(pg[w].meta));
+        const float t = __builtin_ldexpf(x[w][i] * scale, q.exp + ek[w]);
         x[w][i] = t < kLowest ? kLowest : t;
       }
       by[w] = 1.0f;

@@ -5,7 +5,7 @@ import pytest
 
 import kv8
 import kv8_close
-from kv8 import BF16, F16, F32, PAGE, Step, typed
+from kv8 import BF16, F16, F32, PAGE, Step, typed, value
 from kv8_close import assert_close
 from test_gpu_kv8 import Call, GpuPool, pool_of, queries
 from test_gpu_mxfp4 import Buffers, buf  # noqa: F401
@@ -191,3 +191,32 @@ def test_the_f32_attention_refuses_rows_to_spare(dev, buf):
         attend(rows)
     attend(3)
     assert np.allclose(buf.down(out, q)[:3], 1)
+
+
+@pytest.mark.parametrize("t,heads,kv,hd", [(F32, 6, 2, 64), (BF16, 7, 1, 128), (F16, 12, 2, 256)])
+def test_results_do_not_hang_on_pages_of_others(dev, buf, t, heads, kv, hd):
+    """The pool's first page, which no sequence here has, changes no bit of a result, whatever it holds: contexts and
+    lists of odd numbers of pages among them."""
+    rng = np.random.default_rng(80 + hd)
+    for ctx, new in (([37, 300, 1], [1, 1, 1]), ([90, 3000], [4, 1]), ([700, 75], [150, 11])):
+        step = Step(rng, kv, hd, ctx, new, t)
+        q, qv, _ = queries(rng, step, heads, t)
+        pool = GpuPool(dev, buf, kv, hd, step.cache.n + 1)
+        pool.append(step.k_raw, step.v_raw, step.slots + PAGE, t)
+        step.tables = np.where(step.tables >= 0, step.tables + 1, -7).astype(np.int32)
+        call = Call(dev, buf, step, pool, heads, t, q)
+        sel = np.stack([rng.permutation(step.width)[:3] for _ in range(step.rows * kv)]).reshape(step.rows, kv, 3).astype(np.int32)
+        sel[..., 0] = 0
+        count = np.full((step.rows, kv), 3, np.int32)
+        first = None
+        for size in (None, 0.0, 1.0, 2.0 ** 15, 2.0 ** -14):  # (as it was allocated, then written)
+            if size is not None:
+                rows = typed(np.full((PAGE, kv * hd), size) * rng.choice([-1, 1], (PAGE, kv * hd)), t)[0]
+                pool.append(rows, rows, np.arange(PAGE), t)
+            if size == 2.0 ** 15 and t != F16:
+                rows = typed(rows.astype(np.float32) if t == F32 else value(rows, t) * 2.0 ** 100, t)[0]
+                pool.append(rows, rows, np.arange(PAGE), t)
+            got = call.attn(), call.sparse(sel, count)
+            first = first or got
+            for a, b in zip(got, first):
+                assert np.array_equal(a, b), (ctx, size)
